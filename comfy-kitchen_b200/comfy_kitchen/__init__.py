@@ -30,6 +30,17 @@ __all__ = [
     "dequantize_mxfp8",
     "scaled_mm_nvfp4",
     "scaled_mm_mxfp8",
+    "layer_norm",
+    "layer_norm_forward",
+    "layer_norm_forward_mxfp8",
+    "layer_norm_backward",
+    "layer_norm_backward_mxfp8",
+    "gelu_checkpointed",
+    "gelu_mxfp8_forward",
+    "gelu_mxfp8_backward",
+    "linear_checkpointed",
+    "linear_weight_grad_mxfp8",
+    "linear_input_grad_mxfp8",
     "swap_nibbles",
     "to_blocked",
     "from_blocked",
@@ -167,3 +178,19 @@ def list_backends() -> dict:
 def use_backend(name: str):
     """Context manager forcing one backend for the calling thread."""
     return registry.use_backend(name)
+
+
+# ---- training (needs the functions above: the tensor layouts are built on them) ---------------
+from .training import (  # noqa: E402
+    gelu_checkpointed,
+    gelu_mxfp8_backward,
+    gelu_mxfp8_forward,
+    layer_norm,
+    layer_norm_backward,
+    layer_norm_backward_mxfp8,
+    layer_norm_forward,
+    layer_norm_forward_mxfp8,
+    linear_checkpointed,
+    linear_input_grad_mxfp8,
+    linear_weight_grad_mxfp8,
+)

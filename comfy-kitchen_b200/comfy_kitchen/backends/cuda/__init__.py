@@ -36,6 +36,14 @@ __all__ = [
     "linear_mxfp8_from_float",
     "nvfp4_tensor_scale",
     "quantize_nvfp4_dynamic",
+    "layer_norm_forward",
+    "layer_norm_forward_mxfp8",
+    "layer_norm_backward",
+    "layer_norm_backward_mxfp8",
+    "gelu_mxfp8_forward",
+    "gelu_mxfp8_backward",
+    "linear_weight_grad_mxfp8",
+    "linear_input_grad_mxfp8",
     "check_device_status",
 ]
 
@@ -51,6 +59,7 @@ _host = None  # the wrappers' native half (csrc/host), bound to the loaded libra
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _L = ctypes.c_int64
+_F = ctypes.c_float
 
 # symbol -> argument types (return type is int unless listed in _RESTYPE)
 _SIGNATURES = {
@@ -86,11 +95,20 @@ _SIGNATURES = {
     "ck_peer_status": [_P],
     "ck_dequantize_nvfp4": [_P, _P, _P, _P, _I, _L, _L, _I, _P],
     "ck_dequantize_mxfp8": [_P, _P, _P, _I, _L, _L, _P],
+    "ck_layer_norm_forward": [_P, _I, _L, _L, _L, _L, _L, _P, _P, _I, _L, _L, _L, _F, _F, _P, _P, _P, _P, _P, _P],
+    "ck_layer_norm_backward_workspace_bytes": [_L, _L, _L],
+    "ck_layer_norm_backward": [_P, _I, _L, _L, _L, _L, _L, _P, _L, _L, _L, _P, _P, _P, _P, _P, _I, _L, _L, _F, _P, _P, _P, _P, _L, _P],
+    "ck_gelu_mxfp8_forward": [_P, _I, _P, _P, _P, _L, _L, _P],
+    "ck_gelu_mxfp8_backward": [_P, _I, _P, _P, _P, _L, _L, _P],
+    "ck_linear_grad_mxfp8_workspace_bytes": [_I, _I, _I, _L, _L, _L],
+    "ck_linear_weight_grad_mxfp8": [_P, _I, _P, _P, _P, _I, _P, _L, _L, _L, _P, _L, _P],
+    "ck_linear_input_grad_mxfp8": [_P, _I, _P, _P, _P, _I, _L, _L, _L, _P, _L, _P],
 }
 _RESTYPE = {"ck_last_error": ctypes.c_char_p, "ck_nvfp4_tensor_scale_scratch_bytes": ctypes.c_int64,
             "ck_quantize_nvfp4_dynamic_scratch_bytes": ctypes.c_int64, "ck_quantize_nvfp4_dynamic_whole_input_bytes": ctypes.c_int64,
             "ck_scaled_mm_workspace_bytes": ctypes.c_int64, "ck_linear_nvfp4_from_float_workspace_bytes": ctypes.c_int64,
-            "ck_linear_mxfp8_from_float_workspace_bytes": ctypes.c_int64}
+            "ck_linear_mxfp8_from_float_workspace_bytes": ctypes.c_int64, "ck_layer_norm_backward_workspace_bytes": ctypes.c_int64,
+            "ck_linear_grad_mxfp8_workspace_bytes": ctypes.c_int64}
 
 
 def library_path() -> str:
@@ -732,6 +750,248 @@ def scaled_mm_mxfp8(a: torch.Tensor, b: torch.Tensor, block_scale_a: torch.Tenso
 
 
 # ------------------------------------------------------------------------------------------
+# training
+# ------------------------------------------------------------------------------------------
+def _row_levels(t: torch.Tensor, align: int = 1) -> tuple[torch.Tensor, int, int, int]:
+    """``(tensor, inner, outer_stride, inner_stride)``: row r of the tensor (its last dimension is a row) starts at
+    ``(r // inner) * outer_stride + (r % inner) * inner_stride`` elements.  A tensor whose rows do not lie so, or not on
+    ``align``-byte boundaries, is copied."""
+    cols = t.shape[-1]
+    if not t.is_contiguous() and (t.stride(-1) == 1 or cols == 1):
+        levels: list[tuple[int, int]] = []  # (size, stride), outermost first
+        for size, stride in zip(t.shape[:-1], t.stride()[:-1]):
+            if size == 1:
+                continue
+            if levels and levels[-1][1] == size * stride:
+                levels[-1] = (levels[-1][0] * size, stride)
+            else:
+                levels.append((size, stride))
+        if len(levels) <= 2 and t.data_ptr() % align == 0 and all(stride * t.element_size() % align == 0 for _, stride in levels):
+            inner, inner_stride = levels[-1] if levels else (1, cols)
+            return t, inner, levels[0][1] if len(levels) == 2 else 0, inner_stride
+        t = t.contiguous()
+    elif not t.is_contiguous():
+        t = t.contiguous()
+    elif t.data_ptr() % align or cols * t.element_size() % align:
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t, t.numel() // cols, 0, cols
+
+
+def _norm_params(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None):
+    """``(weight, bias, dtype code, groups, weight_stride, bias_stride)`` of a layer norm's parameters: ``[cols]``, or
+    ``[groups, cols]`` (with ones in between, if any) where ``groups`` is x's first dimension."""
+    cols, shape, groups = x.shape[-1], None, 1
+    strides = [0, 0]
+    params = [weight, bias]
+    for i, p in enumerate(params):
+        if p is None:
+            continue
+        if shape is None:
+            shape, dtype = p.shape, p.dtype
+        assert p.shape == shape and p.dtype == dtype, "weight and bias must have the same shape and dtype"
+        assert p.device == x.device, "weight and bias must be on x's device"
+        assert p.dim() >= 1 and p.shape[-1] == cols, f"weight and bias must have rows of {cols}"
+        if p.dim() > 1:
+            groups = p.shape[0]
+            assert p.numel() == groups * cols and x.dim() > 1 and x.shape[0] == groups, "one weight row for each of x's first dimension"
+        p = _plain(p)
+        if cols > 1 and p.stride(-1) != 1:
+            p = p.contiguous()
+        params[i] = p
+        strides[i] = p.stride(0) if p.dim() > 1 else 0
+    code = DTYPE_TO_CODE[x.dtype] if shape is None else DTYPE_TO_CODE.get(dtype, 9)
+    return params[0], params[1], code, groups, strides[0], strides[1]
+
+
+def _layer_norm_forward(x, weight, bias, eps, weight_offset, stats: bool, copy: bool):
+    lib = load_library()
+    x = _plain(x)
+    assert x.dim() >= 1 and x.shape[-1] > 0, "layer norm needs rows of one element at least"
+    cols = x.shape[-1]
+    assert not copy or cols % 32 == 0, f"num_cols must be divisible by 32, got {cols}"
+    rows, dev = x.numel() // cols, x.device
+    weight, bias, code, groups, w_stride, b_stride = _norm_params(x, weight, bias)
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    mean = rstd = codes = scales = None
+    if stats:
+        mean, rstd = torch.empty(rows, dtype=torch.float32, device=dev), torch.empty(rows, dtype=torch.float32, device=dev)
+    if copy:
+        codes = torch.empty((rows, cols), dtype=torch.float8_e4m3fn, device=dev)
+        scales = torch.empty((roundup(rows, 128), roundup(cols // 32, 4)), dtype=torch.float8_e8m0fnu, device=dev)
+    if rows > 0:
+        x, inner, outer_stride, inner_stride = _row_levels(x, 16 if copy else 1)
+        with _on_device(dev):
+            _check(lib.ck_layer_norm_forward(x.data_ptr(), DTYPE_TO_CODE[x.dtype], rows, cols, inner, outer_stride, inner_stride, _ptr(weight),
+                                             _ptr(bias), code, groups, w_stride, b_stride, weight_offset, eps, y.data_ptr(), _ptr(mean), _ptr(rstd),
+                                             _ptr(codes), _ptr(scales), _stream(dev)), "layer_norm_forward")
+    return y, mean, rstd, codes, scales
+
+
+def layer_norm_forward(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, eps: float = 1e-5,
+                       weight_offset: float = 0.0) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``(y, mean, rstd)`` of a layer norm over the last dimension: ``y = (x - mean) * rstd * (weight_offset + weight) + bias``, the
+    statistics in fp32, one for each row.  ``weight`` and ``bias``: ``[cols]``, or ``[groups, cols]`` for x's first dimension; of
+    x's dtype or fp32."""
+    return _layer_norm_forward(x, weight, bias, eps, weight_offset, True, False)[:3]
+
+
+def layer_norm_inference(x, weight=None, bias=None, eps: float = 1e-5, weight_offset: float = 0.0) -> torch.Tensor:
+    """:func:`layer_norm_forward` for callers that need no statistics."""
+    return _layer_norm_forward(x, weight, bias, eps, weight_offset, False, False)[0]
+
+
+def layer_norm_forward_mxfp8(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, eps: float = 1e-5,
+                             weight_offset: float = 0.0) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """:func:`layer_norm_forward` and, from the same pass, ``quantize_mxfp8(x)``: ``(y, mean, rstd, codes, block_scales)``."""
+    return _layer_norm_forward(x, weight, bias, eps, weight_offset, True, True)
+
+
+def _layer_norm_backward(dy, x, codes, scales, mean, rstd, weight, weight_offset, groups, param_dtype, weight_grad, bias_grad):
+    lib = load_library()
+    dy = _plain(dy)
+    cols = dy.shape[-1]
+    rows, dev = dy.numel() // cols, dy.device
+    assert mean.numel() == rstd.numel() == rows and mean.dtype == rstd.dtype == torch.float32 and mean.is_contiguous() and rstd.is_contiguous(), \
+        "mean and rstd must hold one fp32 value for each row"
+    w_stride = 0
+    if weight is not None:
+        weight = _plain(weight)
+        assert weight.shape[-1] == cols and weight.numel() == groups * cols and weight.dtype == param_dtype, "Invalid weight shape or dtype"
+        if cols > 1 and weight.stride(-1) != 1:
+            weight = weight.contiguous()
+        w_stride = weight.stride(0) if weight.dim() > 1 else 0
+    code = DTYPE_TO_CODE.get(param_dtype, 9)
+    dx = torch.empty(dy.shape, dtype=dy.dtype, device=dev)
+    make = torch.empty if rows > 0 else torch.zeros
+    dweight = make((groups, cols), dtype=param_dtype, device=dev) if weight_grad else None
+    dbias = make((groups, cols), dtype=param_dtype, device=dev) if bias_grad else None
+    if rows > 0:
+        x_inner = x_outer_stride = x_inner_stride = 0
+        if x is not None:
+            x = _plain(x)
+            assert x.shape == dy.shape and x.dtype == dy.dtype and x.device == dev, "x must have dy's shape, dtype and device"
+            x, x_inner, x_outer_stride, x_inner_stride = _row_levels(x)
+        else:
+            codes, scales = _plain(codes), _plain(scales)
+            assert codes.shape == (rows, cols) and scales.shape == (roundup(rows, 128), roundup(cols // 32, 4)), "Invalid codes or scale shape"
+            assert codes.is_contiguous() and scales.is_contiguous(), "codes and scales must be contiguous"
+        dy, inner, outer_stride, inner_stride = _row_levels(dy)
+        need = _workspace_bytes("ck_layer_norm_backward_workspace_bytes", rows, cols, groups) if weight_grad or bias_grad else 0
+        with _on_device(dev):
+            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+            _check(lib.ck_layer_norm_backward(dy.data_ptr(), DTYPE_TO_CODE[dy.dtype], rows, cols, inner, outer_stride, inner_stride, _ptr(x), x_inner,
+                                              x_outer_stride, x_inner_stride, _ptr(codes), _ptr(scales), mean.data_ptr(), rstd.data_ptr(), _ptr(weight),
+                                              code, groups, w_stride, weight_offset, dx.data_ptr(), _ptr(dweight), _ptr(dbias), _ptr(ws), need,
+                                              _stream(dev)), "layer_norm_backward")
+    return dx, dweight, dbias
+
+
+def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, weight: torch.Tensor | None = None,
+                        weight_offset: float = 0.0, groups: int = 1, param_dtype: torch.dtype | None = None, weight_grad: bool = True,
+                        bias_grad: bool = True):
+    """``(dx, dweight, dbias)`` of :func:`layer_norm_forward`; the parameters' gradients are ``[groups, cols]`` of ``param_dtype``
+    (the weight's dtype, or dy's without one), or None where they are not wanted.  Sums over rows are added in a fixed order."""
+    param_dtype = param_dtype or (dy.dtype if weight is None else weight.dtype)
+    return _layer_norm_backward(dy, x, None, None, mean, rstd, weight, weight_offset, groups, param_dtype, weight_grad, bias_grad)
+
+
+def layer_norm_backward_mxfp8(dy: torch.Tensor, codes: torch.Tensor, block_scales: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
+                              weight: torch.Tensor | None = None, weight_offset: float = 0.0, groups: int = 1,
+                              param_dtype: torch.dtype | None = None, weight_grad: bool = True, bias_grad: bool = True):
+    """:func:`layer_norm_backward` from the MXFP8 copy of x that :func:`layer_norm_forward_mxfp8` made."""
+    param_dtype = param_dtype or (dy.dtype if weight is None else weight.dtype)
+    return _layer_norm_backward(dy, None, codes, block_scales, mean, rstd, weight, weight_offset, groups, param_dtype, weight_grad, bias_grad)
+
+
+def _aligned(t: torch.Tensor, align: int) -> torch.Tensor:
+    """The tensor, contiguous and on an ``align``-byte boundary."""
+    t = _plain(t)
+    if not t.is_contiguous():
+        t = t.contiguous()
+    return t.clone() if t.data_ptr() % align else t
+
+
+def gelu_mxfp8_forward(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``(gelu_tanh(x), *quantize_mxfp8(x))`` of a 2-D tensor in one pass."""
+    lib = load_library()
+    x = _aligned(x, 32)
+    rows, cols = x.shape
+    assert cols > 0 and cols % 32 == 0, f"num_cols must be divisible by 32, got {cols}"
+    y = torch.empty_like(x)
+    codes = torch.empty((rows, cols), device=x.device, dtype=torch.float8_e4m3fn)
+    scales = torch.empty((roundup(rows, 128), roundup(cols // 32, 4)), device=x.device, dtype=torch.float8_e8m0fnu)
+    if rows > 0:
+        with _on_device(x.device):
+            _check(lib.ck_gelu_mxfp8_forward(x.data_ptr(), DTYPE_TO_CODE[x.dtype], y.data_ptr(), codes.data_ptr(), scales.data_ptr(), rows, cols,
+                                             _stream(x.device)), "gelu_mxfp8_forward")
+    return y, codes, scales
+
+
+def gelu_mxfp8_backward(dy: torch.Tensor, codes: torch.Tensor, block_scales: torch.Tensor) -> torch.Tensor:
+    """``dy * gelu_tanh'(u)`` with u the values that stand in the MXFP8 copy (all 2-D)."""
+    lib = load_library()
+    dy, codes, block_scales = _aligned(dy, 32), _plain(codes), _plain(block_scales)
+    rows, cols = dy.shape
+    assert codes.shape == (rows, cols) and cols % 32 == 0 and block_scales.shape == (roundup(rows, 128), roundup(cols // 32, 4)), \
+        "Invalid codes or scale shape"
+    assert codes.is_contiguous() and block_scales.is_contiguous(), "codes and scales must be contiguous"
+    dx = torch.empty_like(dy)
+    if rows > 0:
+        with _on_device(dy.device):
+            _check(lib.ck_gelu_mxfp8_backward(dy.data_ptr(), DTYPE_TO_CODE[dy.dtype], codes.data_ptr(), block_scales.data_ptr(), dx.data_ptr(), rows,
+                                              cols, _stream(dy.device)), "gelu_mxfp8_backward")
+    return dx
+
+
+def _linear_grad_args(dy, codes, scales, rows: int):
+    dy, codes, scales = _aligned(dy, 16), _plain(codes), _plain(scales)
+    n, k = dy.shape[1], codes.shape[1]
+    assert codes.shape[0] == rows, "Matrix dimensions do not match"
+    assert k > 0 and k % 32 == 0 and n > 0 and n % 8 == 0, "K must be a multiple of 32 and N of 8"
+    assert scales.shape == (roundup(rows, 128), roundup(k // 32, 4)), "Invalid scale shape"
+    assert codes.is_contiguous() and scales.is_contiguous(), "codes and scales must be contiguous"
+    return dy, codes, scales, n, k
+
+
+def linear_weight_grad_mxfp8(dy: torch.Tensor, x_codes: torch.Tensor, x_block_scales: torch.Tensor, out_dtype: torch.dtype | None = None,
+                             bias_grad: bool = False) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """``(dweight [N, K], dbias [N] or None)`` of a linear layer from ``dy`` [M, N] and the MXFP8 copy [M, K] of its input, in
+    ``out_dtype`` (dy's by default): fp32 accumulation of exact products, one rounding."""
+    lib = load_library()
+    dy, codes, scales, n, k = _linear_grad_args(dy, x_codes, x_block_scales, dy.shape[0])
+    m, dev, out_dtype = dy.shape[0], dy.device, out_dtype or dy.dtype
+    make = torch.empty if m > 0 else torch.zeros
+    dweight = make((n, k), dtype=out_dtype, device=dev)
+    dbias = make((n,), dtype=out_dtype, device=dev) if bias_grad else None
+    if m > 0:
+        need = _workspace_bytes("ck_linear_grad_mxfp8_workspace_bytes", 1, DTYPE_TO_CODE[dy.dtype], int(bias_grad), m, n, k)
+        with _on_device(dev):
+            ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+            _check(lib.ck_linear_weight_grad_mxfp8(dy.data_ptr(), DTYPE_TO_CODE[dy.dtype], codes.data_ptr(), scales.data_ptr(), dweight.data_ptr(),
+                                                   DTYPE_TO_CODE[out_dtype], _ptr(dbias), m, n, k, ws.data_ptr(), need, _stream(dev)),
+                   "linear_weight_grad_mxfp8")
+    return dweight, dbias
+
+
+def linear_input_grad_mxfp8(dy: torch.Tensor, w_codes: torch.Tensor, w_block_scales: torch.Tensor,
+                            out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """``dx`` [M, K] = ``dy`` [M, N] times a linear layer's MXFP8 weight [N, K], in ``out_dtype`` (dy's by default): fp32
+    accumulation of exact products, one rounding."""
+    lib = load_library()
+    dy, codes, scales, n, k = _linear_grad_args(dy, w_codes, w_block_scales, dy.shape[1])
+    m, dev, out_dtype = dy.shape[0], dy.device, out_dtype or dy.dtype
+    dx = torch.empty((m, k), dtype=out_dtype, device=dev)
+    if m > 0:
+        need = _workspace_bytes("ck_linear_grad_mxfp8_workspace_bytes", 0, DTYPE_TO_CODE[dy.dtype], 0, m, n, k)
+        with _on_device(dev):
+            ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+            _check(lib.ck_linear_input_grad_mxfp8(dy.data_ptr(), DTYPE_TO_CODE[dy.dtype], codes.data_ptr(), scales.data_ptr(), dx.data_ptr(),
+                                                  DTYPE_TO_CODE[out_dtype], m, n, k, ws.data_ptr(), need, _stream(dev)),
+                   "linear_input_grad_mxfp8")
+    return dx
+
+
+# ------------------------------------------------------------------------------------------
 # registration
 # ------------------------------------------------------------------------------------------
 def _build_constraints() -> dict:
@@ -776,7 +1036,33 @@ def _build_constraints() -> dict:
                     "block_scale_b": ParamConstraint(dtypes=frozenset({torch.float8_e8m0fnu})),
                     "out_dtype": ParamConstraint(dtypes=floats)},
             default_devices=cuda_only, min_compute_capability=blackwell),
+        **_training_constraints(cuda_only, floats, f32, blackwell),
     }
+
+
+def _training_constraints(cuda_only, floats, f32, blackwell) -> dict:
+    from comfy_kitchen.constraints import DivisibleBy, ExactDims, FunctionConstraints, MinDims, ParamConstraint
+
+    any_rows = ParamConstraint(dtypes=floats, shape_rules=(MinDims(1),))
+    matrix = ParamConstraint(dtypes=floats, shape_rules=(ExactDims(2),))
+    params, stats = ParamConstraint(dtypes=floats), ParamConstraint(dtypes=f32)
+    codes = ParamConstraint(dtypes=frozenset({torch.float8_e4m3fn}), shape_rules=(ExactDims(2), DivisibleBy(1, 32)))
+    scales = ParamConstraint(dtypes=frozenset({torch.float8_e8m0fnu}))
+    forward = {"x": any_rows, "weight": params, "bias": params}
+    backward = {"dy": any_rows, "mean": stats, "rstd": stats, "weight": params}
+    copy = {"codes": codes, "block_scales": scales}
+    by_name = {
+        "layer_norm_forward": forward,
+        "layer_norm_inference": forward,
+        "layer_norm_forward_mxfp8": forward,
+        "layer_norm_backward": {**backward, "x": any_rows},
+        "layer_norm_backward_mxfp8": {**backward, **copy},
+        "gelu_mxfp8_forward": {"x": ParamConstraint(dtypes=floats, shape_rules=(ExactDims(2), DivisibleBy(1, 32)))},
+        "gelu_mxfp8_backward": {"dy": matrix, **copy},
+        "linear_weight_grad_mxfp8": {"dy": matrix, "x_codes": codes, "x_block_scales": scales, "out_dtype": ParamConstraint(dtypes=floats)},
+        "linear_input_grad_mxfp8": {"dy": matrix, "w_codes": codes, "w_block_scales": scales, "out_dtype": ParamConstraint(dtypes=floats)},
+    }
+    return {name: FunctionConstraints(params=p, default_devices=cuda_only, min_compute_capability=blackwell) for name, p in by_name.items()}
 
 
 _constraints: dict = {}  # as registered

@@ -183,7 +183,148 @@ def _(a, b, block_scale_a, block_scale_b, bias, output_dtype_code):
     return a.new_empty((a.shape[0], b.shape[0]), dtype=DTYPE_CODE_TO_DTYPE[output_dtype_code])
 
 
+# ---- training (no counterpart in the reference) --------------------------------------------------------------------
+# Gradients of x, weight and bias are attached to the two forward operators of the norm and to GELU's, for calls that the dispatcher has
+# to see (tracing, transforms); eager calls go through the autograd functions of comfy_kitchen/training.py.
+def _mxfp8_empty(x, rows, cols):
+    return (x.new_empty((rows, cols), dtype=torch.float8_e4m3fn),
+            x.new_empty((roundup(rows, 128), roundup(cols // 32, 4)), dtype=torch.float8_e8m0fnu))
+
+
+@torch.library.custom_op("comfy_kitchen::layer_norm_forward", mutates_args=())
+def _op_layer_norm_forward(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None, eps: float,
+                           weight_offset: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return _impl("layer_norm_forward", {"x": x, "weight": weight, "bias": bias, "eps": eps, "weight_offset": weight_offset})
+
+
+@_op_layer_norm_forward.register_fake
+def _(x, weight, bias, eps, weight_offset):
+    rows = x.numel() // x.shape[-1]
+    return x.new_empty(x.shape), x.new_empty((rows,), dtype=torch.float32), x.new_empty((rows,), dtype=torch.float32)
+
+
+@torch.library.custom_op("comfy_kitchen::layer_norm_forward_mxfp8", mutates_args=())
+def _op_layer_norm_forward_mxfp8(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None, eps: float, weight_offset: float
+                                 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    return _impl("layer_norm_forward_mxfp8", {"x": x, "weight": weight, "bias": bias, "eps": eps, "weight_offset": weight_offset})
+
+
+@_op_layer_norm_forward_mxfp8.register_fake
+def _(x, weight, bias, eps, weight_offset):
+    rows = x.numel() // x.shape[-1]
+    return (x.new_empty(x.shape), x.new_empty((rows,), dtype=torch.float32), x.new_empty((rows,), dtype=torch.float32),
+            *_mxfp8_empty(x, rows, x.shape[-1]))
+
+
+@torch.library.custom_op("comfy_kitchen::layer_norm_backward", mutates_args=())
+def _op_layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, weight: torch.Tensor | None,
+                            weight_offset: float, groups: int, param_dtype_code: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return _impl("layer_norm_backward", {"dy": dy, "x": x, "mean": mean, "rstd": rstd, "weight": weight, "weight_offset": weight_offset,
+                                         "groups": groups, "param_dtype": DTYPE_CODE_TO_DTYPE[param_dtype_code]})
+
+
+@_op_layer_norm_backward.register_fake
+def _(dy, x, mean, rstd, weight, weight_offset, groups, param_dtype_code):
+    params = (groups, dy.shape[-1])
+    dtype = DTYPE_CODE_TO_DTYPE[param_dtype_code]
+    return dy.new_empty(dy.shape), dy.new_empty(params, dtype=dtype), dy.new_empty(params, dtype=dtype)
+
+
+@torch.library.custom_op("comfy_kitchen::layer_norm_backward_mxfp8", mutates_args=())
+def _op_layer_norm_backward_mxfp8(dy: torch.Tensor, codes: torch.Tensor, block_scales: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
+                                  weight: torch.Tensor | None, weight_offset: float, groups: int, param_dtype_code: int
+                                  ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return _impl("layer_norm_backward_mxfp8", {"dy": dy, "codes": codes, "block_scales": block_scales, "mean": mean, "rstd": rstd, "weight": weight,
+                                               "weight_offset": weight_offset, "groups": groups, "param_dtype": DTYPE_CODE_TO_DTYPE[param_dtype_code]})
+
+
+@_op_layer_norm_backward_mxfp8.register_fake
+def _(dy, codes, block_scales, mean, rstd, weight, weight_offset, groups, param_dtype_code):
+    params = (groups, dy.shape[-1])
+    dtype = DTYPE_CODE_TO_DTYPE[param_dtype_code]
+    return dy.new_empty(dy.shape), dy.new_empty(params, dtype=dtype), dy.new_empty(params, dtype=dtype)
+
+
+def _norm_setup(ctx, inputs, output):
+    x, weight, bias, _, ctx.weight_offset = inputs
+    some = weight if weight is not None else bias
+    ctx.param_shape, ctx.param_dtype = (some.shape, some.dtype) if some is not None else (None, x.dtype)
+    ctx.groups = some.shape[0] if some is not None and some.dim() > 1 else 1
+    held = (output[3], output[4]) if len(output) == 5 else (x,)
+    ctx.save_for_backward(*held, output[1], output[2], weight)
+
+
+def _norm_backward(ctx, dy, *_):  # mean, rstd and the copy carry no gradient
+    *held, mean, rstd, weight = ctx.saved_tensors
+    op = torch.ops.comfy_kitchen.layer_norm_backward_mxfp8 if len(held) == 2 else torch.ops.comfy_kitchen.layer_norm_backward
+    dx, dweight, dbias = op(dy, *held, mean, rstd, weight, ctx.weight_offset, ctx.groups, DTYPE_TO_CODE[ctx.param_dtype])
+    need = ctx.needs_input_grad
+    return dx if need[0] else None, dweight.view(ctx.param_shape) if need[1] else None, dbias.view(ctx.param_shape) if need[2] else None, None, None
+
+
+_op_layer_norm_forward.register_autograd(_norm_backward, setup_context=_norm_setup)
+_op_layer_norm_forward_mxfp8.register_autograd(_norm_backward, setup_context=_norm_setup)
+
+
+@torch.library.custom_op("comfy_kitchen::gelu_mxfp8_forward", mutates_args=())
+def _op_gelu_mxfp8_forward(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return _impl("gelu_mxfp8_forward", {"x": x})
+
+
+@_op_gelu_mxfp8_forward.register_fake
+def _(x):
+    return (x.new_empty(x.shape), *_mxfp8_empty(x, x.shape[0], x.shape[1]))
+
+
+@torch.library.custom_op("comfy_kitchen::gelu_mxfp8_backward", mutates_args=())
+def _op_gelu_mxfp8_backward(dy: torch.Tensor, codes: torch.Tensor, block_scales: torch.Tensor) -> torch.Tensor:
+    return _impl("gelu_mxfp8_backward", {"dy": dy, "codes": codes, "block_scales": block_scales})
+
+
+@_op_gelu_mxfp8_backward.register_fake
+def _(dy, codes, block_scales):
+    return dy.new_empty(dy.shape)
+
+
+def _gelu_setup(ctx, inputs, output):
+    ctx.save_for_backward(output[1], output[2])
+
+
+def _gelu_backward(ctx, dy, *_):
+    return torch.ops.comfy_kitchen.gelu_mxfp8_backward(dy, *ctx.saved_tensors)
+
+
+_op_gelu_mxfp8_forward.register_autograd(_gelu_backward, setup_context=_gelu_setup)
+
+
+@torch.library.custom_op("comfy_kitchen::linear_weight_grad_mxfp8", mutates_args=())
+def _op_linear_weight_grad_mxfp8(dy: torch.Tensor, x_codes: torch.Tensor, x_block_scales: torch.Tensor, output_dtype_code: int,
+                                 bias_grad: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    dweight, dbias = _impl("linear_weight_grad_mxfp8", {"dy": dy, "x_codes": x_codes, "x_block_scales": x_block_scales,
+                                                        "out_dtype": DTYPE_CODE_TO_DTYPE[output_dtype_code], "bias_grad": bias_grad})
+    return dweight, dbias if bias_grad else dweight.new_empty((0,))
+
+
+@_op_linear_weight_grad_mxfp8.register_fake
+def _(dy, x_codes, x_block_scales, output_dtype_code, bias_grad):
+    dtype = DTYPE_CODE_TO_DTYPE[output_dtype_code]
+    return dy.new_empty((dy.shape[1], x_codes.shape[1]), dtype=dtype), dy.new_empty((dy.shape[1] if bias_grad else 0,), dtype=dtype)
+
+
+@torch.library.custom_op("comfy_kitchen::linear_input_grad_mxfp8", mutates_args=())
+def _op_linear_input_grad_mxfp8(dy: torch.Tensor, w_codes: torch.Tensor, w_block_scales: torch.Tensor, output_dtype_code: int) -> torch.Tensor:
+    return _impl("linear_input_grad_mxfp8", {"dy": dy, "w_codes": w_codes, "w_block_scales": w_block_scales,
+                                             "out_dtype": DTYPE_CODE_TO_DTYPE[output_dtype_code]})
+
+
+@_op_linear_input_grad_mxfp8.register_fake
+def _(dy, w_codes, w_block_scales, output_dtype_code):
+    return dy.new_empty((dy.shape[0], w_codes.shape[1]), dtype=DTYPE_CODE_TO_DTYPE[output_dtype_code])
+
+
 if _registrations is not None and hasattr(_op_quantize_nvfp4, "_backend_fns") and hasattr(_op_quantize_nvfp4, "_disabled_kernel"):
     for _op in (_op_quantize_nvfp4, _op_dequantize_nvfp4, _op_scaled_mm_nvfp4, _op_quantize_mxfp8, _op_dequantize_mxfp8,
-                _op_scaled_mm_mxfp8):
+                _op_scaled_mm_mxfp8, _op_layer_norm_forward, _op_layer_norm_forward_mxfp8, _op_layer_norm_backward,
+                _op_layer_norm_backward_mxfp8, _op_gelu_mxfp8_forward, _op_gelu_mxfp8_backward, _op_linear_weight_grad_mxfp8,
+                _op_linear_input_grad_mxfp8):
         _remember(_op)

@@ -294,6 +294,67 @@ CK_API int ck_scaled_mm_mxfp8_ws(const void* a, const void* b, const void* block
                           int out_dtype, int64_t M, int64_t N, int64_t K, void* workspace,
                           int64_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------ training */
+/*
+ * The operators below have no counterpart in the reference, which has no training code.
+ *
+ * Layer norm over the last dimension, with the row's statistics and all sums in fp32 and one rounding at the end:
+ *   h = (x - mean) * rstd,  y = h * f + bias,  f = weight_offset + weight (1 where weight is null)
+ * x: [rows, cols] f32/f16/bf16 whose row r starts at (r / inner) * x_outer_stride + (r % inner) * x_inner_stride elements (rows are
+ * contiguous; inner = rows for one level).  weight, bias (each may be null): one row of cols for every rows / groups consecutive
+ * rows, weight_stride / bias_stride elements apart, of param_dtype, which is dtype or f32.  y: [rows, cols] contiguous.
+ * mean, rstd: [rows] f32 for the backward pass, or both null.  codes, block_scales: null, or the MXFP8 copy of x as
+ * ck_quantize_mxfp8 writes it (cols % 32 == 0, x's rows on 16-byte boundaries, cols at most 65536, f32 32768).
+ */
+CK_API int ck_layer_norm_forward(const void* x, int dtype, int64_t rows, int64_t cols, int64_t inner, int64_t x_outer_stride,
+                          int64_t x_inner_stride, const void* weight, const void* bias, int param_dtype,
+                          int64_t groups, int64_t weight_stride, int64_t bias_stride, float weight_offset, float eps,
+                          void* y, float* mean, float* rstd, void* codes, void* block_scales, void* stream);
+
+/*
+ * Its gradients.  With g = dy * f:
+ *   dx = rstd * (g - mean_k(g) - h * mean_k(g * h)),  dweight = sum over a group's rows of dy * h,  dbias = sum of dy
+ * h comes from x (rows in two levels, as dy's), or, where x is null, from its MXFP8 copy.  dx: [rows, cols] contiguous of dtype;
+ * dweight, dbias: [groups, cols] contiguous of param_dtype, each may be null.  The sums over rows are added in a fixed order.  workspace:
+ * device memory, 4-byte aligned, of ck_layer_norm_backward_workspace_bytes bytes (0: none), no requirement on its
+ * contents; calls that can overlap on the GPU need separate ones.
+ */
+CK_API int64_t ck_layer_norm_backward_workspace_bytes(int64_t rows, int64_t cols, int64_t groups);
+CK_API int ck_layer_norm_backward(const void* dy, int dtype, int64_t rows, int64_t cols, int64_t dy_inner, int64_t dy_outer_stride,
+                           int64_t dy_inner_stride, const void* x, int64_t x_inner, int64_t x_outer_stride,
+                           int64_t x_inner_stride, const void* codes, const void* block_scales, const float* mean,
+                           const float* rstd, const void* weight, int param_dtype, int64_t groups, int64_t weight_stride,
+                           float weight_offset, void* dx, void* dweight, void* dbias, void* workspace,
+                           int64_t workspace_bytes, void* stream);
+
+/*
+ * GELU (tanh form) whose input is kept in MXFP8.  Forward: y = x / 2 * (1 + tanh(sqrt(2/pi) * (x + 0.044715 x^3))) and the copy
+ * of x as ck_quantize_mxfp8 writes it.  Backward: dx = dy * gelu'(u) with u the value that stands in the copy.  fp32 arithmetic,
+ * one rounding.  [rows, cols] contiguous, cols % 32 == 0; x, y, dy, dx and codes 32-byte aligned, block_scales 4-byte.
+ */
+CK_API int ck_gelu_mxfp8_forward(const void* x, int dtype, void* y, void* codes, void* block_scales, int64_t rows,
+                          int64_t cols, void* stream);
+CK_API int ck_gelu_mxfp8_backward(const void* dy, int dtype, const void* codes, const void* block_scales, void* dx,
+                           int64_t rows, int64_t cols, void* stream);
+
+/*
+ * Gradients of a linear layer y[M,N] = x[M,K] . w[N,K]^T + b one operand of which is held in MXFP8 (E4M3 codes, tiled E8M0 scales
+ * of 32-element blocks along K):
+ *   weight: dweight[N,K] = dy[M,N]^T . deq(x)[M,K], and dbias[N] = sum over m of dy (dbias may be null)
+ *   input:  dx[M,K] = dy[M,N] . deq(w)[N,K]
+ * dy: f32/f16/bf16, row-major, 16-byte aligned; results of out_dtype, 32-byte aligned.  The MXFP8 values enter as
+ * ck_dequantize_mxfp8 gives them in bf16 (exact for magnitudes of 2^-126 on), dy exactly; fp32 accumulation, one rounding, sums in a
+ * fixed order.  K % 32 == 0, N % 8 == 0.  workspace: device memory, 256-byte aligned, of ck_linear_grad_mxfp8_workspace_bytes bytes
+ * (0: shape not supported), no requirement on its contents; calls that can overlap on the GPU need separate ones.
+ */
+CK_API int64_t ck_linear_grad_mxfp8_workspace_bytes(int of_weight, int dy_dtype, int with_bias, int64_t M, int64_t N, int64_t K);
+CK_API int ck_linear_weight_grad_mxfp8(const void* dy, int dy_dtype, const void* x_codes, const void* x_block_scales,
+                                void* dweight, int out_dtype, void* dbias, int64_t M, int64_t N, int64_t K,
+                                void* workspace, int64_t workspace_bytes, void* stream);
+CK_API int ck_linear_input_grad_mxfp8(const void* dy, int dy_dtype, const void* w_codes, const void* w_block_scales,
+                               void* dx, int out_dtype, int64_t M, int64_t N, int64_t K, void* workspace,
+                               int64_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------------ multi-GPU (one node) */
 /*
  * Column-sharded GEMM with the all-gather of the output fused into the epilogue.  No
