@@ -61,7 +61,7 @@ def build_host(force: bool = False, verbose: bool = False) -> str:
     if torch is None:
         raise RuntimeError("torch is not installed")
     torch_dir = list(torch.submodule_search_locations)[0]
-    if not force and not _stale(HOST_PATH, [HOST_SRC, os.path.join(torch_dir, "version.py")]):
+    if not force and not _stale(HOST_PATH, [HOST_SRC, *glob.glob(os.path.join(os.path.dirname(HOST_SRC), "*.h")), os.path.join(torch_dir, "version.py")]):
         return HOST_PATH
     include, libs = os.path.join(torch_dir, "include"), os.path.join(torch_dir, "lib")
     cuda_include = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(_nvcc()))), "include")

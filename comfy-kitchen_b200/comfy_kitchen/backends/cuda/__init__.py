@@ -145,7 +145,9 @@ def load_library():
 _HOST_NAMES = ("ck_quantize_nvfp4", "ck_quantize_nvfp4_dynamic_scratch_bytes", "ck_quantize_nvfp4_dynamic_whole_input_bytes",
                "ck_quantize_nvfp4_dynamic", "ck_quantize_mxfp8", "ck_dequantize_nvfp4", "ck_dequantize_mxfp8", "ck_scaled_mm_workspace_bytes", "ck_scaled_mm_nvfp4_ws",
                "ck_scaled_mm_mxfp8_ws", "ck_linear_nvfp4_from_float_workspace_bytes", "ck_linear_nvfp4_from_float",
-               "ck_linear_mxfp8_from_float_workspace_bytes", "ck_linear_mxfp8_from_float")
+               "ck_linear_mxfp8_from_float_workspace_bytes", "ck_linear_mxfp8_from_float", "ck_layer_norm_forward",
+               "ck_layer_norm_backward_workspace_bytes", "ck_layer_norm_backward", "ck_gelu_mxfp8_forward", "ck_gelu_mxfp8_backward",
+               "ck_linear_grad_mxfp8_workspace_bytes", "ck_linear_weight_grad_mxfp8", "ck_linear_input_grad_mxfp8", "ck_last_error")
 
 
 def _load_host(lib) -> None:
@@ -957,6 +959,10 @@ def linear_weight_grad_mxfp8(dy: torch.Tensor, x_codes: torch.Tensor, x_block_sc
                              bias_grad: bool = False) -> tuple[torch.Tensor, torch.Tensor | None]:
     """``(dweight [N, K], dbias [N] or None)`` of a linear layer from ``dy`` [M, N] and the MXFP8 copy [M, K] of its input, in
     ``out_dtype`` (dy's by default): fp32 accumulation of exact products, one rounding."""
+    if _host is not None:
+        out = _host.linear_weight_grad_mxfp8(dy, x_codes, x_block_scales, out_dtype, bias_grad)
+        if out is not None:
+            return out
     lib = load_library()
     dy, codes, scales, n, k = _linear_grad_args(dy, x_codes, x_block_scales, dy.shape[0])
     m, dev, out_dtype = dy.shape[0], dy.device, out_dtype or dy.dtype
@@ -977,6 +983,10 @@ def linear_input_grad_mxfp8(dy: torch.Tensor, w_codes: torch.Tensor, w_block_sca
                             out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """``dx`` [M, K] = ``dy`` [M, N] times a linear layer's MXFP8 weight [N, K], in ``out_dtype`` (dy's by default): fp32
     accumulation of exact products, one rounding."""
+    if _host is not None:
+        out = _host.linear_input_grad_mxfp8(dy, w_codes, w_block_scales, out_dtype)
+        if out is not None:
+            return out
     lib = load_library()
     dy, codes, scales, n, k = _linear_grad_args(dy, w_codes, w_block_scales, dy.shape[1])
     m, dev, out_dtype = dy.shape[0], dy.device, out_dtype or dy.dtype
@@ -1067,12 +1077,26 @@ def _training_constraints(cuda_only, floats, f32, blackwell) -> dict:
 
 _constraints: dict = {}  # as registered
 _stock = {name: globals()[name] for name in ("quantize_nvfp4", "quantize_nvfp4_dynamic", "quantize_mxfp8", "dequantize_nvfp4",
-                                             "dequantize_mxfp8", "scaled_mm_nvfp4", "scaled_mm_mxfp8")}
+                                             "dequantize_mxfp8", "scaled_mm_nvfp4", "scaled_mm_mxfp8", "layer_norm_forward",
+                                             "layer_norm_forward_mxfp8", "layer_norm_inference", "layer_norm_backward",
+                                             "layer_norm_backward_mxfp8", "gelu_mxfp8_forward", "gelu_mxfp8_backward",
+                                             "linear_weight_grad_mxfp8", "linear_input_grad_mxfp8")}
 
 
 def host_function(name: str):
     """The native half of this module's function ``name``, or None: also where somebody has put another function in its place."""
     return getattr(_host, name) if _host is not None and globals()[name] is _stock[name] else None
+
+
+def host_step(name: str, functions: tuple[str, ...]):
+    """The native function ``name``, which does the work of this module's ``functions`` (a forward pass and its gradients), or None
+    unless the registry would send every call of them here."""
+    if _host is None:
+        return None
+    for function in functions:
+        if globals()[function] is not _stock[function] or not registry.leaves_no_choice(function, _this_module, _constraints.get(function)):
+            return None
+    return getattr(_host, name)
 
 
 def host_operator(name: str):

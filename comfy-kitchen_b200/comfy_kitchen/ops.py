@@ -68,6 +68,19 @@ def host_operator(name: str):
     return _cuda_backend.host_operator(name)
 
 
+def host_step(name: str, functions: tuple[str, ...]):
+    """As :func:`host_operator` for a native function that does the work of several operators (a forward pass and its gradients)."""
+    if torch.compiler.is_compiling() or torch.autograd.forward_ad._current_level >= 0:
+        return None
+    for function in functions:
+        if replaced(function):
+            return None
+    global _cuda_backend
+    if _cuda_backend is None:
+        from .backends import cuda as _cuda_backend  # imports this module
+    return _cuda_backend.host_step(name, functions)
+
+
 _cuda_backend = None
 
 

@@ -23,7 +23,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 from torch.autograd.function import once_differentiable
 
-from .ops import _MAY_BE_PENDING, _PLAIN_TYPES, DTYPE_TO_CODE, _impl, dispatcher_adds_nothing, replaced
+from .ops import _MAY_BE_PENDING, _PLAIN_TYPES, DTYPE_TO_CODE, _impl, dispatcher_adds_nothing, host_operator, host_step, replaced
 from .tensor import QuantizedTensor, TensorCoreMXFP8Layout
 from .tensor.blockwise import quantized_linear
 
@@ -84,6 +84,11 @@ def linear_weight_grad_mxfp8(dy: torch.Tensor, x_codes: torch.Tensor, x_block_sc
     """``(dy.T @ x, dy.sum(0) or None)`` with ``dy`` [M, N] and x [M, K] held in MXFP8, in ``out_dtype`` (dy's by default).
 
     fp32 accumulation of exact products, one rounding; N a multiple of 8, K of 32."""
+    host = host_operator("linear_weight_grad_mxfp8")
+    if host is not None:
+        out = host(dy, x_codes, x_block_scales, out_dtype, bias_grad)
+        if out is not None:
+            return out
     dweight, dbias = _call("linear_weight_grad_mxfp8", {"dy": dy, "x_codes": x_codes, "x_block_scales": x_block_scales,
                                                         "out_dtype": out_dtype or dy.dtype, "bias_grad": bool(bias_grad)})
     return dweight, dbias if bias_grad else None
@@ -94,6 +99,11 @@ def linear_input_grad_mxfp8(dy: torch.Tensor, w_codes: torch.Tensor, w_block_sca
     """``dy @ w`` with ``dy`` [M, N] and a linear layer's weight w [N, K] held in MXFP8, in ``out_dtype`` (dy's by default).
 
     fp32 accumulation of exact products, one rounding; N a multiple of 8, K of 32."""
+    host = host_operator("linear_input_grad_mxfp8")
+    if host is not None:
+        out = host(dy, w_codes, w_block_scales, out_dtype)
+        if out is not None:
+            return out
     return _call("linear_input_grad_mxfp8", {"dy": dy, "w_codes": w_codes, "w_block_scales": w_block_scales, "out_dtype": out_dtype or dy.dtype})
 
 
@@ -118,6 +128,9 @@ def _groups(*params) -> int:
 def _param_grads(ctx, dweight, dbias):
     shape = ctx.param_shape
     return (dweight.view(shape) if ctx.needs_input_grad[1] else None), (dbias.view(shape) if ctx.needs_input_grad[2] else None)
+
+
+_NORM_OPERATORS = ("layer_norm_forward", "layer_norm_forward_mxfp8", "layer_norm_backward", "layer_norm_backward_mxfp8")
 
 
 class _LayerNorm(torch.autograd.Function):
@@ -158,14 +171,22 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     fp32 with one rounding.  With ``checkpoint`` the backward pass works from an MXFP8 copy of x (the last dimension a
     multiple of 32) instead of x itself."""
     eps, weight_offset = float(eps), float(weight_offset)
+    host = host_step("layer_norm", _NORM_OPERATORS)
+    if host is not None:
+        y = host(x, weight, bias, eps, weight_offset, checkpoint)
+        if y is not None:
+            return y
     if checkpoint and x.shape[-1] % BLOCK != 0:
         raise ValueError(f"an MXFP8 checkpoint needs rows of a multiple of {BLOCK}, got {x.shape[-1]}")
-    if _eager((x, weight, bias)) and not (replaced("layer_norm_forward") or replaced("layer_norm_forward_mxfp8")):
+    if _eager((x, weight, bias)) and not any(replaced(name) for name in _NORM_OPERATORS):
         if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
             return _LayerNorm.apply(x, weight, bias, eps, weight_offset, checkpoint)
         return _impl("layer_norm_inference", {"x": x, "weight": weight, "bias": bias, "eps": eps, "weight_offset": weight_offset})
     op = torch.ops.comfy_kitchen.layer_norm_forward_mxfp8 if checkpoint else torch.ops.comfy_kitchen.layer_norm_forward
     return op(x, weight, bias, eps, weight_offset)[0]
+
+
+_GELU_OPERATORS = ("gelu_mxfp8_forward", "gelu_mxfp8_backward")
 
 
 class _Gelu(torch.autograd.Function):
@@ -184,11 +205,16 @@ class _Gelu(torch.autograd.Function):
 
 def gelu_checkpointed(x: torch.Tensor) -> torch.Tensor:
     """Tanh-form GELU whose backward pass works from an MXFP8 copy of x (the last dimension a multiple of 32)."""
+    host = host_step("gelu_checkpointed", _GELU_OPERATORS)
+    if host is not None:
+        y = host(x)
+        if y is not None:
+            return y
     if x.dim() == 0 or x.shape[-1] % BLOCK != 0:
         raise ValueError(f"an MXFP8 checkpoint needs rows of a multiple of {BLOCK}, got {tuple(x.shape)}")
     shape = x.shape
     x2 = x if len(shape) == 2 else x.reshape(-1, shape[-1])
-    if _eager((x2,)) and not replaced("gelu_mxfp8_forward"):
+    if _eager((x2,)) and not any(replaced(name) for name in _GELU_OPERATORS):
         y = _Gelu.apply(x2)
     else:
         y = torch.ops.comfy_kitchen.gelu_mxfp8_forward(x2)[0]

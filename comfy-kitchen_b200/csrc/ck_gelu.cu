@@ -71,10 +71,10 @@ gelu_mxfp8_forward_kernel(const T* x, T* y, uint8_t* codes, uint8_t* scales, int
     float amax = 0.0f;
 #pragma unroll
     for (int i = 0; i < 32; ++i) amax = fmaxf(amax, fabsf(u[i]));
-    const quant::Mxfp8Scale s = quant::mxfp8_scale(amax);
+    const quant::Mxfp8Scale s = block_scale(amax);
     Vec256 out;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) out.w[i] = quant::mxfp8_four(u + 4 * i, s);
+    for (int i = 0; i < 8; ++i) out.w[i] = block_codes(make_float2(u[4 * i], u[4 * i + 1]), make_float2(u[4 * i + 2], u[4 * i + 3]), s);
     st_global_256(codes + at, out);
     byte = s.byte;
 #pragma unroll

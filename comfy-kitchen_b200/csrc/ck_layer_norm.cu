@@ -31,6 +31,7 @@ struct ForwardArgs {
   uint8_t* scales;
   uint32_t rows, rows_padded;
   int64_t cols;
+  int* status;  // for waits that give up (ck_gemm_status)
   bool params_f32;      // else of x's type
   bool params_aligned;  // weights and biases start on vectors
 };
@@ -99,18 +100,18 @@ __device__ __forceinline__ float row_sum(float v, float* buf) {
 // The MXFP8 copy of a row of which each lane holds kVec elements: codes beside the arithmetic's registers, a scale byte for
 // every 32 elements, four of them in one 4-byte store.  Bits as ck_quantize_mxfp8 writes them.  All lanes of a warp come here.
 template <int kVec>
-__device__ __forceinline__ void store_mxfp8(const float (&f)[kVec], bool inside, const ForwardArgs& a, uint32_t row, int64_t vec) {
+__device__ __forceinline__ void store_mxfp8(const float2 (&f)[kVec / 2], bool inside, const ForwardArgs& a, uint32_t row, int64_t vec) {
   constexpr int kLanes = 32 / kVec;  // lanes of a block
   float amax = 0.0f;
 #pragma unroll
-  for (int j = 0; j < kVec; ++j) amax = fmaxf(amax, fabsf(f[j]));
+  for (int j = 0; j < kVec / 2; ++j) amax = fmaxf(amax, fmaxf(fabsf(f[j].x), fabsf(f[j].y)));
 #pragma unroll
   for (int o = 1; o < kLanes; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
-  const quant::Mxfp8Scale s = quant::mxfp8_scale(amax);
+  const quant::Mxfp8Scale s = block_scale(amax);
   if (inside) {
     uint32_t words[kVec / 4];
 #pragma unroll
-    for (int j = 0; j < kVec / 4; ++j) words[j] = quant::mxfp8_four(f + 4 * j, s);
+    for (int j = 0; j < kVec / 4; ++j) words[j] = block_codes(f[2 * j], f[2 * j + 1], s);
     uint8_t* to = a.codes + static_cast<int64_t>(row) * a.cols + vec * kVec;
     if constexpr (kVec == 8) {
       *reinterpret_cast<uint2*>(to) = make_uint2(words[0], words[1]);
@@ -118,13 +119,10 @@ __device__ __forceinline__ void store_mxfp8(const float (&f)[kVec], bool inside,
       *reinterpret_cast<uint32_t*>(to) = words[0];
     }
   }
-  const uint32_t byte = inside ? s.byte : 0u;
-  const int lane = threadIdx.x & 31;
-  const int first = lane & ~(4 * kLanes - 1);
-  uint32_t word = 0;
-#pragma unroll
-  for (int b = 0; b < 4; ++b) word |= __shfl_sync(0xFFFFFFFFu, byte, first + b * kLanes) << (8 * b);
-  if (inside && lane == first) {
+  uint32_t word = inside ? s.byte : 0u;
+  word |= __shfl_down_sync(0xFFFFFFFFu, word, kLanes) << 8;
+  word |= __shfl_down_sync(0xFFFFFFFFu, word, 2 * kLanes) << 16;
+  if (inside && (threadIdx.x & (4 * kLanes - 1)) == 0) {
     const int64_t block = vec * kVec >> 5;
     *reinterpret_cast<uint32_t*>(a.scales + swizzled_scale_offset(row, block, ceil_div(a.cols >> 5, 4))) = word;
   }
@@ -173,7 +171,7 @@ __global__ void __launch_bounds__(kMaxThreads) layer_norm_forward_kernel(const F
       for (int j = 0; j < kVec; ++j) square = fmaf(f[j] - mean, f[j] - mean, square);
     }
   }
-  const float rstd = 1.0f / sqrtf(row_sum<1>(square, buf) / static_cast<float>(a.cols) + a.eps);
+  const float rstd = inverse_root(row_sum<1>(square, buf) / static_cast<float>(a.cols) + a.eps);
   if constexpr (kCopy) {
     if (!live && row < a.rows_padded) clear_scales_of_row(a, row);
   }
@@ -187,9 +185,13 @@ __global__ void __launch_bounds__(kMaxThreads) layer_norm_forward_kernel(const F
   for (int i = 0; i < kNum; ++i) {
     const int64_t v = threadIdx.x + i * blockDim.x;
     const bool inside = live && v < vecs;
+    if constexpr (kCopy) {
+      float2 pairs[kVec / 2];
+      unpack(raw[i], pairs);
+      store_mxfp8<kVec>(pairs, inside, a, row, v);
+    }
     float f[kVec];
     unpack(raw[i], f);
-    if constexpr (kCopy) store_mxfp8<kVec>(f, inside, a, row, v);
     if (inside) {
       float w[kVec], b[kVec];
       if (a.weight != nullptr) load_param<T, kVec>(a.weight, group * a.weight_stride + v * kVec, a.params_f32, a.params_aligned, w);
@@ -201,6 +203,193 @@ __global__ void __launch_bounds__(kMaxThreads) layer_norm_forward_kernel(const F
       }
       store(y + v * kVec, pack<T, kVec>(f));
     }
+  }
+}
+
+// ---- rows that come through shared memory
+// A block's row is a bulk copy into a ring of stages, issued that many rows ahead by one thread, so that what is in flight
+// does not depend on registers or on where the warps stand.  Barriers of the ring are mbarriers whose waits are bounded (mbar_wait).
+struct Ring {
+  uint32_t full;        // shared address of the stages' barriers
+  volatile int* abort;  // a wait gave up
+};
+constexpr int kMaxRing = 4;
+
+// A team of blockDim.x threads takes a row at a time; the block's rows are of one group, whose factors f and biases stand in shared memory
+// as fp32 (`shared_params`) where there is room.  A row is unpacked once and stays in registers as fp32.  Mean and variance take one
+// meeting of the team's warps: each brings the mean of what it holds and the squares about that.
+template <typename T, int kVec, int kNum, bool kCopy>
+__global__ void __launch_bounds__(1024) layer_norm_forward_ring_kernel(const ForwardArgs a, const uint32_t chunks, const uint32_t chunk_rows,
+                                                                       const int stages, const bool shared_params) {
+  constexpr int kPairs = kVec / 2;
+  extern __shared__ __align__(128) uint8_t shared_bytes[];  // factors, biases, the teams' rings
+  __shared__ __align__(8) uint64_t full[32][kMaxRing];
+  __shared__ float2 buf[2][32];   // [turn][warp of the block]: mean and squares
+  __shared__ float counts[32];    // elements that a team's warp holds
+  __shared__ int abort_flag;
+  pdl_launch_dependents();
+  const int team = threadIdx.y, teams = blockDim.y, width = blockDim.x, warps = width >> 5, warp = threadIdx.x >> 5;
+  const uint32_t group = blockIdx.x / chunks, chunk = blockIdx.x - group * chunks;
+  const uint32_t begin = chunk * chunk_rows, end = min(a.rows_per_group, begin + chunk_rows), row0 = group * a.rows_per_group;
+  const int vecs = static_cast<int>(a.cols / kVec);
+  const float inv_cols = 1.0f / static_cast<float>(a.cols);
+  const uint32_t row_bytes = static_cast<uint32_t>(a.cols) * sizeof(T), stage_bytes = (row_bytes + 127) & ~127u;
+  const uint32_t param_bytes = (static_cast<uint32_t>(a.cols) * 4 + 127) & ~127u;
+  const bool weight = a.weight != nullptr, bias = a.bias != nullptr;
+  float* const factor_buf = reinterpret_cast<float*>(shared_bytes);
+  float* const bias_buf = reinterpret_cast<float*>(shared_bytes + (shared_params && weight ? param_bytes : 0u));
+  const uint8_t* const ring = shared_bytes + (shared_params ? ((weight ? param_bytes : 0u) + (bias ? param_bytes : 0u)) : 0u) + team * stages * stage_bytes;
+  const uint32_t ring_at = sm100::smem_u32(ring), full_at = sm100::smem_u32(full[team]);
+  const auto load_row = [&](uint32_t r, int s) {  // by one thread of the team
+    sm100::mbar_arrive_expect_tx(full_at + s * 8, row_bytes);
+    sm100::bulk_load_1d(ring_at + s * stage_bytes, static_cast<const T*>(a.x) + a.x_rows.offset(row0 + r), row_bytes, full_at + s * 8);
+  };
+  int held = 0;
+#pragma unroll
+  for (int i = 0; i < kNum; ++i) held += max(0, min(32, vecs - warp * 32 - i * width)) * kVec;
+  const float inv_held = held > 0 ? 1.0f / static_cast<float>(held) : 0.0f;
+  if (team == 0 && (threadIdx.x & 31) == 0) counts[warp] = static_cast<float>(held);
+  if (threadIdx.x == 0) {
+    if (team == 0) abort_flag = 0;
+    for (int s = 0; s < stages; ++s) sm100::mbar_init(&full[team][s], 1);
+    sm100::fence_barrier_init();
+    pdl_wait();
+    for (int s = 0; s < stages; ++s) {
+      const uint32_t r = begin + team + s * teams;
+      if (r < end) load_row(r, s);
+    }
+  }
+  pdl_wait();
+  constexpr int kPart = 4;  // four of a vector lie together and the vectors 16 bytes apart: a warp's 16-byte loads meet no bank twice
+  const int part_stride = vecs * kPart;
+  if (shared_params) {
+    for (int v = team * width + threadIdx.x; v < vecs; v += width * teams) {
+      float f[kVec];
+      if (weight) {
+        load_param<T, kVec>(a.weight, group * a.weight_stride + static_cast<int64_t>(v) * kVec, a.params_f32, a.params_aligned, f);
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) factor_buf[j / kPart * part_stride + v * kPart + j % kPart] = a.offset + f[j];
+      }
+      if (bias) {
+        load_param<T, kVec>(a.bias, group * a.bias_stride + static_cast<int64_t>(v) * kVec, a.params_f32, a.params_aligned, f);
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) bias_buf[j / kPart * part_stride + v * kPart + j % kPart] = f[j];
+      }
+    }
+  }
+  __syncthreads();
+  const auto read_params = [&](const float* from, int v, float2(&f)[kPairs]) {
+#pragma unroll
+    for (int q = 0; q < kVec / kPart; ++q) {
+      const float4 part = *reinterpret_cast<const float4*>(from + q * part_stride + v * kPart);
+      f[2 * q] = make_float2(part.x, part.y);
+      f[2 * q + 1] = make_float2(part.z, part.w);
+    }
+  };
+  int stage = 0, turn = 0;
+  uint32_t phase = 0;
+  for (uint32_t r = begin + team; r < end; r += teams, turn ^= 1) {
+    if (!sm100::mbar_wait(full_at + stage * 8, phase, &abort_flag)) break;
+    float2 f[kNum][kPairs];
+    float2 sum = both(0.0f);
+#pragma unroll
+    for (int i = 0; i < kNum; ++i) {
+      const int v = threadIdx.x + i * width;
+      if (v < vecs) {
+        unpack(*reinterpret_cast<const Raw<T, kVec>*>(ring + stage * stage_bytes + v * 16), f[i]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) f[i][j] = both(0.0f);
+      }
+#pragma unroll
+      for (int j = 0; j < kPairs; ++j) sum = add_x2(sum, f[i][j]);
+    }
+    const float mine = warp_sum(sum.x + sum.y) * inv_held;
+    float2 square = both(0.0f);
+#pragma unroll
+    for (int i = 0; i < kNum; ++i) {
+      if (static_cast<int>(threadIdx.x) + i * width < vecs) {
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) {
+          const float2 d = add_x2(f[i][j], both(-mine));
+          square = fma_x2(d, d, square);
+        }
+      }
+    }
+    float mean = mine, squares = warp_sum(square.x + square.y);
+    if (warps > 1) {
+      float2* const slots = buf[turn] + team * warps;
+      if ((threadIdx.x & 31) == 0) slots[warp] = make_float2(mine, squares);
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(width) : "memory");
+      mean = 0.0f;
+      for (int w = 0; w < warps; ++w) mean = fmaf(slots[w].x, counts[w], mean);
+      mean *= inv_cols;
+      squares = 0.0f;
+      for (int w = 0; w < warps; ++w) {
+        const float d = slots[w].x - mean;
+        squares += fmaf(d * d, counts[w], slots[w].y);
+      }
+    } else {
+      __syncwarp();
+    }
+    const float rstd = inverse_root(squares * inv_cols + a.eps);
+    const uint32_t row = row0 + r;
+    if (threadIdx.x == 0) {
+      if (r + stages * teams < end) load_row(r + stages * teams, stage);  // all have read the stage
+      if (a.mean != nullptr) {
+        a.mean[row] = mean;
+        a.rstd[row] = rstd;
+      }
+    }
+    if (++stage == stages) {
+      stage = 0;
+      phase ^= 1u;
+    }
+    T* const y = static_cast<T*>(a.y) + static_cast<int64_t>(row) * a.cols;
+#pragma unroll
+    for (int i = 0; i < kNum; ++i) {
+      const int v = threadIdx.x + i * width;
+      if constexpr (kCopy) store_mxfp8<kVec>(f[i], v < vecs, a, row, v);
+      if (v >= vecs) continue;
+      float2 w[kPairs], b[kPairs];
+      if (shared_params) {
+        if (weight) read_params(factor_buf, v, w);
+        if (bias) read_params(bias_buf, v, b);
+      } else {
+        float p[kVec];
+        if (weight) {
+          load_param<T, kVec>(a.weight, group * a.weight_stride + static_cast<int64_t>(v) * kVec, a.params_f32, a.params_aligned, p);
+#pragma unroll
+          for (int j = 0; j < kPairs; ++j) w[j] = make_float2(a.offset + p[2 * j], a.offset + p[2 * j + 1]);
+        }
+        if (bias) {
+          load_param<T, kVec>(a.bias, group * a.bias_stride + static_cast<int64_t>(v) * kVec, a.params_f32, a.params_aligned, p);
+#pragma unroll
+          for (int j = 0; j < kPairs; ++j) b[j] = make_float2(p[2 * j], p[2 * j + 1]);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kPairs; ++j) {
+        f[i][j] = mul_x2(add_x2(f[i][j], both(-mean)), both(rstd));
+        if (weight && bias) {
+          f[i][j] = fma_x2(f[i][j], w[j], b[j]);
+        } else if (weight) {
+          f[i][j] = mul_x2(f[i][j], w[j]);
+        } else if (bias) {
+          f[i][j] = add_x2(f[i][j], b[j]);
+        }
+      }
+      store(y + static_cast<int64_t>(v) * kVec, pack<T, kVec>(f[i]));
+    }
+  }
+  if constexpr (kCopy) {  // the scales' padding rows
+    if (blockIdx.x == gridDim.x - 1) {
+      for (uint32_t row = a.rows + team; row < a.rows_padded; row += teams) clear_scales_of_row(a, row);
+    }
+  }
+  if (abort_flag) {
+    if (threadIdx.x == 0 && team == 0) atomicExch(a.status, 1);
+    for (int i = 0; i < 200; ++i) __nanosleep(1000);  // copies that are in flight land before the memory is released
   }
 }
 
@@ -220,7 +409,7 @@ __global__ void __launch_bounds__(512) layer_norm_forward_wide_kernel(const Forw
     const float d = to_float(x[k]) - mean;
     square = fmaf(d, d, square);
   }
-  const float rstd = 1.0f / sqrtf(row_sum<1>(square, buf) / static_cast<float>(a.cols) + a.eps);
+  const float rstd = inverse_root(row_sum<1>(square, buf) / static_cast<float>(a.cols) + a.eps);
   if (threadIdx.x == 0 && a.mean != nullptr) {
     a.mean[row] = mean;
     a.rstd[row] = rstd;
@@ -256,6 +445,7 @@ struct BackwardArgs {
   float* partials;  // [groups * chunks][2][cols], where a group's rows are several blocks'
   uint32_t rows_per_group, groups, chunks, chunk_rows;
   int64_t cols;
+  int* status;  // for waits that give up (ck_gemm_status)
 };
 
 // The input's vector v of `row` in fp32, from the type it was given in or from its copy.
@@ -449,6 +639,232 @@ __global__ void __launch_bounds__(512) layer_norm_backward_kernel(const Backward
   }
 }
 
+// The same where rows are long enough to come through shared memory (see the forward pass): a team's rows of dy and of x or its codes are
+// bulk copies into its own ring, a few rows ahead, and what a thread holds of a row is read from there once.
+template <typename T, int kVec, int kNum, bool kCopy>
+__global__ void __launch_bounds__(512) layer_norm_backward_ring_kernel(const BackwardArgs a, const int stages) {
+  constexpr int kMaxTeams = 15, kPairs = kVec / 2;
+  extern __shared__ __align__(128) uint8_t shared_bytes[];  // factors f, then the teams' rings; the teams' column sums in the end
+  __shared__ __align__(8) uint64_t full[kMaxTeams][kMaxRing];
+  __shared__ float2 row_buf[2][16];  // [turn][warp of the block]
+  __shared__ int abort_flag;
+  pdl_launch_dependents();
+  const int team = threadIdx.y, teams = blockDim.y, width = blockDim.x, warps = width >> 5, lane = threadIdx.x & 31;
+  const uint32_t group = blockIdx.x / a.chunks, chunk = blockIdx.x - group * a.chunks;
+  const uint32_t begin = chunk * a.chunk_rows, end = min(a.rows_per_group, begin + a.chunk_rows), row0 = group * a.rows_per_group;
+  const int vecs = static_cast<int>(a.cols / kVec);
+  const float inv_cols = 1.0f / static_cast<float>(a.cols);
+  const uint32_t dy_bytes = static_cast<uint32_t>(a.cols) * sizeof(T), x_bytes = static_cast<uint32_t>(a.cols) * (kCopy ? 1 : sizeof(T));
+  const uint32_t x_at = (dy_bytes + 127) & ~127u, stage_bytes = x_at + ((x_bytes + 127) & ~127u);
+  const uint32_t factor_bytes = a.weight != nullptr ? (static_cast<uint32_t>(a.cols) * 4 + 127) & ~127u : 0u;
+  float* const shared_buf = reinterpret_cast<float*>(shared_bytes);
+  uint8_t* const ring = shared_bytes + factor_bytes + team * stages * stage_bytes;
+  const uint32_t ring_at = sm100::smem_u32(ring), full_at = sm100::smem_u32(full[team]);
+  const auto load_row = [&](uint32_t r, int s) {  // by one thread of the team
+    const uint32_t row = row0 + r, to = ring_at + s * stage_bytes, bar = full_at + s * 8;
+    sm100::mbar_arrive_expect_tx(bar, dy_bytes + x_bytes);
+    sm100::bulk_load_1d(to, static_cast<const T*>(a.dy) + a.dy_rows.offset(row), dy_bytes, bar);
+    const void* x = kCopy ? static_cast<const void*>(a.codes + static_cast<int64_t>(row) * a.cols)
+                          : static_cast<const void*>(static_cast<const T*>(a.x) + a.x_rows.offset(row));
+    sm100::bulk_load_1d(to + x_at, x, x_bytes, bar);
+  };
+  if (threadIdx.x == 0) {
+    if (team == 0) abort_flag = 0;
+    for (int s = 0; s < stages; ++s) sm100::mbar_init(&full[team][s], 1);
+    sm100::fence_barrier_init();
+    pdl_wait();
+    for (int s = 0; s < stages; ++s) {
+      const uint32_t r = begin + team + s * teams;
+      if (r < end) load_row(r, s);
+    }
+  }
+  pdl_wait();
+  // factors in shared memory, as above
+  constexpr int kPart = 4;
+  const int part_stride = vecs * kPart;
+  if (a.weight != nullptr) {
+    for (int v = team * width + threadIdx.x; v < vecs; v += width * teams) {
+      float f[kVec];
+      load_param<T, kVec>(a.weight, group * a.weight_stride + static_cast<int64_t>(v) * kVec, a.params_f32, a.params_aligned, f);
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) shared_buf[j / kPart * part_stride + v * kPart + j % kPart] = a.offset + f[j];
+    }
+  }
+  __syncthreads();
+  const auto factors = [&](int i, float2(&f)[kPairs]) {
+    if (a.weight == nullptr) {
+#pragma unroll
+      for (int j = 0; j < kPairs; ++j) f[j] = both(1.0f);
+      return;
+    }
+    const int v = min(static_cast<int>(threadIdx.x) + i * width, vecs - 1);
+#pragma unroll
+    for (int q = 0; q < kVec / kPart; ++q) {
+      const float4 part = *reinterpret_cast<const float4*>(shared_buf + q * part_stride + v * kPart);
+      f[2 * q] = make_float2(part.x, part.y);
+      f[2 * q + 1] = make_float2(part.z, part.w);
+    }
+  };
+  float2 dw[kNum][kPairs], db[kNum][kPairs];
+#pragma unroll
+  for (int i = 0; i < kNum; ++i) {
+#pragma unroll
+    for (int j = 0; j < kPairs; ++j) dw[i][j] = db[i][j] = both(0.0f);
+  }
+  // what comes beside a row, read a row ahead
+  float next_mean = 0.0f, next_rstd = 0.0f;
+  uint32_t next_byte[kNum] = {};
+  const int64_t quads = ceil_div(a.cols >> 5, 4);
+  const auto beside = [&](uint32_t r) {
+    if (r >= end) return;
+    next_mean = a.mean[row0 + r];
+    next_rstd = a.rstd[row0 + r];
+    if constexpr (kCopy) {
+#pragma unroll
+      for (int i = 0; i < kNum; ++i) {
+        const int v = threadIdx.x + i * width;
+        if (v < vecs) next_byte[i] = a.scales[swizzled_scale_offset(row0 + r, v * kVec >> 5, quads)];
+      }
+    }
+  };
+  beside(begin + team);
+  int stage = 0, turn = 0;
+  uint32_t phase = 0;
+  for (uint32_t r = begin + team; r < end; r += teams, turn ^= 1) {
+    const float mean = next_mean, rstd = next_rstd;
+    float factor[kNum];
+#pragma unroll
+    for (int i = 0; i < kNum; ++i) factor[i] = e8m0_factor(next_byte[i]);
+    beside(r + teams);
+    if (!sm100::mbar_wait(full_at + stage * 8, phase, &abort_flag)) break;
+    const uint8_t* const from = ring + stage * stage_bytes;
+    Raw<T, kVec> dy[kNum];
+    std::conditional_t<kCopy, Raw<uint32_t, kVec / 4>, Raw<T, kVec>> x[kNum];
+#pragma unroll
+    for (int i = 0; i < kNum; ++i) {
+      const int v = threadIdx.x + i * width;
+      const bool inside = v < vecs;
+      dy[i] = inside ? *reinterpret_cast<const Raw<T, kVec>*>(from + v * 16) : zeros<T, kVec>();
+      if constexpr (kCopy) {
+        if (inside) {
+          x[i] = *reinterpret_cast<const Raw<uint32_t, kVec / 4>*>(from + x_at + v * kVec);
+        } else {
+#pragma unroll
+          for (int j = 0; j < kVec / 4; ++j) x[i].v[j] = 0u;
+        }
+      } else {
+        x[i] = inside ? *reinterpret_cast<const Raw<T, kVec>*>(from + x_at + v * 16) : zeros<T, kVec>();
+      }
+    }
+    const auto values = [&](int i, float2(&h)[kPairs]) {
+      if constexpr (kCopy) {
+#pragma unroll
+        for (int j = 0; j < kVec / 4; ++j) {
+          h[2 * j] = mul_x2(e4m3_pair(x[i].v[j] & 0xFFFFu), both(factor[i]));
+          h[2 * j + 1] = mul_x2(e4m3_pair(x[i].v[j] >> 16), both(factor[i]));
+        }
+      } else {
+        unpack(x[i], h);
+      }
+#pragma unroll
+      for (int j = 0; j < kPairs; ++j) h[j] = mul_x2(add_x2(h[j], both(-mean)), both(rstd));
+    };
+    float2 s1 = both(0.0f), s2 = both(0.0f);
+#pragma unroll
+    for (int i = 0; i < kNum; ++i) {
+      float2 h[kPairs], d[kPairs], f[kPairs];
+      values(i, h);
+      unpack(dy[i], d);
+      factors(i, f);
+#pragma unroll
+      for (int j = 0; j < kPairs; ++j) {
+        const float2 g = mul_x2(d[j], f[j]);
+        s1 = add_x2(s1, g);
+        s2 = fma_x2(g, h[j], s2);
+        dw[i][j] = fma_x2(d[j], h[j], dw[i][j]);
+        db[i][j] = add_x2(db[i][j], d[j]);
+      }
+    }
+    // both sums in five exchanges: the lower half of a warp goes on with one, the upper with the other
+    float sum = (lane < 16 ? s1.x + s1.y : s2.x + s2.y) + __shfl_xor_sync(0xFFFFFFFFu, lane < 16 ? s2.x + s2.y : s1.x + s1.y, 16);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    float c1, c2;
+    if (warps > 1) {  // the team's warps meet; two buffers in turn, so that one meeting a row is enough
+      float2* const slots = row_buf[turn] + team * warps;
+      if (lane == 0) slots[threadIdx.x >> 5].x = sum;
+      if (lane == 16) slots[threadIdx.x >> 5].y = sum;
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(width) : "memory");
+      float2 all = both(0.0f);
+      for (int w = 0; w < warps; ++w) all = add_x2(all, slots[w]);
+      c1 = all.x * inv_cols;
+      c2 = all.y * inv_cols;
+    } else {
+      c1 = __shfl_sync(0xFFFFFFFFu, sum, 0) * inv_cols;
+      c2 = __shfl_sync(0xFFFFFFFFu, sum, 16) * inv_cols;
+    }
+    if (threadIdx.x == 0 && r + stages * teams < end) load_row(r + stages * teams, stage);  // all have read the stage
+    if (++stage == stages) {
+      stage = 0;
+      phase ^= 1u;
+    }
+    T* const dx = static_cast<T*>(a.dx) + static_cast<int64_t>(row0 + r) * a.cols;
+#pragma unroll
+    for (int i = 0; i < kNum; ++i) {
+      const int v = threadIdx.x + i * width;
+      if (v < vecs) {
+        float2 h[kPairs], d[kPairs], f[kPairs];
+        values(i, h);
+        unpack(dy[i], d);
+        factors(i, f);
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) d[j] = mul_x2(fma_x2(h[j], both(-c2), fma_x2(d[j], f[j], both(-c1))), both(rstd));
+        store(dx + v * kVec, pack<T, kVec>(d));
+      }
+    }
+  }
+  __syncthreads();  // the ring is the column sums' now
+  if (abort_flag) {
+    if (threadIdx.x == 0 && team == 0) atomicExch(a.status, 1);
+    for (int i = 0; i < 200; ++i) __nanosleep(1000);  // copies that are in flight land before the memory is released
+    return;
+  }
+  if (a.dweight == nullptr && a.dbias == nullptr) return;
+  const int threads = width * teams, at = team * width + threadIdx.x;
+#pragma unroll
+  for (int i = 0; i < kNum; ++i) {
+    if (teams > 1) {
+      if (i > 0) __syncthreads();
+#pragma unroll
+      for (int j = 0; j < kPairs; ++j) {
+        shared_buf[(2 * j) * threads + at] = dw[i][j].x;
+        shared_buf[(2 * j + 1) * threads + at] = dw[i][j].y;
+        shared_buf[(kVec + 2 * j) * threads + at] = db[i][j].x;
+        shared_buf[(kVec + 2 * j + 1) * threads + at] = db[i][j].y;
+      }
+      __syncthreads();
+    }
+    const int v = threadIdx.x + i * width;
+#pragma unroll
+    for (int j = 0; j < 2 * kVec; ++j) {
+      if (j % teams != team || v >= vecs) continue;
+      const float2 own = j < kVec ? dw[i][j % kVec / 2] : db[i][j % kVec / 2];
+      float s = j % 2 == 0 ? own.x : own.y;
+      if (teams > 1) {
+        s = 0.0f;
+        for (int t = 0; t < teams; ++t) s += shared_buf[j * threads + t * width + threadIdx.x];
+      }
+      const int64_t k = static_cast<int64_t>(v) * kVec + j % kVec;
+      if (a.partials != nullptr) {
+        a.partials[(static_cast<int64_t>(blockIdx.x) * 2 + j / kVec) * a.cols + k] = s;
+      } else {
+        void* to = j < kVec ? a.dweight : a.dbias;
+        if (to != nullptr) store_param<T>(to, group * a.cols + k, a.params_f32, s);
+      }
+    }
+  }
+}
+
 // Rows of any width: dx by blocks that go over their row twice, then the column sums by blocks of 32 columns.
 template <typename T>
 __device__ __forceinline__ float normalized(const BackwardArgs& a, uint32_t row, int64_t k) {
@@ -565,12 +981,55 @@ int launch_forward_num(const ForwardArgs& a, int warps, cudaStream_t s) {
   return CK_OK;
 }
 
+template <typename T, int kVec, int kNum, bool kCopy>
+int launch_forward_ring_num(ForwardArgs a, int warps, cudaStream_t s) {
+  constexpr int64_t kRoom = 216 * 1024;
+  const int64_t stage = round_up(a.cols * static_cast<int64_t>(sizeof(T)), 128), param = round_up(a.cols * 4, 128);
+  int64_t params = (a.weight != nullptr ? param : 0) + (a.bias != nullptr ? param : 0);
+  const bool shared_params = params + 2 * stage <= kRoom;
+  if (!shared_params) params = 0;
+  int64_t teams = 32 / warps;
+  if (warps > 1 && teams > 15) teams = 15;  // named barriers 1 to 15
+  while (teams > 1 && params + 2 * teams * stage > kRoom) --teams;
+  int64_t stages = (kRoom - params) / (teams * stage);
+  if (stages > kMaxRing) stages = kMaxRing;
+  // one block an SM, and no block with less than a row for each team
+  const int64_t groups = a.rows / a.rows_per_group;
+  int64_t chunks = sm_count() / groups;
+  if (chunks > ceil_div(a.rows_per_group, teams)) chunks = ceil_div(a.rows_per_group, teams);
+  if (chunks < 1) chunks = 1;
+  const uint32_t chunk_rows = static_cast<uint32_t>(ceil_div(a.rows_per_group, chunks));
+  chunks = ceil_div(a.rows_per_group, chunk_rows);
+  const int smem = static_cast<int>(params + teams * stages * stage);
+  auto kernel = layer_norm_forward_ring_kernel<T, kVec, kNum, kCopy>;
+  CK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  if (int rc = gemm_status_word(&a.status)) return rc;
+  CK_CUDA(launch_pdl(kernel, dim3(static_cast<unsigned>(groups * chunks)), dim3(32 * warps, static_cast<unsigned>(teams)), smem, s, a,
+                     static_cast<uint32_t>(chunks), chunk_rows, static_cast<int>(stages), shared_params));
+  return CK_OK;
+}
+
+// 24 elements a thread
+template <typename T, int kVec, bool kCopy>
+int launch_forward_ring(const ForwardArgs& a, cudaStream_t s) {
+  constexpr int kUnit = 8 / kVec;
+  const int64_t vecs = a.cols / kVec;
+  const int warps = static_cast<int>(ceil_div(vecs, 32 * 3 * kUnit));
+  const int64_t num = ceil_div(vecs, 32 * warps * kUnit);
+  if (num == 1) return launch_forward_ring_num<T, kVec, kUnit, kCopy>(a, warps, s);
+  if (num == 2) return launch_forward_ring_num<T, kVec, 2 * kUnit, kCopy>(a, warps, s);
+  return launch_forward_ring_num<T, kVec, 3 * kUnit, kCopy>(a, warps, s);
+}
+
 // Warps of a row: as few as hold it, eight vectors a lane (no barrier crosses a warp then, and a lane has its loads in flight
 // together); where the rows alone do not fill the chip, as many as leave one vector a lane, up to 32.
 template <typename T, int kVec, bool kCopy>
 int launch_forward(const ForwardArgs& a, cudaStream_t s) {
   const int64_t vecs = ceil_div(a.cols, kVec);
   if (vecs > 32 * 32 * 8) return fail(CK_ERR_UNSUPPORTED, "layer_norm_forward: a copy of rows of %lld is not supported", (long long)a.cols);
+  if constexpr (kVec > 1) {
+    if (a.cols <= 32 * 32 * 24 && a.rows > 2 * sm_count() && a.rows_per_group >= 16) return launch_forward_ring<T, kVec, kCopy>(a, s);
+  }
   int warps = static_cast<int>(ceil_div(vecs, 32 * 8));
   while (warps < 32 && static_cast<int64_t>(warps) * 32 < vecs && static_cast<int64_t>(a.rows) * warps < 8 * sm_count()) ++warps;
   const int num = static_cast<int>(ceil_div(vecs, 32 * warps));
@@ -602,31 +1061,42 @@ int forward_typed(const ForwardArgs& given, cudaStream_t s) {
 // ---- backward: how the rows are shared out
 struct Plan {
   bool wide;      // rows that a block's threads do not hold
+  bool ring;      // rows that come through shared memory
   int num;        // vectors of a thread
   int warps;      // of a team
   int teams;      // of a block
   int rows;       // that a team takes at a time
+  int stages;     // of a team's ring
+  int smem;       // bytes
   uint32_t chunks, chunk_rows;  // blocks of a group, rows of each
 };
 
-Plan plan_backward(int64_t cols, int vec, int64_t groups, int64_t rows_per_group) {
+// size: of an element; weight: whether there is one.
+Plan plan_backward(int64_t cols, int size, int vec, bool copy, bool weight, int64_t groups, int64_t rows_per_group) {
   Plan p = {};
   const int64_t vecs = ceil_div(cols, vec);
-  const int most = vec == 1 ? 8 : 4;  // vectors of a thread
-  p.wide = vecs > 512 * most;
-  int64_t step;
-  if (p.wide) {
-    p.num = p.warps = p.teams = p.rows = 1;
-    step = 64;
-  } else {
-    const int wanted = vec == 1 ? 4 : 3;
-    p.warps = static_cast<int>(ceil_div(vecs, 32 * wanted));
+  p.wide = vecs > 512 * (vec == 1 ? 8 : 4);
+  p.ring = vec > 1 && vecs >= 64 && !p.wide;
+  int64_t step = 64;
+  if (!p.wide) {
+    p.warps = static_cast<int>(ceil_div(vecs, 32 * (vec == 1 ? 4 : 3)));
     if (p.warps > 16) p.warps = 16;
     p.num = static_cast<int>(ceil_div(vecs, 32 * p.warps));
-    p.teams = p.warps >= 16 ? 1 : 16 / p.warps;
+    p.teams = 16 / p.warps;
     if (p.teams > 15) p.teams = 15;  // named barriers 1 to 15
-    p.rows = p.num <= 2 ? 2 : 1;
+    p.rows = !p.ring && p.num <= 2 ? 2 : 1;
     step = static_cast<int64_t>(p.teams) * p.rows;
+    const int64_t sums = p.teams > 1 ? 2 * vec * 32 * p.warps * p.teams * 4 : 0, factors = weight ? round_up(cols * 4, 128) : 0;
+    if (p.ring) {
+      const int64_t stage = round_up(cols * size, 128) + round_up(cols * (copy ? 1 : size), 128);
+      int64_t stages = (208 * 1024 - factors) / (p.teams * stage);
+      p.stages = static_cast<int>(stages > kMaxRing ? kMaxRing : stages);
+      p.wide = p.stages < 2;
+      p.smem = static_cast<int>(factors + p.teams * p.stages * stage);
+      if (sums > p.smem) p.smem = static_cast<int>(sums);
+    } else {
+      p.smem = static_cast<int>(sums > factors ? sums : factors);
+    }
   }
   // one block an SM, and no block with less than one round of its teams
   int64_t chunks = sm_count() / groups;
@@ -639,32 +1109,45 @@ Plan plan_backward(int64_t cols, int vec, int64_t groups, int64_t rows_per_group
 
 template <typename T, int kVec, int kNum, int kRows, bool kCopy>
 int launch_backward_num(const BackwardArgs& a, const Plan& p, cudaStream_t s) {
-  const dim3 block(32 * p.warps, p.teams);
-  const int64_t sums = p.teams > 1 ? 2 * kVec * 32 * p.warps * p.teams * 4 : 0, factors = a.weight != nullptr ? a.cols * 4 : 0;
-  const int64_t smem = sums > factors ? sums : factors;
   auto kernel = layer_norm_backward_kernel<T, kVec, kNum, kRows, kCopy>;
-  if (smem > 32 * 1024) CK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-  CK_CUDA(launch_pdl(kernel, dim3(a.groups * a.chunks), block, smem, s, a));
+  if (p.smem > 32 * 1024) CK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, p.smem));
+  CK_CUDA(launch_pdl(kernel, dim3(a.groups * a.chunks), dim3(32 * p.warps, p.teams), p.smem, s, a));
+  return CK_OK;
+}
+
+template <typename T, int kVec, int kNum, bool kCopy>
+int launch_backward_ring(BackwardArgs a, const Plan& p, cudaStream_t s) {
+  if (int rc = gemm_status_word(&a.status)) return rc;
+  auto kernel = layer_norm_backward_ring_kernel<T, kVec, kNum, kCopy>;
+  if (p.smem > 32 * 1024) CK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, p.smem));
+  CK_CUDA(launch_pdl(kernel, dim3(a.groups * a.chunks), dim3(32 * p.warps, p.teams), p.smem, s, a, p.stages));
   return CK_OK;
 }
 
 template <typename T, int kVec, bool kCopy>
 int launch_backward(const BackwardArgs& a, const Plan& p, cudaStream_t s) {
-  switch (p.num) {
-    case 1: return launch_backward_num<T, kVec, 1, 2, kCopy>(a, p, s);
-    case 2: return launch_backward_num<T, kVec, 2, 2, kCopy>(a, p, s);
-    case 3: return launch_backward_num<T, kVec, 3, 1, kCopy>(a, p, s);
-    case 4: return launch_backward_num<T, kVec, 4, 1, kCopy>(a, p, s);
-    default:
-      if constexpr (kVec == 1) return launch_backward_num<T, 1, 8, 1, false>(a, p, s);
-      return fail(CK_ERR_UNSUPPORTED, "layer_norm_backward: no kernel for %d vectors", p.num);
+  if constexpr (kVec == 1) {
+    switch (p.num) {
+      case 1: return launch_backward_num<T, 1, 1, 2, false>(a, p, s);
+      case 2: return launch_backward_num<T, 1, 2, 2, false>(a, p, s);
+      case 3: case 4: return launch_backward_num<T, 1, 4, 1, false>(a, p, s);
+      default: return launch_backward_num<T, 1, 8, 1, false>(a, p, s);
+    }
+  } else if (p.ring) {
+    switch (p.num) {
+      case 2: return launch_backward_ring<T, kVec, 2, kCopy>(a, p, s);
+      case 3: return launch_backward_ring<T, kVec, 3, kCopy>(a, p, s);
+      default: return launch_backward_ring<T, kVec, 4, kCopy>(a, p, s);
+    }
+  } else {  // fewer than 64 vectors
+    return p.num == 1 ? launch_backward_num<T, kVec, 1, 2, kCopy>(a, p, s) : launch_backward_num<T, kVec, 2, 2, kCopy>(a, p, s);
   }
 }
 
 int backward_vec(const BackwardArgs& a, int dtype) {
   const int size = dtype == CK_DTYPE_F32 ? 4 : 2, vec = 16 / size;
   const bool vectors = a.cols % vec == 0 && on_vectors(a.dy, a.dy_rows, size) && reinterpret_cast<uintptr_t>(a.dx) % 16 == 0 &&
-                       (a.x != nullptr ? on_vectors(a.x, a.x_rows, size) : reinterpret_cast<uintptr_t>(a.codes) % 8 == 0);
+                       (a.x != nullptr ? on_vectors(a.x, a.x_rows, size) : reinterpret_cast<uintptr_t>(a.codes) % 16 == 0);
   return vectors ? vec : 1;
 }
 
@@ -673,7 +1156,7 @@ int backward_typed(const BackwardArgs& given, int dtype, void* workspace, int64_
   BackwardArgs a = given;
   a.params_aligned = a.weight == nullptr || on_vectors(a.weight, a.weight_stride, a.params_f32 ? 4 : sizeof(T));
   const int vec = backward_vec(a, dtype);
-  Plan p = plan_backward(a.cols, vec, a.groups, a.rows_per_group);
+  Plan p = plan_backward(a.cols, sizeof(T), vec, a.x == nullptr, a.weight != nullptr, a.groups, a.rows_per_group);
   p.wide = p.wide || (vec == 1 && a.x == nullptr);
   a.chunks = p.chunks;
   a.chunk_rows = p.chunk_rows;
@@ -768,8 +1251,9 @@ extern "C" int64_t ck_layer_norm_backward_workspace_bytes(int64_t rows, int64_t 
   using namespace ck;
   if (rows <= 0 || cols <= 0 || groups <= 0 || rows % groups != 0) return 0;
   int64_t most = 0;  // over the forms that alignment decides between
-  for (int vec : {1, 4, 8}) {
-    const Plan p = plan_backward(cols, vec, groups, rows / groups);
+  for (int form = 0; form < 12; ++form) {
+    const int vec = form % 3 == 0 ? 1 : form % 3 == 1 ? 4 : 8;
+    const Plan p = plan_backward(cols, vec == 4 ? 4 : 2, vec, form / 3 % 2 != 0, form / 6 != 0, groups, rows / groups);
     const int64_t need = p.chunks > 1 ? groups * p.chunks * 2 * cols * 4 : 0;
     if (need > most) most = need;
   }

@@ -4,8 +4,8 @@
 
 #include <type_traits>
 
-#include "ck_common.cuh"
 #include "ck_quant_math.cuh"
+#include "ck_sm100.cuh"
 
 namespace ck {
 namespace rows {
@@ -124,13 +124,57 @@ __device__ __forceinline__ void e4m3_four(uint32_t word, float factor, float* f)
   f[3] = hi.y * factor;
 }
 
+// The same as pairs of fp32 numbers, the form that one instruction computes on.
+template <typename T, int kVec>
+__device__ __forceinline__ void unpack(const Raw<T, kVec>& r, float2 (&f)[kVec / 2]) {
+  float v[kVec];
+  unpack(r, v);
+#pragma unroll
+  for (int i = 0; i < kVec / 2; ++i) f[i] = make_float2(v[2 * i], v[2 * i + 1]);
+}
+template <typename T, int kVec>
+__device__ __forceinline__ Raw<T, kVec> pack(const float2 (&f)[kVec / 2]) {
+  float v[kVec];
+#pragma unroll
+  for (int i = 0; i < kVec / 2; ++i) {
+    v[2 * i] = f[i].x;
+    v[2 * i + 1] = f[i].y;
+  }
+  return pack<T, kVec>(v);
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+// 1 / sqrt(v): the hardware's estimate and a Newton step.  Where the step would meet infinities the estimate is the value.
+__device__ __forceinline__ float inverse_root(float v) {
+  const float r = rsqrtf(v);
+  const float better = r * fmaf(-0.5f * v * r, r, 1.5f);
+  return v > 0.0f && v < 3e38f ? better : r;
+}
+
+// The scale of an MXFP8 block as quant::mxfp8_scale has it, by integers where neither the byte nor its factor is special: with
+// amax = m 2^E and 448 = 1.75 2^8 the exponent is E - 8, and one more where m > 1.75.  (The rounded quotient amax / 448 that the definition
+// takes the logarithm of says the same: the fp32 number above 1.75 2^E gives 1 + 2^-23.8, which rounds to 1 + 2^-23, not to 1.)
+__device__ __forceinline__ quant::Mxfp8Scale block_scale(float amax) {
+  const uint32_t e = ((__float_as_uint(amax) + 0x1FFFFFu) >> 23) - 8u;
+  if (e - 1u < 250u && __float_as_uint(amax) < 0x7F800000u) return {__uint_as_float((254u - e) << 23), e, false};
+  return quant::mxfp8_scale(amax);
+}
+
+// Four values of a block -> four codes.
+__device__ __forceinline__ uint32_t block_codes(float2 a, float2 b, const quant::Mxfp8Scale& s) {
+  a = mul_x2(a, both(s.inv));
+  b = mul_x2(b, both(s.inv));
+  const uint32_t w = quant::f32x2_to_e4m3x2(a.y, a.x) | (quant::f32x2_to_e4m3x2(b.y, b.x) << 16);
+  return s.dead ? 0u : w;
+}
+
 // Rows in two levels: row r is row r % inner of outer index r / inner.
 struct RowStrides {
   int64_t outer_stride;  // elements
   int64_t inner_stride;
   uint32_t inner;
   __device__ __forceinline__ int64_t offset(uint32_t row) const {
-    const uint32_t o = row / inner;
+    const uint32_t o = row < inner ? 0u : row / inner;
     return static_cast<int64_t>(o) * outer_stride + static_cast<int64_t>(row - o * inner) * inner_stride;
   }
 };

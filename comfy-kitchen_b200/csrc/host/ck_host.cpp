@@ -17,12 +17,18 @@
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstdint>
 #include <cstdlib>
+#include <memory>
+#include <optional>
+#include <vector>
 
 namespace {
 
@@ -49,6 +55,17 @@ struct Library {
   int64_t (*linear_mxfp8_from_float_workspace_bytes)(int64_t, int64_t);
   int (*linear_mxfp8_from_float)(const void*, int, const void*, const void*, const void*, int, void*, int, int64_t, int64_t, int64_t, void*,
                                  int64_t, void*);
+  int (*layer_norm_forward)(const void*, int, int64_t, int64_t, int64_t, int64_t, int64_t, const void*, const void*, int, int64_t, int64_t, int64_t, float,
+                            float, void*, float*, float*, void*, void*, void*);
+  int64_t (*layer_norm_backward_workspace_bytes)(int64_t, int64_t, int64_t);
+  int (*layer_norm_backward)(const void*, int, int64_t, int64_t, int64_t, int64_t, int64_t, const void*, int64_t, int64_t, int64_t, const void*, const void*,
+                             const float*, const float*, const void*, int, int64_t, int64_t, float, void*, void*, void*, void*, int64_t, void*);
+  int (*gelu_mxfp8_forward)(const void*, int, void*, void*, void*, int64_t, int64_t, void*);
+  int (*gelu_mxfp8_backward)(const void*, int, const void*, const void*, void*, int64_t, int64_t, void*);
+  int64_t (*linear_grad_mxfp8_workspace_bytes)(int, int, int, int64_t, int64_t, int64_t);
+  int (*linear_weight_grad_mxfp8)(const void*, int, const void*, const void*, void*, int, void*, int64_t, int64_t, int64_t, void*, int64_t, void*);
+  int (*linear_input_grad_mxfp8)(const void*, int, const void*, const void*, void*, int, int64_t, int64_t, int64_t, void*, int64_t, void*);
+  const char* (*last_error)();
 };
 Library lib = {};
 PyTypeObject* parameter_type = nullptr;
@@ -436,6 +453,9 @@ PyObject* linear_mxfp8_from_float(PyObject*, Args a, Py_ssize_t n_args) {  // x,
   });
 }
 
+// ---- training ---------------------------------------------------------------------------------
+#include "ck_host_training.h"
+
 // ---- set-up -----------------------------------------------------------------------------------
 // bind({name: address of ck_<name>}, torch.nn.Parameter)
 PyObject* bind(PyObject*, Args a, Py_ssize_t n_args) {
@@ -466,6 +486,15 @@ PyObject* bind(PyObject*, Args a, Py_ssize_t n_args) {
   CK_TAKE(linear_nvfp4_from_float);
   CK_TAKE(linear_mxfp8_from_float_workspace_bytes);
   CK_TAKE(linear_mxfp8_from_float);
+  CK_TAKE(layer_norm_forward);
+  CK_TAKE(layer_norm_backward_workspace_bytes);
+  CK_TAKE(layer_norm_backward);
+  CK_TAKE(gelu_mxfp8_forward);
+  CK_TAKE(gelu_mxfp8_backward);
+  CK_TAKE(linear_grad_mxfp8_workspace_bytes);
+  CK_TAKE(linear_weight_grad_mxfp8);
+  CK_TAKE(linear_input_grad_mxfp8);
+  CK_TAKE(last_error);
 #undef CK_TAKE
   if (!complete) {
     if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "bind: an entry point is missing");
@@ -488,6 +517,10 @@ PyMethodDef methods[] = {CK_METHOD(bind),
                          CK_METHOD(scaled_mm_mxfp8),
                          CK_METHOD(linear_nvfp4_from_float),
                          CK_METHOD(linear_mxfp8_from_float),
+                         CK_METHOD(layer_norm),
+                         CK_METHOD(gelu_checkpointed),
+                         CK_METHOD(linear_weight_grad_mxfp8),
+                         CK_METHOD(linear_input_grad_mxfp8),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_ck_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
