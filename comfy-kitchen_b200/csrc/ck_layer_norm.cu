@@ -370,7 +370,8 @@ __global__ void __launch_bounds__(1024) layer_norm_forward_ring_kernel(const For
       }
 #pragma unroll
       for (int j = 0; j < kPairs; ++j) {
-        f[i][j] = mul_x2(add_x2(f[i][j], both(-mean)), both(rstd));
+        // in one step for 16-bit types, where a mean of that many times the deviation leaves no digits in x anyway
+        f[i][j] = sizeof(T) == 2 ? fma_x2(f[i][j], both(rstd), both(-mean * rstd)) : mul_x2(add_x2(f[i][j], both(-mean)), both(rstd));
         if (weight && bias) {
           f[i][j] = fma_x2(f[i][j], w[j], b[j]);
         } else if (weight) {
@@ -610,24 +611,18 @@ __global__ void __launch_bounds__(512) layer_norm_backward_kernel(const Backward
   const int threads = width * teams, at = team * width + threadIdx.x;
 #pragma unroll
   for (int i = 0; i < kNum; ++i) {
-    if (teams > 1) {
-      __syncthreads();
+    __syncthreads();
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) {
-        column_buf[j * threads + at] = dw[i][j];
-        column_buf[(kVec + j) * threads + at] = db[i][j];
-      }
-      __syncthreads();
+    for (int j = 0; j < kVec; ++j) {
+      column_buf[j * threads + at] = dw[i][j];
+      column_buf[(kVec + j) * threads + at] = db[i][j];
     }
+    __syncthreads();
     const int64_t v = threadIdx.x + i * width;
-#pragma unroll
-    for (int j = 0; j < 2 * kVec; ++j) {
-      if (j % teams != team || v >= vecs) continue;
-      float s = j < kVec ? dw[i][j % kVec] : db[i][j % kVec];
-      if (teams > 1) {
-        s = 0.0f;
-        for (int t = 0; t < teams; ++t) s += column_buf[j * threads + t * width + threadIdx.x];
-      }
+    if (v >= vecs) continue;
+    for (int j = team; j < 2 * kVec; j += teams) {
+      float s = 0.0f;
+      for (int t = 0; t < teams; ++t) s += column_buf[j * threads + t * width + threadIdx.x];
       const int64_t k = v * kVec + j % kVec;
       if (a.partials != nullptr) {
         a.partials[(static_cast<int64_t>(blockIdx.x) * 2 + j / kVec) * a.cols + k] = s;
@@ -738,51 +733,37 @@ __global__ void __launch_bounds__(512) layer_norm_backward_ring_kernel(const Bac
     beside(r + teams);
     if (!sm100::mbar_wait(full_at + stage * 8, phase, &abort_flag)) break;
     const uint8_t* const from = ring + stage * stage_bytes;
-    Raw<T, kVec> dy[kNum];
-    std::conditional_t<kCopy, Raw<uint32_t, kVec / 4>, Raw<T, kVec>> x[kNum];
-#pragma unroll
-    for (int i = 0; i < kNum; ++i) {
-      const int v = threadIdx.x + i * width;
-      const bool inside = v < vecs;
-      dy[i] = inside ? *reinterpret_cast<const Raw<T, kVec>*>(from + v * 16) : zeros<T, kVec>();
-      if constexpr (kCopy) {
-        if (inside) {
-          x[i] = *reinterpret_cast<const Raw<uint32_t, kVec / 4>*>(from + x_at + v * kVec);
-        } else {
-#pragma unroll
-          for (int j = 0; j < kVec / 4; ++j) x[i].v[j] = 0u;
-        }
-      } else {
-        x[i] = inside ? *reinterpret_cast<const Raw<T, kVec>*>(from + x_at + v * 16) : zeros<T, kVec>();
-      }
-    }
-    const auto values = [&](int i, float2(&h)[kPairs]) {
-      if constexpr (kCopy) {
-#pragma unroll
-        for (int j = 0; j < kVec / 4; ++j) {
-          h[2 * j] = mul_x2(e4m3_pair(x[i].v[j] & 0xFFFFu), both(factor[i]));
-          h[2 * j + 1] = mul_x2(e4m3_pair(x[i].v[j] >> 16), both(factor[i]));
-        }
-      } else {
-        unpack(x[i], h);
-      }
-#pragma unroll
-      for (int j = 0; j < kPairs; ++j) h[j] = mul_x2(add_x2(h[j], both(-mean)), both(rstd));
-    };
+    // unpacked once: dy and h stay in registers for both passes
+    float2 d[kNum][kPairs], h[kNum][kPairs];
+    const float2 rstd2 = both(rstd), shift = both(sizeof(T) == 2 ? -mean * rstd : -mean);
     float2 s1 = both(0.0f), s2 = both(0.0f);
 #pragma unroll
     for (int i = 0; i < kNum; ++i) {
-      float2 h[kPairs], d[kPairs], f[kPairs];
-      values(i, h);
-      unpack(dy[i], d);
+      const int v = min(static_cast<int>(threadIdx.x) + i * width, vecs - 1);
+      Raw<T, kVec> raw = *reinterpret_cast<const Raw<T, kVec>*>(from + v * 16);
+      if (static_cast<int>(threadIdx.x) + i * width >= vecs) raw = zeros<T, kVec>();  // past the row's end: dy = 0, whatever h
+      unpack(raw, d[i]);
+      if constexpr (kCopy) {
+        const auto codes = *reinterpret_cast<const Raw<uint32_t, kVec / 4>*>(from + x_at + v * kVec);
+#pragma unroll
+        for (int j = 0; j < kVec / 4; ++j) {
+          h[i][2 * j] = mul_x2(e4m3_pair(codes.v[j] & 0xFFFFu), both(factor[i]));
+          h[i][2 * j + 1] = mul_x2(e4m3_pair(codes.v[j] >> 16), both(factor[i]));
+        }
+      } else {
+        unpack(*reinterpret_cast<const Raw<T, kVec>*>(from + x_at + v * 16), h[i]);
+      }
+      float2 f[kPairs];
       factors(i, f);
 #pragma unroll
       for (int j = 0; j < kPairs; ++j) {
-        const float2 g = mul_x2(d[j], f[j]);
+        // (x - mean) / std; in one step for 16-bit types, where a mean of that many times the deviation leaves no digits in x anyway
+        h[i][j] = sizeof(T) == 2 ? fma_x2(h[i][j], rstd2, shift) : mul_x2(add_x2(h[i][j], shift), rstd2);
+        const float2 g = mul_x2(d[i][j], f[j]);
         s1 = add_x2(s1, g);
-        s2 = fma_x2(g, h[j], s2);
-        dw[i][j] = fma_x2(d[j], h[j], dw[i][j]);
-        db[i][j] = add_x2(db[i][j], d[j]);
+        s2 = fma_x2(g, h[i][j], s2);
+        dw[i][j] = fma_x2(d[i][j], h[i][j], dw[i][j]);
+        db[i][j] = add_x2(db[i][j], d[i][j]);
       }
     }
     // both sums in five exchanges: the lower half of a warp goes on with one, the upper with the other
@@ -792,8 +773,7 @@ __global__ void __launch_bounds__(512) layer_norm_backward_ring_kernel(const Bac
     float c1, c2;
     if (warps > 1) {  // the team's warps meet; two buffers in turn, so that one meeting a row is enough
       float2* const slots = row_buf[turn] + team * warps;
-      if (lane == 0) slots[threadIdx.x >> 5].x = sum;
-      if (lane == 16) slots[threadIdx.x >> 5].y = sum;
+      if ((lane & 15) == 0) reinterpret_cast<float*>(slots + (threadIdx.x >> 5))[lane >> 4] = sum;
       asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(width) : "memory");
       float2 all = both(0.0f);
       for (int w = 0; w < warps; ++w) all = add_x2(all, slots[w]);
@@ -813,13 +793,13 @@ __global__ void __launch_bounds__(512) layer_norm_backward_ring_kernel(const Bac
     for (int i = 0; i < kNum; ++i) {
       const int v = threadIdx.x + i * width;
       if (v < vecs) {
-        float2 h[kPairs], d[kPairs], f[kPairs];
-        values(i, h);
-        unpack(dy[i], d);
+        float2 f[kPairs];
         factors(i, f);
 #pragma unroll
-        for (int j = 0; j < kPairs; ++j) d[j] = mul_x2(fma_x2(h[j], both(-c2), fma_x2(d[j], f[j], both(-c1))), both(rstd));
-        store(dx + v * kVec, pack<T, kVec>(d));
+        for (int j = 0; j < kPairs; ++j) {
+          d[i][j] = mul_x2(fma_x2(h[i][j], both(-c2), fma_x2(d[i][j], f[j], both(-c1))), rstd2);
+        }
+        store(dx + v * kVec, pack<T, kVec>(d[i]));
       }
     }
   }
@@ -831,35 +811,42 @@ __global__ void __launch_bounds__(512) layer_norm_backward_ring_kernel(const Bac
   }
   if (a.dweight == nullptr && a.dbias == nullptr) return;
   const int threads = width * teams, at = team * width + threadIdx.x;
+  const auto put = [&](int j, int v, float s) {  // sum j (of kVec for dw, then of kVec for db) of vector v
+    const int64_t k = static_cast<int64_t>(v) * kVec + j % kVec;
+    if (a.partials != nullptr) {
+      a.partials[(static_cast<int64_t>(blockIdx.x) * 2 + j / kVec) * a.cols + k] = s;
+    } else {
+      void* const to = j < kVec ? a.dweight : a.dbias;
+      if (to != nullptr) store_param<T>(to, group * a.cols + k, a.params_f32, s);
+    }
+  };
 #pragma unroll
   for (int i = 0; i < kNum; ++i) {
-    if (teams > 1) {
-      if (i > 0) __syncthreads();
-#pragma unroll
-      for (int j = 0; j < kPairs; ++j) {
-        shared_buf[(2 * j) * threads + at] = dw[i][j].x;
-        shared_buf[(2 * j + 1) * threads + at] = dw[i][j].y;
-        shared_buf[(kVec + 2 * j) * threads + at] = db[i][j].x;
-        shared_buf[(kVec + 2 * j + 1) * threads + at] = db[i][j].y;
-      }
-      __syncthreads();
-    }
     const int v = threadIdx.x + i * width;
+    if (teams == 1) {
+      if (v < vecs) {
 #pragma unroll
-    for (int j = 0; j < 2 * kVec; ++j) {
-      if (j % teams != team || v >= vecs) continue;
-      const float2 own = j < kVec ? dw[i][j % kVec / 2] : db[i][j % kVec / 2];
-      float s = j % 2 == 0 ? own.x : own.y;
-      if (teams > 1) {
-        s = 0.0f;
-        for (int t = 0; t < teams; ++t) s += shared_buf[j * threads + t * width + threadIdx.x];
+        for (int j = 0; j < kVec; ++j) {
+          put(j, v, j % 2 == 0 ? dw[i][j / 2].x : dw[i][j / 2].y);
+          put(kVec + j, v, j % 2 == 0 ? db[i][j / 2].x : db[i][j / 2].y);
+        }
       }
-      const int64_t k = static_cast<int64_t>(v) * kVec + j % kVec;
-      if (a.partials != nullptr) {
-        a.partials[(static_cast<int64_t>(blockIdx.x) * 2 + j / kVec) * a.cols + k] = s;
-      } else {
-        void* to = j < kVec ? a.dweight : a.dbias;
-        if (to != nullptr) store_param<T>(to, group * a.cols + k, a.params_f32, s);
+      continue;
+    }
+    if (i > 0) __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kPairs; ++j) {
+      shared_buf[(2 * j) * threads + at] = dw[i][j].x;
+      shared_buf[(2 * j + 1) * threads + at] = dw[i][j].y;
+      shared_buf[(kVec + 2 * j) * threads + at] = db[i][j].x;
+      shared_buf[(kVec + 2 * j + 1) * threads + at] = db[i][j].y;
+    }
+    __syncthreads();
+    if (v < vecs) {
+      for (int j = team; j < 2 * kVec; j += teams) {
+        float s = 0.0f;
+        for (int t = 0; t < teams; ++t) s += shared_buf[j * threads + t * width + threadIdx.x];
+        put(j, v, s);
       }
     }
   }
@@ -1075,18 +1062,19 @@ struct Plan {
 Plan plan_backward(int64_t cols, int size, int vec, bool copy, bool weight, int64_t groups, int64_t rows_per_group) {
   Plan p = {};
   const int64_t vecs = ceil_div(cols, vec);
-  p.wide = vecs > 512 * (vec == 1 ? 8 : 4);
+  const int unit = vec == 4 ? 2 : 1;  // 24 elements a thread, or up to 32 (one by one: 4, up to 8)
+  p.wide = vecs > 512 * (vec == 1 ? 8 : vec == 4 ? 6 : 4);
   p.ring = vec > 1 && vecs >= 64 && !p.wide;
   int64_t step = 64;
   if (!p.wide) {
-    p.warps = static_cast<int>(ceil_div(vecs, 32 * (vec == 1 ? 4 : 3)));
+    p.warps = static_cast<int>(ceil_div(vecs, 32 * (vec == 1 ? 4 : 3 * unit)));
     if (p.warps > 16) p.warps = 16;
-    p.num = static_cast<int>(ceil_div(vecs, 32 * p.warps));
+    p.num = static_cast<int>(ceil_div(vecs, 32 * p.warps * unit)) * unit;
     p.teams = 16 / p.warps;
     if (p.teams > 15) p.teams = 15;  // named barriers 1 to 15
     p.rows = !p.ring && p.num <= 2 ? 2 : 1;
     step = static_cast<int64_t>(p.teams) * p.rows;
-    const int64_t sums = p.teams > 1 ? 2 * vec * 32 * p.warps * p.teams * 4 : 0, factors = weight ? round_up(cols * 4, 128) : 0;
+    const int64_t sums = 2 * vec * 32 * p.warps * p.teams * 4, factors = weight ? round_up(cols * 4, 128) : 0;
     if (p.ring) {
       const int64_t stage = round_up(cols * size, 128) + round_up(cols * (copy ? 1 : size), 128);
       int64_t stages = (208 * 1024 - factors) / (p.teams * stage);
@@ -1134,10 +1122,18 @@ int launch_backward(const BackwardArgs& a, const Plan& p, cudaStream_t s) {
       default: return launch_backward_num<T, 1, 8, 1, false>(a, p, s);
     }
   } else if (p.ring) {
-    switch (p.num) {
-      case 2: return launch_backward_ring<T, kVec, 2, kCopy>(a, p, s);
-      case 3: return launch_backward_ring<T, kVec, 3, kCopy>(a, p, s);
-      default: return launch_backward_ring<T, kVec, 4, kCopy>(a, p, s);
+    if constexpr (kVec == 4) {
+      switch (p.num) {
+        case 2: return launch_backward_ring<T, 4, 2, kCopy>(a, p, s);
+        case 4: return launch_backward_ring<T, 4, 4, kCopy>(a, p, s);
+        default: return launch_backward_ring<T, 4, 6, kCopy>(a, p, s);
+      }
+    } else {
+      switch (p.num) {
+        case 1: case 2: return launch_backward_ring<T, 8, 2, kCopy>(a, p, s);
+        case 3: return launch_backward_ring<T, 8, 3, kCopy>(a, p, s);
+        default: return launch_backward_ring<T, 8, 4, kCopy>(a, p, s);
+      }
     }
   } else {  // fewer than 64 vectors
     return p.num == 1 ? launch_backward_num<T, kVec, 1, 2, kCopy>(a, p, s) : launch_backward_num<T, kVec, 2, 2, kCopy>(a, p, s);
