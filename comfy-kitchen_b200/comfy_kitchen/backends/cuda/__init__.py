@@ -946,12 +946,11 @@ def gelu_mxfp8_backward(dy: torch.Tensor, codes: torch.Tensor, block_scales: tor
 
 
 def _linear_grad_args(dy, codes, scales, rows: int):
-    dy, codes, scales = _aligned(dy, 16), _plain(codes), _plain(scales)
+    dy, codes, scales = _aligned(dy, 16), _aligned(codes, 32), _aligned(scales, 16)
     n, k = dy.shape[1], codes.shape[1]
     assert codes.shape[0] == rows, "Matrix dimensions do not match"
     assert k > 0 and k % 32 == 0 and n > 0 and n % 8 == 0, "K must be a multiple of 32 and N of 8"
     assert scales.shape == (roundup(rows, 128), roundup(k // 32, 4)), "Invalid scale shape"
-    assert codes.is_contiguous() and scales.is_contiguous(), "codes and scales must be contiguous"
     return dy, codes, scales, n, k
 
 

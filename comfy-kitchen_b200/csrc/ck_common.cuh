@@ -68,6 +68,11 @@ int scaled_mm_small_m(bool is_mxfp8, const void* a, const void* b, const void* s
                       const float* tsb, const float* alpha, const void* bias, int bias_dtype, void* out, int out_dtype,
                       int64_t M, int64_t N, int64_t K, cudaStream_t stream);
 
+// A linear layer's input gradient through an MXFP8 weight for few rows (ck_grad_few_rows.cu).
+bool grad_few_rows_applies(int64_t M, int64_t N, int64_t K, int planes);
+int grad_few_rows(const void* dy, int planes, const void* codes, const void* scales, void* out, int out_dtype, int64_t M, int64_t N, int64_t K,
+                  cudaStream_t stream);
+
 // ---- programmatic dependent launch ------------------------------------------------------
 // The streaming kernels and the GEMMs of this library are launched with programmatic stream
 // serialization: each kernel lets its successor start being scheduled at once

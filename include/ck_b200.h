@@ -342,7 +342,7 @@ CK_API int ck_gelu_mxfp8_backward(const void* dy, int dtype, const void* codes, 
  * of 32-element blocks along K):
  *   weight: dweight[N,K] = dy[M,N]^T . deq(x)[M,K], and dbias[N] = sum over m of dy (dbias may be null)
  *   input:  dx[M,K] = dy[M,N] . deq(w)[N,K]
- * dy: f32/f16/bf16, row-major, 16-byte aligned; results of out_dtype, 32-byte aligned.  The MXFP8 values enter as
+ * dy: f32/f16/bf16, row-major, 16-byte aligned; codes 32-byte, block scales 16-byte aligned; results of out_dtype, 32-byte aligned.  The MXFP8 values enter as
  * ck_dequantize_mxfp8 gives them in bf16 (exact for magnitudes of 2^-126 on), dy exactly; fp32 accumulation, one rounding, sums in a
  * fixed order.  K % 32 == 0, N % 8 == 0.  workspace: device memory, 256-byte aligned, of ck_linear_grad_mxfp8_workspace_bytes bytes
  * (0: shape not supported), no requirement on its contents; calls that can overlap on the GPU need separate ones.

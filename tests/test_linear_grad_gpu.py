@@ -76,7 +76,8 @@ def test_weight(ck, dtype, m, n, k):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("m,n,k", SIZES + [(2, 3000, 512), (8, 4096, 1024), (16, 1024, 2048), (40, 2048, 32), (128, 2048, 2048)])
+@pytest.mark.parametrize("m,n,k", SIZES + [(2, 3000, 512), (8, 4096, 1024), (16, 1024, 2048), (40, 2048, 32), (128, 2048, 2048), (16, 12288, 128),
+                                           (72, 12288, 256), (128, 12288, 384), (200, 12288, 128), (208, 6000, 256), (209, 6000, 256)])
 def test_input(ck, dtype, m, n, k):
     _input(ck, m, n, k, dtype)
 
