@@ -877,7 +877,7 @@ def _layer_norm_backward(dy, x, codes, scales, mean, rstd, weight, weight_offset
             codes, scales = _plain(codes), _plain(scales)
             assert codes.shape == (rows, cols) and scales.shape == (roundup(rows, 128), roundup(cols // 32, 4)), "Invalid codes or scale shape"
             assert codes.is_contiguous() and scales.is_contiguous(), "codes and scales must be contiguous"
-        dy, inner, outer_stride, inner_stride = _row_levels(dy)
+        dy, inner, outer_stride, inner_stride = _row_levels(dy, 16 if x is None else 1)
         need = _workspace_bytes("ck_layer_norm_backward_workspace_bytes", rows, cols, groups) if weight_grad or bias_grad else 0
         with _on_device(dev):
             ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None

@@ -1,0 +1,185 @@
+// What the forward and the backward pass of layer norm share: parameters, sums over a row's warps, a thread's columns, and rows that come through
+// a ring in shared memory.
+//
+//   m = mean_k x,  v = mean_k (x - m)^2,  i = 1 / sqrt(v + eps),  h = (x - m) i
+//   y = h f + b,   f = offset + w (1 without a weight)
+//   g = dy f,      dx = i (g - mean_k g - h mean_k(g h)),   dw = sum_rows dy h,   db = sum_rows dy
+//
+// w and b belong to groups of consecutive rows (one group: the learned weight of a layer; one for each sample: modulation).
+// Rows are taken in two levels of strides, so that a slice of the tokens of a longer buffer needs no copy.  All
+// sums and statistics are fp32; a row stays in registers between its passes, so its mean is subtracted before
+// squares are taken.  Results are rounded to their types once.
+#pragma once
+
+#include "ck_rows.cuh"
+
+namespace ck {
+namespace {
+
+using namespace rows;
+
+// ---- parameters: fp32, or of x's type
+template <typename W, int kVec>
+__device__ __forceinline__ void load_param_of(const W* p, bool aligned, float (&f)[kVec]) {
+  Raw<W, kVec> r;
+  if (kVec > 1 && aligned) {
+    r = *reinterpret_cast<const Raw<W, kVec>*>(p);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) r.v[i] = p[i];
+  }
+  unpack(r, f);
+}
+
+// kVec weights or biases from element `at` on: fp32 or of the type T.
+template <typename T, int kVec>
+__device__ __forceinline__ void load_param(const void* base, int64_t at, bool f32, bool aligned, float (&f)[kVec]) {
+  if (!std::is_same<T, float>::value && f32) {
+    if constexpr (kVec == 8) {  // two 16-byte loads
+      float lo[4], hi[4];
+      load_param_of<float, 4>(static_cast<const float*>(base) + at, aligned, lo);
+      load_param_of<float, 4>(static_cast<const float*>(base) + at + 4, aligned, hi);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        f[i] = lo[i];
+        f[4 + i] = hi[i];
+      }
+    } else {
+      load_param_of<float, kVec>(static_cast<const float*>(base) + at, aligned, f);
+    }
+  } else {
+    load_param_of<T, kVec>(static_cast<const T*>(base) + at, aligned, f);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ float param(const void* base, int64_t at, bool f32) {
+  return f32 ? static_cast<const float*>(base)[at] : to_float(static_cast<const T*>(base)[at]);
+}
+
+template <typename T>
+__device__ __forceinline__ void store_param(void* base, int64_t at, bool f32, float v) {
+  if (f32) {
+    static_cast<float*>(base)[at] = v;
+  } else {
+    static_cast<T*>(base)[at] = from_float<T>(v);
+  }
+}
+
+// ---- sums
+// Sum over the warps of one row (threadIdx.y); `buf`: a slot for each warp of the block, another one for each sum of a kernel.
+template <int kSlot>
+__device__ __forceinline__ float row_sum(float v, float* buf) {
+  v = warp_sum(v);
+  const int warps = blockDim.x >> 5;
+  if (warps == 1) return v;
+  float* mine = buf + kSlot * 32 + threadIdx.y * warps;
+  if ((threadIdx.x & 31) == 0) mine[threadIdx.x >> 5] = v;
+  __syncthreads();
+  float s = 0.0f;
+  for (int i = 0; i < warps; ++i) s += mine[i];
+  return s;
+}
+
+// ---- rows that come through shared memory
+// A team's row is a bulk copy into a ring of stages, issued that many rows ahead by one thread, so that what is in flight
+// does not depend on registers or on where the warps stand.  Barriers of the ring are mbarriers whose waits are bounded (mbar_wait).
+constexpr int kMaxRing = 4;
+
+// A row that does not lie on 16-byte boundaries is copied where it does, at the same place in its 16 bytes; what is before and behind
+// (up to 15 bytes each) comes by plain loads of one element a lane, read ahead of a row's arithmetic and stored behind it.
+template <typename T>
+struct RowInRing {
+  uint32_t bytes;  // of a row
+
+  __host__ __device__ static constexpr int64_t stage_bytes(int64_t row_bytes) { return round_up(row_bytes + 15, 128); }
+
+  __device__ __forceinline__ static uint32_t offset(const T* row) { return static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row) & 15u); }
+  __device__ __forceinline__ uint32_t head(const T* row) const { return min((16u - offset(row)) & 15u, bytes); }
+  // what the bulk copy of a row brings
+  __device__ __forceinline__ uint32_t bulk_bytes(const T* row) const { return (bytes - head(row)) & ~15u; }
+  // by one thread; its bytes are expected by the barrier already
+  __device__ __forceinline__ void fetch(const T* row, uint32_t stage, uint32_t bar) const {
+    const uint32_t h = head(row), n = bulk_bytes(row);
+    if (n > 0) sm100::bulk_load_1d(stage + offset(row) + h, reinterpret_cast<const uint8_t*>(row) + h, n, bar);
+  }
+  // element `*at` of the row is lane's (of sixteen) to bring: eight before the copy, eight behind it
+  __device__ __forceinline__ bool edge(const T* row, int lane, uint32_t* at) const {
+    const uint32_t h = head(row), tail = (bytes - h) & 15u, e = static_cast<uint32_t>(lane & 7) * sizeof(T);
+    *at = ((lane & 8) != 0 ? bytes - tail + e : e) / sizeof(T);
+    return e < ((lane & 8) != 0 ? tail : h);
+  }
+};
+
+// The columns of a thread of a team that takes such rows, in turns of two columns, which are a pair of fp32 numbers in registers: beside one another
+// where rows lie on the boundaries of pairs (kVec = 2), else as far apart as the team is wide.
+template <typename T, int kVec>
+struct Columns {
+  static constexpr int kPairs = 1, kTurn = 2;
+
+  int thread, width, cols;
+
+  __device__ __forceinline__ int column(int turn, int e) const { return kVec == 1 ? thread + (2 * turn + e) * width : 2 * (thread + turn * width) + e; }
+  __device__ __forceinline__ bool has(int turn, int e = 0) const { return column(turn, e) < cols; }
+
+  __device__ __forceinline__ void read(const uint8_t* row, int turn, float2 (&f)[kPairs]) const {
+    const T* const p = reinterpret_cast<const T*>(row) + column(turn, 0);
+    if constexpr (kVec == 1) {
+      f[0] = make_float2(has(turn) ? to_float(p[0]) : 0.0f, has(turn, 1) ? to_float(p[width]) : 0.0f);
+    } else if (has(turn)) {
+      unpack(*reinterpret_cast<const Raw<T, kVec>*>(p), f);
+    } else {
+      f[0] = both(0.0f);
+    }
+  }
+
+  __device__ __forceinline__ void write(T* row, int turn, const float2 (&f)[kPairs]) const {
+    T* const p = row + column(turn, 0);
+    if constexpr (kVec == 1) {
+      if (has(turn)) p[0] = from_float<T>(f[0].x);
+      if (has(turn, 1)) p[width] = from_float<T>(f[0].y);
+    } else if (has(turn)) {
+      store(p, pack<T, kVec>(f));
+    }
+  }
+
+  // parameters as fp32 in shared memory, by all threads of a block
+  __device__ __forceinline__ void share(float* to, const void* from, int64_t at, bool f32, float offset, int t, int threads) const {
+    for (int c = t; c < cols; c += threads) to[c] = offset + param<T>(from, at + c, f32);
+  }
+  // a turn of them; past the row's end any that are there
+  __device__ __forceinline__ void shared_params(const float* from, int turn, float2 (&f)[kPairs]) const {
+    if constexpr (kVec == 2) {
+      f[0] = *reinterpret_cast<const float2*>(from + min(column(turn, 0), cols - 2));
+    } else {
+      f[0] = make_float2(from[min(column(turn, 0), cols - 1)], from[min(column(turn, 1), cols - 1)]);
+    }
+  }
+};
+
+// ---- host side
+template <typename T>
+constexpr int kVecOf = 16 / static_cast<int>(sizeof(T));
+
+bool on_vectors(const void* p, int64_t elements, int size) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && elements * size % 16 == 0;
+}
+bool on_bytes(const void* p, const RowStrides& r, int size, int bytes) {
+  return reinterpret_cast<uintptr_t>(p) % bytes == 0 && r.outer_stride * size % bytes == 0 && r.inner_stride * size % bytes == 0;
+}
+bool on_vectors(const void* p, const RowStrides& r, int size) { return on_bytes(p, r, size, 16); }
+
+bool is_float_code(int dtype) { return dtype == CK_DTYPE_F32 || dtype == CK_DTYPE_F16 || dtype == CK_DTYPE_BF16; }
+
+int check_shapes(const char* op, int dtype, int param_dtype, int64_t rows, int64_t inner, int64_t cols, int64_t groups) {
+  CK_REQUIRE(is_float_code(dtype), "%s: unsupported dtype code %d", op, dtype);
+  CK_REQUIRE(param_dtype == dtype || param_dtype == CK_DTYPE_F32, "%s: parameters are fp32 or of the input's type, got dtype code %d", op, param_dtype);
+  CK_REQUIRE(rows > 0 && cols > 0 && inner > 0 && groups > 0, "%s: empty input [%lld, %lld]", op, (long long)rows, (long long)cols);
+  CK_REQUIRE(rows <= 0x7FFFFF00 && cols <= 0x7FFFFFFF && inner <= rows, "%s: input too large [%lld, %lld]", op, (long long)rows, (long long)cols);
+  CK_REQUIRE(rows % groups == 0, "%s: %lld rows do not form %lld groups", op, (long long)rows, (long long)groups);
+  CK_REQUIRE(groups <= 32767, "%s: %lld groups, at most 32767", op, (long long)groups);
+  return CK_OK;
+}
+
+}  // namespace
+}  // namespace ck

@@ -158,7 +158,7 @@ struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
     const int code = static_cast<int>(held["code"].toInt());
     const int64_t groups = held["groups"].toInt();
     const bool want_weight = has_weight && ctx->needs_input_grad(1), want_bias = has_bias && ctx->needs_input_grad(1 + has_weight);
-    const Rows dy = rows_in_levels(grads[0], 1);
+    const Rows dy = rows_in_levels(grads[0], copy ? 16 : 1);
     const Tensor dx = result(grads[0].sizes(), grads[0].scalar_type(), c.device);
     const ScalarType param = code == 0 ? ScalarType::Float : code == 1 ? ScalarType::Half : ScalarType::BFloat16;
     const std::vector<int64_t> shape = has_weight || has_bias ? held["shape"].toIntVector() : std::vector<int64_t>{};

@@ -102,6 +102,18 @@ def test_affine(ck, dtype, rows, cols):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", [(2000, 1), (2000, 7), (1500, 33), (700, 129), (700, 130), (600, 257), (600, 1001), (500, 3070), (400, 5001), (350, 9754),
+                                       (310, 12287), (300, 12290), (300, 16383)])
+def test_many_rows_off_vectors(ck, dtype, rows, cols):
+    """Rows that do not lie on 16-byte boundaries, in every place of 16 bytes, from one to many of them a team."""
+    x = _made((rows, cols), dtype, 50, 2.0, 0.3)
+    _run(ck, x, _made((cols,), dtype, 51, 0.2, 1.0), _made((cols,), dtype, 52, 0.2))
+    if cols > 8:
+        wide = _made((rows, cols + 3), dtype, 53)
+        _run(ck, wide[:, 1:cols + 1], _made((cols,), torch.float32, 54, 0.2, 1.0), None, dy=_made((rows, cols + 5), dtype, 55)[:, 2:cols + 2])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,cols", [(1, 32), (5, 96), (129, 512), (1003, 1024), (64, 3072), (300, 4096), (17, 12288), (4, 16384), (2, 32768)])
 def test_from_the_mxfp8_copy(ck, dtype, rows, cols):
     x = _made((rows, cols), dtype, 4, 2.0, 0.3)
