@@ -913,20 +913,29 @@ def _aligned(t: torch.Tensor, align: int) -> torch.Tensor:
     return t.clone() if t.data_ptr() % align else t
 
 
-def gelu_mxfp8_forward(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """``(gelu_tanh(x), *quantize_mxfp8(x))`` of a 2-D tensor in one pass."""
+def _gelu_forward(x: torch.Tensor, copy: bool):
     lib = load_library()
     x = _aligned(x, 32)
     rows, cols = x.shape
     assert cols > 0 and cols % 32 == 0, f"num_cols must be divisible by 32, got {cols}"
     y = torch.empty_like(x)
-    codes = torch.empty((rows, cols), device=x.device, dtype=torch.float8_e4m3fn)
-    scales = torch.empty((roundup(rows, 128), roundup(cols // 32, 4)), device=x.device, dtype=torch.float8_e8m0fnu)
+    codes = torch.empty((rows, cols), device=x.device, dtype=torch.float8_e4m3fn) if copy else None
+    scales = torch.empty((roundup(rows, 128), roundup(cols // 32, 4)), device=x.device, dtype=torch.float8_e8m0fnu) if copy else None
     if rows > 0:
         with _on_device(x.device):
-            _check(lib.ck_gelu_mxfp8_forward(x.data_ptr(), DTYPE_TO_CODE[x.dtype], y.data_ptr(), codes.data_ptr(), scales.data_ptr(), rows, cols,
+            _check(lib.ck_gelu_mxfp8_forward(x.data_ptr(), DTYPE_TO_CODE[x.dtype], y.data_ptr(), _ptr(codes), _ptr(scales), rows, cols,
                                              _stream(x.device)), "gelu_mxfp8_forward")
     return y, codes, scales
+
+
+def gelu_mxfp8_forward(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``(gelu_tanh(x), *quantize_mxfp8(x))`` of a 2-D tensor in one pass."""
+    return _gelu_forward(x, True)
+
+
+def gelu_inference(x: torch.Tensor) -> torch.Tensor:
+    """:func:`gelu_mxfp8_forward` for callers that need no copy."""
+    return _gelu_forward(x, False)[0]
 
 
 def gelu_mxfp8_backward(dy: torch.Tensor, codes: torch.Tensor, block_scales: torch.Tensor) -> torch.Tensor:
@@ -1060,13 +1069,15 @@ def _training_constraints(cuda_only, floats, f32, blackwell) -> dict:
     forward = {"x": any_rows, "weight": params, "bias": params}
     backward = {"dy": any_rows, "mean": stats, "rstd": stats, "weight": params}
     copy = {"codes": codes, "block_scales": scales}
+    blocks = {"x": ParamConstraint(dtypes=floats, shape_rules=(ExactDims(2), DivisibleBy(1, 32)))}
     by_name = {
         "layer_norm_forward": forward,
         "layer_norm_inference": forward,
         "layer_norm_forward_mxfp8": forward,
         "layer_norm_backward": {**backward, "x": any_rows},
         "layer_norm_backward_mxfp8": {**backward, **copy},
-        "gelu_mxfp8_forward": {"x": ParamConstraint(dtypes=floats, shape_rules=(ExactDims(2), DivisibleBy(1, 32)))},
+        "gelu_mxfp8_forward": blocks,
+        "gelu_inference": blocks,
         "gelu_mxfp8_backward": {"dy": matrix, **copy},
         "linear_weight_grad_mxfp8": {"dy": matrix, "x_codes": codes, "x_block_scales": scales, "out_dtype": ParamConstraint(dtypes=floats)},
         "linear_input_grad_mxfp8": {"dy": matrix, "w_codes": codes, "w_block_scales": scales, "out_dtype": ParamConstraint(dtypes=floats)},
@@ -1078,7 +1089,7 @@ _constraints: dict = {}  # as registered
 _stock = {name: globals()[name] for name in ("quantize_nvfp4", "quantize_nvfp4_dynamic", "quantize_mxfp8", "dequantize_nvfp4",
                                              "dequantize_mxfp8", "scaled_mm_nvfp4", "scaled_mm_mxfp8", "layer_norm_forward",
                                              "layer_norm_forward_mxfp8", "layer_norm_inference", "layer_norm_backward",
-                                             "layer_norm_backward_mxfp8", "gelu_mxfp8_forward", "gelu_mxfp8_backward",
+                                             "layer_norm_backward_mxfp8", "gelu_mxfp8_forward", "gelu_inference", "gelu_mxfp8_backward",
                                              "linear_weight_grad_mxfp8", "linear_input_grad_mxfp8")}
 
 

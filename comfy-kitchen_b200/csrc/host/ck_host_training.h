@@ -217,18 +217,26 @@ PyObject* layer_norm(PyObject*, Args a, Py_ssize_t n_args) {  // x, weight, bias
   });
 }
 
+Tensor gelu_forward(const Tensor& x, const Call& c, Tensor* codes, Tensor* scales) {  // null: no copy
+  const Tensor from = rows_in_levels(x, 32).t.contiguous();
+  const int64_t cols = x.size(-1), rows = x.numel() / cols;
+  Tensor y = result(x.sizes(), x.scalar_type(), c.device);
+  if (codes != nullptr) {
+    *codes = result({rows, cols}, ScalarType::Float8_e4m3fn, c.device);
+    *scales = result({round_up(rows, 128), round_up(cols / 32, 4)}, ScalarType::Float8_e8m0fnu, c.device);
+  }
+  if (lib.gelu_mxfp8_forward(from.const_data_ptr(), code_of(x.scalar_type()), y.mutable_data_ptr(), codes != nullptr ? codes->mutable_data_ptr() : nullptr,
+                             codes != nullptr ? scales->mutable_data_ptr() : nullptr, rows, cols, c.stream) != 0) {
+    library_error("gelu_mxfp8_forward");
+  }
+  return y;
+}
+
 struct GeluNode : torch::autograd::Function<GeluNode> {
   static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x) {
     const Call c;
-    const Tensor from = rows_in_levels(x, 32).t.contiguous();
-    const int64_t cols = x.size(-1), rows = x.numel() / cols;
-    const Tensor y = result(x.sizes(), x.scalar_type(), c.device);
-    const Tensor codes = result({rows, cols}, ScalarType::Float8_e4m3fn, c.device);
-    const Tensor scales = result({round_up(rows, 128), round_up(cols / 32, 4)}, ScalarType::Float8_e8m0fnu, c.device);
-    if (lib.gelu_mxfp8_forward(from.const_data_ptr(), code_of(x.scalar_type()), y.mutable_data_ptr(), codes.mutable_data_ptr(), scales.mutable_data_ptr(),
-                               rows, cols, c.stream) != 0) {
-      library_error("gelu_mxfp8_forward");
-    }
+    Tensor codes, scales;
+    Tensor y = gelu_forward(x, c, &codes, &scales);
     ctx->save_for_backward({codes, scales});
     return y;
   }
@@ -258,7 +266,7 @@ PyObject* gelu_checkpointed(PyObject*, Args a, Py_ssize_t n_args) {  // x
     Tensor y;
     {
       const WithoutGil released;
-      y = GeluNode::apply(*x);
+      y = c10::GradMode::is_enabled() && x->requires_grad() ? GeluNode::apply(*x) : gelu_forward(*x, c, nullptr, nullptr);
     }
     return THPVariable_Wrap(std::move(y));
   });

@@ -329,7 +329,7 @@ CK_API int ck_layer_norm_backward(const void* dy, int dtype, int64_t rows, int64
 
 /*
  * GELU (tanh form) whose input is kept in MXFP8.  Forward: y = x / 2 * (1 + tanh(sqrt(2/pi) * (x + 0.044715 x^3))) and the copy
- * of x as ck_quantize_mxfp8 writes it.  Backward: dx = dy * gelu'(u) with u the value that stands in the copy.  fp32 arithmetic,
+ * of x as ck_quantize_mxfp8 writes it (null codes and block_scales: no copy).  Backward: dx = dy * gelu'(u) with u the value that stands in the copy.  fp32 arithmetic,
  * one rounding.  [rows, cols] contiguous, cols % 32 == 0; x, y, dy, dx and codes 32-byte aligned, block_scales 4-byte.
  */
 CK_API int ck_gelu_mxfp8_forward(const void* x, int dtype, void* y, void* codes, void* block_scales, int64_t rows,
