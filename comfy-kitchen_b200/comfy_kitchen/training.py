@@ -25,7 +25,7 @@ from torch.autograd.function import once_differentiable
 
 from .ops import _MAY_BE_PENDING, _PLAIN_TYPES, DTYPE_TO_CODE, _impl, dispatcher_adds_nothing, host_operator, host_step, replaced
 from .tensor import QuantizedTensor, TensorCoreMXFP8Layout
-from .tensor.blockwise import quantized_linear
+from .tensor.blockwise import crop
 
 BLOCK = 32  # elements of one scale
 
@@ -215,7 +215,7 @@ def gelu_checkpointed(x: torch.Tensor) -> torch.Tensor:
     shape = x.shape
     x2 = x if len(shape) == 2 else x.reshape(-1, shape[-1])
     if _eager((x2,)) and not any(replaced(name) for name in _GELU_OPERATORS):
-        y = _Gelu.apply(x2)
+        y = _Gelu.apply(x2) if torch.is_grad_enabled() and x2.requires_grad else _impl("gelu_inference", {"x": x2})
     else:
         y = torch.ops.comfy_kitchen.gelu_mxfp8_forward(x2)[0]
     return y if len(shape) == 2 else y.view(shape)
@@ -229,7 +229,8 @@ class _Linear(torch.autograd.Function):
         codes = scales = None
         if ctx.needs_input_grad[1]:
             codes, scales = _call("quantize_mxfp8", {"x": x.contiguous(), "pad_32x": False})
-        ctx.save_for_backward(codes, scales, weight)
+        ctx.save_for_backward(codes, scales, weight if ctx.needs_input_grad[0] else None)
+        ctx.weight_dtype = weight.dtype
         return F.linear(x, weight, bias)
 
     @staticmethod
@@ -239,7 +240,7 @@ class _Linear(torch.autograd.Function):
         dx = dy @ weight if ctx.needs_input_grad[0] else None
         dweight = dbias = None
         if ctx.needs_input_grad[1]:
-            dweight, dbias = linear_weight_grad_mxfp8(dy, codes, scales, weight.dtype, ctx.needs_input_grad[2])
+            dweight, dbias = linear_weight_grad_mxfp8(dy, codes, scales, ctx.weight_dtype, ctx.needs_input_grad[2])
         elif ctx.needs_input_grad[2]:
             dbias = dy.sum(0)
         return dx, dweight, dbias
@@ -250,18 +251,22 @@ class _FrozenLinear(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias):
-        ctx.weight = weight
+        ctx.save_for_backward(weight._qdata, weight._params.scale)
+        ctx.shape = weight._params.orig_shape
+        padded = weight._qdata.shape[0] - ctx.shape[0]  # rows up to the scale block's size
+        if bias is not None and padded:
+            bias = F.pad(bias, (0, padded))
         with torch.no_grad():
-            return quantized_linear(QuantizedTensor.from_float(x.contiguous(), "TensorCoreMXFP8Layout"), weight, bias)
+            y = TensorCoreMXFP8Layout.scaled_mm(QuantizedTensor.from_float(x.contiguous(), "TensorCoreMXFP8Layout"), weight, bias, x.dtype)
+        return crop(y, x.shape[0], ctx.shape[0])
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        weight = ctx.weight
         dx = None
         if ctx.needs_input_grad[0]:
-            rows, cols = weight._params.orig_shape
-            codes, scales = weight._qdata, weight._params.scale
+            codes, scales = ctx.saved_tensors
+            rows, cols = ctx.shape
             padded = dy if codes.shape[0] == rows else F.pad(dy, (0, codes.shape[0] - rows))
             dx = linear_input_grad_mxfp8(padded, codes, scales)
             dx = dx if codes.shape[1] == cols else dx[:, :cols]
@@ -271,24 +276,29 @@ class _FrozenLinear(torch.autograd.Function):
 def linear_checkpointed(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None) -> torch.Tensor:
     """``F.linear(x, weight, bias)`` for training.
 
-    A dense ``weight`` [N, K] (of x's dtype; N a multiple of 8, K of 32): the result is the dense product, and the weight's and the bias's
-    gradients come from an MXFP8 copy of x, which is all that is kept of it.  A ``QuantizedTensor`` in the MXFP8 layout: x is
-    quantized and multiplied as in ``MXFP8Linear``, the weight stays frozen, and the input's gradient is taken through it (the
-    quantization of x passes its gradient on unchanged)."""
+    A dense ``weight`` [N, K] (of x's dtype, or of any under autocast; N a multiple of 8, K of 32): the result is the dense product, and the weight's
+    and the bias's gradients come from an MXFP8 copy of x, which is all that is kept of it.  A ``QuantizedTensor`` in the MXFP8
+    layout: x is quantized and multiplied as in ``MXFP8Linear``, the weight stays frozen, and the input's gradient is taken
+    through it (the quantization of x passes its gradient on unchanged)."""
     shape = x.shape
-    x2 = x if x.dim() == 2 else x.reshape(-1, shape[-1])
-    if isinstance(weight, QuantizedTensor):
-        if weight.layout_cls is not TensorCoreMXFP8Layout or weight._params.transposed:
-            raise ValueError("linear_checkpointed takes a dense weight or one in the MXFP8 layout")
-        n = weight._params.orig_shape[0]
-        y = _FrozenLinear.apply(x2, weight, bias)
-    else:
-        n, k = weight.shape
+    frozen = isinstance(weight, QuantizedTensor)
+    if frozen and (weight.layout_cls is not TensorCoreMXFP8Layout or weight._params.transposed):
+        raise ValueError("linear_checkpointed takes a dense weight or one in the MXFP8 layout")
+    n, k = weight._params.orig_shape if frozen else weight.shape
+    if x.dim() == 0 or shape[-1] != k:
+        raise ValueError(f"the weight is [{n}, {k}], the input {tuple(shape)}")
+    if not frozen:
         if k % BLOCK != 0 or n % 8 != 0:
             raise ValueError(f"an MXFP8 checkpoint needs input features of a multiple of {BLOCK} and output features of 8, got [{n}, {k}]")
+        if x.is_cuda and torch.is_autocast_enabled("cuda"):
+            dtype = torch.get_autocast_dtype("cuda")
+            x, weight, bias = x.to(dtype), weight.to(dtype), bias if bias is None else bias.to(dtype)
         if weight.dtype != x.dtype:
             raise ValueError(f"the weight is {weight.dtype}, the input {x.dtype}")
-        y = _Linear.apply(x2, weight, bias)
+    if not torch.is_grad_enabled() and not frozen:
+        return F.linear(x, weight, bias)
+    x2 = x if x.dim() == 2 else x.reshape(-1, k)
+    y = (_FrozenLinear if frozen else _Linear).apply(x2, weight, bias)
     return y if x.dim() == 2 else y.view(*shape[:-1], n)
 
 
