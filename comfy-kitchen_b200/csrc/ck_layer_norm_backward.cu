@@ -213,8 +213,8 @@ __global__ void __launch_bounds__(512) layer_norm_backward_kernel(const Backward
 
 // The same where rows are long enough to come through shared memory (see the forward pass): a team's rows of dy and of x or its codes are
 // bulk copies into its own ring, a few rows ahead, and what a thread holds of a row is read from there once.
-template <typename T, int kVec, int kNum, bool kCopy>
-__global__ void __launch_bounds__(512) layer_norm_backward_ring_kernel(const BackwardArgs a, const int stages) {
+template <typename T, int kVec, int kNum, int kThreads, bool kCopy, bool kExact>
+__global__ void __launch_bounds__(kThreads) layer_norm_backward_ring_kernel(const BackwardArgs a, const int stages) {
   constexpr int kMaxTeams = 15, kPairs = kVec / 2;
   extern __shared__ __align__(128) uint8_t shared_bytes[];  // factors f, then the teams' rings; the teams' column sums in the end
   __shared__ __align__(8) uint64_t full[kMaxTeams][kMaxRing];
@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(512) layer_norm_backward_ring_kernel(const Bac
   const float inv_cols = 1.0f / static_cast<float>(a.cols);
   const uint32_t dy_bytes = static_cast<uint32_t>(a.cols) * sizeof(T), x_bytes = static_cast<uint32_t>(a.cols) * (kCopy ? 1 : sizeof(T));
   const uint32_t x_at = (dy_bytes + 127) & ~127u, stage_bytes = x_at + ((x_bytes + 127) & ~127u);
-  const uint32_t factor_bytes = a.weight != nullptr ? (static_cast<uint32_t>(a.cols) * 4 + 127) & ~127u : 0u;
+  const uint32_t factor_bytes = (static_cast<uint32_t>(a.cols) * 4 + 127) & ~127u;
   float* const shared_buf = reinterpret_cast<float*>(shared_bytes);
   uint8_t* const ring = shared_bytes + factor_bytes + team * stages * stage_bytes;
   const uint32_t ring_at = sm100::smem_u32(ring), full_at = sm100::smem_u32(full[team]);
@@ -251,25 +251,20 @@ __global__ void __launch_bounds__(512) layer_norm_backward_ring_kernel(const Bac
     }
   }
   pdl_wait();
+  const auto has = [&](int i) { return kExact || static_cast<int>(threadIdx.x) + i * width < vecs; };
+  const auto vec_of = [&](int i) { return kExact ? static_cast<int>(threadIdx.x) + i * width : min(static_cast<int>(threadIdx.x) + i * width, vecs - 1); };
   // factors in shared memory, as above
   constexpr int kPart = 4;
   const int part_stride = vecs * kPart;
-  if (a.weight != nullptr) {
-    for (int v = team * width + threadIdx.x; v < vecs; v += width * teams) {
-      float f[kVec];
-      load_param<T, kVec>(a.weight, group * a.weight_stride + static_cast<int64_t>(v) * kVec, a.params_f32, a.params_aligned, f);
+  for (int v = team * width + threadIdx.x; v < vecs; v += width * teams) {
+    float f[kVec];
+    if (a.weight != nullptr) load_param<T, kVec>(a.weight, group * a.weight_stride + static_cast<int64_t>(v) * kVec, a.params_f32, a.params_aligned, f);
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) shared_buf[j / kPart * part_stride + v * kPart + j % kPart] = a.offset + f[j];
-    }
+    for (int j = 0; j < kVec; ++j) shared_buf[j / kPart * part_stride + v * kPart + j % kPart] = a.weight != nullptr ? a.offset + f[j] : 1.0f;
   }
   __syncthreads();
   const auto factors = [&](int i, float2(&f)[kPairs]) {
-    if (a.weight == nullptr) {
-#pragma unroll
-      for (int j = 0; j < kPairs; ++j) f[j] = both(1.0f);
-      return;
-    }
-    const int v = min(static_cast<int>(threadIdx.x) + i * width, vecs - 1);
+    const int v = vec_of(i);
 #pragma unroll
     for (int q = 0; q < kVec / kPart; ++q) {
       const float4 part = *reinterpret_cast<const float4*>(shared_buf + q * part_stride + v * kPart);
@@ -287,16 +282,19 @@ __global__ void __launch_bounds__(512) layer_norm_backward_ring_kernel(const Bac
   float next_mean = 0.0f, next_rstd = 0.0f;
   uint32_t next_byte[kNum] = {};
   const int64_t quads = ceil_div(a.cols >> 5, 4);
+  const uint8_t* scale_at[kNum];  // in row 0
+  if constexpr (kCopy) {
+#pragma unroll
+    for (int i = 0; i < kNum; ++i) scale_at[i] = a.scales + swizzled_scale_offset(0, vec_of(i) * kVec >> 5, quads);
+  }
   const auto beside = [&](uint32_t r) {
     if (r >= end) return;
     next_mean = a.mean[row0 + r];
     next_rstd = a.rstd[row0 + r];
     if constexpr (kCopy) {
+      const int64_t row_at = swizzled_scale_offset(row0 + r, 0, quads);
 #pragma unroll
-      for (int i = 0; i < kNum; ++i) {
-        const int v = threadIdx.x + i * width;
-        if (v < vecs) next_byte[i] = a.scales[swizzled_scale_offset(row0 + r, v * kVec >> 5, quads)];
-      }
+      for (int i = 0; i < kNum; ++i) next_byte[i] = scale_at[i][row_at];
     }
   };
   beside(begin + team);
@@ -316,9 +314,9 @@ __global__ void __launch_bounds__(512) layer_norm_backward_ring_kernel(const Bac
     float2 s1 = both(0.0f), s2 = both(0.0f);
 #pragma unroll
     for (int i = 0; i < kNum; ++i) {
-      const int v = min(static_cast<int>(threadIdx.x) + i * width, vecs - 1);
+      const int v = vec_of(i);
       Raw<T, kVec> raw = *reinterpret_cast<const Raw<T, kVec>*>(from + v * 16);
-      if (static_cast<int>(threadIdx.x) + i * width >= vecs) raw = zeros<T, kVec>();  // past the row's end: dy = 0, whatever h
+      if (!has(i)) raw = zeros<T, kVec>();  // past the row's end: dy = 0, whatever h
       unpack(raw, d[i]);
       if constexpr (kCopy) {
         const auto codes = *reinterpret_cast<const Raw<uint32_t, kVec / 4>*>(from + x_at + v * kVec);
@@ -369,7 +367,7 @@ __global__ void __launch_bounds__(512) layer_norm_backward_ring_kernel(const Bac
 #pragma unroll
     for (int i = 0; i < kNum; ++i) {
       const int v = threadIdx.x + i * width;
-      if (v < vecs) {
+      if (has(i)) {
         float2 f[kPairs];
         factors(i, f);
 #pragma unroll
@@ -387,43 +385,38 @@ __global__ void __launch_bounds__(512) layer_norm_backward_ring_kernel(const Bac
     return;
   }
   if (a.dweight == nullptr && a.dbias == nullptr) return;
-  const int threads = width * teams, at = team * width + threadIdx.x;
-  const auto put = [&](int j, int v, float s) {  // sum j (of kVec for dw, then of kVec for db) of vector v
-    const int64_t k = static_cast<int64_t>(v) * kVec + j % kVec;
-    if (a.partials != nullptr) {
-      a.partials[(static_cast<int64_t>(blockIdx.x) * 2 + j / kVec) * a.cols + k] = s;
-    } else {
-      void* const to = j < kVec ? a.dweight : a.dbias;
-      if (to != nullptr) store_param<T>(to, group * a.cols + k, a.params_f32, s);
-    }
-  };
+  // The teams' sums of all columns side by side in shared memory, then four columns a thread, added in the teams' order.
+  const int threads = width * teams, at = team * width + threadIdx.x, cols = static_cast<int>(a.cols);
 #pragma unroll
   for (int i = 0; i < kNum; ++i) {
-    const int v = threadIdx.x + i * width;
-    if (teams == 1) {
-      if (v < vecs) {
+    if (!has(i)) continue;
+    float* const to = shared_buf + team * cols + (threadIdx.x + i * width) * kVec;
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) {
-          put(j, v, j % 2 == 0 ? dw[i][j / 2].x : dw[i][j / 2].y);
-          put(kVec + j, v, j % 2 == 0 ? db[i][j / 2].x : db[i][j / 2].y);
-        }
+    for (int j = 0; j < kPairs; j += 2) {
+      *reinterpret_cast<float4*>(to + 2 * j) = make_float4(dw[i][j].x, dw[i][j].y, dw[i][j + 1].x, dw[i][j + 1].y);
+      *reinterpret_cast<float4*>(to + teams * cols + 2 * j) = make_float4(db[i][j].x, db[i][j].y, db[i][j + 1].x, db[i][j + 1].y);
+    }
+  }
+  __syncthreads();
+  for (int which = 0; which < 2; ++which) {
+    void* const result = which == 0 ? a.dweight : a.dbias;
+#pragma unroll 2
+    for (int k = 4 * at; k < cols; k += 4 * threads) {
+      float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (int t = 0; t < teams; ++t) {
+        const float4 f = *reinterpret_cast<const float4*>(shared_buf + (which * teams + t) * cols + k);
+        s.x += f.x;
+        s.y += f.y;
+        s.z += f.z;
+        s.w += f.w;
       }
-      continue;
-    }
-    if (i > 0) __syncthreads();
-#pragma unroll
-    for (int j = 0; j < kPairs; ++j) {
-      shared_buf[(2 * j) * threads + at] = dw[i][j].x;
-      shared_buf[(2 * j + 1) * threads + at] = dw[i][j].y;
-      shared_buf[(kVec + 2 * j) * threads + at] = db[i][j].x;
-      shared_buf[(kVec + 2 * j + 1) * threads + at] = db[i][j].y;
-    }
-    __syncthreads();
-    if (v < vecs) {
-      for (int j = team; j < 2 * kVec; j += teams) {
-        float s = 0.0f;
-        for (int t = 0; t < teams; ++t) s += shared_buf[j * threads + t * width + threadIdx.x];
-        put(j, v, s);
+      if (a.partials != nullptr) {
+        *reinterpret_cast<float4*>(a.partials + (static_cast<int64_t>(blockIdx.x) * 2 + which) * cols + k) = s;
+      } else if (result != nullptr) {
+        store_param<T>(result, group * a.cols + k, a.params_f32, s.x);
+        store_param<T>(result, group * a.cols + k + 1, a.params_f32, s.y);
+        store_param<T>(result, group * a.cols + k + 2, a.params_f32, s.z);
+        store_param<T>(result, group * a.cols + k + 3, a.params_f32, s.w);
       }
     }
   }
@@ -750,30 +743,39 @@ Plan plan_backward(int64_t cols, int size, int vec, bool copy, bool weight, int6
   const bool whole = vec * size == 16;
   const int turn = vec == 1 ? 2 : vec, unit = 8 / turn;  // turns of eight columns
   p.ring = cols >= (whole ? 512 : 129) && !(copy && !whole);
-  p.wide = p.ring ? cols > 512 * (size == 4 || !whole ? 24 : 32) : copy && !whole;
+  p.wide = p.ring ? cols > (!whole ? 512 * 24 : size == 4 ? 256 * 48 : 512 * 32) : copy && !whole;
   int64_t step = 64;
+  int most = 8;
   if (!p.wide) {
     if (p.ring) {
-      // 24 columns a thread, or whole 16-bit vectors up to 32
-      p.warps = static_cast<int>(ceil_div(cols, 32 * 24));
-      if (p.warps > 16) p.warps = 16;
-      p.num = static_cast<int>(ceil_div(cols, 32 * 8 * p.warps)) * unit;
+      if (whole) {
+        p.warps = cols > 256 * 48 ? 16 : static_cast<int>(ceil_div(cols, 32 * 48));
+        if (cols <= 32 * 24 || p.warps > 8) most = 16;
+        const int64_t eights = ceil_div(cols, 32 * 8 * p.warps);
+        p.num = static_cast<int>(eights <= 2 ? 2 : eights <= 4 ? eights : 6) * unit;  // as there are kernels
+      } else {
+        p.warps = static_cast<int>(ceil_div(cols, 32 * 24));
+        p.num = static_cast<int>(ceil_div(cols, 32 * 8 * p.warps)) * unit;
+        most = 16;
+      }
     } else {
       const int64_t vecs = ceil_div(cols, whole ? vec : 1);
       p.warps = 1;
       p.num = static_cast<int>(ceil_div(vecs, 32));
     }
-    p.teams = 16 / p.warps;
+    if (!p.ring) most = 16;
+    p.teams = most / p.warps;
     if (p.teams > 15) p.teams = 15;  // named barriers 1 to 15
     p.rows = !p.ring && p.num <= 2 ? 2 : 1;
     step = static_cast<int64_t>(p.teams) * p.rows;
-    const int64_t sums = 2 * (whole ? vec : 2) * 32 * p.warps * p.teams * 4, factors = weight ? round_up(cols * 4, 128) : 0;
+    const int64_t sums = p.ring && whole ? 2 * p.teams * cols * 4 : 2 * (whole ? vec : 2) * 32 * p.warps * p.teams * 4;
+    const int64_t factors = weight || (p.ring && whole) ? round_up(cols * 4, 128) : 0;
     if (p.ring) {
       const int64_t dy_stage = round_up(cols * size + (whole ? 0 : 15), 128), stage = dy_stage + (copy ? round_up(cols, 128) : dy_stage);
       while (p.teams > 1 && factors + 2 * p.teams * stage > kRingRoom) --p.teams;
       const int64_t stages = (kRingRoom - factors) / (p.teams * stage);
       p.stages = static_cast<int>(stages > kMaxRing ? kMaxRing : stages);
-      p.wide = p.stages < 2;
+      p.wide = p.stages < (whole ? 1 : 2);
       p.smem = static_cast<int>(factors + p.teams * p.stages * stage);
       if (sums > p.smem) p.smem = static_cast<int>(sums);
       step = p.teams;
@@ -798,10 +800,17 @@ int launch_backward_num(const BackwardArgs& a, const Plan& p, cudaStream_t s) {
   return CK_OK;
 }
 
-template <typename T, int kVec, int kNum, bool kCopy>
+template <typename T, int kVec, int kNum, int kThreads, bool kCopy>
 int launch_backward_ring(BackwardArgs a, const Plan& p, cudaStream_t s) {
   if (int rc = gemm_status_word(&a.status)) return rc;
-  auto kernel = layer_norm_backward_ring_kernel<T, kVec, kNum, kCopy>;
+  // Where the columns fill all threads nothing is asked for each vector.  Where a thread reads 48 columns of both dy and x, asking keeps the reads of
+  // later vectors behind the arithmetic of earlier ones, which is worth more (36864 x 3072 bf16: 114 us against 132; from the copy 128 against
+  // 111); 32 columns of each of 512 threads leave no registers for either.
+  constexpr bool kCanFill = kNum * kVec <= 24 || (kThreads == 256 && (kCopy || kNum * kVec <= 32));
+  auto kernel = layer_norm_backward_ring_kernel<T, kVec, kNum, kThreads, kCopy, false>;
+  if constexpr (kCanFill) {
+    if (a.cols == int64_t{32} * p.warps * kNum * kVec) kernel = layer_norm_backward_ring_kernel<T, kVec, kNum, kThreads, kCopy, true>;
+  }
   if (p.smem > 32 * 1024) CK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, p.smem));
   CK_CUDA(launch_pdl(kernel, dim3(a.groups * a.chunks), dim3(32 * p.warps, p.teams), p.smem, s, a, p.stages));
   return CK_OK;
@@ -824,10 +833,13 @@ int launch_backward(const BackwardArgs& a, const Plan& p, cudaStream_t s) {
     if constexpr (!kWhole) {
       return p.num == kUnit ? launch_backward_off_vectors<T, kVec, kUnit>(a, p, s) : launch_backward_off_vectors<T, kVec, 3 * kUnit>(a, p, s);
     } else {
-      if (p.num <= 2 * kUnit) return launch_backward_ring<T, kVec, 2 * kUnit, kCopy>(a, p, s);
-      if (sizeof(T) == 4 || p.num == 3 * kUnit) return launch_backward_ring<T, kVec, 3 * kUnit, kCopy>(a, p, s);
-      if constexpr (sizeof(T) == 2) return launch_backward_ring<T, kVec, 4 * kUnit, kCopy>(a, p, s);
-      return fail(CK_ERR_UNSUPPORTED, "layer_norm_backward: no kernel for %d turns", p.num);
+      if (p.num == 2 * kUnit) return launch_backward_ring<T, kVec, 2 * kUnit, 512, kCopy>(a, p, s);
+      if (p.num == 3 * kUnit) return launch_backward_ring<T, kVec, 3 * kUnit, 512, kCopy>(a, p, s);
+      if constexpr (sizeof(T) == 2) {
+        if (p.warps > 8) return launch_backward_ring<T, kVec, 4 * kUnit, 512, kCopy>(a, p, s);
+      }
+      if (p.num == 4 * kUnit) return launch_backward_ring<T, kVec, 4 * kUnit, 256, kCopy>(a, p, s);
+      return launch_backward_ring<T, kVec, 6 * kUnit, 256, kCopy>(a, p, s);
     }
   }
   if constexpr (kWhole) {  // fewer than 512 columns
@@ -865,7 +877,7 @@ int backward_typed(const BackwardArgs& given, void* workspace, int64_t workspace
   const bool sums = a.dweight != nullptr || a.dbias != nullptr;
   const int64_t need = static_cast<int64_t>(a.groups) * p.chunks * 2 * a.cols * 4;
   if (sums && p.chunks > 1) {
-    CK_REQUIRE(workspace != nullptr && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 4 == 0,
+    CK_REQUIRE(workspace != nullptr && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
                "layer_norm_backward: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
     a.partials = static_cast<float*>(workspace);
   }

@@ -316,7 +316,7 @@ CK_API int ck_layer_norm_forward(const void* x, int dtype, int64_t rows, int64_t
  *   dx = rstd * (g - mean_k(g) - h * mean_k(g * h)),  dweight = sum over a group's rows of dy * h,  dbias = sum of dy
  * h comes from x (rows in two levels, as dy's), or, where x is null, from its MXFP8 copy.  dx: [rows, cols] contiguous of dtype;
  * dweight, dbias: [groups, cols] contiguous of param_dtype, each may be null.  The sums over rows are added in a fixed order.  workspace:
- * device memory, 4-byte aligned, of ck_layer_norm_backward_workspace_bytes bytes (0: none), no requirement on its
+ * device memory, 16-byte aligned, of ck_layer_norm_backward_workspace_bytes bytes (0: none), no requirement on its
  * contents; calls that can overlap on the GPU need separate ones.
  */
 CK_API int64_t ck_layer_norm_backward_workspace_bytes(int64_t rows, int64_t cols, int64_t groups);
