@@ -349,6 +349,150 @@ __global__ void __launch_bounds__(kVec * kNum <= 16 ? 1024 : 512) layer_norm_for
   }
 }
 
+// The same for rows that do not lie on 16-byte boundaries (Columns and RowInRing in ck_layer_norm.cuh), without a copy.
+template <typename T, int kVec, int kNum>
+__global__ void __launch_bounds__(512) layer_norm_forward_off_vectors_kernel(const ForwardArgs a, const uint32_t chunks, const uint32_t chunk_rows,
+                                                                             const int stages) {
+  using Cols = Columns<T, kVec>;
+  using Row = RowInRing<T>;
+  extern __shared__ __align__(128) uint8_t shared_bytes[];  // factors, biases, the teams' rings
+  __shared__ __align__(8) uint64_t full[16][kMaxRing];
+  __shared__ float2 buf[2][16];  // [turn][warp of the block]: mean and squares
+  __shared__ float counts[16];   // elements that a team's warp holds
+  __shared__ int abort_flag;
+  pdl_launch_dependents();
+  const int team = threadIdx.y, teams = blockDim.y, width = blockDim.x, warps = width >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t group = blockIdx.x / chunks, chunk = blockIdx.x - group * chunks;
+  const uint32_t begin = chunk * chunk_rows, end = min(a.rows_per_group, begin + chunk_rows), row0 = group * a.rows_per_group;
+  const Cols own = {static_cast<int>(threadIdx.x), width, static_cast<int>(a.cols)};
+  const Row in = {static_cast<uint32_t>(a.cols) * static_cast<uint32_t>(sizeof(T))};
+  const float inv_cols = 1.0f / static_cast<float>(a.cols);
+  const uint32_t stage_bytes = static_cast<uint32_t>(Row::stage_bytes(in.bytes)), param_bytes = (static_cast<uint32_t>(a.cols) * 4 + 127) & ~127u;
+  float* const factor_buf = reinterpret_cast<float*>(shared_bytes);
+  float* const bias_buf = reinterpret_cast<float*>(shared_bytes + param_bytes);
+  uint8_t* const ring = shared_bytes + 2 * param_bytes + team * stages * stage_bytes;
+  const uint32_t ring_at = sm100::smem_u32(ring), full_at = sm100::smem_u32(full[team]);
+  const auto row_of = [&](uint32_t r) { return static_cast<const T*>(a.x) + a.x_rows.offset(row0 + r); };
+  const auto load_row = [&](uint32_t r, int s) {  // by one thread of the team
+    const T* const row = row_of(r);
+    sm100::mbar_arrive_expect_tx(full_at + s * 8, in.bulk_bytes(row));
+    in.fetch(row, ring_at + s * stage_bytes, full_at + s * 8);
+  };
+  // sixteen lanes of a team's first warp bring what lies beside the copy
+  const auto put_edge = [&](const T* row, int s, uint32_t e, T v) { reinterpret_cast<T*>(ring + s * stage_bytes + Row::offset(row))[e] = v; };
+  float held = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kNum; ++i) held += (own.has(i) ? 1.0f : 0.0f) + (own.has(i, 1) ? 1.0f : 0.0f);
+  held = warp_sum(held);
+  const float inv_held = held > 0.0f ? 1.0f / held : 0.0f;
+  if (team == 0 && lane == 0) counts[warp] = held;
+  if (threadIdx.x == 0) {
+    if (team == 0) abort_flag = 0;
+    for (int s = 0; s < stages; ++s) sm100::mbar_init(&full[team][s], 1);
+    sm100::fence_barrier_init();
+  }
+  pdl_wait();
+  if (warp == 0) {
+    __syncwarp();
+    for (int s = 0; s < stages; ++s) {
+      const uint32_t r = begin + team + s * teams;
+      if (r >= end) break;
+      if (lane == 0) load_row(r, s);
+      const T* const row = row_of(r);
+      uint32_t e;
+      if (lane < 16 && in.edge(row, lane, &e)) put_edge(row, s, e, row[e]);
+    }
+  }
+  for (int c = team * width + threadIdx.x; c < own.cols; c += width * teams) {
+    factor_buf[c] = a.weight != nullptr ? a.offset + param<T>(a.weight, group * a.weight_stride + c, a.params_f32) : 1.0f;
+    bias_buf[c] = a.bias != nullptr ? param<T>(a.bias, group * a.bias_stride + c, a.params_f32) : 0.0f;
+  }
+  __syncthreads();
+  int stage = 0, turn = 0;
+  uint32_t phase = 0;
+  for (uint32_t r = begin + team; r < end; r += teams, turn ^= 1) {
+    const uint32_t next = r + stages * teams;  // the row that comes into this one's stage
+    T edge = from_float<T>(0.0f);
+    uint32_t edge_at = 0;
+    bool has_edge = false;
+    if (warp == 0 && lane < 16 && next < end) {
+      const T* const row = row_of(next);
+      has_edge = in.edge(row, lane, &edge_at);
+      if (has_edge) edge = row[edge_at];
+    }
+    if (!sm100::mbar_wait(full_at + stage * 8, phase, &abort_flag)) break;
+    const uint8_t* const from = ring + stage * stage_bytes + Row::offset(row_of(r));
+    float2 f[kNum];
+    float2 sum[2] = {both(0.0f), both(0.0f)};
+    Cols at = own.again();
+#pragma unroll
+    for (int i = 0; i < kNum; ++i) {
+      float2 v[1];
+      at.read(from, i, v);  // zeros past the row's end
+      f[i] = v[0];
+      sum[i & 1] = add_x2(sum[i & 1], f[i]);
+    }
+    sum[0] = add_x2(sum[0], sum[1]);
+    const float mine = warp_sum(sum[0].x + sum[0].y) * inv_held;
+    float2 square[2] = {both(0.0f), both(0.0f)};
+    at = own.again();
+#pragma unroll
+    for (int i = 0; i < kNum; ++i) {
+      const float2 d = add_x2(f[i], make_float2(at.has(i) ? -mine : 0.0f, at.has(i, 1) ? -mine : 0.0f));
+      square[i & 1] = fma_x2(d, d, square[i & 1]);
+    }
+    square[0] = add_x2(square[0], square[1]);
+    float mean = mine, squares = warp_sum(square[0].x + square[0].y);
+    if (warps > 1) {
+      float2* const slots = buf[turn] + team * warps;
+      if (lane == 0) slots[warp] = make_float2(mine, squares);
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(width) : "memory");
+      mean = 0.0f;
+      for (int w = 0; w < warps; ++w) mean = fmaf(slots[w].x, counts[w], mean);
+      mean *= inv_cols;
+      squares = 0.0f;
+      for (int w = 0; w < warps; ++w) {
+        const float d = slots[w].x - mean;
+        squares += fmaf(d * d, counts[w], slots[w].y);
+      }
+    } else {
+      __syncwarp();
+    }
+    const float rstd = inverse_root(squares * inv_cols + a.eps);
+    const uint32_t row = row0 + r;
+    if (threadIdx.x == 0) {
+      if (next < end) load_row(next, stage);  // all have read the stage
+      if (a.mean != nullptr) {
+        a.mean[row] = mean;
+        a.rstd[row] = rstd;
+      }
+    }
+    if (has_edge) put_edge(row_of(next), stage, edge_at, edge);  // read behind the team's next meeting
+    if (++stage == stages) {
+      stage = 0;
+      phase ^= 1u;
+    }
+    T* const y = static_cast<T*>(a.y) + static_cast<int64_t>(row) * a.cols;
+    at = own.again();
+    const float2 scale = both(rstd), shift = both(sizeof(T) == 2 ? -mean * rstd : -mean);
+#pragma unroll
+    for (int i = 0; i < kNum; ++i) {
+      if (!at.has(i)) continue;
+      // as in the kernel for whole vectors
+      float2 v[1] = {sizeof(T) == 2 ? fma_x2(f[i], scale, shift) : mul_x2(add_x2(f[i], shift), scale)};
+      float2 w[1], b[1];
+      at.shared_params(factor_buf, i, w);
+      at.shared_params(bias_buf, i, b);
+      v[0] = fma_x2(v[0], w[0], b[0]);
+      at.write(y, i, v);
+    }
+  }
+  if (abort_flag) {
+    if (threadIdx.x == 0 && team == 0) atomicExch(a.status, 1);
+    for (int i = 0; i < 200; ++i) __nanosleep(1000);  // copies that are in flight land before the memory is released
+  }
+}
+
 // Rows of any width and alignment, which do not stay in registers: a block goes over its row three times, the second and third out of L1.
 template <typename T, int kVec>
 __global__ void __launch_bounds__(512) layer_norm_forward_wide_kernel(const ForwardArgs a) {
@@ -414,13 +558,13 @@ struct RingPlan {
 
 // A block of up to 16 warps an SM, or of 32 with a short row each.  A row's warps: as few as hold it, and as many more as the rows leave idle: those that
 // fit into the ring, or those that an SM gets.
-RingPlan plan_ring(int64_t rows, int64_t cols, int64_t size) {
+RingPlan plan_ring(int64_t rows, int64_t cols, int64_t size, bool whole) {
   constexpr int64_t kRoom = 216 * 1024;
-  const int64_t stage = round_up(cols * size, 128), params = 2 * round_up(cols * 4, 128), columns = 16 / size * 32;
+  const int64_t stage = round_up(cols * size + (whole ? 0 : 15), 128), params = 2 * round_up(cols * 4, 128), columns = 16 / size * 32;
   RingPlan p = {};
   p.warps = static_cast<int>(ceil_div(cols, 32 * 96));
   if (p.warps > 16 || params + 2 * stage > kRoom) return p;
-  int64_t teams = cols <= 512 ? 32 : 16 / p.warps;
+  int64_t teams = cols <= 512 && whole ? 32 : 16 / p.warps;
   if (teams > (kRoom - params) / (2 * stage)) teams = (kRoom - params) / (2 * stage);
   if (teams > ceil_div(rows, sm_count())) teams = ceil_div(rows, sm_count());
   int64_t warps = teams > 16 ? 1 : 16 / teams;
@@ -433,8 +577,7 @@ RingPlan plan_ring(int64_t rows, int64_t cols, int64_t size) {
   return p;
 }
 
-template <typename T, int kVec, int kNum, bool kCopy>
-int launch_forward_ring_num(ForwardArgs a, const RingPlan& p, cudaStream_t s) {
+int launch_ring(void (*kernel)(ForwardArgs, uint32_t, uint32_t, int), ForwardArgs a, const RingPlan& p, cudaStream_t s) {
   // one block an SM, and no block with less than a row for each team
   const int64_t groups = a.rows / a.rows_per_group;
   int64_t chunks = sm_count() / groups;
@@ -442,13 +585,17 @@ int launch_forward_ring_num(ForwardArgs a, const RingPlan& p, cudaStream_t s) {
   if (chunks < 1) chunks = 1;
   const uint32_t chunk_rows = static_cast<uint32_t>(ceil_div(a.rows_per_group, chunks));
   chunks = ceil_div(a.rows_per_group, chunk_rows);
-  const bool exact = a.cols == int64_t{32} * p.warps * kNum * kVec;
-  auto kernel = exact ? layer_norm_forward_ring_kernel<T, kVec, kNum, kCopy, true> : layer_norm_forward_ring_kernel<T, kVec, kNum, kCopy, false>;
   CK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, p.smem));
   if (int rc = gemm_status_word(&a.status)) return rc;
   CK_CUDA(launch_pdl(kernel, dim3(static_cast<unsigned>(groups * chunks)), dim3(32 * p.warps, p.teams), p.smem, s, a, static_cast<uint32_t>(chunks),
                      chunk_rows, p.stages));
   return CK_OK;
+}
+
+template <typename T, int kVec, int kNum, bool kCopy>
+int launch_forward_ring_num(const ForwardArgs& a, const RingPlan& p, cudaStream_t s) {
+  const bool exact = a.cols == int64_t{32} * p.warps * kNum * kVec;
+  return launch_ring(exact ? layer_norm_forward_ring_kernel<T, kVec, kNum, kCopy, true> : layer_norm_forward_ring_kernel<T, kVec, kNum, kCopy, false>, a, p, s);
 }
 
 template <typename T, int kVec, bool kCopy>
@@ -470,7 +617,7 @@ int launch_forward(const ForwardArgs& a, cudaStream_t s) {
   if constexpr (kVec * sizeof(T) == 16) {
     // (30000 x 256 bf16 with a copy, which gives eight lanes of a warp work: 19.2 us against 15.5; without one 11.8 against 12.4)
     if (a.rows > 2 * sm_count() && a.rows_per_group >= 16 && reinterpret_cast<uintptr_t>(a.codes) % 32 == 0 && (!kCopy || a.cols > 256)) {
-      const RingPlan p = plan_ring(a.rows, a.cols, sizeof(T));
+      const RingPlan p = plan_ring(a.rows, a.cols, sizeof(T), true);
       if (p.smem > 0 && a.rows / a.rows_per_group <= 2 * sm_count()) return launch_forward_ring<T, kVec, kCopy>(a, p, s);
     }
   }
@@ -506,11 +653,23 @@ int forward_typed(const ForwardArgs& given, cudaStream_t s) {
     return launch_forward<T, kVec, true>(a, s);
   }
   if (vectors && a.cols <= int64_t{32} * 32 * 8 * kVec) return launch_forward<T, kVec, false>(a, s);
-  // Rows in registers need a wide block from a few thousand columns of a few bytes on, of which an SM holds one: with many such rows three ways over them
-  // are faster.  9036 x 9754 bf16: 211 us against 373, 9000 x 4097 fp32 133 against 155, but 36864 x 3070 bf16 461 against 257.
-  const bool wide = a.cols > 4096 && a.rows > 2 * sm_count();
-  if (!wide && !vectors && pairs && a.cols <= 2 * 32 * 32 * 8) return launch_forward<T, 2, false>(a, s);
-  if (!wide && !vectors && a.cols <= 32 * 32 * 8) return launch_forward<T, 1, false>(a, s);
+  if (!vectors) {
+    if (a.rows > 2 * sm_count() && a.rows_per_group >= 16 && a.cols > 384 && a.rows / a.rows_per_group <= 2 * sm_count()) {
+      const RingPlan p = plan_ring(a.rows, a.cols, sizeof(T), false);
+      if (p.smem > 0) {
+        const auto by_num = [&](auto vec) {
+          constexpr int kV = decltype(vec)::value;
+          const int64_t num = ceil_div(a.cols, 64 * p.warps);  // pairs
+          return launch_ring(num <= 16 ? layer_norm_forward_off_vectors_kernel<T, kV, 16>
+                                       : num <= 32 ? layer_norm_forward_off_vectors_kernel<T, kV, 32> : layer_norm_forward_off_vectors_kernel<T, kV, 48>,
+                             a, p, s);
+        };
+        return pairs ? by_num(std::integral_constant<int, 2>()) : by_num(std::integral_constant<int, 1>());
+      }
+    }
+    if (pairs && a.cols <= 2 * 32 * 32 * 8) return launch_forward<T, 2, false>(a, s);
+    if (a.cols <= 32 * 32 * 8) return launch_forward<T, 1, false>(a, s);
+  }
   auto kernel = vectors ? layer_norm_forward_wide_kernel<T, kVec> : pairs ? layer_norm_forward_wide_kernel<T, 2> : layer_norm_forward_wide_kernel<T, 1>;
   const int64_t vecs = a.cols / (vectors ? kVec : pairs ? 2 : 1);
   const unsigned threads = vecs >= 512 ? 512 : static_cast<unsigned>(round_up(vecs, 32));

@@ -119,17 +119,23 @@ struct Columns {
 
   int thread, width, cols;
 
+  // The same, computed again: what a pass over a row knows of its columns' places and ends is not kept in registers for the next one.
+  __device__ __forceinline__ Columns again() const {
+    Columns c = *this;
+    asm volatile("" : "+r"(c.thread), "+r"(c.width), "+r"(c.cols));
+    return c;
+  }
+
   __device__ __forceinline__ int column(int turn, int e) const { return kVec == 1 ? thread + (2 * turn + e) * width : 2 * (thread + turn * width) + e; }
   __device__ __forceinline__ bool has(int turn, int e = 0) const { return column(turn, e) < cols; }
 
   __device__ __forceinline__ void read(const uint8_t* row, int turn, float2 (&f)[kPairs]) const {
-    const T* const p = reinterpret_cast<const T*>(row) + column(turn, 0);
     if constexpr (kVec == 1) {
+      const T* const p = reinterpret_cast<const T*>(row) + column(turn, 0);
       f[0] = make_float2(has(turn) ? to_float(p[0]) : 0.0f, has(turn, 1) ? to_float(p[width]) : 0.0f);
-    } else if (has(turn)) {
-      unpack(*reinterpret_cast<const Raw<T, kVec>*>(p), f);
-    } else {
-      f[0] = both(0.0f);
+    } else {  // no branch: a place of the row, or zeros for what was there
+      unpack(*reinterpret_cast<const Raw<T, kVec>*>(reinterpret_cast<const T*>(row) + min(column(turn, 0), cols - 2)), f);
+      if (!has(turn)) f[0] = both(0.0f);
     }
   }
 

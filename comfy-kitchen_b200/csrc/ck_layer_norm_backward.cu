@@ -423,8 +423,8 @@ __global__ void __launch_bounds__(kThreads) layer_norm_backward_ring_kernel(cons
 }
 
 // The same for rows that do not lie on 16-byte boundaries (Columns and RowInRing in ck_layer_norm.cuh).
-template <typename T, int kVec, int kNum>
-__global__ void __launch_bounds__(512) layer_norm_backward_off_vectors_kernel(const BackwardArgs a, const int stages) {
+template <typename T, int kVec, int kNum, int kThreads>
+__global__ void __launch_bounds__(kThreads) layer_norm_backward_off_vectors_kernel(const BackwardArgs a, const int stages) {
   using Cols = Columns<T, kVec>;
   using Row = RowInRing<T>;
   constexpr int kMaxTeams = 15, kPairs = Cols::kPairs, kTurn = Cols::kTurn;
@@ -480,9 +480,10 @@ __global__ void __launch_bounds__(512) layer_norm_backward_off_vectors_kernel(co
     own.share(shared_buf, a.weight, group * a.weight_stride, a.params_f32, a.offset, team * width + threadIdx.x, width * teams);
   }
   __syncthreads();
+  Cols at = own;
   const auto factors = [&](int i, float2(&f)[kPairs]) {
     if (a.weight != nullptr) {
-      own.shared_params(shared_buf, i, f);
+      at.shared_params(shared_buf, i, f);
     } else {
 #pragma unroll
       for (int j = 0; j < kPairs; ++j) f[j] = both(1.0f);
@@ -524,10 +525,11 @@ __global__ void __launch_bounds__(512) layer_norm_backward_off_vectors_kernel(co
     float2 d[kNum][kPairs], h[kNum][kPairs];
     const float2 rstd2 = both(rstd), shift = both(sizeof(T) == 2 ? -mean * rstd : -mean);
     float2 s1 = both(0.0f), s2 = both(0.0f);
+    at = own.again();
 #pragma unroll
     for (int i = 0; i < kNum; ++i) {
-      own.read(dy_from, i, d[i]);  // past the row's end: dy = 0, and h something finite
-      own.read(x_from, i, h[i]);
+      at.read(dy_from, i, d[i]);  // past the row's end: dy = 0, and h something finite
+      at.read(x_from, i, h[i]);
       float2 f[kPairs];
       factors(i, f);
 #pragma unroll
@@ -566,16 +568,17 @@ __global__ void __launch_bounds__(512) layer_norm_backward_off_vectors_kernel(co
       phase ^= 1u;
     }
     T* const dx = static_cast<T*>(a.dx) + static_cast<int64_t>(row0 + r) * a.cols;
+    at = own.again();
 #pragma unroll
     for (int i = 0; i < kNum; ++i) {
-      if (!own.has(i)) continue;
+      if (!at.has(i)) continue;
       float2 f[kPairs];
       factors(i, f);
 #pragma unroll
       for (int j = 0; j < kPairs; ++j) {
         d[i][j] = mul_x2(fma_x2(h[i][j], both(-c2), fma_x2(d[i][j], f[j], both(-c1))), rstd2);
       }
-      own.write(dx, i, d[i]);
+      at.write(dx, i, d[i]);
     }
   }
   __syncthreads();  // the ring is the column sums' now
@@ -585,42 +588,30 @@ __global__ void __launch_bounds__(512) layer_norm_backward_off_vectors_kernel(co
     return;
   }
   if (a.dweight == nullptr && a.dbias == nullptr) return;
-  const int threads = width * teams, at = team * width + threadIdx.x;
-  const auto put = [&](int i, int e, float s) {  // sum e of turn i: of kTurn for dw, then of kTurn for db
-    if (!own.has(i, e % kTurn)) return;
-    const int64_t k = own.column(i, e % kTurn);
-    if (a.partials != nullptr) {
-      a.partials[(static_cast<int64_t>(blockIdx.x) * 2 + e / kTurn) * a.cols + k] = s;
-    } else {
-      void* const to = e < kTurn ? a.dweight : a.dbias;
-      if (to != nullptr) store_param<T>(to, group * a.cols + k, a.params_f32, s);
-    }
-  };
+  const int threads = width * teams, place = team * width + threadIdx.x, cols = own.cols;  // as in the kernel for whole vectors
+  at = own.again();
 #pragma unroll
   for (int i = 0; i < kNum; ++i) {
-    if (teams == 1) {
 #pragma unroll
-      for (int j = 0; j < kPairs; ++j) {
-        put(i, 2 * j, dw[i][j].x);
-        put(i, 2 * j + 1, dw[i][j].y);
-        put(i, kTurn + 2 * j, db[i][j].x);
-        put(i, kTurn + 2 * j + 1, db[i][j].y);
-      }
-      continue;
+    for (int e = 0; e < kTurn; ++e) {
+      if (!at.has(i, e)) continue;
+      float* const to = shared_buf + team * cols + at.column(i, e);
+      to[0] = e == 0 ? dw[i][0].x : dw[i][0].y;
+      to[teams * cols] = e == 0 ? db[i][0].x : db[i][0].y;
     }
-    if (i > 0) __syncthreads();
-#pragma unroll
-    for (int j = 0; j < kPairs; ++j) {
-      shared_buf[(2 * j) * threads + at] = dw[i][j].x;
-      shared_buf[(2 * j + 1) * threads + at] = dw[i][j].y;
-      shared_buf[(kTurn + 2 * j) * threads + at] = db[i][j].x;
-      shared_buf[(kTurn + 2 * j + 1) * threads + at] = db[i][j].y;
-    }
-    __syncthreads();
-    for (int e = team; e < 2 * kTurn; e += teams) {
+  }
+  __syncthreads();
+  for (int which = 0; which < 2; ++which) {
+    void* const result = which == 0 ? a.dweight : a.dbias;
+#pragma unroll 4
+    for (int k = place; k < cols; k += threads) {
       float s = 0.0f;
-      for (int t = 0; t < teams; ++t) s += shared_buf[e * threads + t * width + threadIdx.x];
-      put(i, e, s);
+      for (int t = 0; t < teams; ++t) s += shared_buf[(which * teams + t) * cols + k];
+      if (a.partials != nullptr) {
+        a.partials[(static_cast<int64_t>(blockIdx.x) * 2 + which) * cols + k] = s;
+      } else if (result != nullptr) {
+        store_param<T>(result, group * a.cols + k, a.params_f32, s);
+      }
     }
   }
 }
@@ -743,20 +734,19 @@ Plan plan_backward(int64_t cols, int size, int vec, bool copy, bool weight, int6
   const bool whole = vec * size == 16;
   const int turn = vec == 1 ? 2 : vec, unit = 8 / turn;  // turns of eight columns
   p.ring = cols >= (whole ? 512 : 129) && !(copy && !whole);
-  p.wide = p.ring ? cols > (!whole ? 512 * 24 : size == 4 ? 256 * 48 : 512 * 32) : copy && !whole;
+  p.wide = p.ring ? cols > (whole && size == 2 ? 512 * 32 : 256 * 48) : copy && !whole;
   int64_t step = 64;
   int most = 8;
   if (!p.wide) {
     if (p.ring) {
+      // 24 columns a thread of 512, beyond that 48 a thread of 256; whole 16-bit vectors of the widest rows 32 of 512
+      p.warps = whole && cols > 256 * 48 ? 16 : static_cast<int>(ceil_div(cols, 32 * 48));
+      if (cols <= 32 * 24 || p.warps > 8) most = 16;
+      const int64_t eights = ceil_div(cols, 32 * 8 * p.warps);
       if (whole) {
-        p.warps = cols > 256 * 48 ? 16 : static_cast<int>(ceil_div(cols, 32 * 48));
-        if (cols <= 32 * 24 || p.warps > 8) most = 16;
-        const int64_t eights = ceil_div(cols, 32 * 8 * p.warps);
         p.num = static_cast<int>(eights <= 2 ? 2 : eights <= 4 ? eights : 6) * unit;  // as there are kernels
       } else {
-        p.warps = static_cast<int>(ceil_div(cols, 32 * 24));
-        p.num = static_cast<int>(ceil_div(cols, 32 * 8 * p.warps)) * unit;
-        most = 16;
+        p.num = eights <= 1 ? 4 : eights <= 3 ? 12 : 24;  // pairs
       }
     } else {
       const int64_t vecs = ceil_div(cols, whole ? vec : 1);
@@ -768,7 +758,7 @@ Plan plan_backward(int64_t cols, int size, int vec, bool copy, bool weight, int6
     if (p.teams > 15) p.teams = 15;  // named barriers 1 to 15
     p.rows = !p.ring && p.num <= 2 ? 2 : 1;
     step = static_cast<int64_t>(p.teams) * p.rows;
-    const int64_t sums = p.ring && whole ? 2 * p.teams * cols * 4 : 2 * (whole ? vec : 2) * 32 * p.warps * p.teams * 4;
+    const int64_t sums = p.ring ? 2 * p.teams * cols * 4 : 2 * (whole ? vec : 2) * 32 * p.warps * p.teams * 4;
     const int64_t factors = weight || (p.ring && whole) ? round_up(cols * 4, 128) : 0;
     if (p.ring) {
       const int64_t dy_stage = round_up(cols * size + (whole ? 0 : 15), 128), stage = dy_stage + (copy ? round_up(cols, 128) : dy_stage);
@@ -816,10 +806,10 @@ int launch_backward_ring(BackwardArgs a, const Plan& p, cudaStream_t s) {
   return CK_OK;
 }
 
-template <typename T, int kVec, int kNum>
+template <typename T, int kVec, int kNum, int kThreads>
 int launch_backward_off_vectors(BackwardArgs a, const Plan& p, cudaStream_t s) {
   if (int rc = gemm_status_word(&a.status)) return rc;
-  auto kernel = layer_norm_backward_off_vectors_kernel<T, kVec, kNum>;
+  auto kernel = layer_norm_backward_off_vectors_kernel<T, kVec, kNum, kThreads>;
   if (p.smem > 32 * 1024) CK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, p.smem));
   CK_CUDA(launch_pdl(kernel, dim3(a.groups * a.chunks), dim3(32 * p.warps, p.teams), p.smem, s, a, p.stages));
   return CK_OK;
@@ -831,7 +821,9 @@ int launch_backward(const BackwardArgs& a, const Plan& p, cudaStream_t s) {
   constexpr int kUnit = kVec == 1 ? 4 : 8 / kVec;  // turns of eight columns
   if (p.ring) {
     if constexpr (!kWhole) {
-      return p.num == kUnit ? launch_backward_off_vectors<T, kVec, kUnit>(a, p, s) : launch_backward_off_vectors<T, kVec, 3 * kUnit>(a, p, s);
+      if (p.num == 4) return launch_backward_off_vectors<T, kVec, 4, 512>(a, p, s);
+      if (p.num == 12) return launch_backward_off_vectors<T, kVec, 12, 512>(a, p, s);
+      return launch_backward_off_vectors<T, kVec, 24, 256>(a, p, s);
     } else {
       if (p.num == 2 * kUnit) return launch_backward_ring<T, kVec, 2 * kUnit, 512, kCopy>(a, p, s);
       if (p.num == 3 * kUnit) return launch_backward_ring<T, kVec, 3 * kUnit, 512, kCopy>(a, p, s);
