@@ -1,7 +1,7 @@
 // A linear layer's input gradient through its MXFP8 weight for few rows, sm_100a:  dX[M, K] = dY[M, N] . W[N, K].
 //
 // Bound by the weight's bytes (N K 33/32): the 38.9 MB of a 12288 x 3072 weight take 5.9 us at the copy rate.  The GEMM of ck_grad_gemm.cu would
-// have the weight written as bf16 first and read that back (17 + 24 us for 8 rows; 20 here, 22.6 for 128 rows).  Here the weight is decoded on its way into the operand: a CTA takes
+// have the weight written as bf16 first and read that back (17 + 24 us for 8 rows; 20.6 here, 23.3 for 128 rows).  Here the weight is decoded on its way into the operand: a CTA takes
 // 128 columns of W and a range of its rows; codes and scales of 64 rows at a time come by TMA, sixteen warps decode them (exactly, to
 // bf16) and write them to shared memory as an MN-major operand, the columns of W being the MMA's 128 rows; dY comes by TMA as the
 // other operand, its rows being the MMA's columns (16 to 208 of them); one thread issues the MMAs.  Decoding has no
@@ -26,7 +26,7 @@ constexpr int kThreads = 32 * (kCodeWarps + 2);  // beside them the loads of dY 
 constexpr int kHeldBytes = kDeep * kCols * 2;    // of a stage
 constexpr int kBoxBytes = kDeep * 128;           // 64 columns of it
 // Four groups of warps decode stages in turn: a stage is a chain of waits, conversions, stores and a fence, which sixteen warps at one stage
-// ran through in step (28 us for 8 rows of 12288 x 3072, now 20; codes read into registers ahead of their use, 24 whether 5, 8 or 12 stages ahead).
+// ran through in step (28 us for 8 rows of 12288 x 3072, in turn 20; codes read into registers ahead of their use, 24 whether 5, 8 or 12 stages ahead).
 constexpr int kGroups = 4, kGroupWarps = kCodeWarps / kGroups;
 // The operands' stages, at least four: a group's wait for its stage to be free goes by the parity of the phase, and what it has waited for
 // before must leave no doubt which phase that is.  At its step j it knows that the MMAs of step j - 4 - stages are done (its step before
@@ -47,6 +47,7 @@ struct FewRowsArgs {
   int M, N, K;
   int padded;  // M as a multiple of 16
   int planes;  // bf16 numbers whose sum is an element of dY
+  int parts;   // accumulators that the first of them take in turn; the others have one each, in front of these
   int stages, raw_stages;
   int steps_per_split;  // of 64 rows of W
   int* status;          // for waits that give up (ck_gemm_status)
@@ -99,8 +100,9 @@ grad_few_rows_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_co
   const int split = blockIdx.x, splits = gridDim.x, strip = blockIdx.y;
   const int steps = (a.N + kDeep - 1) / kDeep, first = split * a.steps_per_split, last = min(steps, first + a.steps_per_split);
   const int plane_bytes = a.padded * 128, stage_bytes = kHeldBytes + a.planes * plane_bytes;
+  const int minor = a.planes - 1, accumulators = minor + min(a.parts, last - first);
   uint32_t tmem_cols = 32;
-  while (static_cast<int>(tmem_cols) < a.padded) tmem_cols *= 2;
+  while (static_cast<int>(tmem_cols) < (minor + a.parts) * a.padded) tmem_cols *= 2;
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int s = 0; s < a.stages; ++s) {
@@ -182,16 +184,21 @@ grad_few_rows_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_co
     const int quarter = warp & 3, k = strip * kCols + quarter * 32 + lane;
     float* const sums = reinterpret_cast<float*>(smem);  // [padded][kCols], where a cluster adds
     for (int m0 = (warp >> 2) * 16; m0 < a.padded; m0 += kCodeWarps * 4) {
-      uint32_t v[16];
-      tmem_load_32x16(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + m0, v);
-      tmem_load_wait();
+      float f[16] = {};
+      for (int n = 0; n < accumulators; ++n) {
+        uint32_t v[16];
+        tmem_load_32x16(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + n * a.padded + m0, v);
+        tmem_load_wait();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) f[i] += __uint_as_float(v[i]);
+      }
       if (splits > 1) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sums[(m0 + i) * kCols + quarter * 32 + lane] = __uint_as_float(v[i]);
+        for (int i = 0; i < 16; ++i) sums[(m0 + i) * kCols + quarter * 32 + lane] = f[i];
       } else if (k < a.K) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          if (m0 + i < a.M) store_result(a, static_cast<int64_t>(m0 + i) * a.K + k, __uint_as_float(v[i]));
+          if (m0 + i < a.M) store_result(a, static_cast<int64_t>(m0 + i) * a.K + k, f[i]);
         }
       }
       __syncwarp();
@@ -239,7 +246,7 @@ grad_few_rows_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_co
     if (elect_one()) {
       // kind::f16: bf16 operands, fp32 sums, A (W's columns) MN-major in boxes of 64 columns, B (dY's rows) K-major
       const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (static_cast<uint32_t>(a.padded >> 3) << 17) | ((kCols >> 4) << 24);
-      int stage = 0;
+      int stage = 0, part = 0;
       uint32_t phase = 0;
       for (int step = first; step < last; ++step) {
         mbar_wait(full + stage * 8, phase, &abort_flag);
@@ -247,13 +254,16 @@ grad_few_rows_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_co
         const uint32_t at = smem_u32(smem) + stage * stage_bytes;
         const uint64_t held = make_smem_desc(at, kBoxBytes, 1024, 2);
         for (int p = 0; p < a.planes; ++p) {
+          const uint32_t to = tmem + (p == 0 ? (minor + part) * a.padded : (minor - p) * a.padded);  // the smallest in front
+          const bool begins = step == first + (p == 0 ? part : 0);
           const uint64_t dy = make_operand_desc_sw128(at + kHeldBytes + p * plane_bytes);
 #pragma unroll
           for (int i = 0; i < kDeep / 16; ++i) {  // 16 rows of 128 bytes, 32 bytes
-            mma_bf16(tmem, held + i * (2048 >> 4), dy + i * (32 >> 4), idesc, step != first || p != 0 || i != 0);
+            mma_bf16(to, held + i * (2048 >> 4), dy + i * (32 >> 4), idesc, !begins || i != 0);
           }
         }
         tc_commit<1>(empty + stage * 8);
+        if (++part == a.parts) part = 0;
         if (++stage == a.stages) {
           stage = 0;
           phase ^= 1u;
@@ -365,6 +375,11 @@ int grad_few_rows(const void* dy, int planes, const void* codes, const void* sca
   a.K = static_cast<int>(K);
   a.padded = static_cast<int>(round_up(M, 16));
   a.planes = planes;
+  // An accumulator cuts what it adds to its own magnitude.  So the second and third numbers of dY's elements have their own, and for a result in fp32 four
+  // take the first numbers in turn: 9 rows of fp32 through 6208 x 2624 were off by 3.1e-6 of the result with one for all.
+  a.parts = 512 / a.padded - (planes - 1);
+  if (a.parts > (out_dtype == CK_DTYPE_F32 ? 4 : 1)) a.parts = out_dtype == CK_DTYPE_F32 ? 4 : 1;
+  CK_REQUIRE(a.parts >= 1, "linear_input_grad_mxfp8: %d accumulators", a.parts);
   const int stage = kHeldBytes + planes * a.padded * 128, steps = static_cast<int>(ceil_div(N, kDeep)), strips = static_cast<int>(ceil_div(K, kCols));
   a.raw_stages = (kSmem - 1024 - kMaxRaw * kRawBytes) / stage >= kMinStages ? kMaxRaw : kGroups;
   a.stages = (kSmem - 1024 - a.raw_stages * kRawBytes) / stage;

@@ -147,7 +147,8 @@ grad_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         const int m0 = tile_m * kPairRows + static_cast<int>(rank) * 128, n0 = tile_n * kPairCols + static_cast<int>(rank) * 128;
         const int end = min(all_stages, (split + 1) * p.stages_per_split);
         for (int ks = split * p.stages_per_split; ks < end; ++ks) {
-          const int plane = ks / p.deep_stages, l0 = (ks - plane * p.deep_stages) * kDeep;
+          // dY's smallest numbers first: what an accumulator adds is cut to the magnitude that it has reached
+          const int behind = ks / p.deep_stages, plane = p.planes - 1 - behind, l0 = (ks - behind * p.deep_stages) * kDeep;
           mbar_wait(empty + s * 8, ph ^ 1, abort_flag);
           const uint32_t bar = full + s * 8, a_to = a_addr + s * kOperandBytes, b_to = b_addr + s * kOperandBytes;
           if (rank == 0) mbar_arrive_expect_tx(bar, 2 * 2 * kOperandBytes);  // both CTAs' loads report to the leader

@@ -192,3 +192,16 @@ def test_refusals(ck):
         ck.linear_weight_grad_mxfp8(_made((64, 16), torch.bfloat16, 18), codes.view(torch.uint8), scales)
     with pytest.raises(ck.NoCapableBackendError):
         ck.linear_input_grad_mxfp8(_made((64, 64), torch.bfloat16, 18).cpu(), codes.cpu(), scales.cpu())
+
+
+@pytest.mark.parametrize("m,n,k", [(9, 6208, 512), (64, 12288, 128), (300, 560, 512), (300, 4096, 512)])
+def test_small_numbers_of_dy_are_added_before_large_ones(ck, m, n, k):
+    """An fp32 dY enters as three bf16 numbers, 2^-8 and 2^-16 of the first.  An accumulator loses up to 2^-23 of what it has reached with each addition of
+    16 steps: 2048 steps of first numbers at most lose 128 * 2^-23 * 0.5 in the mean, towards zero, so 7.6e-6 if all sums
+    had one size; they grow as the root of the number of steps, which leaves two thirds, and half of the additions leave the sum smaller: 2.6e-6.  With the
+    others added at the same magnitude, three times the additions, it would be 7.6e-6."""
+    dy = _made((m, n), torch.float32, 19)
+    codes, scales, w = _held(ck, n, k, 20)
+    dx = ck.linear_input_grad_mxfp8(dy, codes, scales)
+    want = dy.double() @ w
+    assert (dx.double() - want).norm() <= 2.6e-6 * want.norm()
