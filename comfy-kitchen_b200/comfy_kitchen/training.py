@@ -295,6 +295,8 @@ def linear_checkpointed(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tenso
             x, weight, bias = x.to(dtype), weight.to(dtype), bias if bias is None else bias.to(dtype)
         if weight.dtype != x.dtype:
             raise ValueError(f"the weight is {weight.dtype}, the input {x.dtype}")
+    if x.numel() == 0:  # nothing to keep
+        return F.linear(x, weight.dequantize().to(x.dtype) if frozen else weight, bias)
     if not torch.is_grad_enabled() and not frozen:
         return F.linear(x, weight, bias)
     x2 = x if x.dim() == 2 else x.reshape(-1, k)
@@ -309,6 +311,8 @@ class CheckpointedLayerNorm(nn.LayerNorm):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if len(self.normalized_shape) != 1:
             raise ValueError("CheckpointedLayerNorm is over the last dimension")
+        if x.shape[-1:] != torch.Size(self.normalized_shape):
+            raise ValueError(f"the norm is over rows of {self.normalized_shape[0]}, the input {tuple(x.shape)}")
         return layer_norm(x, self.weight, self.bias, self.eps, checkpoint=True)
 
 

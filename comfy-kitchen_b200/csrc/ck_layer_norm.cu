@@ -262,8 +262,9 @@ __global__ void __launch_bounds__(kVec * kNum <= 16 ? 1024 : 512) layer_norm_for
   };
   int stage = 0, turn = 0;
   uint32_t phase = 0;
+  bool landed = true;  // after a wait that gave up the team still meets for each row, with no more copies, and the result is void
   for (uint32_t r = begin + team; r < end; r += teams, turn ^= 1) {
-    if (!sm100::mbar_wait(full_at + stage * 8, phase, &abort_flag)) break;
+    landed = sm100::mbar_wait(full_at + stage * 8, phase, &abort_flag) && landed;
     const uint8_t* const from = ring + stage * stage_bytes;
     const uint32_t row = row0 + r;
     if constexpr (kCopy) copy_row<T>(from, threadIdx.x, width, a, row);
@@ -311,7 +312,7 @@ __global__ void __launch_bounds__(kVec * kNum <= 16 ? 1024 : 512) layer_norm_for
     }
     const float rstd = inverse_root(squares * inv_cols + a.eps);
     if (threadIdx.x == 0) {
-      if (r + stages * teams < end) load_row(r + stages * teams, stage);  // all have read the stage
+      if (landed && r + stages * teams < end) load_row(r + stages * teams, stage);  // all have read the stage
       if (a.mean != nullptr) {
         a.mean[row] = mean;
         a.rstd[row] = rstd;
@@ -343,13 +344,13 @@ __global__ void __launch_bounds__(kVec * kNum <= 16 ? 1024 : 512) layer_norm_for
       for (uint32_t row = a.rows + team; row < a.rows_padded; row += teams) clear_scales_of_row(a, row);
     }
   }
-  if (abort_flag) {
-    if (threadIdx.x == 0 && team == 0) atomicExch(a.status, 1);
+  if (!landed) {
+    if ((threadIdx.x & 31) == 0) atomicExch(a.status, 1);
     for (int i = 0; i < 200; ++i) __nanosleep(1000);  // copies that are in flight land before the memory is released
   }
 }
 
-// The same for rows that do not lie on 16-byte boundaries (Columns and RowInRing in ck_layer_norm.cuh), without a copy.  36864 x 3071 fp16: 153 us
+// The same for rows that do not lie on 16-byte boundaries (Columns and RowInRing in ck_layer_norm.cuh), without a copy.  36864 x 3071 fp16: 135 us
 // against 455 for rows in registers without a ring, an element a load either way.
 template <typename T, int kVec, int kNum>
 __global__ void __launch_bounds__(512) layer_norm_forward_off_vectors_kernel(const ForwardArgs a, const uint32_t chunks, const uint32_t chunk_rows,
@@ -411,6 +412,7 @@ __global__ void __launch_bounds__(512) layer_norm_forward_off_vectors_kernel(con
   __syncthreads();
   int stage = 0, turn = 0;
   uint32_t phase = 0;
+  bool landed = true;  // after a wait that gave up the team still meets for each row, with no more copies, and the result is void
   for (uint32_t r = begin + team; r < end; r += teams, turn ^= 1) {
     const uint32_t next = r + stages * teams;  // the row that comes into this one's stage
     T edge = from_float<T>(0.0f);
@@ -421,7 +423,7 @@ __global__ void __launch_bounds__(512) layer_norm_forward_off_vectors_kernel(con
       has_edge = in.edge(row, lane, &edge_at);
       if (has_edge) edge = row[edge_at];
     }
-    if (!sm100::mbar_wait(full_at + stage * 8, phase, &abort_flag)) break;
+    landed = sm100::mbar_wait(full_at + stage * 8, phase, &abort_flag) && landed;
     const uint8_t* const from = ring + stage * stage_bytes + Row::offset(row_of(r));
     float2 f[kNum];
     float2 sum[2] = {both(0.0f), both(0.0f)};
@@ -462,7 +464,7 @@ __global__ void __launch_bounds__(512) layer_norm_forward_off_vectors_kernel(con
     const float rstd = inverse_root(squares * inv_cols + a.eps);
     const uint32_t row = row0 + r;
     if (threadIdx.x == 0) {
-      if (next < end) load_row(next, stage);  // all have read the stage
+      if (landed && next < end) load_row(next, stage);  // all have read the stage
       if (a.mean != nullptr) {
         a.mean[row] = mean;
         a.rstd[row] = rstd;
@@ -488,8 +490,8 @@ __global__ void __launch_bounds__(512) layer_norm_forward_off_vectors_kernel(con
       at.write(y, i, v);
     }
   }
-  if (abort_flag) {
-    if (threadIdx.x == 0 && team == 0) atomicExch(a.status, 1);
+  if (!landed) {
+    if ((threadIdx.x & 31) == 0) atomicExch(a.status, 1);
     for (int i = 0; i < 200; ++i) __nanosleep(1000);  // copies that are in flight land before the memory is released
   }
 }

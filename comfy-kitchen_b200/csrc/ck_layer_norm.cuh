@@ -130,11 +130,12 @@ struct Columns {
   __device__ __forceinline__ bool has(int turn, int e = 0) const { return column(turn, e) < cols; }
 
   __device__ __forceinline__ void read(const uint8_t* row, int turn, float2 (&f)[kPairs]) const {
+    const T* const at = reinterpret_cast<const T*>(row);
     if constexpr (kVec == 1) {
-      const T* const p = reinterpret_cast<const T*>(row) + column(turn, 0);
+      const T* const p = at + column(turn, 0);
       f[0] = make_float2(has(turn) ? to_float(p[0]) : 0.0f, has(turn, 1) ? to_float(p[width]) : 0.0f);
     } else {  // no branch: a place of the row, or zeros for what was there
-      unpack(*reinterpret_cast<const Raw<T, kVec>*>(reinterpret_cast<const T*>(row) + min(column(turn, 0), cols - 2)), f);
+      unpack(*reinterpret_cast<const Raw<T, kVec>*>(at + min(column(turn, 0), cols - 2)), f);
       if (!has(turn)) f[0] = both(0.0f);
     }
   }

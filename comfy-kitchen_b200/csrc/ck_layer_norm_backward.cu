@@ -302,13 +302,14 @@ __global__ void __launch_bounds__(kThreads) layer_norm_backward_ring_kernel(cons
   beside(begin + team);
   int stage = 0, turn = 0;
   uint32_t phase = 0;
+  bool landed = true;  // after a wait that gave up the team still meets for each row, with no more copies, and the result is void
   for (uint32_t r = begin + team; r < end; r += teams, turn ^= 1) {
     const float mean = next_mean, rstd = next_rstd;
     float factor[kNum];
 #pragma unroll
     for (int i = 0; i < kNum; ++i) factor[i] = e8m0_factor(next_byte[i]);
     beside(r + teams);
-    if (!sm100::mbar_wait(full_at + stage * 8, phase, &abort_flag)) break;
+    landed = sm100::mbar_wait(full_at + stage * 8, phase, &abort_flag) && landed;
     const uint8_t* const from = ring + stage * stage_bytes;
     // unpacked once: dy and h stay in registers for both passes
     float2 d[kNum][kPairs], h[kNum][kPairs];
@@ -360,7 +361,7 @@ __global__ void __launch_bounds__(kThreads) layer_norm_backward_ring_kernel(cons
       c1 = __shfl_sync(0xFFFFFFFFu, sum, 0) * inv_cols;
       c2 = __shfl_sync(0xFFFFFFFFu, sum, 16) * inv_cols;
     }
-    if (threadIdx.x == 0 && r + stages * teams < end) load_row(r + stages * teams, stage);  // all have read the stage
+    if (threadIdx.x == 0 && landed && r + stages * teams < end) load_row(r + stages * teams, stage);  // all have read the stage
     if (++stage == stages) {
       stage = 0;
       phase ^= 1u;
@@ -380,9 +381,9 @@ __global__ void __launch_bounds__(kThreads) layer_norm_backward_ring_kernel(cons
       }
     }
   }
+  if (!landed && (threadIdx.x & 31) == 0) atomicExch(a.status, 1);
   __syncthreads();  // the ring is the column sums' now
   if (abort_flag) {
-    if (threadIdx.x == 0 && team == 0) atomicExch(a.status, 1);
     for (int i = 0; i < 200; ++i) __nanosleep(1000);  // copies that are in flight land before the memory is released
     return;
   }
@@ -424,7 +425,7 @@ __global__ void __launch_bounds__(kThreads) layer_norm_backward_ring_kernel(cons
   }
 }
 
-// The same for rows that do not lie on 16-byte boundaries (Columns and RowInRing in ck_layer_norm.cuh): 36864 x 3071 fp16 227 us, against 677 for
+// The same for rows that do not lie on 16-byte boundaries (Columns and RowInRing in ck_layer_norm.cuh): 36864 x 3071 fp16 246 us, against 677 for
 // 24 columns a thread whose places the compiler kept in registers over all rows.
 template <typename T, int kVec, int kNum, int kThreads>
 __global__ void __launch_bounds__(kThreads) layer_norm_backward_off_vectors_kernel(const BackwardArgs a, const int stages) {
@@ -508,6 +509,7 @@ __global__ void __launch_bounds__(kThreads) layer_norm_backward_off_vectors_kern
   beside(begin + team);
   int stage = 0, turn = 0;
   uint32_t phase = 0;
+  bool landed = true;  // after a wait that gave up the team still meets for each row, with no more copies, and the result is void
   for (uint32_t r = begin + team; r < end; r += teams, turn ^= 1) {
     const float mean = next_mean, rstd = next_rstd;
     beside(r + teams);
@@ -520,7 +522,7 @@ __global__ void __launch_bounds__(kThreads) layer_norm_backward_off_vectors_kern
       has_edge = in.edge(row, lane & 15, &edge_at);
       if (has_edge) edge = row[edge_at];
     }
-    if (!sm100::mbar_wait(full_at + stage * 8, phase, &abort_flag)) break;
+    landed = sm100::mbar_wait(full_at + stage * 8, phase, &abort_flag) && landed;
     const uint8_t* const from = ring + stage * stage_bytes;
     const uint8_t* const dy_from = from + Row::offset(dy_row(r));
     const uint8_t* const x_from = from + dy_stage + Row::offset(x_row(r));
@@ -564,7 +566,7 @@ __global__ void __launch_bounds__(kThreads) layer_norm_backward_off_vectors_kern
       c2 = __shfl_sync(0xFFFFFFFFu, sum, 16) * inv_cols;
       __syncwarp();
     }
-    if (threadIdx.x == 0 && next < end) load_row(next, stage);  // all have read the stage
+    if (threadIdx.x == 0 && landed && next < end) load_row(next, stage);  // all have read the stage
     if (has_edge) put_edge(edge_row(next), stage, edge_at, edge);  // read behind the team's next meeting
     if (++stage == stages) {
       stage = 0;
@@ -584,9 +586,9 @@ __global__ void __launch_bounds__(kThreads) layer_norm_backward_off_vectors_kern
       at.write(dx, i, d[i]);
     }
   }
+  if (!landed && (threadIdx.x & 31) == 0) atomicExch(a.status, 1);
   __syncthreads();  // the ring is the column sums' now
   if (abort_flag) {
-    if (threadIdx.x == 0 && team == 0) atomicExch(a.status, 1);
     for (int i = 0; i < 200; ++i) __nanosleep(1000);  // copies that are in flight land before the memory is released
     return;
   }

@@ -100,6 +100,36 @@ def test_gradients_that_are_not_wanted(ck):
         assert not ck.linear_checkpointed(x, w, b).requires_grad and not ck.gelu_checkpointed(x).requires_grad
 
 
+@pytest.mark.parametrize("shape", [(0, 64), (2, 0, 64)])
+def test_no_tokens(ck, shape):
+    from comfy_kitchen.tensor import QuantizedTensor
+
+    mlp = ck.training.CheckpointedMLP(64, 96, device="cuda")
+    x = torch.empty(shape, device="cuda", requires_grad=True)
+    mlp(x).sum().backward()
+    assert x.grad.shape == shape and all((p.grad == 0).all() for p in mlp.parameters())
+    frozen = QuantizedTensor.from_float(_made((96, 64), torch.float32, 42), "TensorCoreMXFP8Layout")
+    y = ck.linear_checkpointed(x, frozen)
+    assert y.shape == (*shape[:-1], 96) and torch.autograd.grad(y.sum(), x)[0].shape == shape
+
+
+def test_more_than_2_31_elements(ck):
+    x = _made((66000, 32768), torch.bfloat16, 43)
+    last = x[-128:]
+    y, mean, rstd, codes, scales = ck.layer_norm_forward_mxfp8(x)
+    want = ck.layer_norm_forward_mxfp8(last.clone())
+    assert torch.equal(y[-128:], want[0]) and torch.equal(codes[-128:].view(torch.uint8), want[3].view(torch.uint8))
+    dx = ck.layer_norm_backward_mxfp8(x, codes, scales, mean, rstd)[0]
+    held = ck.dequantize_mxfp8(want[3], want[4], torch.float32).double()
+    h = (held - want[1].double().unsqueeze(1)) * want[2].double().unsqueeze(1)
+    d = last.double()
+    exact = want[2].double().unsqueeze(1) * (d - d.mean(1, keepdim=True) - h * (d * h).mean(1, keepdim=True))
+    assert (dx[-128:].double() - exact).norm() <= 2.0**-8 * exact.norm()
+    del y, dx
+    u, gelu_codes, _ = ck.gelu_mxfp8_forward(x)
+    assert torch.equal(gelu_codes[-128:].view(torch.uint8), want[3].view(torch.uint8)) and torch.equal(u[-128:], ck.gelu_mxfp8_forward(last.clone())[0])
+
+
 def test_expanded_gradient(ck):
     """The gradient of a sum is one number for all elements, with strides of zero."""
     x, w = _made((40, 64), torch.float32, 15), _made((16, 64), torch.float32, 16).requires_grad_()
@@ -270,6 +300,8 @@ def test_refusals(ck):
         ck.linear_checkpointed(x, frozen.t())
     with pytest.raises(ValueError, match="last dimension"):
         ck.training.CheckpointedLayerNorm((4, 64), device="cuda", dtype=torch.bfloat16)(x)
+    with pytest.raises(ValueError, match="rows of 32"):
+        ck.training.CheckpointedLayerNorm(32, elementwise_affine=False)(x)
     with pytest.raises(RuntimeError):  # no gradients of gradients
         w = _made((16, 64), torch.bfloat16, 40).requires_grad_()
         (g,) = torch.autograd.grad(ck.linear_checkpointed(x, w), w, _made((4, 16), torch.bfloat16, 41).requires_grad_(), create_graph=True)
