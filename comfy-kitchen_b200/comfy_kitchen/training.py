@@ -25,16 +25,23 @@ from torch.autograd.function import once_differentiable
 
 from .ops import _MAY_BE_PENDING, _PLAIN_TYPES, DTYPE_TO_CODE, _impl, dispatcher_adds_nothing, host_operator, host_step, replaced
 from .tensor import QuantizedTensor, TensorCoreMXFP8Layout
-from .tensor.blockwise import crop
+from .tensor.blockwise import crop, strict_status_check
 
 BLOCK = 32  # elements of one scale
+
+
+def _run(name: str, kwargs: dict):
+    """An operator straight from the registry; under CK_STRICT=1 a wait in its kernels that gave up raises here."""
+    out = _impl(name, kwargs)
+    strict_status_check(name)
+    return out
 
 
 def _call(name: str, kwargs: dict):
     """An operator without a gradient: straight to the registry where the dispatcher would add nothing."""
     tensors = [v for v in kwargs.values() if isinstance(v, torch.Tensor)]
     if not replaced(name) and dispatcher_adds_nothing(tensors):
-        return _impl(name, kwargs)
+        return _run(name, kwargs)
     return getattr(torch.ops.comfy_kitchen, name)(*[DTYPE_TO_CODE[v] if isinstance(v, torch.dtype) else v for v in kwargs.values()])
 
 
@@ -138,10 +145,10 @@ class _LayerNorm(torch.autograd.Function):
     def forward(ctx, x, weight, bias, eps, weight_offset, checkpoint):
         kwargs = {"x": x, "weight": weight, "bias": bias, "eps": eps, "weight_offset": weight_offset}
         if checkpoint:
-            y, mean, rstd, codes, scales = _impl("layer_norm_forward_mxfp8", kwargs)
+            y, mean, rstd, codes, scales = _run("layer_norm_forward_mxfp8", kwargs)
             ctx.save_for_backward(codes, scales, mean, rstd, weight)
         else:
-            y, mean, rstd = _impl("layer_norm_forward", kwargs)
+            y, mean, rstd = _run("layer_norm_forward", kwargs)
             ctx.save_for_backward(x, mean, rstd, weight)
         some = weight if weight is not None else bias
         ctx.param_shape, ctx.param_dtype = (some.shape, some.dtype) if some is not None else (None, x.dtype)
@@ -155,9 +162,9 @@ class _LayerNorm(torch.autograd.Function):
         kwargs = {"dy": dy, "mean": mean, "rstd": rstd, "weight": weight, "weight_offset": ctx.weight_offset, "groups": ctx.groups,
                   "param_dtype": ctx.param_dtype, "weight_grad": ctx.needs_input_grad[1], "bias_grad": ctx.needs_input_grad[2]}
         if len(held) == 2:
-            dx, dweight, dbias = _impl("layer_norm_backward_mxfp8", {**kwargs, "codes": held[0], "block_scales": held[1]})
+            dx, dweight, dbias = _run("layer_norm_backward_mxfp8", {**kwargs, "codes": held[0], "block_scales": held[1]})
         else:
-            dx, dweight, dbias = _impl("layer_norm_backward", {**kwargs, "x": held[0]})
+            dx, dweight, dbias = _run("layer_norm_backward", {**kwargs, "x": held[0]})
         return (dx if ctx.needs_input_grad[0] else None, *_param_grads(ctx, dweight, dbias), None, None, None)
 
 
@@ -181,7 +188,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     if _eager((x, weight, bias)) and not any(replaced(name) for name in _NORM_OPERATORS):
         if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
             return _LayerNorm.apply(x, weight, bias, eps, weight_offset, checkpoint)
-        return _impl("layer_norm_inference", {"x": x, "weight": weight, "bias": bias, "eps": eps, "weight_offset": weight_offset})
+        return _run("layer_norm_inference", {"x": x, "weight": weight, "bias": bias, "eps": eps, "weight_offset": weight_offset})
     op = torch.ops.comfy_kitchen.layer_norm_forward_mxfp8 if checkpoint else torch.ops.comfy_kitchen.layer_norm_forward
     return op(x, weight, bias, eps, weight_offset)[0]
 
@@ -192,7 +199,7 @@ _GELU_OPERATORS = ("gelu_mxfp8_forward", "gelu_mxfp8_backward")
 class _Gelu(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x):
-        y, codes, scales = _impl("gelu_mxfp8_forward", {"x": x})
+        y, codes, scales = _run("gelu_mxfp8_forward", {"x": x})
         ctx.save_for_backward(codes, scales)
         return y
 
@@ -200,7 +207,7 @@ class _Gelu(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         codes, scales = ctx.saved_tensors
-        return _impl("gelu_mxfp8_backward", {"dy": dy, "codes": codes, "block_scales": scales})
+        return _run("gelu_mxfp8_backward", {"dy": dy, "codes": codes, "block_scales": scales})
 
 
 def gelu_checkpointed(x: torch.Tensor) -> torch.Tensor:
@@ -215,7 +222,7 @@ def gelu_checkpointed(x: torch.Tensor) -> torch.Tensor:
     shape = x.shape
     x2 = x if len(shape) == 2 else x.reshape(-1, shape[-1])
     if _eager((x2,)) and not any(replaced(name) for name in _GELU_OPERATORS):
-        y = _Gelu.apply(x2) if torch.is_grad_enabled() and x2.requires_grad else _impl("gelu_inference", {"x": x2})
+        y = _Gelu.apply(x2) if torch.is_grad_enabled() and x2.requires_grad else _run("gelu_inference", {"x": x2})
     else:
         y = torch.ops.comfy_kitchen.gelu_mxfp8_forward(x2)[0]
     return y if len(shape) == 2 else y.view(shape)
@@ -258,6 +265,7 @@ class _FrozenLinear(torch.autograd.Function):
             bias = F.pad(bias, (0, padded))
         with torch.no_grad():
             y = TensorCoreMXFP8Layout.scaled_mm(QuantizedTensor.from_float(x.contiguous(), "TensorCoreMXFP8Layout"), weight, bias, x.dtype)
+        strict_status_check("linear_checkpointed")
         return crop(y, x.shape[0], ctx.shape[0])
 
     @staticmethod

@@ -280,6 +280,27 @@ def test_the_example(ck):
     assert ours["kept_bytes"] < 0.7 * dense["kept_bytes"]
 
 
+def test_strict_mode_reports_a_wait_that_gave_up(ck, monkeypatch):
+    """The status word is set from the host here; no kernel is made to fail."""
+    from comfy_kitchen.backends import cuda as backend
+
+    lib = backend.load_library()
+    x, w = _made((600, 64), torch.bfloat16, 44).requires_grad_(), _made((16, 64), torch.bfloat16, 45).requires_grad_()
+    codes, scales = ck.quantize_mxfp8(x.detach())
+    dy = _made((600, 16), torch.bfloat16, 46)
+    backend.check_device_status("clean start")
+    monkeypatch.setenv("CK_STRICT", "1")
+    for call in (lambda: ck.layer_norm(x), lambda: ck.layer_norm(x.detach()), lambda: ck.layer_norm(x, checkpoint=True),
+                 lambda: ck.linear_weight_grad_mxfp8(dy, codes, scales), lambda: ck.linear_input_grad_mxfp8(x.detach(), *ck.quantize_mxfp8(w.detach().t().contiguous()
+                                                                                                           .repeat(1, 2)))):
+        call()
+        assert lib.ck_debug_set_gemm_status(1) == 0
+        with pytest.raises(RuntimeError, match="gave up"):
+            call()
+    monkeypatch.setenv("CK_STRICT", "0")
+    backend.check_device_status("cleared")
+
+
 def test_refusals(ck):
     from comfy_kitchen.tensor import QuantizedTensor
 
