@@ -340,9 +340,7 @@ __global__ void __launch_bounds__(kVec * kNum <= 16 ? 1024 : 512) layer_norm_for
     }
   }
   if constexpr (kCopy) {  // the scales' padding rows
-    if (blockIdx.x == gridDim.x - 1) {
-      for (uint32_t row = a.rows + team; row < a.rows_padded; row += teams) clear_scales_of_row(a, row);
-    }
+    for (uint32_t row = a.rows + blockIdx.x * teams + team; row < a.rows_padded; row += gridDim.x * teams) clear_scales_of_row(a, row);
   }
   if (!landed) {
     if ((threadIdx.x & 31) == 0) atomicExch(a.status, 1);
