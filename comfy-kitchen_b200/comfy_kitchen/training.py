@@ -137,7 +137,8 @@ def _param_grads(ctx, dweight, dbias):
     return (dweight.view(shape) if ctx.needs_input_grad[1] else None), (dbias.view(shape) if ctx.needs_input_grad[2] else None)
 
 
-_NORM_OPERATORS = ("layer_norm_forward", "layer_norm_forward_mxfp8", "layer_norm_backward", "layer_norm_backward_mxfp8")
+_NORM_OPERATORS = {False: ("layer_norm_forward", "layer_norm_backward"), True: ("layer_norm_forward_mxfp8", "layer_norm_backward_mxfp8")}
+_NORM_INFERENCE = ("layer_norm_forward",)
 
 
 class _LayerNorm(torch.autograd.Function):
@@ -178,18 +179,20 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     fp32 with one rounding.  With ``checkpoint`` the backward pass works from an MXFP8 copy of x (the last dimension a
     multiple of 32) instead of x itself."""
     eps, weight_offset = float(eps), float(weight_offset)
-    host = host_step("layer_norm", _NORM_OPERATORS)
+    graph = torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad))
+    operators = _NORM_OPERATORS[bool(checkpoint)] if graph else _NORM_INFERENCE  # a copy that nothing reads is not made
+    host = host_step("layer_norm", operators)
     if host is not None:
         y = host(x, weight, bias, eps, weight_offset, checkpoint)
         if y is not None:
             return y
     if checkpoint and x.shape[-1] % BLOCK != 0:
         raise ValueError(f"an MXFP8 checkpoint needs rows of a multiple of {BLOCK}, got {x.shape[-1]}")
-    if _eager((x, weight, bias)) and not any(replaced(name) for name in _NORM_OPERATORS):
-        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+    if _eager((x, weight, bias)) and not any(replaced(name) for name in operators):
+        if graph:
             return _LayerNorm.apply(x, weight, bias, eps, weight_offset, checkpoint)
         return _run("layer_norm_inference", {"x": x, "weight": weight, "bias": bias, "eps": eps, "weight_offset": weight_offset})
-    op = torch.ops.comfy_kitchen.layer_norm_forward_mxfp8 if checkpoint else torch.ops.comfy_kitchen.layer_norm_forward
+    op = torch.ops.comfy_kitchen.layer_norm_forward_mxfp8 if checkpoint and graph else torch.ops.comfy_kitchen.layer_norm_forward
     return op(x, weight, bias, eps, weight_offset)[0]
 
 
@@ -212,7 +215,9 @@ class _Gelu(torch.autograd.Function):
 
 def gelu_checkpointed(x: torch.Tensor) -> torch.Tensor:
     """Tanh-form GELU whose backward pass works from an MXFP8 copy of x (the last dimension a multiple of 32)."""
-    host = host_step("gelu_checkpointed", _GELU_OPERATORS)
+    graph = torch.is_grad_enabled() and x.requires_grad
+    operators = _GELU_OPERATORS if graph else _GELU_OPERATORS[:1]
+    host = host_step("gelu_checkpointed", operators)
     if host is not None:
         y = host(x)
         if y is not None:
@@ -221,8 +226,8 @@ def gelu_checkpointed(x: torch.Tensor) -> torch.Tensor:
         raise ValueError(f"an MXFP8 checkpoint needs rows of a multiple of {BLOCK}, got {tuple(x.shape)}")
     shape = x.shape
     x2 = x if len(shape) == 2 else x.reshape(-1, shape[-1])
-    if _eager((x2,)) and not any(replaced(name) for name in _GELU_OPERATORS):
-        y = _Gelu.apply(x2) if torch.is_grad_enabled() and x2.requires_grad else _run("gelu_inference", {"x": x2})
+    if _eager((x2,)) and not any(replaced(name) for name in operators):
+        y = _Gelu.apply(x2) if graph else _run("gelu_inference", {"x": x2})
     else:
         y = torch.ops.comfy_kitchen.gelu_mxfp8_forward(x2)[0]
     return y if len(shape) == 2 else y.view(shape)
