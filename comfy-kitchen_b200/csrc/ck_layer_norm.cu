@@ -379,7 +379,7 @@ __global__ void __launch_bounds__(512) layer_norm_forward_off_vectors_kernel(con
     in.fetch(row, ring_at + s * stage_bytes, full_at + s * 8);
   };
   // sixteen lanes of a team's first warp bring what lies beside the copy
-  const auto put_edge = [&](const T* row, int s, uint32_t e, T v) { reinterpret_cast<T*>(ring + s * stage_bytes + Row::offset(row))[e] = v; };
+  const auto put_edge = [&](const T* row, int s, uint32_t e, T v) { Row::put(ring + s * stage_bytes, row, e, v); };
   float held = 0.0f;
 #pragma unroll
   for (int i = 0; i < kNum; ++i) held += (own.has(i) ? 1.0f : 0.0f) + (own.has(i, 1) ? 1.0f : 0.0f);

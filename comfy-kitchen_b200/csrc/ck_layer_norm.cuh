@@ -103,6 +103,12 @@ struct RowInRing {
     const uint32_t h = head(row), n = bulk_bytes(row);
     if (n > 0) sm100::bulk_load_1d(stage + offset(row) + h, reinterpret_cast<const uint8_t*>(row) + h, n, bar);
   }
+  // An element beside the copy.  The bulk copy of a later row, which may lie otherwise in its 16 bytes, writes the same place through the async
+  // proxy: the fence puts this store before it, for the thread that issues that copy behind the team's next meeting.
+  __device__ __forceinline__ static void put(uint8_t* stage, const T* row, uint32_t at, T v) {
+    reinterpret_cast<T*>(stage + offset(row))[at] = v;
+    sm100::fence_proxy_async();
+  }
   // element `*at` of the row is lane's (of sixteen) to bring: eight before the copy, eight behind it
   __device__ __forceinline__ bool edge(const T* row, int lane, uint32_t* at) const {
     const uint32_t h = head(row), tail = (bytes - h) & 15u, e = static_cast<uint32_t>(lane & 7) * sizeof(T);

@@ -460,9 +460,7 @@ __global__ void __launch_bounds__(kThreads) layer_norm_backward_off_vectors_kern
   };
   // Sixteen lanes of a team's first warp bring what lies beside the copies of a row of dy, the others that of x.
   const auto edge_row = [&](uint32_t r) { return lane < 16 ? dy_row(r) : x_row(r); };
-  const auto put_edge = [&](const T* row, int s, uint32_t at, T v) {
-    reinterpret_cast<T*>(ring + s * stage_bytes + (lane < 16 ? 0u : dy_stage) + Row::offset(row))[at] = v;
-  };
+  const auto put_edge = [&](const T* row, int s, uint32_t at, T v) { Row::put(ring + s * stage_bytes + (lane < 16 ? 0u : dy_stage), row, at, v); };
   if (threadIdx.x == 0) {
     if (team == 0) abort_flag = 0;
     for (int s = 0; s < stages; ++s) sm100::mbar_init(&full[team][s], 1);
