@@ -859,6 +859,7 @@ def _layer_norm_backward(dy, x, codes, scales, mean, rstd, weight, weight_offset
     if weight is not None:
         weight = _plain(weight)
         assert weight.shape[-1] == cols and weight.numel() == groups * cols and weight.dtype == param_dtype, "Invalid weight shape or dtype"
+        assert weight.dim() == 1 or weight.shape[0] == groups, "one weight row for each group, in the first dimension"
         if cols > 1 and weight.stride(-1) != 1:
             weight = weight.contiguous()
         w_stride = weight.stride(0) if weight.dim() > 1 else 0

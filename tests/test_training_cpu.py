@@ -142,3 +142,20 @@ def test_refusals_without_a_gpu():
         ck.gelu_checkpointed(torch.zeros(()))
     with pytest.raises(ValueError, match="output features"):
         ck.linear_checkpointed(x, torch.zeros(12, 64))
+
+
+def test_norm_backward_takes_a_weight_with_one_row_for_each_group(monkeypatch):
+    """A weight whose first dimension is not the groups has its rows elsewhere than a group's number times its stride: refused before any launch."""
+    from comfy_kitchen.backends import cuda
+
+    monkeypatch.setattr(cuda, "load_library", lambda: None)  # nothing is launched, whatever is here
+    with FakeTensorMode():
+        dy, stats = torch.empty(8, 64, device="cuda"), torch.empty(8, device="cuda")
+        codes = torch.empty(8, 64, device="cuda", dtype=torch.float8_e4m3fn)
+        scales = torch.empty(128, 4, device="cuda", dtype=torch.float8_e8m0fnu)
+        for shape in ((2, 2, 64), (1, 4, 64), (2, 1, 2, 64)):
+            w = torch.empty(shape, device="cuda")
+            for call in (lambda: cuda.layer_norm_backward(dy, dy, stats, stats, w, 0.0, 4),
+                         lambda: cuda.layer_norm_backward_mxfp8(dy, codes, scales, stats, stats, w, 0.0, 4)):
+                with pytest.raises(AssertionError, match="weight"):
+                    call()
