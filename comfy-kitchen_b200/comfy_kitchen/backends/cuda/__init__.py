@@ -779,6 +779,10 @@ def _row_levels(t: torch.Tensor, align: int = 1) -> tuple[torch.Tensor, int, int
     return t, t.numel() // cols, 0, cols
 
 
+def _on_one_device(first: torch.Tensor, *others) -> None:
+    assert all(t is None or t.device == first.device for t in others), "all tensors of a call must be on one device"
+
+
 def _norm_params(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None):
     """``(weight, bias, dtype code, groups, weight_stride, bias_stride)`` of a layer norm's parameters: ``[cols]``, or
     ``[groups, cols]`` (with ones in between, if any) where ``groups`` is x's first dimension."""
@@ -855,6 +859,7 @@ def _layer_norm_backward(dy, x, codes, scales, mean, rstd, weight, weight_offset
     rows, dev = dy.numel() // cols, dy.device
     assert mean.numel() == rstd.numel() == rows and mean.dtype == rstd.dtype == torch.float32 and mean.is_contiguous() and rstd.is_contiguous(), \
         "mean and rstd must hold one fp32 value for each row"
+    _on_one_device(dy, mean, rstd, weight, x, codes, scales)
     w_stride = 0
     if weight is not None:
         weight = _plain(weight)
@@ -872,7 +877,7 @@ def _layer_norm_backward(dy, x, codes, scales, mean, rstd, weight, weight_offset
         x_inner = x_outer_stride = x_inner_stride = 0
         if x is not None:
             x = _plain(x)
-            assert x.shape == dy.shape and x.dtype == dy.dtype and x.device == dev, "x must have dy's shape, dtype and device"
+            assert x.shape == dy.shape and x.dtype == dy.dtype, "x must have dy's shape and dtype"
             x, x_inner, x_outer_stride, x_inner_stride = _row_levels(x)
         else:
             codes, scales = _plain(codes), _plain(scales)
@@ -942,6 +947,7 @@ def gelu_inference(x: torch.Tensor) -> torch.Tensor:
 def gelu_mxfp8_backward(dy: torch.Tensor, codes: torch.Tensor, block_scales: torch.Tensor) -> torch.Tensor:
     """``dy * gelu_tanh'(u)`` with u the values that stand in the MXFP8 copy (all 2-D)."""
     lib = load_library()
+    _on_one_device(dy, codes, block_scales)
     dy, codes, block_scales = _aligned(dy, 32), _plain(codes), _plain(block_scales)
     rows, cols = dy.shape
     assert codes.shape == (rows, cols) and cols % 32 == 0 and block_scales.shape == (roundup(rows, 128), roundup(cols // 32, 4)), \
@@ -956,6 +962,7 @@ def gelu_mxfp8_backward(dy: torch.Tensor, codes: torch.Tensor, block_scales: tor
 
 
 def _linear_grad_args(dy, codes, scales, rows: int):
+    _on_one_device(dy, codes, scales)
     dy, codes, scales = _aligned(dy, 16), _aligned(codes, 32), _aligned(scales, 16)
     n, k = dy.shape[1], codes.shape[1]
     assert codes.shape[0] == rows, "Matrix dimensions do not match"

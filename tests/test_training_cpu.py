@@ -159,3 +159,26 @@ def test_norm_backward_takes_a_weight_with_one_row_for_each_group(monkeypatch):
                          lambda: cuda.layer_norm_backward_mxfp8(dy, codes, scales, stats, stats, w, 0.0, 4)):
                 with pytest.raises(AssertionError, match="weight"):
                     call()
+
+
+def test_gradients_take_operands_of_one_device(monkeypatch):
+    """A kernel on one GPU cannot read another one's memory: operands that lie elsewhere are refused before any launch."""
+    from comfy_kitchen.backends import cuda
+
+    monkeypatch.setattr(cuda, "load_library", lambda: None)  # nothing is launched, whatever is here
+    monkeypatch.setattr(cuda, "_host", None)
+    with FakeTensorMode():
+        def made(shape, dtype=torch.float32):
+            return [torch.empty(shape, device=d, dtype=dtype) for d in ("cuda:0", "cuda:1")]
+
+        dy, stats, w = made((8, 64)), made((8,)), made((64,))
+        codes, scales = made((8, 64), torch.float8_e4m3fn), made((128, 4), torch.float8_e8m0fnu)
+        for other in range(3):
+            mean, rstd, weight = (t[i == other] for i, t in enumerate((stats, stats, w)))
+            with pytest.raises(AssertionError, match="device"):
+                cuda.layer_norm_backward(dy[0], dy[0], mean, rstd, weight)
+        for c, s in ((codes[1], scales[0]), (codes[0], scales[1])):
+            for call in (lambda: cuda.layer_norm_backward_mxfp8(dy[0], c, s, stats[0], stats[0]), lambda: cuda.gelu_mxfp8_backward(dy[0], c, s),
+                         lambda: cuda.linear_weight_grad_mxfp8(dy[0], c, s), lambda: cuda.linear_input_grad_mxfp8(dy[0][:, :8], c, s)):
+                with pytest.raises(AssertionError, match="device"):
+                    call()
