@@ -205,3 +205,26 @@ def test_small_numbers_of_dy_are_added_before_large_ones(ck, m, n, k):
     dx = ck.linear_input_grad_mxfp8(dy, codes, scales)
     want = dy.double() @ w
     assert (dx.double() - want).norm() <= 2.6e-6 * want.norm()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [8, 40, 72, 128, 200, 264])
+def test_padding_of_the_scales_is_not_read(ck, dtype, n):
+    """Scales come in tiles of 128 rows and four blocks; what stands in those past the matrix's rows and columns must not reach a result: 0xFF is
+    infinite, and the codes of rows past the last one are zeros."""
+    k = 160
+    codes, scales, _ = _held(ck, n, k, 21)
+    bad = scales.clone()
+    tall, wide = scales.shape[0] // 128, scales.shape[1] // 4
+    rows = torch.arange(tall * 128, device="cuda").view(tall, 1, 4, 32, 1).transpose(2, 3)  # tile row, tile column, row % 32, row // 32, block
+    blocks = torch.arange(wide * 4, device="cuda").view(1, wide, 1, 1, 4)
+    tiles = bad.view(torch.uint8).view(tall, wide, 32, 4, 4)
+    tiles[((rows >= n) | (blocks >= k // 32)).expand(tiles.shape)] = 0xFF
+    assert (bad.view(torch.uint8) == 0xFF).sum() == scales.numel() - n * (k // 32)
+    for m in (1, 5, 33, 300):  # decoded inside the product, and before it
+        dy = _made((m, n), dtype, 22)
+        got, clean = (ck.linear_input_grad_mxfp8(dy, codes, s) for s in (bad, scales))
+        assert torch.isfinite(clean).all() and torch.equal(got, clean), m
+    x_dy = _made((n, 64), dtype, 23)
+    got, clean = (ck.linear_weight_grad_mxfp8(x_dy, codes, s, bias_grad=True) for s in (bad, scales))
+    assert torch.equal(got[0], clean[0]) and torch.equal(got[1], clean[1])
