@@ -560,25 +560,25 @@ struct RingPlan {
 // A block of up to 16 warps an SM, or of 32 with a short row each.  A row's warps: as few as hold it, and as many more as the rows leave idle: those that
 // fit into the ring, or those that an SM gets.
 RingPlan plan_ring(int64_t rows, int64_t cols, int64_t size, bool whole) {
-  constexpr int64_t kRoom = 216 * 1024;
   const int64_t stage = round_up(cols * size + (whole ? 0 : 15), 128), params = 2 * round_up(cols * 4, 128), columns = 16 / size * 32;
   RingPlan p = {};
   p.warps = static_cast<int>(ceil_div(cols, 32 * 96));
-  if (p.warps > 16 || params + 2 * stage > kRoom) return p;
+  if (p.warps > 16 || params + 2 * stage > kRingRoom) return p;
   int64_t teams = cols <= 512 && whole ? 32 : 16 / p.warps;
-  if (teams > (kRoom - params) / (2 * stage)) teams = (kRoom - params) / (2 * stage);
+  if (teams > (kRingRoom - params) / (2 * stage)) teams = (kRingRoom - params) / (2 * stage);
   if (teams > ceil_div(rows, sm_count())) teams = ceil_div(rows, sm_count());
   int64_t warps = teams > 16 ? 1 : 16 / teams;
   if (warps > ceil_div(cols, columns)) warps = ceil_div(cols, columns);
   if (warps > p.warps) p.warps = static_cast<int>(warps);
   p.teams = static_cast<int>(teams);
-  const int64_t stages = (kRoom - params) / (teams * stage);
+  const int64_t stages = (kRingRoom - params) / (teams * stage);
   p.stages = static_cast<int>(stages > kMaxRing ? kMaxRing : stages);
   p.smem = static_cast<int>(params + teams * p.stages * stage);
   return p;
 }
 
-int launch_ring(void (*kernel)(ForwardArgs, uint32_t, uint32_t, int), ForwardArgs a, const RingPlan& p, cudaStream_t s) {
+template <auto kKernel>
+int launch_ring(ForwardArgs a, const RingPlan& p, cudaStream_t s) {
   // one block an SM, and no block with less than a row for each team
   const int64_t groups = a.rows / a.rows_per_group;
   int64_t chunks = sm_count() / groups;
@@ -586,17 +586,17 @@ int launch_ring(void (*kernel)(ForwardArgs, uint32_t, uint32_t, int), ForwardArg
   if (chunks < 1) chunks = 1;
   const uint32_t chunk_rows = static_cast<uint32_t>(ceil_div(a.rows_per_group, chunks));
   chunks = ceil_div(a.rows_per_group, chunk_rows);
-  CK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, p.smem));
+  if (int rc = allow_ring_room<kKernel>()) return rc;
   if (int rc = gemm_status_word(&a.status)) return rc;
-  CK_CUDA(launch_pdl(kernel, dim3(static_cast<unsigned>(groups * chunks)), dim3(32 * p.warps, p.teams), p.smem, s, a, static_cast<uint32_t>(chunks),
+  CK_CUDA(launch_pdl(kKernel, dim3(static_cast<unsigned>(groups * chunks)), dim3(32 * p.warps, p.teams), p.smem, s, a, static_cast<uint32_t>(chunks),
                      chunk_rows, p.stages));
   return CK_OK;
 }
 
 template <typename T, int kVec, int kNum, bool kCopy>
 int launch_forward_ring_num(const ForwardArgs& a, const RingPlan& p, cudaStream_t s) {
-  const bool exact = a.cols == int64_t{32} * p.warps * kNum * kVec;
-  return launch_ring(exact ? layer_norm_forward_ring_kernel<T, kVec, kNum, kCopy, true> : layer_norm_forward_ring_kernel<T, kVec, kNum, kCopy, false>, a, p, s);
+  if (a.cols == int64_t{32} * p.warps * kNum * kVec) return launch_ring<layer_norm_forward_ring_kernel<T, kVec, kNum, kCopy, true>>(a, p, s);
+  return launch_ring<layer_norm_forward_ring_kernel<T, kVec, kNum, kCopy, false>>(a, p, s);
 }
 
 template <typename T, int kVec, bool kCopy>
@@ -661,9 +661,9 @@ int forward_typed(const ForwardArgs& given, cudaStream_t s) {
         const auto by_num = [&](auto vec) {
           constexpr int kV = decltype(vec)::value;
           const int64_t num = ceil_div(a.cols, 64 * p.warps);  // pairs
-          return launch_ring(num <= 16 ? layer_norm_forward_off_vectors_kernel<T, kV, 16>
-                                       : num <= 32 ? layer_norm_forward_off_vectors_kernel<T, kV, 32> : layer_norm_forward_off_vectors_kernel<T, kV, 48>,
-                             a, p, s);
+          if (num <= 16) return launch_ring<layer_norm_forward_off_vectors_kernel<T, kV, 16>>(a, p, s);
+          if (num <= 32) return launch_ring<layer_norm_forward_off_vectors_kernel<T, kV, 32>>(a, p, s);
+          return launch_ring<layer_norm_forward_off_vectors_kernel<T, kV, 48>>(a, p, s);
         };
         return pairs ? by_num(std::integral_constant<int, 2>()) : by_num(std::integral_constant<int, 1>());
       }

@@ -11,6 +11,8 @@
 // squares are taken.  Results are rounded to their types once.
 #pragma once
 
+#include <atomic>
+
 #include "ck_rows.cuh"
 
 namespace ck {
@@ -181,6 +183,22 @@ bool on_bytes(const void* p, const RowStrides& r, int size, int bytes) {
   return reinterpret_cast<uintptr_t>(p) % bytes == 0 && r.outer_stride * size % bytes == 0 && r.inner_stride * size % bytes == 0;
 }
 bool on_vectors(const void* p, const RowStrides& r, int size) { return on_bytes(p, r, size, 16); }
+
+constexpr int kRingRoom = 216 * 1024;  // of shared memory, for parameters and rings
+
+// What a kernel may be launched with is state of the function on its device: one bound for all calls, set before the first of them, so that calls of
+// several threads, whose plans differ, do not take it from one another.
+template <auto kKernel>
+int allow_ring_room() {
+  static std::atomic<bool> allowed[64];
+  int dev = 0;
+  CK_CUDA(cudaGetDevice(&dev));
+  const bool known = dev >= 0 && dev < 64;
+  if (known && allowed[dev].load(std::memory_order_acquire)) return CK_OK;
+  CK_CUDA(cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingRoom));
+  if (known) allowed[dev].store(true, std::memory_order_release);
+  return CK_OK;
+}
 
 bool is_float_code(int dtype) { return dtype == CK_DTYPE_F32 || dtype == CK_DTYPE_F16 || dtype == CK_DTYPE_BF16; }
 

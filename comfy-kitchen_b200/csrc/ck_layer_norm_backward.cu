@@ -717,8 +717,6 @@ __global__ void __launch_bounds__(512) layer_norm_join_kernel(const float* parti
 // host side
 // ---------------------------------------------------------------------------
 // ---- backward: how the rows are shared out
-constexpr int64_t kRingRoom = 216 * 1024;  // of shared memory, for factors and rings
-
 struct Plan {
   bool wide;      // rows that a block's threads do not hold
   bool ring;      // rows that come through shared memory
@@ -787,35 +785,34 @@ Plan plan_backward(int64_t cols, int size, int vec, bool copy, bool weight, int6
 
 template <typename T, int kVec, int kNum, int kRows, bool kCopy>
 int launch_backward_num(const BackwardArgs& a, const Plan& p, cudaStream_t s) {
-  auto kernel = layer_norm_backward_kernel<T, kVec, kNum, kRows, kCopy>;
-  if (p.smem > 32 * 1024) CK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, p.smem));
-  CK_CUDA(launch_pdl(kernel, dim3(a.groups * a.chunks), dim3(32 * p.warps, p.teams), p.smem, s, a));
+  // 480 threads' column sums at most: 30 KB, which needs no leave
+  CK_CUDA(launch_pdl(layer_norm_backward_kernel<T, kVec, kNum, kRows, kCopy>, dim3(a.groups * a.chunks), dim3(32 * p.warps, p.teams), p.smem, s, a));
+  return CK_OK;
+}
+
+template <auto kKernel>
+int launch_rows_in_ring(BackwardArgs a, const Plan& p, cudaStream_t s) {
+  if (int rc = allow_ring_room<kKernel>()) return rc;
+  if (int rc = gemm_status_word(&a.status)) return rc;
+  CK_CUDA(launch_pdl(kKernel, dim3(a.groups * a.chunks), dim3(32 * p.warps, p.teams), p.smem, s, a, p.stages));
   return CK_OK;
 }
 
 template <typename T, int kVec, int kNum, int kThreads, bool kCopy>
-int launch_backward_ring(BackwardArgs a, const Plan& p, cudaStream_t s) {
-  if (int rc = gemm_status_word(&a.status)) return rc;
+int launch_backward_ring(const BackwardArgs& a, const Plan& p, cudaStream_t s) {
   // Where the columns fill all threads nothing is asked for each vector.  Where a thread reads 48 columns of both dy and x, asking keeps the reads of
   // later vectors behind the arithmetic of earlier ones, which is worth more (36864 x 3072 bf16: 114 us against 132; from the copy 128 against
   // 111); 32 columns of each of 512 threads leave no registers for either.
   constexpr bool kCanFill = kNum * kVec <= 24 || (kThreads == 256 && (kCopy || kNum * kVec <= 32));
-  auto kernel = layer_norm_backward_ring_kernel<T, kVec, kNum, kThreads, kCopy, false>;
   if constexpr (kCanFill) {
-    if (a.cols == int64_t{32} * p.warps * kNum * kVec) kernel = layer_norm_backward_ring_kernel<T, kVec, kNum, kThreads, kCopy, true>;
+    if (a.cols == int64_t{32} * p.warps * kNum * kVec) return launch_rows_in_ring<layer_norm_backward_ring_kernel<T, kVec, kNum, kThreads, kCopy, true>>(a, p, s);
   }
-  if (p.smem > 32 * 1024) CK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, p.smem));
-  CK_CUDA(launch_pdl(kernel, dim3(a.groups * a.chunks), dim3(32 * p.warps, p.teams), p.smem, s, a, p.stages));
-  return CK_OK;
+  return launch_rows_in_ring<layer_norm_backward_ring_kernel<T, kVec, kNum, kThreads, kCopy, false>>(a, p, s);
 }
 
 template <typename T, int kVec, int kNum, int kThreads>
-int launch_backward_off_vectors(BackwardArgs a, const Plan& p, cudaStream_t s) {
-  if (int rc = gemm_status_word(&a.status)) return rc;
-  auto kernel = layer_norm_backward_off_vectors_kernel<T, kVec, kNum, kThreads>;
-  if (p.smem > 32 * 1024) CK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, p.smem));
-  CK_CUDA(launch_pdl(kernel, dim3(a.groups * a.chunks), dim3(32 * p.warps, p.teams), p.smem, s, a, p.stages));
-  return CK_OK;
+int launch_backward_off_vectors(const BackwardArgs& a, const Plan& p, cudaStream_t s) {
+  return launch_rows_in_ring<layer_norm_backward_off_vectors_kernel<T, kVec, kNum, kThreads>>(a, p, s);
 }
 
 template <typename T, int kVec, bool kCopy>
