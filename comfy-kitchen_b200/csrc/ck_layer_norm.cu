@@ -223,11 +223,14 @@ __global__ void __launch_bounds__(kVec * kNum <= 16 ? 1024 : 512) layer_norm_for
     sm100::bulk_load_1d(ring_at + s * stage_bytes, static_cast<const T*>(a.x) + a.x_rows.offset(row0 + r), row_bytes, full_at + s * 8);
   };
   const auto has = [&](int i) { return kExact || static_cast<int>(threadIdx.x) + i * width < vecs; };
-  int held = 0;
+  int held = 32 * kNum * kVec;
+  if constexpr (!kExact) {
+    held = 0;
 #pragma unroll
-  for (int i = 0; i < kNum; ++i) held += max(0, min(32, vecs - warp * 32 - i * width)) * kVec;
-  const float inv_held = held > 0 ? 1.0f / static_cast<float>(held) : 0.0f;
-  if (team == 0 && (threadIdx.x & 31) == 0) counts[warp] = static_cast<float>(held);
+    for (int i = 0; i < kNum; ++i) held += max(0, min(32, vecs - warp * 32 - i * width)) * kVec;
+  }
+  const float count = static_cast<float>(held), inv_held = held > 0 ? 1.0f / count : 0.0f;
+  if (team == 0 && (threadIdx.x & 31) == 0) counts[warp] = count;
   if (threadIdx.x == 0) {
     if (team == 0) abort_flag = 0;
     for (int s = 0; s < stages; ++s) sm100::mbar_init(&full[team][s], 1);
@@ -282,7 +285,7 @@ __global__ void __launch_bounds__(kVec * kNum <= 16 ? 1024 : 512) layer_norm_for
       for (int j = 0; j < kPairs; ++j) sum[j & 1] = add_x2(sum[j & 1], f[i][j]);
     }
     sum[0] = add_x2(sum[0], sum[1]);
-    const float mine = warp_sum(sum[0].x + sum[0].y) * inv_held;
+    const float mine = mean_of(warp_sum(sum[0].x + sum[0].y), count, inv_held);
     float2 square[2] = {both(0.0f), both(0.0f)};
 #pragma unroll
     for (int i = 0; i < kNum; ++i) {
@@ -291,6 +294,7 @@ __global__ void __launch_bounds__(kVec * kNum <= 16 ? 1024 : 512) layer_norm_for
       for (int j = 0; j < kPairs; ++j) {
         const float2 d = add_x2(f[i][j], minus);
         square[j & 1] = fma_x2(d, d, square[j & 1]);
+        if constexpr (kCopy) f[i][j] = d;
       }
     }
     square[0] = add_x2(square[0], square[1]);
@@ -299,14 +303,9 @@ __global__ void __launch_bounds__(kVec * kNum <= 16 ? 1024 : 512) layer_norm_for
       float2* const slots = buf[turn] + team * warps;
       if ((threadIdx.x & 31) == 0) slots[warp] = make_float2(mine, squares);
       asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(width) : "memory");
-      mean = 0.0f;
-      for (int w = 0; w < warps; ++w) mean = fmaf(slots[w].x, counts[w], mean);
-      mean *= inv_cols;
-      squares = 0.0f;
-      for (int w = 0; w < warps; ++w) {
-        const float d = slots[w].x - mean;
-        squares += fmaf(d * d, counts[w], slots[w].y);
-      }
+      const Moments all = join_moments(slots, counts, warps, static_cast<float>(a.cols), inv_cols);
+      mean = all.mean;
+      squares = all.squares;
     } else {
       __syncwarp();
     }
@@ -323,6 +322,10 @@ __global__ void __launch_bounds__(kVec * kNum <= 16 ? 1024 : 512) layer_norm_for
       phase ^= 1u;
     }
     T* const y = static_cast<T*>(a.y) + static_cast<int64_t>(row) * a.cols;
+    // h = (x - mean) / std, the difference first: a product of x and 1 / std would leave its rounding in the result where eps and not the deviation bounds
+    // 1 / std.  Or, in one step, from x - mine and what the warp's mean is off, a few deviations at most: beside a copy, where it takes 58.8 us
+    // instead of 60.2 (18432 x 3072 bf16); without one 14.1 instead of 13.5 (4096 x 3072).
+    const float2 scale = both(rstd), shift = both(kCopy ? (mine - mean) * rstd : -mean);
 #pragma unroll
     for (int i = 0; i < kNum; ++i) {
       if (!has(i)) continue;
@@ -332,9 +335,8 @@ __global__ void __launch_bounds__(kVec * kNum <= 16 ? 1024 : 512) layer_norm_for
       read_params(bias_buf, v, b);
 #pragma unroll
       for (int j = 0; j < kPairs; ++j) {
-        // in one step for 16-bit types, where a mean of that many times the deviation leaves no digits in x anyway
-        f[i][j] = sizeof(T) == 2 ? fma_x2(f[i][j], both(rstd), both(-mean * rstd)) : mul_x2(add_x2(f[i][j], both(-mean)), both(rstd));
-        f[i][j] = fma_x2(f[i][j], w[j], b[j]);
+        const float2 h = kCopy ? fma_x2(f[i][j], scale, shift) : mul_x2(add_x2(f[i][j], shift), scale);
+        f[i][j] = fma_x2(h, w[j], b[j]);
       }
       store(y + static_cast<int64_t>(v) * kVec, pack<T, kVec>(f[i]));
     }
@@ -434,13 +436,13 @@ __global__ void __launch_bounds__(512) layer_norm_forward_off_vectors_kernel(con
       sum[i & 1] = add_x2(sum[i & 1], f[i]);
     }
     sum[0] = add_x2(sum[0], sum[1]);
-    const float mine = warp_sum(sum[0].x + sum[0].y) * inv_held;
+    const float mine = mean_of(warp_sum(sum[0].x + sum[0].y), held, inv_held);
     float2 square[2] = {both(0.0f), both(0.0f)};
     at = own.again();
 #pragma unroll
     for (int i = 0; i < kNum; ++i) {
-      const float2 d = add_x2(f[i], make_float2(at.has(i) ? -mine : 0.0f, at.has(i, 1) ? -mine : 0.0f));
-      square[i & 1] = fma_x2(d, d, square[i & 1]);
+      f[i] = add_x2(f[i], make_float2(at.has(i) ? -mine : 0.0f, at.has(i, 1) ? -mine : 0.0f));
+      square[i & 1] = fma_x2(f[i], f[i], square[i & 1]);
     }
     square[0] = add_x2(square[0], square[1]);
     float mean = mine, squares = warp_sum(square[0].x + square[0].y);
@@ -448,14 +450,9 @@ __global__ void __launch_bounds__(512) layer_norm_forward_off_vectors_kernel(con
       float2* const slots = buf[turn] + team * warps;
       if (lane == 0) slots[warp] = make_float2(mine, squares);
       asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(width) : "memory");
-      mean = 0.0f;
-      for (int w = 0; w < warps; ++w) mean = fmaf(slots[w].x, counts[w], mean);
-      mean *= inv_cols;
-      squares = 0.0f;
-      for (int w = 0; w < warps; ++w) {
-        const float d = slots[w].x - mean;
-        squares += fmaf(d * d, counts[w], slots[w].y);
-      }
+      const Moments all = join_moments(slots, counts, warps, static_cast<float>(a.cols), inv_cols);
+      mean = all.mean;
+      squares = all.squares;
     } else {
       __syncwarp();
     }
@@ -475,12 +472,11 @@ __global__ void __launch_bounds__(512) layer_norm_forward_off_vectors_kernel(con
     }
     T* const y = static_cast<T*>(a.y) + static_cast<int64_t>(row) * a.cols;
     at = own.again();
-    const float2 scale = both(rstd), shift = both(sizeof(T) == 2 ? -mean * rstd : -mean);
+    const float2 scale = both(rstd), shift = both((mine - mean) * rstd);  // as in the kernel for whole vectors, in one step
 #pragma unroll
     for (int i = 0; i < kNum; ++i) {
       if (!at.has(i)) continue;
-      // as in the kernel for whole vectors
-      float2 v[1] = {sizeof(T) == 2 ? fma_x2(f[i], scale, shift) : mul_x2(add_x2(f[i], shift), scale)};
+      float2 v[1] = {fma_x2(f[i], scale, shift)};
       float2 w[1], b[1];
       at.shared_params(factor_buf, i, w);
       at.shared_params(bias_buf, i, b);

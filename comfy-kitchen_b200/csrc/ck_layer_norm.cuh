@@ -83,10 +83,34 @@ __device__ __forceinline__ float row_sum(float v, float* buf) {
   return s;
 }
 
+// total / count with one more step than the product with 1 / count: the rounded quotient, so that a row of equal numbers whose sum is exact has that
+// number for its mean.  Where eps and not the deviation bounds 1 / std (316 for 1e-5), a unit in the last place of 1000 would be 0.02 in h.
+__device__ __forceinline__ float mean_of(float total, float count, float inv_count) {
+  const float q = total * inv_count;
+  const float better = fmaf(fmaf(-q, count, total), inv_count, q);
+  return fabsf(q) < __uint_as_float(0x7F800000u) ? better : q;
+}
+
+// What a row's warps hold, joined: `slots` has each one's mean and the squares about it, `counts` its number of elements.
+struct Moments {
+  float mean, squares;
+};
+__device__ __forceinline__ Moments join_moments(const float2* slots, const float* counts, int warps, float cols, float inv_cols) {
+  Moments m = {0.0f, 0.0f};
+  for (int w = 0; w < warps; ++w) m.mean = fmaf(slots[w].x, counts[w], m.mean);
+  m.mean = mean_of(m.mean, cols, inv_cols);
+  for (int w = 0; w < warps; ++w) {
+    const float d = slots[w].x - m.mean;
+    m.squares += fmaf(d * d, counts[w], slots[w].y);
+  }
+  return m;
+}
+
 // ---- rows that come through shared memory
 // A team's row is a bulk copy into a ring of stages, issued that many rows ahead by one thread, so that what is in flight
 // does not depend on registers or on where the warps stand.  Barriers of the ring are mbarriers whose waits are bounded (mbar_wait).
-constexpr int kMaxRing = 4;
+// Two rows of each team: with four, 10000 x 1152 fp16 takes 15.4 us forward instead of 13.9, 36864 x 3072 bf16 from the copy 105 backward instead of 102.
+constexpr int kMaxRing = 2;
 
 // A row that does not lie on 16-byte boundaries is copied where it does, at the same place in its 16 bytes; what is before and behind
 // (up to 15 bytes each) comes by plain loads of one element a lane, read ahead of a row's arithmetic and stored behind it.

@@ -218,6 +218,9 @@ __global__ void __launch_bounds__(512) layer_norm_backward_kernel(const Backward
 template <typename T, int kVec, int kNum, int kThreads, bool kCopy, bool kExact>
 __global__ void __launch_bounds__(kThreads) layer_norm_backward_ring_kernel(const BackwardArgs a, const int stages) {
   constexpr int kMaxTeams = 15, kPairs = kVec / 2;
+  // g stays in registers for the second pass; or dy, and the factors are read again, where 48 columns a thread of 16-bit x or of an fp32 row's copy leave
+  // the compiler an order of reads that is worth more (36864 x 3072 bf16: 111 us against 118; 4096 x 12288 fp32 from the copy 86 against 95)
+  constexpr bool kAgain = kNum * kVec == 48 && sizeof(T) == (kCopy ? 4 : 2);
   extern __shared__ __align__(128) uint8_t shared_bytes[];  // factors f, then the teams' rings; the teams' column sums in the end
   __shared__ __align__(8) uint64_t full[kMaxTeams][kMaxRing];
   __shared__ float2 row_buf[2][16];  // [turn][warp of the block]
@@ -311,9 +314,9 @@ __global__ void __launch_bounds__(kThreads) layer_norm_backward_ring_kernel(cons
     beside(r + teams);
     landed = sm100::mbar_wait(full_at + stage * 8, phase, &abort_flag) && landed;
     const uint8_t* const from = ring + stage * stage_bytes;
-    // unpacked once: dy and h stay in registers for both passes
+    // unpacked once: g (or dy) and h stay in registers for the second pass
     float2 d[kNum][kPairs], h[kNum][kPairs];
-    const float2 rstd2 = both(rstd), shift = both(sizeof(T) == 2 ? -mean * rstd : -mean);
+    const float2 rstd2 = both(rstd), minus = both(-mean);
     float2 s1 = both(0.0f), s2 = both(0.0f);
 #pragma unroll
     for (int i = 0; i < kNum; ++i) {
@@ -325,8 +328,8 @@ __global__ void __launch_bounds__(kThreads) layer_norm_backward_ring_kernel(cons
         const auto codes = *reinterpret_cast<const Raw<uint32_t, kVec / 4>*>(from + x_at + v * kVec);
 #pragma unroll
         for (int j = 0; j < kVec / 4; ++j) {
-          h[i][2 * j] = mul_x2(e4m3_pair(codes.v[j] & 0xFFFFu), both(factor[i]));
-          h[i][2 * j + 1] = mul_x2(e4m3_pair(codes.v[j] >> 16), both(factor[i]));
+          h[i][2 * j] = fma_x2(e4m3_pair(codes.v[j] & 0xFFFFu), both(factor[i]), minus);
+          h[i][2 * j + 1] = fma_x2(e4m3_pair(codes.v[j] >> 16), both(factor[i]), minus);
         }
       } else {
         unpack(*reinterpret_cast<const Raw<T, kVec>*>(from + x_at + v * 16), h[i]);
@@ -335,13 +338,13 @@ __global__ void __launch_bounds__(kThreads) layer_norm_backward_ring_kernel(cons
       factors(i, f);
 #pragma unroll
       for (int j = 0; j < kPairs; ++j) {
-        // (x - mean) / std; in one step for 16-bit types, where a mean of that many times the deviation leaves no digits in x anyway
-        h[i][j] = sizeof(T) == 2 ? fma_x2(h[i][j], rstd2, shift) : mul_x2(add_x2(h[i][j], shift), rstd2);
+        h[i][j] = mul_x2(kCopy ? h[i][j] : add_x2(h[i][j], minus), rstd2);
+        dw[i][j] = fma_x2(d[i][j], h[i][j], dw[i][j]);
+        db[i][j] = add_x2(db[i][j], d[i][j]);
         const float2 g = mul_x2(d[i][j], f[j]);
         s1 = add_x2(s1, g);
         s2 = fma_x2(g, h[i][j], s2);
-        dw[i][j] = fma_x2(d[i][j], h[i][j], dw[i][j]);
-        db[i][j] = add_x2(db[i][j], d[i][j]);
+        if constexpr (!kAgain) d[i][j] = g;
       }
     }
     // both sums in five exchanges: the lower half of a warp goes on with one, the upper with the other
@@ -367,15 +370,16 @@ __global__ void __launch_bounds__(kThreads) layer_norm_backward_ring_kernel(cons
       phase ^= 1u;
     }
     T* const dx = static_cast<T*>(a.dx) + static_cast<int64_t>(row0 + r) * a.cols;
+    const float2 c1r = both(-c1 * rstd), c2r = both(-c2 * rstd);
 #pragma unroll
     for (int i = 0; i < kNum; ++i) {
       const int v = threadIdx.x + i * width;
       if (has(i)) {
         float2 f[kPairs];
-        factors(i, f);
+        if constexpr (kAgain) factors(i, f);
 #pragma unroll
         for (int j = 0; j < kPairs; ++j) {
-          d[i][j] = mul_x2(fma_x2(h[i][j], both(-c2), fma_x2(d[i][j], f[j], both(-c1))), rstd2);
+          d[i][j] = kAgain ? mul_x2(fma_x2(h[i][j], both(-c2), fma_x2(d[i][j], f[j], both(-c1))), rstd2) : fma_x2(h[i][j], c2r, fma_x2(d[i][j], rstd2, c1r));
         }
         store(dx + v * kVec, pack<T, kVec>(d[i]));
       }
@@ -524,9 +528,9 @@ __global__ void __launch_bounds__(kThreads) layer_norm_backward_off_vectors_kern
     const uint8_t* const from = ring + stage * stage_bytes;
     const uint8_t* const dy_from = from + Row::offset(dy_row(r));
     const uint8_t* const x_from = from + dy_stage + Row::offset(x_row(r));
-    // unpacked once: dy and h stay in registers for both passes
+    // unpacked once: g and h stay in registers for the second pass
     float2 d[kNum][kPairs], h[kNum][kPairs];
-    const float2 rstd2 = both(rstd), shift = both(sizeof(T) == 2 ? -mean * rstd : -mean);
+    const float2 rstd2 = both(rstd), minus = both(-mean);
     float2 s1 = both(0.0f), s2 = both(0.0f);
     at = own.again();
 #pragma unroll
@@ -537,13 +541,12 @@ __global__ void __launch_bounds__(kThreads) layer_norm_backward_off_vectors_kern
       factors(i, f);
 #pragma unroll
       for (int j = 0; j < kPairs; ++j) {
-        // (x - mean) / std; in one step for 16-bit types, where a mean of that many times the deviation leaves no digits in x anyway
-        h[i][j] = sizeof(T) == 2 ? fma_x2(h[i][j], rstd2, shift) : mul_x2(add_x2(h[i][j], shift), rstd2);
-        const float2 g = mul_x2(d[i][j], f[j]);
-        s1 = add_x2(s1, g);
-        s2 = fma_x2(g, h[i][j], s2);
+        h[i][j] = mul_x2(add_x2(h[i][j], minus), rstd2);
         dw[i][j] = fma_x2(d[i][j], h[i][j], dw[i][j]);
         db[i][j] = add_x2(db[i][j], d[i][j]);
+        d[i][j] = mul_x2(d[i][j], f[j]);  // g from here on
+        s1 = add_x2(s1, d[i][j]);
+        s2 = fma_x2(d[i][j], h[i][j], s2);
       }
     }
     // both sums in five exchanges: the lower half of a warp goes on with one, the upper with the other
@@ -571,16 +574,13 @@ __global__ void __launch_bounds__(kThreads) layer_norm_backward_off_vectors_kern
       phase ^= 1u;
     }
     T* const dx = static_cast<T*>(a.dx) + static_cast<int64_t>(row0 + r) * a.cols;
+    const float2 c1r = both(-c1 * rstd), c2r = both(-c2 * rstd);
     at = own.again();
 #pragma unroll
     for (int i = 0; i < kNum; ++i) {
       if (!at.has(i)) continue;
-      float2 f[kPairs];
-      factors(i, f);
 #pragma unroll
-      for (int j = 0; j < kPairs; ++j) {
-        d[i][j] = mul_x2(fma_x2(h[i][j], both(-c2), fma_x2(d[i][j], f[j], both(-c1))), rstd2);
-      }
+      for (int j = 0; j < kPairs; ++j) d[i][j] = fma_x2(h[i][j], c2r, fma_x2(d[i][j], rstd2, c1r));
       at.write(dx, i, d[i]);
     }
   }
