@@ -265,9 +265,10 @@ def _norm_setup(ctx, inputs, output):
     ctx.groups = some.shape[0] if some is not None and some.dim() > 1 else 1
     held = (output[3], output[4]) if len(output) == 5 else (x,)
     ctx.save_for_backward(*held, output[1], output[2], weight)
+    ctx.mark_non_differentiable(*output[1:])  # mean, rstd and the copy carry no gradient
 
 
-def _norm_backward(ctx, dy, *_):  # mean, rstd and the copy carry no gradient
+def _norm_backward(ctx, dy, *_):
     *held, mean, rstd, weight = ctx.saved_tensors
     op = torch.ops.comfy_kitchen.layer_norm_backward_mxfp8 if len(held) == 2 else torch.ops.comfy_kitchen.layer_norm_backward
     dx, dweight, dbias = op(dy, *held, mean, rstd, weight, ctx.weight_offset, ctx.groups, DTYPE_TO_CODE[ctx.param_dtype])
@@ -301,6 +302,7 @@ def _(dy, codes, block_scales):
 
 def _gelu_setup(ctx, inputs, output):
     ctx.save_for_backward(output[1], output[2])
+    ctx.mark_non_differentiable(output[1], output[2])
 
 
 def _gelu_backward(ctx, dy, *_):

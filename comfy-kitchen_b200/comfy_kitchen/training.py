@@ -14,7 +14,7 @@ statistics of the dense input).
 * :class:`CheckpointedLayerNorm`, :class:`CheckpointedGELU`, :class:`CheckpointedLinear`, :class:`CheckpointedMLP`: modules around them.
 
 The functions that these are built from (``layer_norm_forward`` ... ``linear_input_grad_mxfp8``) are operators of the package like
-the quantizers; gradients of gradients are not available.
+the quantizers; statistics and copies that they return carry no gradient, and gradients of gradients are not available.
 """
 from __future__ import annotations
 
@@ -48,7 +48,7 @@ def _call(name: str, kwargs: dict):
 # ---- the operators -----------------------------------------------------------------------------
 def layer_norm_forward(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, eps: float = 1e-5,
                        weight_offset: float = 0.0) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """``(y, mean, rstd)`` of :func:`layer_norm`: the result and the fp32 statistics of each row."""
+    """``(y, mean, rstd)`` of :func:`layer_norm`: the result and the fp32 statistics of each row, which carry no gradient."""
     return _call("layer_norm_forward", {"x": x, "weight": weight, "bias": bias, "eps": float(eps), "weight_offset": float(weight_offset)})
 
 

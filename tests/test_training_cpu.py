@@ -182,3 +182,30 @@ def test_gradients_take_operands_of_one_device(monkeypatch):
                          lambda: cuda.linear_weight_grad_mxfp8(dy[0], c, s), lambda: cuda.linear_input_grad_mxfp8(dy[0][:, :8], c, s)):
                 with pytest.raises(AssertionError, match="device"):
                     call()
+
+
+def test_only_the_results_carry_gradients(monkeypatch):
+    """Statistics and copies have no gradient, and say so, instead of one of zeros: the operators' formulas over stand-ins for their kernels."""
+    from comfy_kitchen import ops
+
+    def stand_in(name, kwargs):
+        if name.endswith("backward") or name.endswith("backward_mxfp8"):
+            dy = kwargs["dy"]
+            return 2 * dy if name.startswith("gelu") else (2 * dy, 3 * dy.sum(0, keepdim=True), 5 * dy.sum(0, keepdim=True))
+        x = kwargs["x"].detach()
+        copy = torch.zeros(x.shape, dtype=torch.uint8).view(torch.float8_e4m3fn), torch.zeros(128, 4, dtype=torch.uint8).view(torch.float8_e8m0fnu)
+        return (2 * x, *(() if name.startswith("gelu") else (x.mean(-1), x.std(-1))), *(copy if name.endswith("mxfp8") or name.startswith("gelu") else ()))
+
+    monkeypatch.setattr(ops, "_impl", stand_in)
+    x, w, b = (torch.ones(s, requires_grad=True) for s in ((4, 64), (64,), (64,)))
+    op = torch.ops.comfy_kitchen
+    for leaves, out in (((x, w, b), op.layer_norm_forward(x, w, b, 1e-5, 0.0)), ((x, w, b), op.layer_norm_forward_mxfp8(x, w, b, 1e-5, 0.0)),
+                        ((x,), op.gelu_mxfp8_forward(x)), ((x, w), ck.layer_norm_forward(x, w))):
+        assert out[0].requires_grad and not any(t.requires_grad for t in out[1:])
+        grads = torch.autograd.grad(out[0], leaves, torch.ones_like(x))
+        assert all(torch.equal(g, torch.full_like(t, c)) for g, t, c in zip(grads, leaves, (2, 12, 20)))
+        if out[1].dtype == torch.float32:  # a loss of the result and a statistic: the result's part alone
+            mixed = torch.autograd.grad((ck.layer_norm_forward(x, w)[0] + out[1].unsqueeze(1)).sum(), x)[0]
+            assert torch.equal(mixed, torch.full_like(x, 2))
+            with pytest.raises(RuntimeError, match="does not require grad"):
+                torch.autograd.grad(out[1].sum(), x)
