@@ -126,6 +126,9 @@ torch::autograd::variable_list once(torch::autograd::variable_list grads) {
   return grads;
 }
 
+// A gradient as it stands in memory: a view whose negation is pending (the imaginary part of a conjugate) or a symbolic zero is laid out.
+Tensor materialized(const Tensor& grad) { return grad._is_zerotensor() ? at::zeros(grad.sizes(), grad.options()) : grad.resolve_neg(); }
+
 struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
   static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias,
                         const NormParams& p, double eps, double offset, bool copy) {
@@ -148,7 +151,8 @@ struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, const torch::autograd::variable_list& grads) {
     torch::autograd::variable_list out(7);
     if (!grads[0].defined()) return out;
-    const c10::cuda::CUDAGuard on(grads[0].device());
+    const Tensor grad = materialized(grads[0]);
+    const c10::cuda::CUDAGuard on(grad.device());
     const Call c;
     const auto saved = ctx->get_saved_variables();
     const Tensor &mean = saved[0], &rstd = saved[1], &weight = saved[2];
@@ -158,8 +162,8 @@ struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
     const int code = static_cast<int>(held["code"].toInt());
     const int64_t groups = held["groups"].toInt();
     const bool want_weight = has_weight && ctx->needs_input_grad(1), want_bias = has_bias && ctx->needs_input_grad(1 + has_weight);
-    const Rows dy = rows_in_levels(grads[0], copy ? 16 : 1);
-    const Tensor dx = result(grads[0].sizes(), grads[0].scalar_type(), c.device);
+    const Rows dy = rows_in_levels(grad, copy ? 16 : 1);
+    const Tensor dx = result(grad.sizes(), grad.scalar_type(), c.device);
     const ScalarType param = code == 0 ? ScalarType::Float : code == 1 ? ScalarType::Half : ScalarType::BFloat16;
     const std::vector<int64_t> shape = has_weight || has_bias ? held["shape"].toIntVector() : std::vector<int64_t>{};
     Tensor dweight, dbias;
@@ -247,7 +251,7 @@ struct GeluNode : torch::autograd::Function<GeluNode> {
     const Call c;
     const auto saved = ctx->get_saved_variables();
     const int64_t cols = grads[0].size(-1);
-    Tensor dy = grads[0].contiguous();
+    Tensor dy = materialized(grads[0]).contiguous();
     if (reinterpret_cast<uintptr_t>(dy.const_data_ptr()) % 32 != 0) dy = dy.clone();
     const Tensor dx = result(dy.sizes(), dy.scalar_type(), c.device);
     if (lib.gelu_mxfp8_backward(dy.const_data_ptr(), code_of(dy.scalar_type()), saved[0].const_data_ptr(), saved[1].const_data_ptr(), dx.mutable_data_ptr(),

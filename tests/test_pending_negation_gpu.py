@@ -47,3 +47,25 @@ def test_symbolic_zero(cuda_device):
             ck.quantize_mxfp8(zero)
     else:
         _same(ck.quantize_mxfp8(zero), through_dispatcher)
+
+
+@pytest.mark.parametrize("checkpoint", [False, True])
+def test_gradients_with_a_pending_negation(cuda_device, checkpoint):
+    """A gradient may arrive as such a view too: contiguous, or the imaginary part of a conjugate."""
+    gen = torch.Generator(device=cuda_device).manual_seed(2)
+    x, w, b, dy = (torch.randn(s, generator=gen, device=cuda_device) for s in ((48, 64), (64,), (64,), (48, 64)))
+    for strided in (False, True):
+        pending = _negated(dy) if strided else torch._neg_view(dy)
+        for call in (lambda *t: ck.layer_norm(*t, checkpoint=checkpoint), lambda x, w, b: ck.gelu_checkpointed(x * w + b),
+                     lambda x, w, b: ck.linear_checkpointed(x * b, w.repeat(64, 1))):
+            got, want = (torch.autograd.grad(call(*leaves), leaves, g, allow_unused=True)
+                         for leaves in [[t.clone().requires_grad_() for t in (x, w, b)]] for g in (pending, -dy))
+            _same(tuple(t for t in got if t is not None), tuple(t for t in want if t is not None))
+
+
+@pytest.mark.parametrize("checkpoint", [False, True])
+def test_gradients_that_are_symbolic_zeros(cuda_device, checkpoint):
+    x, w = torch.randn(48, 64, device=cuda_device, requires_grad=True), torch.ones(64, device=cuda_device, requires_grad=True)
+    zero = torch._efficientzerotensor((48, 64), device=cuda_device, dtype=torch.float32)
+    for y in (ck.layer_norm(x, w, checkpoint=checkpoint), ck.gelu_checkpointed(x)):
+        assert all(g is None or not g.any() for g in torch.autograd.grad(y, (x, w), zero, allow_unused=True))
