@@ -660,9 +660,9 @@ __global__ void __launch_bounds__(512) layer_norm_columns_wide_kernel(const Back
   __shared__ float buf[2][16][33];
   pdl_launch_dependents();
   pdl_wait();
-  const uint32_t group = blockIdx.x / a.chunks, chunk = blockIdx.x - group * a.chunks;
+  const uint32_t part = blockIdx.y, group = part / a.chunks, chunk = part - group * a.chunks;
   const uint32_t begin = chunk * a.chunk_rows, end = min(a.rows_per_group, begin + a.chunk_rows);
-  const int64_t k = static_cast<int64_t>(blockIdx.y) * 32 + threadIdx.x;
+  const int64_t k = static_cast<int64_t>(blockIdx.x) * 32 + threadIdx.x;
   float dw = 0.0f, db = 0.0f;
   if (k < a.cols) {
     for (uint32_t r = begin + threadIdx.y; r < end; r += 16) {
@@ -680,7 +680,7 @@ __global__ void __launch_bounds__(512) layer_norm_columns_wide_kernel(const Back
 #pragma unroll
     for (int t = 0; t < 16; ++t) s += buf[threadIdx.y][t][threadIdx.x];
     if (a.partials != nullptr) {
-      a.partials[(static_cast<int64_t>(blockIdx.x) * 2 + threadIdx.y) * a.cols + k] = s;
+      a.partials[(static_cast<int64_t>(part) * 2 + threadIdx.y) * a.cols + k] = s;
     } else {
       void* to = threadIdx.y == 0 ? a.dweight : a.dbias;
       if (to != nullptr) store_param<T>(to, group * a.cols + k, a.params_f32, s);
@@ -878,7 +878,8 @@ int backward_typed(const BackwardArgs& given, void* workspace, int64_t workspace
   if (p.wide) {
     CK_CUDA(launch_pdl(layer_norm_backward_wide_kernel<T>, dim3(a.groups * a.rows_per_group), dim3(512), 0, s, a));
     if (sums) {
-      const dim3 grid(a.groups * p.chunks, static_cast<unsigned>(ceil_div(a.cols, 32)));
+      // strips of columns in the dimension that has room for any width; groups are at most 32767, chunks of fewer groups than SMs as many as those
+      const dim3 grid(static_cast<unsigned>(ceil_div(a.cols, 32)), a.groups * p.chunks);
       CK_CUDA(launch_pdl(layer_norm_columns_wide_kernel<T>, grid, dim3(32, 16), 0, s, a));
     }
   } else if (vec == 1) {

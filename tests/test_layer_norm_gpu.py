@@ -295,3 +295,11 @@ def test_refusals(ck):
         leaf = x.detach().requires_grad_()
         (g,) = torch.autograd.grad(ck.layer_norm(leaf), leaf, x, create_graph=True)
         g.sum().backward()
+
+
+@pytest.mark.parametrize("cols", [2_097_120, 2_097_128, 2_200_000])
+def test_gradients_of_very_wide_rows(ck, monkeypatch, cols):
+    """More strips of 32 columns than a grid's second dimension counts.  A thread of 512 adds its columns one after another: the bounds grow as those do."""
+    monkeypatch.setitem(globals(), "U", U * (cols / 512 + 64) / 128)
+    x = _made((2, cols), torch.bfloat16, 46)
+    _run(ck, x, _made((cols,), torch.bfloat16, 47, 0.2, 1.0), _made((cols,), torch.bfloat16, 48))
