@@ -37,23 +37,21 @@ struct CopyVec {
   uint32_t byte;
 };
 
-// A team of blockDim.x threads takes kRows rows at a time, every thread the same columns of all of them: a row's two sums go through
-// shared memory once for all kRows, and the column sums for dw and db stay in registers until the block's rows are
-// done.  Then the teams' sums are added in a fixed order and written: as results where the block has all rows of its group, else as
-// partial sums that a second kernel adds.
+// Short rows, a warp each.  It takes kRows of them at a time, every lane the same columns of all: a row's two sums go over the lanes, and the
+// column sums for dw and db stay in registers until the block's rows are done.  Then the warps' sums are added in a fixed order and
+// written: as results where the block has all rows of its group, else as partial sums that a second kernel adds.
 template <typename T, int kVec, int kNum, int kRows, bool kCopy>
 __global__ void __launch_bounds__(512) layer_norm_backward_kernel(const BackwardArgs a) {
-  constexpr int kMaxWarps = 16;
-  __shared__ __align__(16) float row_buf[2][kMaxWarps][2 * kRows];  // [turn][warp of the block][sums]
-  extern __shared__ __align__(16) float shared_buf[];               // first the factors f, later the teams' column sums
+  const int width = blockDim.x;  // 32; given as a constant the compiler has fewer loads in flight (20000 x 320 fp32 from the copy: 25.5 us against 22.0)
+  extern __shared__ __align__(16) float shared_buf[];  // first the factors f, later the warps' column sums
   pdl_launch_dependents();
-  const int team = threadIdx.y, teams = blockDim.y, width = blockDim.x, warps = width >> 5;
+  const int team = threadIdx.y, teams = blockDim.y;
   const uint32_t group = blockIdx.x / a.chunks, chunk = blockIdx.x - group * a.chunks;
   const uint32_t begin = chunk * a.chunk_rows, end = min(a.rows_per_group, begin + a.chunk_rows);
   const int64_t vecs = a.cols / kVec;
   const float inv_cols = 1.0f / static_cast<float>(a.cols);
   pdl_wait();
-  // The factors as fp32 in shared memory, all teams': in registers they would be a third of what a thread holds.  Four of a vector lie
+  // The factors as fp32 in shared memory, all warps': in registers they would be a third of what a thread holds.  Four of a vector lie
   // together and the vectors 16 bytes apart, so that a warp's 16-byte loads meet no bank twice.
   constexpr int kPart = kVec < 4 ? kVec : 4;
   const int part_stride = static_cast<int>(vecs) * kPart;
@@ -86,8 +84,7 @@ __global__ void __launch_bounds__(512) layer_norm_backward_kernel(const Backward
 #pragma unroll
     for (int j = 0; j < kVec; ++j) dw[i][j] = db[i][j] = 0.0f;
   }
-  int turn = 0;
-  for (uint32_t r0 = begin + team * kRows; r0 < end; r0 += teams * kRows, turn ^= 1) {
+  for (uint32_t r0 = begin + team * kRows; r0 < end; r0 += teams * kRows) {
     Raw<T, kVec> dy[kRows][kNum];
     std::conditional_t<kCopy, CopyVec<kVec>, InputVec<T, kVec>> in[kRows][kNum];
     float mean[kRows], rstd[kRows];
@@ -148,20 +145,6 @@ __global__ void __launch_bounds__(512) layer_norm_backward_kernel(const Backward
       sums[2 * r] = warp_sum(s1);
       sums[2 * r + 1] = warp_sum(s2);
     }
-    if (warps > 1) {  // the team's warps meet; two buffers in turn, so that one meeting a round is enough
-      const int warp0 = team * warps;
-      if ((threadIdx.x & 31) == 0) {
-#pragma unroll
-        for (int s = 0; s < 2 * kRows; ++s) row_buf[turn][warp0 + (threadIdx.x >> 5)][s] = sums[s];
-      }
-      asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(width) : "memory");
-#pragma unroll
-      for (int s = 0; s < 2 * kRows; ++s) sums[s] = 0.0f;
-      for (int w = 0; w < warps; ++w) {
-#pragma unroll
-        for (int s = 0; s < 2 * kRows; ++s) sums[s] += row_buf[turn][warp0 + w][s];
-      }
-    }
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
       if (r0 + r >= end) break;
@@ -183,7 +166,7 @@ __global__ void __launch_bounds__(512) layer_norm_backward_kernel(const Backward
     }
   }
   if (a.dweight == nullptr && a.dbias == nullptr) return;
-  // the teams' column sums
+  // the warps' column sums
   float* column_buf = shared_buf;  // [2 * kVec][threads]
   const int threads = width * teams, at = team * width + threadIdx.x;
 #pragma unroll
@@ -786,7 +769,7 @@ Plan plan_backward(int64_t cols, int size, int vec, bool copy, bool weight, int6
 template <typename T, int kVec, int kNum, int kRows, bool kCopy>
 int launch_backward_num(const BackwardArgs& a, const Plan& p, cudaStream_t s) {
   // 480 threads' column sums at most: 30 KB, which needs no leave
-  CK_CUDA(launch_pdl(layer_norm_backward_kernel<T, kVec, kNum, kRows, kCopy>, dim3(a.groups * a.chunks), dim3(32 * p.warps, p.teams), p.smem, s, a));
+  CK_CUDA(launch_pdl(layer_norm_backward_kernel<T, kVec, kNum, kRows, kCopy>, dim3(a.groups * a.chunks), dim3(32, p.teams), p.smem, s, a));
   return CK_OK;
 }
 
