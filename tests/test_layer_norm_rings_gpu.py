@@ -134,3 +134,15 @@ def test_rows_that_are_nearly_constant(ck, dtype, checkpoint, rows, cols):
     hk = (kept - exact_mean) * exact_rstd
     limit = (off * exact_rstd + hk.abs() * (160 * U + off**2 * exact_rstd**2)).sum(0, keepdim=True) + rows * U * hk.abs().sum(0, keepdim=True)
     assert ((dw.double() - hk.sum(0, keepdim=True)).abs() <= limit).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("checkpoint", [False, True])
+@pytest.mark.parametrize("rows,cols", [(300, 544), (700, 5120), (320, 6016), (1500, 8192), (500, 12288), (310, 13824), (420, 16384), (300, 18432)])
+def test_teams_of_several_warps(ck, dtype, checkpoint, rows, cols):
+    """Whole vectors, a row over two to sixteen warps, up to the widest row that the ring takes: threads that are full, that are not, and that have nothing."""
+    x = _made((rows, cols), dtype, 70, 2.0, 0.3)
+    _run(ck, x, _made((cols,), dtype, 71, 0.2, 1.0), _made((cols,), dtype, 72, 0.2), checkpoint=checkpoint)
+    if cols % 2048 == 0:
+        x = _made((2, rows, cols), dtype, 73)
+        _run(ck, x, _made((2, cols), torch.float32, 74, 0.2), _made((2, cols), torch.float32, 75), 1.0, checkpoint)
