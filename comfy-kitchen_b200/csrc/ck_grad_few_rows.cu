@@ -147,8 +147,11 @@ grad_few_rows_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_co
       for (int i = 0; i < kItems; ++i) {
         const int row = row0 + 4 * kGroupWarps * i;
         codes[i] = *reinterpret_cast<const uint4*>(code_at + raw_stage * kRawBytes + 4 * kGroupWarps * i * kCols);
-        // a tile of scales is two stages high; what stands in its rows past the last one is nobody's (an infinite one would make NaN of zeros)
-        byte[i] = step * kDeep + row < a.N ? scale_at[raw_stage * kRawBytes + (row & 31) * 16 + (row >> 5) * 4 + (step & 1) * 8] : 0;
+        byte[i] = scale_at[raw_stage * kRawBytes + (row & 31) * 16 + (row >> 5) * 4 + (step & 1) * 8];  // a tile of scales is two stages high
+      }
+      if (const int left = a.N - step * kDeep; left < kDeep) {  // what stands in rows past the last one is nobody's: infinite, it would make NaN of zeros
+#pragma unroll
+        for (int i = 0; i < kItems; ++i) byte[i] = row0 + 4 * kGroupWarps * i < left ? byte[i] : 0u;
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&raw_empty_bar[raw_stage]);
