@@ -194,8 +194,8 @@ __device__ __forceinline__ void copy_row(const uint8_t* from, int thread, int wi
 
 // Many rows.  A team of blockDim.x threads takes a row at a time out of its ring; the block's rows are of one group, whose factors f and biases stand
 // in shared memory as fp32.  A row is unpacked once and stays in registers as fp32, up to 96 columns a thread: waiting, sums over
-// lanes and the meeting of a team's warps cost the same for few columns as for many.  36864 x 3072 bf16, a warp a row: 89 us
-// (5.1 TB/s) against 109 with four warps a row; with the copy 112 against 155.  Mean and variance take one meeting: each warp brings the mean of what it holds and the squares about that.
+// lanes and the meeting of a team's warps cost the same for few columns as for many.  36864 x 3072 bf16, a warp a row: 92 us
+// (4.9 TB/s) against 109 with four warps a row; with the copy 113 against 155.  Mean and variance take one meeting: each warp brings the mean of what it holds and the squares about that.
 // kExact: the columns fill all threads.
 template <typename T, int kVec, int kNum, bool kCopy, bool kExact>
 __global__ void __launch_bounds__(kVec * kNum <= 16 ? 1024 : 512) layer_norm_forward_ring_kernel(const ForwardArgs a, const uint32_t chunks, const uint32_t chunk_rows,
@@ -350,7 +350,7 @@ __global__ void __launch_bounds__(kVec * kNum <= 16 ? 1024 : 512) layer_norm_for
   }
 }
 
-// The same for rows that do not lie on 16-byte boundaries (Columns and RowInRing in ck_layer_norm.cuh), without a copy.  36864 x 3071 fp16: 135 us
+// The same for rows that do not lie on 16-byte boundaries (Columns and RowInRing in ck_layer_norm.cuh), without a copy.  36864 x 3071 fp16: 141 us
 // against 455 for rows in registers without a ring, an element a load either way.
 template <typename T, int kVec, int kNum>
 __global__ void __launch_bounds__(512) layer_norm_forward_off_vectors_kernel(const ForwardArgs a, const uint32_t chunks, const uint32_t chunk_rows,
@@ -612,7 +612,7 @@ int launch_forward(const ForwardArgs& a, cudaStream_t s) {
   const int64_t vecs = ceil_div(a.cols, kVec);
   CK_REQUIRE(vecs <= 32 * 32 * 8, "layer_norm_forward: a copy of rows of %lld is not supported", (long long)a.cols);
   if constexpr (kVec * sizeof(T) == 16) {
-    // (30000 x 256 bf16 with a copy, which gives eight lanes of a warp work: 19.2 us against 15.5; without one 11.8 against 12.4)
+    // (30000 x 256 bf16 with a copy, which gives eight lanes of a warp work: 18.6 us against 15.0; without one 10.6 against 12.1)
     if (a.rows > 2 * sm_count() && a.rows_per_group >= 16 && reinterpret_cast<uintptr_t>(a.codes) % 32 == 0 && (!kCopy || a.cols > 256)) {
       const RingPlan p = plan_ring(a.rows, a.cols, sizeof(T), true);
       if (p.smem > 0 && a.rows / a.rows_per_group <= 2 * sm_count()) return launch_forward_ring<T, kVec, kCopy>(a, p, s);

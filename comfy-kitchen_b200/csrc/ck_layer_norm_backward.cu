@@ -197,13 +197,14 @@ __global__ void __launch_bounds__(512) layer_norm_backward_kernel(const Backward
 // The same where rows are long enough to come through shared memory (see the forward pass): a team's rows of dy and of x or its codes are
 // bulk copies into its own ring, a few rows ahead, and what a thread holds of a row is read from there once.  Bound by HBM, and by the instructions
 // that a row costs each warp whatever its columns: 256 threads with 48 columns of 255 registers instead of 512 with 24 took 36864 x 3072 bf16
-// from 125 us to 112 (6.1 TB/s), from the copy from 143 to 110 (5.2 TB/s).
+// from 125 us to 112, from the copy from 143 to 110.  As they stand: 111 (6.1 TB/s) and 102 (5.6 TB/s).
 template <typename T, int kVec, int kNum, int kThreads, bool kCopy, bool kExact>
 __global__ void __launch_bounds__(kThreads) layer_norm_backward_ring_kernel(const BackwardArgs a, const int stages) {
   constexpr int kMaxTeams = 15, kPairs = kVec / 2;
-  // g stays in registers for the second pass; or dy, and the factors are read again, where 48 columns a thread of 16-bit x or of an fp32 row's copy leave
-  // the compiler an order of reads that is worth more (36864 x 3072 bf16: 111 us against 118; 4096 x 12288 fp32 from the copy 86 against 95)
-  constexpr bool kAgain = kNum * kVec == 48 && sizeof(T) == (kCopy ? 4 : 2);
+  // g stays in registers for the second pass.  Or dy, and the factors are read again, where a thread holds 48 columns (but for a copy of 16-bit rows):
+  // there the compiler's order of reads is worth more (36864 x 3072 bf16: 111 us against 118; 4096 x 12288 fp32 from the copy 86 against 95;
+  // 36864 x 3072 bf16 from the copy 102 against 109 the other way round)
+  constexpr bool kAgain = kNum * kVec == 48 && !(kCopy && sizeof(T) == 2);
   extern __shared__ __align__(128) uint8_t shared_bytes[];  // factors f, then the teams' rings; the teams' column sums in the end
   __shared__ __align__(8) uint64_t full[kMaxTeams][kMaxRing];
   __shared__ float2 row_buf[2][16];  // [turn][warp of the block]
@@ -412,7 +413,7 @@ __global__ void __launch_bounds__(kThreads) layer_norm_backward_ring_kernel(cons
   }
 }
 
-// The same for rows that do not lie on 16-byte boundaries (Columns and RowInRing in ck_layer_norm.cuh): 36864 x 3071 fp16 246 us, against 677 for
+// The same for rows that do not lie on 16-byte boundaries (Columns and RowInRing in ck_layer_norm.cuh): 36864 x 3071 fp16 228 us, against 677 for
 // 24 columns a thread whose places the compiler kept in registers over all rows.
 template <typename T, int kVec, int kNum, int kThreads>
 __global__ void __launch_bounds__(kThreads) layer_norm_backward_off_vectors_kernel(const BackwardArgs a, const int stages) {
@@ -784,8 +785,8 @@ int launch_rows_in_ring(BackwardArgs a, const Plan& p, cudaStream_t s) {
 template <typename T, int kVec, int kNum, int kThreads, bool kCopy>
 int launch_backward_ring(const BackwardArgs& a, const Plan& p, cudaStream_t s) {
   // Where the columns fill all threads nothing is asked for each vector.  Where a thread reads 48 columns of both dy and x, asking keeps the reads of
-  // later vectors behind the arithmetic of earlier ones, which is worth more (36864 x 3072 bf16: 114 us against 132; from the copy 128 against
-  // 111); 32 columns of each of 512 threads leave no registers for either.
+  // later vectors behind the arithmetic of earlier ones, which is worth more (36864 x 3072 bf16: 111 us against 114; from the copy 113 against
+  // 102); 32 columns of each of 512 threads leave no registers for either.
   constexpr bool kCanFill = kNum * kVec <= 24 || (kThreads == 256 && (kCopy || kNum * kVec <= 32));
   if constexpr (kCanFill) {
     if (a.cols == int64_t{32} * p.warps * kNum * kVec) return launch_rows_in_ring<layer_norm_backward_ring_kernel<T, kVec, kNum, kThreads, kCopy, true>>(a, p, s);
