@@ -3,8 +3,9 @@
 A layer of a transformer keeps its input for its backward pass, two or four bytes an element.  The functions here keep the
 MXFP8 form that the quantized linears use (E4M3 codes, one E8M0 scale for 32 of a row: 1.03 bytes), write it in
 the same pass that computes the result, and read it in the backward pass without a dense copy in between.  Results of the forward pass are
-those of the dense input; gradients are the exact derivatives at the values that stand in the copy (the norm's with the
-statistics of the dense input).
+those of the dense input.  Gradients are taken at the values that stand in the copy: those of GELU and of a linear layer's weight are the
+exact derivatives there; the norm's are its formula with the copy's values in the input's place beside the statistics of the dense input,
+so not exactly the derivative of anything (these values' own mean and variance are others).
 
 * :func:`layer_norm`: over the last dimension, with a learned weight and bias or with one row of them for each sample
   (``weight_offset=1`` and the scale and shift of a modulated norm).  Differentiable with and without a copy of its input.

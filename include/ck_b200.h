@@ -302,7 +302,7 @@ CK_API int ck_scaled_mm_mxfp8_ws(const void* a, const void* b, const void* block
  *   h = (x - mean) * rstd,  y = h * f + bias,  f = weight_offset + weight (1 where weight is null)
  * x: [rows, cols] f32/f16/bf16 whose row r starts at (r / inner) * x_outer_stride + (r % inner) * x_inner_stride elements (rows are
  * contiguous; inner = rows for one level).  weight, bias (each may be null): one row of cols for every rows / groups consecutive
- * rows, weight_stride / bias_stride elements apart, of param_dtype, which is dtype or f32.  y: [rows, cols] contiguous.
+ * rows, weight_stride / bias_stride elements apart, of param_dtype, which is dtype or f32 (at most 32767 groups).  y: [rows, cols] contiguous.
  * mean, rstd: [rows] f32 for the backward pass, or both null.  codes, block_scales: null, or the MXFP8 copy of x as
  * ck_quantize_mxfp8 writes it (cols % 32 == 0, x's rows on 16-byte boundaries, cols at most 65536, f32 32768).
  */
@@ -344,7 +344,7 @@ CK_API int ck_gelu_mxfp8_backward(const void* dy, int dtype, const void* codes, 
  *   input:  dx[M,K] = dy[M,N] . deq(w)[N,K]
  * dy: f32/f16/bf16, row-major, 16-byte aligned; codes 32-byte, block scales 16-byte aligned; results of out_dtype, 32-byte aligned.  The MXFP8 values enter as
  * ck_dequantize_mxfp8 gives them in bf16 (exact for magnitudes of 2^-126 on), dy exactly; fp32 accumulation, one rounding, sums in a
- * fixed order.  K % 32 == 0, N % 8 == 0.  workspace: device memory, 256-byte aligned, of ck_linear_grad_mxfp8_workspace_bytes bytes
+ * fixed order.  What stands in the scales' padding has no part in them.  K % 32 == 0, N % 8 == 0.  workspace: device memory, 256-byte aligned, of ck_linear_grad_mxfp8_workspace_bytes bytes
  * (0: shape not supported), no requirement on its contents; calls that can overlap on the GPU need separate ones.
  */
 CK_API int64_t ck_linear_grad_mxfp8_workspace_bytes(int of_weight, int dy_dtype, int with_bias, int64_t M, int64_t N, int64_t K);
