@@ -350,7 +350,7 @@ __global__ void __launch_bounds__(kVec * kNum <= 16 ? 1024 : 512) layer_norm_for
   }
 }
 
-// The same for rows that do not lie on 16-byte boundaries (Columns and RowInRing in ck_layer_norm.cuh), without a copy.  36864 x 3071 fp16: 141 us
+// The same for rows that do not lie on 16-byte boundaries (Columns and RowInRing in ck_layer_norm.cuh), without a copy.  36864 x 3071 fp16: 140 us
 // against 455 for rows in registers without a ring, an element a load either way.
 template <typename T, int kVec, int kNum>
 __global__ void __launch_bounds__(512) layer_norm_forward_off_vectors_kernel(const ForwardArgs a, const uint32_t chunks, const uint32_t chunk_rows,
@@ -441,8 +441,8 @@ __global__ void __launch_bounds__(512) layer_norm_forward_off_vectors_kernel(con
     at = own.again();
 #pragma unroll
     for (int i = 0; i < kNum; ++i) {
-      f[i] = add_x2(f[i], make_float2(at.has(i) ? -mine : 0.0f, at.has(i, 1) ? -mine : 0.0f));
-      square[i & 1] = fma_x2(f[i], f[i], square[i & 1]);
+      const float2 d = add_x2(f[i], make_float2(at.has(i) ? -mine : 0.0f, at.has(i, 1) ? -mine : 0.0f));
+      square[i & 1] = fma_x2(d, d, square[i & 1]);
     }
     square[0] = add_x2(square[0], square[1]);
     float mean = mine, squares = warp_sum(square[0].x + square[0].y);
@@ -472,11 +472,11 @@ __global__ void __launch_bounds__(512) layer_norm_forward_off_vectors_kernel(con
     }
     T* const y = static_cast<T*>(a.y) + static_cast<int64_t>(row) * a.cols;
     at = own.again();
-    const float2 scale = both(rstd), shift = both((mine - mean) * rstd);  // as in the kernel for whole vectors, in one step
+    const float2 scale = both(rstd), shift = both(-mean);  // as in the kernel for whole vectors
 #pragma unroll
     for (int i = 0; i < kNum; ++i) {
       if (!at.has(i)) continue;
-      float2 v[1] = {fma_x2(f[i], scale, shift)};
+      float2 v[1] = {mul_x2(add_x2(f[i], shift), scale)};
       float2 w[1], b[1];
       at.shared_params(factor_buf, i, w);
       at.shared_params(bias_buf, i, b);
