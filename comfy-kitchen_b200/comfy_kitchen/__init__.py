@@ -41,6 +41,10 @@ __all__ = [
     "linear_checkpointed",
     "linear_weight_grad_mxfp8",
     "linear_input_grad_mxfp8",
+    "grouped_mm_mxfp8",
+    "grouped_linear_mxfp8",
+    "grouped_input_grad_mxfp8",
+    "quantize_experts_mxfp8",
     "swap_nibbles",
     "to_blocked",
     "from_blocked",
@@ -193,4 +197,10 @@ from .training import (  # noqa: E402
     linear_checkpointed,
     linear_input_grad_mxfp8,
     linear_weight_grad_mxfp8,
+)
+from .experts import (  # noqa: E402
+    grouped_input_grad_mxfp8,
+    grouped_linear_mxfp8,
+    grouped_mm_mxfp8,
+    quantize_experts_mxfp8,
 )

@@ -44,6 +44,9 @@ __all__ = [
     "gelu_mxfp8_backward",
     "linear_weight_grad_mxfp8",
     "linear_input_grad_mxfp8",
+    "grouped_mm_mxfp8",
+    "grouped_linear_mxfp8",
+    "grouped_input_grad_mxfp8",
     "check_device_status",
 ]
 
@@ -103,12 +106,18 @@ _SIGNATURES = {
     "ck_linear_grad_mxfp8_workspace_bytes": [_I, _I, _I, _L, _L, _L],
     "ck_linear_weight_grad_mxfp8": [_P, _I, _P, _P, _P, _I, _P, _L, _L, _L, _P, _L, _P],
     "ck_linear_input_grad_mxfp8": [_P, _I, _P, _P, _P, _I, _L, _L, _L, _P, _L, _P],
+    "ck_grouped_mm_mxfp8_workspace_bytes": [_I, _L, _L, _L],
+    "ck_grouped_mm_mxfp8": [_P, _P, _P, _P, _P, _P, _I, _P, _I, _L, _L, _L, _L, _P, _L, _P],
+    "ck_grouped_linear_mxfp8": [_P, _I, _P, _P, _P, _P, _I, _P, _I, _L, _L, _L, _L, _P, _L, _P],
+    "ck_grouped_input_grad_mxfp8_workspace_bytes": [_I, _L, _L, _L, _L],
+    "ck_grouped_input_grad_mxfp8": [_P, _I, _P, _P, _P, _P, _I, _L, _L, _L, _L, _P, _L, _P],
 }
 _RESTYPE = {"ck_last_error": ctypes.c_char_p, "ck_nvfp4_tensor_scale_scratch_bytes": ctypes.c_int64,
             "ck_quantize_nvfp4_dynamic_scratch_bytes": ctypes.c_int64, "ck_quantize_nvfp4_dynamic_whole_input_bytes": ctypes.c_int64,
             "ck_scaled_mm_workspace_bytes": ctypes.c_int64, "ck_linear_nvfp4_from_float_workspace_bytes": ctypes.c_int64,
             "ck_linear_mxfp8_from_float_workspace_bytes": ctypes.c_int64, "ck_layer_norm_backward_workspace_bytes": ctypes.c_int64,
-            "ck_linear_grad_mxfp8_workspace_bytes": ctypes.c_int64}
+            "ck_linear_grad_mxfp8_workspace_bytes": ctypes.c_int64, "ck_grouped_mm_mxfp8_workspace_bytes": ctypes.c_int64,
+            "ck_grouped_input_grad_mxfp8_workspace_bytes": ctypes.c_int64}
 
 
 def library_path() -> str:
@@ -1018,6 +1027,91 @@ def linear_input_grad_mxfp8(dy: torch.Tensor, w_codes: torch.Tensor, w_block_sca
 
 
 # ------------------------------------------------------------------------------------------
+# experts
+# ------------------------------------------------------------------------------------------
+_MAX_GROUPS = 1024
+
+
+def _experts_args(rows, w_codes, w_scales, offsets, bias, out_cols: bool):
+    """Checks of what the products with experts' weights share; ``rows`` is [M, K], or [M, N] for the gradient (``out_cols``)."""
+    _on_one_device(rows, w_codes, w_scales, offsets, bias)
+    assert w_codes.dim() == 3, "experts' weights are [experts, N, K]"
+    experts, n, k = w_codes.shape
+    assert 1 <= experts <= _MAX_GROUPS, f"1 to {_MAX_GROUPS} experts are supported, got {experts}"
+    assert k > 0 and k % 32 == 0 and n > 0 and n % 8 == 0, "K must be a multiple of 32 and N of 8"
+    assert rows.dim() == 2 and rows.shape[1] == (n if out_cols else k), "Matrix dimensions do not match"
+    assert w_scales.shape == (experts, roundup(n, 128), roundup(k // 32, 4)), "Invalid scale shape"
+    assert offsets.shape == (experts,) and offsets.dtype == torch.int32, "offsets must hold one int32 end for each expert"
+    assert w_codes.is_contiguous() and w_scales.is_contiguous() and offsets.is_contiguous(), "weights, scales and offsets must be contiguous"
+    bias_ptr, bias_code = None, 0
+    if bias is not None:
+        assert bias.shape == (experts, n), f"bias must be [{experts}, {n}]"
+        bias = _plain(bias)
+        bias = bias if bias.is_contiguous() else bias.contiguous()
+        bias_ptr, bias_code = bias.data_ptr(), DTYPE_TO_CODE.get(bias.dtype, 9)
+    return experts, n, k, bias, bias_ptr, bias_code
+
+
+def grouped_mm_mxfp8(a: torch.Tensor, b: torch.Tensor, block_scale_a: torch.Tensor, block_scale_b: torch.Tensor, offsets: torch.Tensor,
+                     bias: torch.Tensor | None = None, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """out[M, N]: row i of expert e = deq(a)[i] @ deq(b)[e].T + bias[e], with E4M3 a [M, K] and b [E, N, K] and their E8M0 scales."""
+    lib = load_library()
+    _on_one_device(a, block_scale_a)
+    a, b, block_scale_a, block_scale_b = _plain(a), _plain(b), _plain(block_scale_a), _plain(block_scale_b)
+    experts, n, k, bias, bias_ptr, bias_code = _experts_args(a, b, block_scale_b, offsets, bias, False)
+    m, dev, out_dtype = a.shape[0], a.device, out_dtype or torch.bfloat16
+    assert block_scale_a.shape == (roundup(m, 128), roundup(k // 32, 4)), "Invalid A scale shape"
+    assert a.is_contiguous() and block_scale_a.is_contiguous(), "operands must be contiguous"
+    out = torch.empty((m, n), dtype=out_dtype, device=dev)
+    if m > 0:
+        need = _workspace_bytes("ck_grouped_mm_mxfp8_workspace_bytes", 0, m, k, experts)
+        with _on_device(dev):
+            ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+            _check(lib.ck_grouped_mm_mxfp8(a.data_ptr(), b.data_ptr(), block_scale_a.data_ptr(), block_scale_b.data_ptr(), offsets.data_ptr(), bias_ptr,
+                                           bias_code, out.data_ptr(), DTYPE_TO_CODE[out_dtype], m, n, k, experts, ws.data_ptr(), need, _stream(dev)),
+                   "grouped_mm_mxfp8")
+    return out
+
+
+def grouped_linear_mxfp8(x: torch.Tensor, w_codes: torch.Tensor, w_block_scales: torch.Tensor, offsets: torch.Tensor,
+                         bias: torch.Tensor | None = None) -> torch.Tensor:
+    """:func:`grouped_mm_mxfp8` of dense rows x [M, K], quantized in the same call, in x's dtype."""
+    lib = load_library()
+    w_codes, w_block_scales = _plain(w_codes), _plain(w_block_scales)
+    experts, n, k, bias, bias_ptr, bias_code = _experts_args(x, w_codes, w_block_scales, offsets, bias, False)
+    x = _aligned(x, 16)
+    m, dev = x.shape[0], x.device
+    out = torch.empty((m, n), dtype=x.dtype, device=dev)
+    if m > 0:
+        need = _workspace_bytes("ck_grouped_mm_mxfp8_workspace_bytes", 1, m, k, experts)
+        with _on_device(dev):
+            ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+            _check(lib.ck_grouped_linear_mxfp8(x.data_ptr(), DTYPE_TO_CODE[x.dtype], w_codes.data_ptr(), w_block_scales.data_ptr(), offsets.data_ptr(),
+                                               bias_ptr, bias_code, out.data_ptr(), DTYPE_TO_CODE[x.dtype], m, n, k, experts, ws.data_ptr(), need,
+                                               _stream(dev)), "grouped_linear_mxfp8")
+    return out
+
+
+def grouped_input_grad_mxfp8(dy: torch.Tensor, w_codes: torch.Tensor, w_block_scales: torch.Tensor, offsets: torch.Tensor,
+                             out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """dx[M, K]: row i of expert e = dy[i] @ deq(w)[e], in ``out_dtype`` (dy's by default)."""
+    lib = load_library()
+    w_codes, w_block_scales = _plain(w_codes), _plain(w_block_scales)
+    experts, n, k, *_ = _experts_args(dy, w_codes, w_block_scales, offsets, None, True)
+    dy, w_codes = _aligned(dy, 16), _aligned(w_codes, 32)
+    m, dev, out_dtype = dy.shape[0], dy.device, out_dtype or dy.dtype
+    dx = torch.empty((m, k), dtype=out_dtype, device=dev)
+    if m > 0:
+        need = _workspace_bytes("ck_grouped_input_grad_mxfp8_workspace_bytes", DTYPE_TO_CODE[dy.dtype], m, n, k, experts)
+        with _on_device(dev):
+            ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+            _check(lib.ck_grouped_input_grad_mxfp8(dy.data_ptr(), DTYPE_TO_CODE[dy.dtype], w_codes.data_ptr(), w_block_scales.data_ptr(),
+                                                   offsets.data_ptr(), dx.data_ptr(), DTYPE_TO_CODE[out_dtype], m, n, k, experts, ws.data_ptr(), need,
+                                                   _stream(dev)), "grouped_input_grad_mxfp8")
+    return dx
+
+
+# ------------------------------------------------------------------------------------------
 # registration
 # ------------------------------------------------------------------------------------------
 def _build_constraints() -> dict:
@@ -1063,6 +1157,7 @@ def _build_constraints() -> dict:
                     "out_dtype": ParamConstraint(dtypes=floats)},
             default_devices=cuda_only, min_compute_capability=blackwell),
         **_training_constraints(cuda_only, floats, f32, blackwell),
+        **_experts_constraints(cuda_only, floats, blackwell),
     }
 
 
@@ -1093,17 +1188,34 @@ def _training_constraints(cuda_only, floats, f32, blackwell) -> dict:
     return {name: FunctionConstraints(params=p, default_devices=cuda_only, min_compute_capability=blackwell) for name, p in by_name.items()}
 
 
+def _experts_constraints(cuda_only, floats, blackwell) -> dict:
+    from comfy_kitchen.constraints import DivisibleBy, ExactDims, FunctionConstraints, ParamConstraint
+
+    rows, offsets = ParamConstraint(dtypes=floats, shape_rules=(ExactDims(2),)), ParamConstraint(dtypes=frozenset({torch.int32}), shape_rules=(ExactDims(1),))
+    e4m3 = frozenset({torch.float8_e4m3fn})
+    codes, scales = ParamConstraint(dtypes=e4m3, shape_rules=(ExactDims(3), DivisibleBy(2, 32))), ParamConstraint(dtypes=frozenset({torch.float8_e8m0fnu}))
+    weight = {"w_codes": codes, "w_block_scales": scales, "offsets": offsets}
+    by_name = {
+        "grouped_mm_mxfp8": {"a": ParamConstraint(dtypes=e4m3, shape_rules=(ExactDims(2), DivisibleBy(1, 32))), "b": codes, "block_scale_a": scales,
+                             "block_scale_b": scales, "offsets": offsets, "bias": ParamConstraint(dtypes=floats), "out_dtype": ParamConstraint(dtypes=floats)},
+        "grouped_linear_mxfp8": {"x": rows, **weight, "bias": ParamConstraint(dtypes=floats)},
+        "grouped_input_grad_mxfp8": {"dy": rows, **weight, "out_dtype": ParamConstraint(dtypes=floats)},
+    }
+    return {name: FunctionConstraints(params=p, default_devices=cuda_only, min_compute_capability=blackwell) for name, p in by_name.items()}
+
+
 _constraints: dict = {}  # as registered
 _stock = {name: globals()[name] for name in ("quantize_nvfp4", "quantize_nvfp4_dynamic", "quantize_mxfp8", "dequantize_nvfp4",
                                              "dequantize_mxfp8", "scaled_mm_nvfp4", "scaled_mm_mxfp8", "layer_norm_forward",
                                              "layer_norm_forward_mxfp8", "layer_norm_inference", "layer_norm_backward",
                                              "layer_norm_backward_mxfp8", "gelu_mxfp8_forward", "gelu_inference", "gelu_mxfp8_backward",
-                                             "linear_weight_grad_mxfp8", "linear_input_grad_mxfp8")}
+                                             "linear_weight_grad_mxfp8", "linear_input_grad_mxfp8", "grouped_mm_mxfp8", "grouped_linear_mxfp8",
+                                             "grouped_input_grad_mxfp8")}
 
 
 def host_function(name: str):
     """The native half of this module's function ``name``, or None: also where somebody has put another function in its place."""
-    return getattr(_host, name) if _host is not None and globals()[name] is _stock[name] else None
+    return getattr(_host, name, None) if _host is not None and globals()[name] is _stock[name] else None
 
 
 def host_step(name: str, functions: tuple[str, ...]):

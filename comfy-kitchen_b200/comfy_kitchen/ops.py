@@ -336,10 +336,58 @@ def _op_linear_input_grad_mxfp8(dy: torch.Tensor, w_codes: torch.Tensor, w_block
 def _(dy, w_codes, w_block_scales, output_dtype_code):
     return dy.new_empty((dy.shape[0], w_codes.shape[1]), dtype=DTYPE_CODE_TO_DTYPE[output_dtype_code])
 
+# ---- experts (no counterpart in the reference) ---------------------------------------------------------------------
+@torch.library.custom_op("comfy_kitchen::grouped_mm_mxfp8", mutates_args=())
+def _op_grouped_mm_mxfp8(a: torch.Tensor, b: torch.Tensor, block_scale_a: torch.Tensor, block_scale_b: torch.Tensor, offsets: torch.Tensor,
+                         bias: torch.Tensor | None, output_dtype_code: int) -> torch.Tensor:
+    return _impl("grouped_mm_mxfp8", {"a": a, "b": b, "block_scale_a": block_scale_a, "block_scale_b": block_scale_b, "offsets": offsets, "bias": bias,
+                                      "out_dtype": DTYPE_CODE_TO_DTYPE[output_dtype_code]})
+
+
+@_op_grouped_mm_mxfp8.register_fake
+def _(a, b, block_scale_a, block_scale_b, offsets, bias, output_dtype_code):
+    return a.new_empty((a.shape[0], b.shape[1]), dtype=DTYPE_CODE_TO_DTYPE[output_dtype_code])
+
+
+@torch.library.custom_op("comfy_kitchen::grouped_linear_mxfp8", mutates_args=())
+def _op_grouped_linear_mxfp8(x: torch.Tensor, w_codes: torch.Tensor, w_block_scales: torch.Tensor, offsets: torch.Tensor,
+                             bias: torch.Tensor | None) -> torch.Tensor:
+    return _impl("grouped_linear_mxfp8", {"x": x, "w_codes": w_codes, "w_block_scales": w_block_scales, "offsets": offsets, "bias": bias})
+
+
+@_op_grouped_linear_mxfp8.register_fake
+def _(x, w_codes, w_block_scales, offsets, bias):
+    return x.new_empty((x.shape[0], w_codes.shape[1]))
+
+
+@torch.library.custom_op("comfy_kitchen::grouped_input_grad_mxfp8", mutates_args=())
+def _op_grouped_input_grad_mxfp8(dy: torch.Tensor, w_codes: torch.Tensor, w_block_scales: torch.Tensor, offsets: torch.Tensor,
+                                 output_dtype_code: int) -> torch.Tensor:
+    return _impl("grouped_input_grad_mxfp8", {"dy": dy, "w_codes": w_codes, "w_block_scales": w_block_scales, "offsets": offsets,
+                                              "out_dtype": DTYPE_CODE_TO_DTYPE[output_dtype_code]})
+
+
+@_op_grouped_input_grad_mxfp8.register_fake
+def _(dy, w_codes, w_block_scales, offsets, output_dtype_code):
+    return dy.new_empty((dy.shape[0], w_codes.shape[2]), dtype=DTYPE_CODE_TO_DTYPE[output_dtype_code])
+
+
+def _grouped_setup(ctx, inputs, output):
+    _, w_codes, w_block_scales, offsets, _ = inputs
+    ctx.save_for_backward(w_codes, w_block_scales, offsets)
+
+
+def _grouped_backward(ctx, dy):
+    dx = torch.ops.comfy_kitchen.grouped_input_grad_mxfp8(dy, *ctx.saved_tensors, DTYPE_TO_CODE[dy.dtype]) if ctx.needs_input_grad[0] else None
+    return dx, None, None, None, None
+
+
+_op_grouped_linear_mxfp8.register_autograd(_grouped_backward, setup_context=_grouped_setup)
+
 
 if _registrations is not None and hasattr(_op_quantize_nvfp4, "_backend_fns") and hasattr(_op_quantize_nvfp4, "_disabled_kernel"):
     for _op in (_op_quantize_nvfp4, _op_dequantize_nvfp4, _op_scaled_mm_nvfp4, _op_quantize_mxfp8, _op_dequantize_mxfp8,
                 _op_scaled_mm_mxfp8, _op_layer_norm_forward, _op_layer_norm_forward_mxfp8, _op_layer_norm_backward,
                 _op_layer_norm_backward_mxfp8, _op_gelu_mxfp8_forward, _op_gelu_mxfp8_backward, _op_linear_weight_grad_mxfp8,
-                _op_linear_input_grad_mxfp8):
+                _op_linear_input_grad_mxfp8, _op_grouped_mm_mxfp8, _op_grouped_linear_mxfp8, _op_grouped_input_grad_mxfp8):
         _remember(_op)

@@ -17,7 +17,11 @@
 //
 // Bound by the tensor pipe and, in a loop, by the power limit: 4608 x 3072 x 12288 bf16 takes 214 us in the GEMM (1.63 PFLOP/s, the pipe 96 % active) and 231
 // with the launch before it; 4608 x 12288 x 3072 to fp32 with db 233 (86 %, the sums in parts) and 264 to 300.
+//
+// Rows that are grouped by expert: dX[i] = dY[i] W_e for the rows i of group e.  The same GEMM over a list of tiles that every CTA makes for itself
+// from the groups' ends; a tile begins at its group's first row, wherever in dY that is, and stores the group's rows alone.
 #include "ck_gemm_kernel.cuh"
+#include "ck_groups.cuh"
 #include "ck_rows.cuh"
 
 namespace ck {
@@ -28,7 +32,8 @@ constexpr int kDeep = 64;                           // contraction steps of a st
 constexpr int kOperandBytes = 128 * kDeep * 2;      // of A or B, stage and CTA
 constexpr int kPairRows = 256, kPairCols = 256;     // a tile
 constexpr int kBoxBytes = 64 * kDeep * 2;           // 64 rows (A) or columns (B) of an MN-major operand
-constexpr int kGradSmem = 1024 + kGradStages * 2 * kOperandBytes + 256;
+constexpr int grad_smem(bool grouped) { return 1024 + kGradStages * 2 * kOperandBytes + 256 + (grouped ? static_cast<int>(sizeof(groups::Table)) : 0); }
+static_assert(grad_smem(true) <= 227 * 1024, "shared memory budget exceeded");
 // Epilogue warps: eight, 128 columns each; for fp32 results, whose sums go on in registers, sixteen of 64.
 constexpr int grad_epilogue_warps(bool parts) { return parts ? 16 : 8; }
 constexpr int grad_threads(bool parts) { return 64 + 32 * grad_epilogue_warps(parts); }  // beside them producer and issuer
@@ -51,6 +56,8 @@ struct GradParams {
   const float* sum_partials;  // db's partial sums [sum_chunks][sum_cols], to be added beside the first main loop; null: none
   int sum_chunks, sum_cols, sum_dtype;
   void* sum_out;
+  const int* offsets;         // grouped rows: the groups' ends
+  int groups;
 };
 
 __device__ __forceinline__ void store_as(void* out, int dtype, int64_t at, float v) {
@@ -93,7 +100,7 @@ __device__ __forceinline__ int part_stages(int stages) {
   return (stages + parts - 1) / parts;
 }
 
-template <typename OutT, bool kMnA>
+template <typename OutT, bool kMnA, bool kGrouped>
 __global__ void __launch_bounds__(grad_threads(kInParts<OutT>), 1)
 grad_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const GradParams p) {
   pdl_launch_dependents();
@@ -111,7 +118,9 @@ grad_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
   uint64_t* acc_empty_bar = acc_full_bar + 2;                                                // epilogue -> MMAs
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty_bar + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  [[maybe_unused]] groups::Table* table = reinterpret_cast<groups::Table*>(smem + kGradStages * 2 * kOperandBytes + 256);
   static_assert((2 * kGradStages + 4) * 8 + 8 <= 256, "barrier area");
+  static_assert(!kGrouped || !kMnA, "the rows of the input's gradient are grouped");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (warp == 0 && lane == 0) {
@@ -129,13 +138,17 @@ grad_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     prefetch_tensormap(&map_b);
   }
   if (warp == 1) tmem_alloc<2>(tmem_slot, 512);
+  if constexpr (kGrouped) {
+    pdl_wait();  // the ends may come from the kernel before this one
+    groups::fill_table(table, p.offsets, p.groups, p.rows, kPairRows);
+  }
   tc_fence_before_sync();
   __syncthreads();
   cluster_sync_all();  // the other CTA's barriers exist before anything reports to them
   tc_fence_after_sync();
   const uint32_t tmem = *tmem_slot;
 
-  const int tiles = p.tiles_m * p.tiles_n, items = tiles * p.splits, all_stages = p.deep_stages * p.planes;
+  const int tiles = (kGrouped ? table->tiles[p.groups] : p.tiles_m) * p.tiles_n, items = tiles * p.splits, all_stages = p.deep_stages * p.planes;
   if (warp == 0) {
     // ---------------------------------------------------------------- loads
     if (elect_one()) {
@@ -145,9 +158,17 @@ grad_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       uint32_t ph = 0;
       for (int item = worker; item < items; item += workers) {
         const int split = item / tiles;
-        int tile_m, tile_n;
-        tile_place(p, item - split * tiles, &tile_m, &tile_n);
-        const int m0 = tile_m * kPairRows + static_cast<int>(rank) * 128, n0 = tile_n * kPairCols + static_cast<int>(rank) * 128;
+        int tile_m, tile_n, group = 0, m0 = static_cast<int>(rank) * 128;
+        if constexpr (kGrouped) {
+          const groups::Tile t = groups::place(table, p.groups, p.tiles_n, kPairRows, item);
+          m0 += t.row;
+          tile_n = t.tile_n;
+          group = t.group;
+        } else {
+          tile_place(p, item - split * tiles, &tile_m, &tile_n);
+          m0 += tile_m * kPairRows;
+        }
+        const int n0 = tile_n * kPairCols + static_cast<int>(rank) * 128;
         const int end = min(all_stages, (split + 1) * p.stages_per_split);
         for (int ks = split * p.stages_per_split; ks < end; ++ks) {
           // dY's smallest numbers first: what an accumulator adds is cut to the magnitude that it has reached
@@ -161,8 +182,13 @@ grad_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
           } else {
             tma_load_3d_pair(a_to, &map_a, bar, l0, m0, plane);
           }
-          tma_load_2d_pair(b_to, &map_b, bar, n0, l0);
-          tma_load_2d_pair(b_to + kBoxBytes, &map_b, bar, n0 + 64, l0);
+          if constexpr (kGrouped) {
+            tma_load_3d_pair(b_to, &map_b, bar, n0, l0, group);
+            tma_load_3d_pair(b_to + kBoxBytes, &map_b, bar, n0 + 64, l0, group);
+          } else {
+            tma_load_2d_pair(b_to, &map_b, bar, n0, l0);
+            tma_load_2d_pair(b_to + kBoxBytes, &map_b, bar, n0 + 64, l0);
+          }
           if (++s == kGradStages) {
             s = 0;
             ph ^= 1u;
@@ -243,14 +269,23 @@ grad_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         if (lane == 0) mbar_arrive_cluster(acc_empty + acc * 8);
       };
       // this thread's row of the tile, its warp's columns
+      int end = p.rows;
       const auto place = [&](int* row, int* col0) {
         int tile_m, tile_n;
-        tile_place(p, item - split * tiles, &tile_m, &tile_n);
-        *row = tile_m * kPairRows + static_cast<int>(rank) * 128 + quarter * 32 + lane;
+        *row = static_cast<int>(rank) * 128 + quarter * 32 + lane;
+        if constexpr (kGrouped) {
+          const groups::Tile t = groups::place(table, p.groups, p.tiles_n, kPairRows, item);
+          *row += t.row;
+          tile_n = t.tile_n;
+          end = t.end;
+        } else {
+          tile_place(p, item - split * tiles, &tile_m, &tile_n);
+          *row += tile_m * kPairRows;
+        }
         *col0 = tile_n * kPairCols + share * kWarpCols;
       };
       const auto write = [&](int row, int col, const uint32_t(&v)[32]) {
-        if (row < p.rows && col < p.cols) {
+        if (row < end && col < p.cols) {
           OutT* out = static_cast<OutT*>(p.out) + (static_cast<int64_t>(split) * p.rows + row) * p.cols + col;
           constexpr int kVec = 32 / static_cast<int>(sizeof(OutT));
 #pragma unroll
@@ -305,6 +340,15 @@ grad_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
           if (c == kWarpBoxes - 1) give_back(acc);  // read to the end
           write(row, col0 + c * 32, v);
         }
+      }
+    }
+    if constexpr (kGrouped) {  // rows behind the last group
+      constexpr int kVec = 16 / static_cast<int>(sizeof(OutT));
+      OutT* out = static_cast<OutT*>(p.out);
+      const int64_t first = static_cast<int64_t>(table->bound[p.groups]) * p.cols, n = static_cast<int64_t>(p.rows) * p.cols;
+      for (int64_t i = first + (static_cast<int64_t>(blockIdx.x) * (kWarps * 32) + threadIdx.x - 64) * kVec; i < n;
+           i += static_cast<int64_t>(gridDim.x) * (kWarps * 32) * kVec) {
+        rows::store(out + i, rows::zeros<OutT, kVec>());
       }
     }
   }
@@ -451,6 +495,32 @@ __global__ void __launch_bounds__(256) prepare_kernel(const PrepareArgs a) {
   prepare_sums<T>(a, block - a.plane_blocks, sum_buf);
 }
 
+// The same for grouped rows: a matrix [N, K] with scales of its own for each group; those of groups without rows are passed over.
+struct GroupedPrepareArgs {
+  PrepareArgs args;  // held_rows: of one matrix
+  const int* offsets;
+  int groups;
+};
+template <typename T>
+__global__ void __launch_bounds__(256) prepare_groups_kernel(const GroupedPrepareArgs g) {
+  pdl_launch_dependents();
+  const int block = blockIdx.x;
+  const PrepareArgs& a = g.args;
+  if (block < a.held_blocks) {
+    const int64_t each = ceil_div(a.held_rows * (a.held_cols >> 5), 256);  // blocks of one matrix
+    const int e = static_cast<int>(block / each);
+    pdl_wait();
+    if (groups::group_end(g.offsets, e, static_cast<int>(a.dy_rows)) <= groups::group_end(g.offsets, e - 1, static_cast<int>(a.dy_rows))) return;
+    PrepareArgs one = a;
+    one.codes += e * a.held_rows * a.held_cols;
+    one.scales += e * round_up(a.held_rows, 128) * round_up(a.held_cols >> 5, 4);
+    one.held += e * a.held_rows * a.held_cols;
+    return prepare_held(one, (block - e * each) * 256 + threadIdx.x);
+  }
+  pdl_wait();
+  if constexpr (!std::is_same<T, __nv_bfloat16>::value) prepare_planes<T>(a, (static_cast<int64_t>(block - a.held_blocks) * 256 + threadIdx.x) * 4);
+}
+
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
@@ -519,14 +589,14 @@ GradLayout grad_layout(bool weight, int dtype, bool bias, int64_t M, int64_t N, 
   return l;
 }
 
-template <typename OutT, bool kMnA>
+template <typename OutT, bool kMnA, bool kGrouped = false>
 int launch_grad_gemm(const CUtensorMap& map_a, const CUtensorMap& map_b, const GradParams& p, cudaStream_t stream) {
-  auto kernel = grad_gemm_kernel<OutT, kMnA>;
+  auto kernel = grad_gemm_kernel<OutT, kMnA, kGrouped>;
   int dev = 0;
   CK_CUDA(cudaGetDevice(&dev));
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(grad_threads(kInParts<OutT>));
-  cfg.dynamicSmemBytes = kGradSmem;
+  cfg.dynamicSmemBytes = grad_smem(kGrouped);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -541,7 +611,7 @@ int launch_grad_gemm(const CUtensorMap& map_a, const CUtensorMap& map_b, const G
   static std::atomic<int> resident_on[64];
   int resident = (dev >= 0 && dev < 64) ? resident_on[dev].load(std::memory_order_acquire) : 0;
   if (resident == 0) {
-    CK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kGradSmem));
+    CK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, grad_smem(kGrouped)));
     resident = sm_count() / 2;
     cfg.gridDim = dim3(resident * 2);
     int clusters = 0;
@@ -649,8 +719,95 @@ int linear_grad(bool weight, const char* op, const void* dy, int dtype, const vo
   }
 }
 
+// ---- grouped rows --------------------------------------------------------------------------------------------
+// Workspace: the groups' matrices in bf16 | dY's planes
+struct GroupedGradLayout {
+  int64_t planes_off, total;
+};
+GroupedGradLayout grouped_grad_layout(int dtype, int64_t M, int64_t N, int64_t K, int64_t E) {
+  GroupedGradLayout l;
+  l.planes_off = round_up(E * N * K * 2, 256);
+  l.total = l.planes_off + (planes_of(dtype) > 1 ? planes_of(dtype) * M * N * 2 : 0);
+  return l;
+}
+
+int check_grouped_grad(const char* op, int dtype, int64_t M, int64_t N, int64_t K, int64_t E) {
+  CK_REQUIRE(is_float(dtype), "%s: unsupported dtype code %d", op, dtype);
+  CK_REQUIRE(M > 0 && N > 0 && K > 0 && M < (1ll << 30) && N < (1ll << 30) && K < (1ll << 30), "%s: bad shape M=%lld N=%lld K=%lld", op,
+             (long long)M, (long long)N, (long long)K);
+  CK_REQUIRE(E > 0 && E <= groups::kMaxGroups, "%s: %lld groups, 1 to %d are supported", op, (long long)E, groups::kMaxGroups);
+  CK_REQUIRE(K % 32 == 0 && N % 8 == 0, "%s: K=%lld must be a multiple of 32 and N=%lld of 8", op, (long long)K, (long long)N);
+  CK_REQUIRE((M / kPairRows + E) * ceil_div(K, kPairCols) < (1ll << 30) && E * ceil_div(N * (K / 32), 256) + ceil_div(M * N, 1024) <= 0x7FFFFFFF,
+             "%s: too large", op);
+  return CK_OK;
+}
+
+int grouped_input_grad(const char* op, const void* dy, int dtype, const void* codes, const void* scales, const int* offsets, void* out, int out_dtype,
+                       int64_t M, int64_t N, int64_t K, int64_t E, void* workspace, int64_t workspace_bytes, cudaStream_t s) {
+  CK_REQUIRE(dy && codes && scales && offsets && out && workspace, "%s: null pointer", op);
+  if (int rc = check_grouped_grad(op, dtype, M, N, K, E)) return rc;
+  CK_REQUIRE(is_float(out_dtype), "%s: unsupported dtype code %d", op, out_dtype);
+  CK_REQUIRE(reinterpret_cast<uintptr_t>(dy) % 16 == 0 && reinterpret_cast<uintptr_t>(codes) % 32 == 0 && reinterpret_cast<uintptr_t>(scales) % 16 == 0 &&
+                 reinterpret_cast<uintptr_t>(out) % 32 == 0 && reinterpret_cast<uintptr_t>(workspace) % 256 == 0 &&
+                 reinterpret_cast<uintptr_t>(offsets) % 4 == 0,
+             "%s: dy, codes, block scales, result and workspace have to be aligned to 16, 32, 16, 32 and 256 bytes", op);
+  const GroupedGradLayout l = grouped_grad_layout(dtype, M, N, K, E);
+  CK_REQUIRE(workspace_bytes >= l.total, "%s: workspace of %lld bytes, %lld needed", op, (long long)workspace_bytes, (long long)l.total);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  const int planes = planes_of(dtype);
+  GroupedPrepareArgs g = {};
+  g.offsets = offsets;
+  g.groups = static_cast<int>(E);
+  g.args.codes = static_cast<const uint8_t*>(codes);
+  g.args.scales = static_cast<const uint8_t*>(scales);
+  g.args.held = reinterpret_cast<__nv_bfloat16*>(ws);
+  g.args.held_rows = N;
+  g.args.held_cols = K;
+  g.args.dy = dy;
+  g.args.planes = reinterpret_cast<__nv_bfloat16*>(ws + l.planes_off);
+  g.args.dy_rows = M;
+  g.args.dy_cols = N;
+  g.args.held_blocks = static_cast<int>(E * ceil_div(N * (K / 32), 256));
+  g.args.plane_blocks = planes > 1 ? static_cast<int>(ceil_div(M * N, 1024)) : 0;
+  auto prepare = dtype == CK_DTYPE_BF16 ? prepare_groups_kernel<__nv_bfloat16> : dtype == CK_DTYPE_F16 ? prepare_groups_kernel<__half> : prepare_groups_kernel<float>;
+  CK_CUDA(launch_pdl(prepare, dim3(static_cast<unsigned>(g.args.held_blocks + g.args.plane_blocks)), dim3(256), 0, s, g));
+  CUtensorMap map_a, map_b;
+  if (int rc = make_plane_map(&map_a, planes > 1 ? g.args.planes : dy, planes, M, N, 128, false)) return rc;
+  if (int rc = make_plane_map(&map_b, ws, E, N, K, kDeep, false)) return rc;
+  GradParams p = {};
+  p.rows = static_cast<int>(M);
+  p.cols = static_cast<int>(K);
+  p.deep_stages = static_cast<int>(ceil_div(N, kDeep));
+  p.planes = planes;
+  p.tiles_m = static_cast<int>(M / kPairRows + (E < M ? E : M));  // the most that the groups can have
+  p.tiles_n = static_cast<int>(ceil_div(K, kPairCols));
+  p.splits = 1;
+  p.stages_per_split = p.deep_stages * planes;
+  p.out = out;
+  p.offsets = offsets;
+  p.groups = static_cast<int>(E);
+  if (int rc = gemm_status_word(&p.status)) return rc;
+  switch (out_dtype) {
+    case CK_DTYPE_BF16: return launch_grad_gemm<__nv_bfloat16, false, true>(map_a, map_b, p, s);
+    case CK_DTYPE_F16: return launch_grad_gemm<__half, false, true>(map_a, map_b, p, s);
+    default: return launch_grad_gemm<float, false, true>(map_a, map_b, p, s);
+  }
+}
+
 }  // namespace
 }  // namespace ck
+
+extern "C" int64_t ck_grouped_input_grad_mxfp8_workspace_bytes(int dy_dtype, int64_t M, int64_t N, int64_t K, int64_t E) {
+  if (ck::check_grouped_grad("grouped_input_grad_mxfp8", dy_dtype, M, N, K, E) != CK_OK) return 0;
+  return ck::grouped_grad_layout(dy_dtype, M, N, K, E).total;
+}
+
+extern "C" int ck_grouped_input_grad_mxfp8(const void* dy, int dy_dtype, const void* w_codes, const void* w_block_scales, const int* offsets, void* dx,
+                                           int out_dtype, int64_t M, int64_t N, int64_t K, int64_t E, void* workspace, int64_t workspace_bytes,
+                                           void* stream) {
+  return ck::grouped_input_grad("grouped_input_grad_mxfp8", dy, dy_dtype, w_codes, w_block_scales, offsets, dx, out_dtype, M, N, K, E, workspace,
+                                workspace_bytes, static_cast<cudaStream_t>(stream));
+}
 
 extern "C" int64_t ck_linear_grad_mxfp8_workspace_bytes(int of_weight, int dy_dtype, int with_bias, int64_t M, int64_t N, int64_t K) {
   using namespace ck;

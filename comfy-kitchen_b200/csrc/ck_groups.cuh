@@ -1,0 +1,110 @@
+// Rows that are grouped by expert: group e has the rows [offsets[e - 1], offsets[e]) of a matrix (the first one from 0 on), ends that
+// lie on the device.  What every kernel on such rows shares: the bounds, kept inside the matrix whatever the ends say, and
+// the walk over the groups' tiles, whose number only the device knows.
+#pragma once
+
+#include "ck_common.cuh"
+
+namespace ck {
+namespace groups {
+
+constexpr int kMaxGroups = 1024;  // 8 KiB of shared memory for the table
+
+// A value that the kernel before this one may have written (see ld_f32_dependent).
+__device__ __forceinline__ int ld_s32_dependent(const int* p) {
+  int v;
+  asm volatile("ld.global.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+
+// First row behind group e, inside the matrix.
+__device__ __forceinline__ int group_end(const int* offsets, int e, int rows) {
+  return e < 0 ? 0 : min(max(ld_s32_dependent(offsets + e), 0), rows);
+}
+
+// Group of a row: the first whose end lies behind it, `count` if none does.  For ends that decrease it is still one whose
+// begin is not behind the row.
+__device__ __forceinline__ int group_of_row(const int* offsets, int count, int row) {
+  int lo = 0, hi = count;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (ld_s32_dependent(offsets + mid) > row) {
+      hi = mid;
+    } else {
+      lo = mid + 1;
+    }
+  }
+  return lo;
+}
+
+// Where the scale tiles (128 rows by 4 blocks, 512 bytes) of a group's own row blocks begin, in row blocks.  A group's first row is its
+// first tile's first row, so groups share no tile: with s and t its begin and end, ceil((t - s) / 128) <= t / 128 - s / 128 + 1
+// (whole quotients), which is the distance to the next group's.
+__host__ __device__ __forceinline__ int64_t first_scale_block(int begin, int e) { return (begin >> 7) + e; }
+__host__ __device__ __forceinline__ int64_t scale_blocks(int64_t rows, int64_t count) { return ceil_div(rows, 128) + count; }
+
+// In shared memory: the groups' bounds, and the numbers of row tiles before each.
+struct Table {
+  int bound[kMaxGroups + 1];  // group e: rows [bound[e], max(bound[e], bound[e + 1]))
+  int tiles[kMaxGroups + 1];  // row tiles of the groups before e
+};
+
+// Filled by all threads of the block, behind pdl_wait.
+__device__ __forceinline__ void fill_table(Table* t, const int* offsets, int count, int rows, int tile_rows) {
+  for (int e = threadIdx.x; e <= count; e += blockDim.x) t->bound[e] = group_end(offsets, e - 1, rows);
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    int before = 0;
+    for (int first = 0; first < count; first += 32) {
+      const int e = first + static_cast<int>(threadIdx.x);
+      const int own = e < count ? (max(t->bound[e + 1] - t->bound[e], 0) + tile_rows - 1) / tile_rows : 0;
+      int sum = own;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xFFFFFFFFu, sum, o);
+        if (static_cast<int>(threadIdx.x) >= o) sum += up;
+      }
+      if (e < count) t->tiles[e] = before + sum - own;
+      before += __shfl_sync(0xFFFFFFFFu, sum, 31);
+    }
+    if (threadIdx.x == 0) t->tiles[count] = before;
+  }
+  __syncthreads();
+}
+
+struct Tile {
+  int group;
+  int row;        // its first row in the matrix
+  int end;        // first row behind the group
+  int index;      // row tile within the group
+  int tile_n;
+};
+
+// Item -> tile.  A group's tiles follow one another, in bands of so many row tiles, down a band's rows first: the tiles that run together share
+// operands in L2.
+__device__ __forceinline__ Tile place(const Table* t, int count, int tiles_n, int tile_rows, int item) {
+  constexpr int kBand = 8;
+  int lo = 0, hi = count - 1;  // the last group with tiles[e] * tiles_n <= item
+  const int before = item / tiles_n;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (t->tiles[mid] <= before) {
+      lo = mid;
+    } else {
+      hi = mid - 1;
+    }
+  }
+  Tile p;
+  p.group = lo;
+  const int tiles_m = t->tiles[lo + 1] - t->tiles[lo], in_group = item - t->tiles[lo] * tiles_n;
+  const int band = in_group / (kBand * tiles_n), in_band = in_group - band * kBand * tiles_n;
+  const int height = min(kBand, tiles_m - band * kBand);
+  p.tile_n = in_band / height;
+  p.index = band * kBand + in_band - p.tile_n * height;
+  p.row = t->bound[lo] + p.index * tile_rows;
+  p.end = max(t->bound[lo], t->bound[lo + 1]);
+  return p;
+}
+
+}  // namespace groups
+}  // namespace ck

@@ -355,6 +355,31 @@ CK_API int ck_linear_input_grad_mxfp8(const void* dy, int dy_dtype, const void* 
                                void* dx, int out_dtype, int64_t M, int64_t N, int64_t K, void* workspace,
                                int64_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------ experts */
+/*
+ * Products of rows that are grouped by expert with the experts' MXFP8 weights, and the rows' gradients through them.  No counterpart in
+ * the reference.  Group e has the rows [offsets[e - 1], offsets[e]) (the first one from 0 on); offsets: [E] int32 on the device, not
+ * decreasing, at most M (other ends give unspecified rows, and no access outside the matrices); E at most 1024.
+ *   mm:         out[M,N]: row i = deq(a)[i] . deq(b)[e]^T + bias[e]     a E4M3 [M, K] with tiled E8M0 scales [roundup(M,128), roundup(K/32,4)]
+ *   linear:     the same with x in f32/f16/bf16, quantized as ck_quantize_mxfp8 does
+ *   input_grad: dx[M,K]: row i = dy[i] . deq(w)[e]                      dy f32/f16/bf16 [M, N], which enters exactly
+ * b, w: E4M3 [E, N, K], each matrix with tiled E8M0 scales [roundup(N,128), roundup(K/32,4)] of its own, one behind another.  bias: [E, N]
+ * f32/f16/bf16 or null.  Rows behind the last group are zeros.  fp32 accumulation, one rounding.  K % 32 == 0, N % 8 == 0.  Pointers are
+ * 16-byte aligned (input_grad: codes and result 32).  workspace: device memory, 256-byte aligned, of the given number of bytes (0: shape
+ * not supported), no requirement on its contents; calls that can overlap on the GPU need separate ones.
+ */
+CK_API int64_t ck_grouped_mm_mxfp8_workspace_bytes(int from_float, int64_t M, int64_t K, int64_t E);
+CK_API int ck_grouped_mm_mxfp8(const void* a, const void* b, const void* block_scale_a, const void* block_scale_b,
+                        const int* offsets, const void* bias, int bias_dtype, void* out, int out_dtype, int64_t M,
+                        int64_t N, int64_t K, int64_t E, void* workspace, int64_t workspace_bytes, void* stream);
+CK_API int ck_grouped_linear_mxfp8(const void* x, int x_dtype, const void* w, const void* w_block_scales, const int* offsets,
+                            const void* bias, int bias_dtype, void* out, int out_dtype, int64_t M, int64_t N,
+                            int64_t K, int64_t E, void* workspace, int64_t workspace_bytes, void* stream);
+CK_API int64_t ck_grouped_input_grad_mxfp8_workspace_bytes(int dy_dtype, int64_t M, int64_t N, int64_t K, int64_t E);
+CK_API int ck_grouped_input_grad_mxfp8(const void* dy, int dy_dtype, const void* w_codes, const void* w_block_scales,
+                                const int* offsets, void* dx, int out_dtype, int64_t M, int64_t N, int64_t K,
+                                int64_t E, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------------ multi-GPU (one node) */
 /*
  * Column-sharded GEMM with the all-gather of the output fused into the epilogue.  No
