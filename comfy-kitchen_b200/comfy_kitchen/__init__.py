@@ -45,6 +45,12 @@ __all__ = [
     "grouped_linear_mxfp8",
     "grouped_input_grad_mxfp8",
     "quantize_experts_mxfp8",
+    "rms_norm",
+    "rms_norm_forward",
+    "rms_norm_backward",
+    "rms_norm_mxfp8",
+    "grad_norm",
+    "clip_grad_norm_",
     "swap_nibbles",
     "to_blocked",
     "from_blocked",
@@ -197,6 +203,14 @@ from .training import (  # noqa: E402
     linear_checkpointed,
     linear_input_grad_mxfp8,
     linear_weight_grad_mxfp8,
+)
+from .norms import (  # noqa: E402
+    clip_grad_norm_,
+    grad_norm,
+    rms_norm,
+    rms_norm_backward,
+    rms_norm_forward,
+    rms_norm_mxfp8,
 )
 from .experts import (  # noqa: E402
     grouped_input_grad_mxfp8,

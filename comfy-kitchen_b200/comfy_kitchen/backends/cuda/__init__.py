@@ -47,6 +47,11 @@ __all__ = [
     "grouped_mm_mxfp8",
     "grouped_linear_mxfp8",
     "grouped_input_grad_mxfp8",
+    "rms_norm_forward",
+    "rms_norm_backward",
+    "rms_norm_mxfp8",
+    "grad_norm",
+    "clip_grads",
     "check_device_status",
 ]
 
@@ -106,6 +111,11 @@ _SIGNATURES = {
     "ck_linear_grad_mxfp8_workspace_bytes": [_I, _I, _I, _L, _L, _L],
     "ck_linear_weight_grad_mxfp8": [_P, _I, _P, _P, _P, _I, _P, _L, _L, _L, _P, _L, _P],
     "ck_linear_input_grad_mxfp8": [_P, _I, _P, _P, _P, _I, _L, _L, _L, _P, _L, _P],
+    "ck_rms_norm_forward": [_P, _I, _L, _L, _L, _L, _L, _P, _L, _L, _L, _P, _I, _F, _F, _P, _P, _P, _P, _P, _P],
+    "ck_rms_norm_backward_workspace_bytes": [_I, _L, _L],
+    "ck_rms_norm_backward": [_P, _I, _L, _L, _L, _L, _L, _P, _L, _L, _L, _P, _L, _L, _L, _P, _P, _I, _F, _P, _P, _P, _L, _P],
+    "ck_clip_grad_norm_workspace_bytes": [_L],
+    "ck_clip_grad_norm": [_P, _P, _P, _L, _F, _P, _P, _L, _P],
     "ck_grouped_mm_mxfp8_workspace_bytes": [_I, _L, _L, _L],
     "ck_grouped_mm_mxfp8": [_P, _P, _P, _P, _P, _P, _I, _P, _I, _L, _L, _L, _L, _P, _L, _P],
     "ck_grouped_linear_mxfp8": [_P, _I, _P, _P, _P, _P, _I, _P, _I, _L, _L, _L, _L, _P, _L, _P],
@@ -117,7 +127,8 @@ _RESTYPE = {"ck_last_error": ctypes.c_char_p, "ck_nvfp4_tensor_scale_scratch_byt
             "ck_scaled_mm_workspace_bytes": ctypes.c_int64, "ck_linear_nvfp4_from_float_workspace_bytes": ctypes.c_int64,
             "ck_linear_mxfp8_from_float_workspace_bytes": ctypes.c_int64, "ck_layer_norm_backward_workspace_bytes": ctypes.c_int64,
             "ck_linear_grad_mxfp8_workspace_bytes": ctypes.c_int64, "ck_grouped_mm_mxfp8_workspace_bytes": ctypes.c_int64,
-            "ck_grouped_input_grad_mxfp8_workspace_bytes": ctypes.c_int64}
+            "ck_grouped_input_grad_mxfp8_workspace_bytes": ctypes.c_int64, "ck_rms_norm_backward_workspace_bytes": ctypes.c_int64,
+            "ck_clip_grad_norm_workspace_bytes": ctypes.c_int64}
 
 
 def library_path() -> str:
@@ -1027,6 +1038,127 @@ def linear_input_grad_mxfp8(dy: torch.Tensor, w_codes: torch.Tensor, w_block_sca
 
 
 # ------------------------------------------------------------------------------------------
+# RMS norm
+# ------------------------------------------------------------------------------------------
+def _rms_args(x, weight, *others):
+    """Checks of what the norm and its gradient share: ``(cols, weight, dtype code of the weight)``."""
+    _on_one_device(x, weight, *others)
+    assert x.dim() >= 1 and x.shape[-1] > 0, "RMS norm needs rows of one element at least"
+    for t in others:
+        assert t is None or (t.shape == x.shape and t.dtype == x.dtype), "all tensors of a call must have the same shape and dtype"
+    cols = x.shape[-1]
+    if weight is None:
+        return cols, None, DTYPE_TO_CODE[x.dtype]
+    assert weight.shape == (cols,), f"the weight must be [{cols}], got {tuple(weight.shape)}"
+    assert weight.dtype in (x.dtype, torch.float32), "the weight must be of the input's dtype or float32"
+    weight = _plain(weight)
+    return cols, weight if weight.is_contiguous() else weight.contiguous(), DTYPE_TO_CODE[weight.dtype]
+
+
+def _rms_norm(x, weight, residual, eps, weight_offset, stats: bool, codes_too: bool):
+    lib = load_library()
+    cols, weight, code = _rms_args(x, weight, residual)
+    assert not codes_too or cols % 32 == 0, f"num_cols must be divisible by 32, got {cols}"
+    x, residual = _plain(x), None if residual is None else _plain(residual)
+    rows, dev = x.numel() // cols, x.device
+    y = codes = scales = None
+    if codes_too:
+        codes = torch.empty((rows, cols), dtype=torch.float8_e4m3fn, device=dev)
+        scales = torch.empty((roundup(rows, 128), roundup(cols // 32, 4)), dtype=torch.float8_e8m0fnu, device=dev)
+        if weight is not None and weight.data_ptr() % 16:
+            weight = weight.clone()
+    else:
+        y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    h = None if residual is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
+    rstd = torch.empty(rows, dtype=torch.float32, device=dev) if stats else None
+    if rows > 0:
+        align = 32 if codes_too else 1
+        x, inner, outer_stride, inner_stride = _row_levels(x, align)
+        r_levels = (None, 0, 0, 0) if residual is None else _row_levels(residual, align)
+        with _on_device(dev):
+            _check(lib.ck_rms_norm_forward(x.data_ptr(), DTYPE_TO_CODE[x.dtype], rows, cols, inner, outer_stride, inner_stride, _ptr(r_levels[0]),
+                                           *r_levels[1:], _ptr(weight), code, weight_offset, eps, _ptr(y), _ptr(h), _ptr(rstd), _ptr(codes), _ptr(scales),
+                                           _stream(dev)), "rms_norm_forward")
+    return y, h, rstd, codes, scales
+
+
+def rms_norm_forward(x: torch.Tensor, weight: torch.Tensor | None = None, residual: torch.Tensor | None = None, eps: float = 1e-6,
+                     weight_offset: float = 0.0) -> tuple[torch.Tensor, torch.Tensor | None, torch.Tensor]:
+    """``(y, h, rstd)``: ``h = x + residual`` (None without one), ``y = h * rstd * (weight_offset + weight)`` and fp32 ``rstd`` of each row."""
+    return _rms_norm(x, weight, residual, eps, weight_offset, True, False)[:3]
+
+
+def rms_norm_inference(x, weight=None, residual=None, eps: float = 1e-6, weight_offset: float = 0.0):
+    """``(y, h)`` of :func:`rms_norm_forward` for callers that need no statistics."""
+    return _rms_norm(x, weight, residual, eps, weight_offset, False, False)[:2]
+
+
+def rms_norm_mxfp8(x: torch.Tensor, weight: torch.Tensor | None = None, residual: torch.Tensor | None = None, eps: float = 1e-6,
+                   weight_offset: float = 0.0) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
+    """``(codes, block_scales, h)``: ``quantize_mxfp8`` of the norm's rows, from one pass."""
+    _, h, _, codes, scales = _rms_norm(x, weight, residual, eps, weight_offset, False, True)
+    return codes, scales, h
+
+
+def rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, rstd: torch.Tensor, weight: torch.Tensor | None = None, dh: torch.Tensor | None = None,
+                      weight_offset: float = 0.0, weight_grad: bool = True) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """``(dx, dweight)`` of :func:`rms_norm_forward`; ``dh`` is what reaches h by other ways.  Sums over rows are added in a fixed order."""
+    lib = load_library()
+    cols, weight, code = _rms_args(dy, weight, h, dh)
+    dy, h, dh = _plain(dy), _plain(h), None if dh is None else _plain(dh)
+    rows, dev = dy.numel() // cols, dy.device
+    assert rstd.shape == (rows,) and rstd.dtype == torch.float32 and rstd.is_contiguous() and rstd.device == dev, "rstd must hold one fp32 value for each row"
+    dx = torch.empty(dy.shape, dtype=dy.dtype, device=dev)
+    weight_grad = weight_grad and weight is not None
+    dweight = (torch.empty if rows > 0 else torch.zeros)(cols, dtype=weight.dtype, device=dev) if weight_grad else None
+    if rows > 0:
+        dy, *dy_levels = _row_levels(dy)
+        h, *h_levels = _row_levels(h)
+        dh, *dh_levels = (None, 0, 0, 0) if dh is None else _row_levels(dh)
+        need = _workspace_bytes("ck_rms_norm_backward_workspace_bytes", DTYPE_TO_CODE[dy.dtype], rows, cols) if weight_grad else 0
+        with _on_device(dev):
+            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+            _check(lib.ck_rms_norm_backward(dy.data_ptr(), DTYPE_TO_CODE[dy.dtype], rows, cols, *dy_levels, h.data_ptr(), *h_levels, _ptr(dh), *dh_levels,
+                                            rstd.data_ptr(), _ptr(weight), code, weight_offset, dx.data_ptr(), _ptr(dweight), _ptr(ws), need, _stream(dev)),
+                   "rms_norm_backward")
+    return dx, dweight
+
+
+# ------------------------------------------------------------------------------------------
+# gradients' norm
+# ------------------------------------------------------------------------------------------
+def _clip(grads, max_norm: float):
+    lib = load_library()
+    assert grads, "no tensors"
+    dev = grads[0].device
+    assert dev.type == "cuda", "gradients must be on the GPU"
+    for g in grads:
+        assert g.device == dev, "all gradients must be on one device"
+        assert g.dtype in (torch.float32, torch.float16, torch.bfloat16), f"gradients of {g.dtype} are not supported"
+        assert g.layout == torch.strided and g.is_contiguous(), "gradients must be contiguous"
+    n = len(grads)
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    need = _workspace_bytes("ck_clip_grad_norm_workspace_bytes", n)
+    with _on_device(dev):
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        _check(lib.ck_clip_grad_norm((ctypes.c_void_p * n)(*[g.data_ptr() for g in grads]), (ctypes.c_int64 * n)(*[g.numel() for g in grads]),
+                                     (ctypes.c_int * n)(*[DTYPE_TO_CODE[g.dtype] for g in grads]), n, max_norm, norm.data_ptr(), ws.data_ptr(), need,
+                                     _stream(dev)), "clip_grad_norm")
+    return norm
+
+
+def grad_norm(grads: list[torch.Tensor]) -> torch.Tensor:
+    """0-d fp32: the 2-norm of all elements of the tensors."""
+    return _clip(grads, -1.0)
+
+
+def clip_grads(grads: list[torch.Tensor], max_norm: float) -> torch.Tensor:
+    """:func:`grad_norm`, and every element times ``min(1, max_norm / (norm + 1e-6))``, in place."""
+    assert max_norm >= 0.0, f"max_norm must not be negative, got {max_norm}"
+    return _clip(grads, max_norm)
+
+
+# ------------------------------------------------------------------------------------------
 # experts
 # ------------------------------------------------------------------------------------------
 _MAX_GROUPS = 1024
@@ -1157,6 +1289,7 @@ def _build_constraints() -> dict:
                     "out_dtype": ParamConstraint(dtypes=floats)},
             default_devices=cuda_only, min_compute_capability=blackwell),
         **_training_constraints(cuda_only, floats, f32, blackwell),
+        **_norm_constraints(cuda_only, floats, f32, blackwell),
         **_experts_constraints(cuda_only, floats, blackwell),
     }
 
@@ -1188,6 +1321,22 @@ def _training_constraints(cuda_only, floats, f32, blackwell) -> dict:
     return {name: FunctionConstraints(params=p, default_devices=cuda_only, min_compute_capability=blackwell) for name, p in by_name.items()}
 
 
+def _norm_constraints(cuda_only, floats, f32, blackwell) -> dict:
+    from comfy_kitchen.constraints import FunctionConstraints, MinDims, ParamConstraint
+
+    any_rows, params = ParamConstraint(dtypes=floats, shape_rules=(MinDims(1),)), ParamConstraint(dtypes=floats)
+    forward = {"x": any_rows, "weight": params, "residual": any_rows}
+    by_name = {
+        "rms_norm_forward": forward,
+        "rms_norm_inference": forward,
+        "rms_norm_mxfp8": forward,
+        "rms_norm_backward": {"dy": any_rows, "h": any_rows, "rstd": ParamConstraint(dtypes=f32), "weight": params, "dh": any_rows},
+        "grad_norm": {},
+        "clip_grads": {},
+    }
+    return {name: FunctionConstraints(params=p, default_devices=cuda_only, min_compute_capability=blackwell) for name, p in by_name.items()}
+
+
 def _experts_constraints(cuda_only, floats, blackwell) -> dict:
     from comfy_kitchen.constraints import DivisibleBy, ExactDims, FunctionConstraints, ParamConstraint
 
@@ -1210,7 +1359,8 @@ _stock = {name: globals()[name] for name in ("quantize_nvfp4", "quantize_nvfp4_d
                                              "layer_norm_forward_mxfp8", "layer_norm_inference", "layer_norm_backward",
                                              "layer_norm_backward_mxfp8", "gelu_mxfp8_forward", "gelu_inference", "gelu_mxfp8_backward",
                                              "linear_weight_grad_mxfp8", "linear_input_grad_mxfp8", "grouped_mm_mxfp8", "grouped_linear_mxfp8",
-                                             "grouped_input_grad_mxfp8")}
+                                             "grouped_input_grad_mxfp8", "rms_norm_forward", "rms_norm_inference", "rms_norm_mxfp8",
+                                             "rms_norm_backward", "grad_norm", "clip_grads")}
 
 
 def host_function(name: str):
@@ -1226,7 +1376,7 @@ def host_step(name: str, functions: tuple[str, ...]):
     for function in functions:
         if globals()[function] is not _stock[function] or not registry.leaves_no_choice(function, _this_module, _constraints.get(function)):
             return None
-    return getattr(_host, name)
+    return getattr(_host, name, None)
 
 
 def host_operator(name: str):

@@ -336,6 +336,88 @@ def _op_linear_input_grad_mxfp8(dy: torch.Tensor, w_codes: torch.Tensor, w_block
 def _(dy, w_codes, w_block_scales, output_dtype_code):
     return dy.new_empty((dy.shape[0], w_codes.shape[1]), dtype=DTYPE_CODE_TO_DTYPE[output_dtype_code])
 
+# ---- RMS norm, clipping (no counterpart in the reference) ----------------------------------------------------------
+# An operator's results are tensors: where there is no residual, h is an empty one.
+@torch.library.custom_op("comfy_kitchen::rms_norm_forward", mutates_args=())
+def _op_rms_norm_forward(x: torch.Tensor, weight: torch.Tensor | None, residual: torch.Tensor | None, eps: float, weight_offset: float
+                         ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    y, h, rstd = _impl("rms_norm_forward", {"x": x, "weight": weight, "residual": residual, "eps": eps, "weight_offset": weight_offset})
+    return y, x.new_empty((0,)) if h is None else h, rstd
+
+
+@_op_rms_norm_forward.register_fake
+def _(x, weight, residual, eps, weight_offset):
+    rows = x.numel() // x.shape[-1]
+    return x.new_empty(x.shape), x.new_empty((0,) if residual is None else x.shape), x.new_empty((rows,), dtype=torch.float32)
+
+
+@torch.library.custom_op("comfy_kitchen::rms_norm_mxfp8", mutates_args=())
+def _op_rms_norm_mxfp8(x: torch.Tensor, weight: torch.Tensor | None, residual: torch.Tensor | None, eps: float, weight_offset: float
+                       ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    codes, scales, h = _impl("rms_norm_mxfp8", {"x": x, "weight": weight, "residual": residual, "eps": eps, "weight_offset": weight_offset})
+    return codes, scales, x.new_empty((0,)) if h is None else h
+
+
+@_op_rms_norm_mxfp8.register_fake
+def _(x, weight, residual, eps, weight_offset):
+    return (*_mxfp8_empty(x, x.numel() // x.shape[-1], x.shape[-1]), x.new_empty((0,) if residual is None else x.shape))
+
+
+@torch.library.custom_op("comfy_kitchen::rms_norm_backward", mutates_args=())
+def _op_rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, rstd: torch.Tensor, weight: torch.Tensor | None, dh: torch.Tensor | None,
+                          weight_offset: float, weight_grad: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    dx, dweight = _impl("rms_norm_backward", {"dy": dy, "h": h, "rstd": rstd, "weight": weight, "dh": dh, "weight_offset": weight_offset,
+                                              "weight_grad": weight_grad})
+    return dx, rstd.new_empty((0,)) if dweight is None else dweight
+
+
+@_op_rms_norm_backward.register_fake
+def _(dy, h, rstd, weight, dh, weight_offset, weight_grad):
+    return dy.new_empty(dy.shape), rstd.new_empty((0,)) if weight is None or not weight_grad else weight.new_empty(weight.shape)
+
+
+def _rms_setup(ctx, inputs, output):
+    x, weight, residual, _, ctx.weight_offset = inputs
+    ctx.save_for_backward(x if residual is None else output[1], output[2], weight)
+    ctx.has_residual = residual is not None
+    ctx.mark_non_differentiable(output[2])
+    ctx.set_materialize_grads(False)
+
+
+def _rms_backward(ctx, dy, dh, _):
+    h, rstd, weight = ctx.saved_tensors
+    need = ctx.needs_input_grad
+    dh = dh if ctx.has_residual else None
+    if dy is None:
+        return dh, None, dh if ctx.has_residual and need[2] else None, None, None
+    dx, dweight = torch.ops.comfy_kitchen.rms_norm_backward(dy, h, rstd, weight, dh, ctx.weight_offset, bool(need[1]))
+    # (a gradient of two inputs is given to each as its own tensor)
+    return dx if need[0] else None, dweight if need[1] else None, dx.clone() if ctx.has_residual and need[2] else None, None, None
+
+
+_op_rms_norm_forward.register_autograd(_rms_backward, setup_context=_rms_setup)
+
+
+@torch.library.custom_op("comfy_kitchen::grad_norm", mutates_args=())
+def _op_grad_norm(grads: list[torch.Tensor]) -> torch.Tensor:
+    return _impl("grad_norm", {"grads": grads})
+
+
+@_op_grad_norm.register_fake
+def _(grads):
+    return grads[0].new_empty((), dtype=torch.float32)
+
+
+@torch.library.custom_op("comfy_kitchen::clip_grads", mutates_args=("grads",))
+def _op_clip_grads(grads: list[torch.Tensor], max_norm: float) -> torch.Tensor:
+    return _impl("clip_grads", {"grads": grads, "max_norm": max_norm})
+
+
+@_op_clip_grads.register_fake
+def _(grads, max_norm):
+    return grads[0].new_empty((), dtype=torch.float32)
+
+
 # ---- experts (no counterpart in the reference) ---------------------------------------------------------------------
 @torch.library.custom_op("comfy_kitchen::grouped_mm_mxfp8", mutates_args=())
 def _op_grouped_mm_mxfp8(a: torch.Tensor, b: torch.Tensor, block_scale_a: torch.Tensor, block_scale_b: torch.Tensor, offsets: torch.Tensor,
@@ -389,5 +471,6 @@ if _registrations is not None and hasattr(_op_quantize_nvfp4, "_backend_fns") an
     for _op in (_op_quantize_nvfp4, _op_dequantize_nvfp4, _op_scaled_mm_nvfp4, _op_quantize_mxfp8, _op_dequantize_mxfp8,
                 _op_scaled_mm_mxfp8, _op_layer_norm_forward, _op_layer_norm_forward_mxfp8, _op_layer_norm_backward,
                 _op_layer_norm_backward_mxfp8, _op_gelu_mxfp8_forward, _op_gelu_mxfp8_backward, _op_linear_weight_grad_mxfp8,
-                _op_linear_input_grad_mxfp8, _op_grouped_mm_mxfp8, _op_grouped_linear_mxfp8, _op_grouped_input_grad_mxfp8):
+                _op_linear_input_grad_mxfp8, _op_grouped_mm_mxfp8, _op_grouped_linear_mxfp8, _op_grouped_input_grad_mxfp8,
+                _op_rms_norm_forward, _op_rms_norm_mxfp8, _op_rms_norm_backward, _op_grad_norm, _op_clip_grads):
         _remember(_op)

@@ -355,6 +355,48 @@ CK_API int ck_linear_input_grad_mxfp8(const void* dy, int dy_dtype, const void* 
                                void* dx, int out_dtype, int64_t M, int64_t N, int64_t K, void* workspace,
                                int64_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------ RMS norm, clipping */
+/*
+ * Root-mean-square norm over the last dimension, with the residual's addition.  No counterpart in the reference.
+ *   h = x + residual (rounded to their type; x itself without a residual),  rstd = 1 / sqrt(mean(h^2) + eps)
+ *   y = h * rstd * f,  f = weight_offset + weight (1 where weight is null)
+ * x, residual: [rows, cols] f32/f16/bf16, rows in two levels as ck_layer_norm_forward has them.  weight: [cols] of param_dtype, which is
+ * dtype or f32.  h: [rows, cols] contiguous, null exactly where residual is.  rstd: [rows] f32 or null.  Either y ([rows, cols] contiguous
+ * of dtype), or codes and block_scales: what ck_quantize_mxfp8 gives for y (cols % 32 == 0; rows of x and residual on
+ * 32-byte boundaries, h and codes too, the weight on a 16-byte one).  fp32 arithmetic, one rounding (codes: behind that to dtype).
+ */
+CK_API int ck_rms_norm_forward(const void* x, int dtype, int64_t rows, int64_t cols, int64_t x_inner, int64_t x_outer_stride,
+                        int64_t x_inner_stride, const void* residual, int64_t r_inner, int64_t r_outer_stride,
+                        int64_t r_inner_stride, const void* weight, int param_dtype, float weight_offset, float eps,
+                        void* y, void* h, float* rstd, void* codes, void* block_scales, void* stream);
+
+/*
+ * Its gradients: with g = dy * f and u = h * rstd
+ *   dx = dh + rstd * (g - u * mean(g * u)),  dweight = sum over the rows of dy * u
+ * dh, the gradient that reaches h by other ways, may be null, and so may dweight ([cols] of param_dtype).  dy, h and dh have their rows in two
+ * levels; dx [rows, cols] is contiguous.  Sums over rows are added in a fixed order.  workspace (not needed without dweight): device memory,
+ * 16-byte aligned, of ck_rms_norm_backward_workspace_bytes bytes, no requirement on its contents; calls that can overlap on the GPU
+ * need separate ones.
+ */
+CK_API int64_t ck_rms_norm_backward_workspace_bytes(int dtype, int64_t rows, int64_t cols);
+CK_API int ck_rms_norm_backward(const void* dy, int dtype, int64_t rows, int64_t cols, int64_t dy_inner, int64_t dy_outer_stride,
+                         int64_t dy_inner_stride, const void* h, int64_t h_inner, int64_t h_outer_stride,
+                         int64_t h_inner_stride, const void* dh, int64_t dh_inner, int64_t dh_outer_stride,
+                         int64_t dh_inner_stride, const float* rstd, const void* weight, int param_dtype,
+                         float weight_offset, void* dx, void* dweight, void* workspace, int64_t workspace_bytes,
+                         void* stream);
+
+/*
+ * The 2-norm of all elements of many tensors, and clipping by it: *norm = sqrt(sum of squares), every element times
+ * min(1, max_norm / (*norm + 1e-6)), in place (not touched where that is 1; a max_norm below zero: the norm alone).  grads, counts, dtypes:
+ * HOST arrays of `tensors` device addresses, numbers of elements and dtype codes (f32/f16/bf16, mixed at will); tensors that overlap are
+ * refused.  norm: f32 on the device.  fp32 squares, sums in a fixed order.  workspace: device memory, 4-byte aligned, of
+ * ck_clip_grad_norm_workspace_bytes bytes, no requirement on its contents; calls that can overlap on the GPU need separate ones.
+ */
+CK_API int64_t ck_clip_grad_norm_workspace_bytes(int64_t tensors);
+CK_API int ck_clip_grad_norm(void* const* grads, const int64_t* counts, const int* dtypes, int64_t tensors, float max_norm,
+                      float* norm, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------------ experts */
 /*
  * Products of rows that are grouped by expert with the experts' MXFP8 weights, and the rows' gradients through them.  No counterpart in
