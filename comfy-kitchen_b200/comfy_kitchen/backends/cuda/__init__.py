@@ -167,7 +167,9 @@ _HOST_NAMES = ("ck_quantize_nvfp4", "ck_quantize_nvfp4_dynamic_scratch_bytes", "
                "ck_scaled_mm_mxfp8_ws", "ck_linear_nvfp4_from_float_workspace_bytes", "ck_linear_nvfp4_from_float",
                "ck_linear_mxfp8_from_float_workspace_bytes", "ck_linear_mxfp8_from_float", "ck_layer_norm_forward",
                "ck_layer_norm_backward_workspace_bytes", "ck_layer_norm_backward", "ck_gelu_mxfp8_forward", "ck_gelu_mxfp8_backward",
-               "ck_linear_grad_mxfp8_workspace_bytes", "ck_linear_weight_grad_mxfp8", "ck_linear_input_grad_mxfp8", "ck_last_error")
+               "ck_linear_grad_mxfp8_workspace_bytes", "ck_linear_weight_grad_mxfp8", "ck_linear_input_grad_mxfp8",
+               "ck_rms_norm_forward", "ck_rms_norm_backward_workspace_bytes", "ck_rms_norm_backward", "ck_clip_grad_norm_workspace_bytes", "ck_clip_grad_norm",
+               "ck_grouped_mm_mxfp8_workspace_bytes", "ck_grouped_mm_mxfp8", "ck_grouped_linear_mxfp8", "ck_grouped_input_grad_mxfp8_workspace_bytes", "ck_grouped_input_grad_mxfp8", "ck_last_error")
 
 
 def _load_host(lib) -> None:
@@ -1365,7 +1367,7 @@ _stock = {name: globals()[name] for name in ("quantize_nvfp4", "quantize_nvfp4_d
 
 def host_function(name: str):
     """The native half of this module's function ``name``, or None: also where somebody has put another function in its place."""
-    return getattr(_host, name, None) if _host is not None and globals()[name] is _stock[name] else None
+    return getattr(_host, name) if _host is not None and globals()[name] is _stock[name] else None
 
 
 def host_step(name: str, functions: tuple[str, ...]):
@@ -1376,7 +1378,7 @@ def host_step(name: str, functions: tuple[str, ...]):
     for function in functions:
         if globals()[function] is not _stock[function] or not registry.leaves_no_choice(function, _this_module, _constraints.get(function)):
             return None
-    return getattr(_host, name, None)
+    return getattr(_host, name)
 
 
 def host_operator(name: str):

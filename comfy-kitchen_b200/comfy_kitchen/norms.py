@@ -127,11 +127,6 @@ class RMSNorm(nn.Module):
 # ---- gradients ---------------------------------------------------------------------------------
 def _list_call(name: str, grads: list[torch.Tensor], *args):
     if _eager(grads) and not replaced(name):
-        host = host_operator(name)
-        if host is not None:
-            out = host(grads, *args)
-            if out is not None:
-                return out
         out = _run(name, {"grads": grads, **({"max_norm": args[0]} if args else {})})
         if args:
             torch.autograd.graph.increment_version(grads)
@@ -157,6 +152,12 @@ def clip_grad_norm_(parameters: Iterable[torch.Tensor] | torch.Tensor, max_norm:
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must not be negative, got {max_norm}")
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    if not error_if_nonfinite:
+        host = host_step("clip_grad_norm", ("clip_grads",))
+        if host is not None:
+            norm = host(parameters, max_norm)
+            if norm is not None:
+                return norm
     grads = list({id(p): p.grad for p in parameters if p.grad is not None}.values())
     if not grads:
         return torch.zeros(())

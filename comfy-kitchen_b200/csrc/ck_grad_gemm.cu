@@ -103,7 +103,8 @@ __device__ __forceinline__ int part_stages(int stages) {
 template <typename OutT, bool kMnA, bool kGrouped>
 __global__ void __launch_bounds__(grad_threads(kInParts<OutT>), 1)
 grad_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const GradParams p) {
-  pdl_launch_dependents();
+  // Grouped rows: launched in plain stream order (launch_grad_gemm), so there is nothing to wait for, and what comes behind starts when this ends.
+  if constexpr (!kGrouped) pdl_launch_dependents();
   const uint32_t rank = cluster_cta_rank();
   const int worker = blockIdx.x >> 1, workers = gridDim.x >> 1;
   constexpr bool kParts = kInParts<OutT>;
@@ -138,21 +139,18 @@ grad_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     prefetch_tensormap(&map_b);
   }
   if (warp == 1) tmem_alloc<2>(tmem_slot, 512);
-  if constexpr (kGrouped) {
-    pdl_wait();  // the ends may come from the kernel before this one
-    groups::fill_table(table, p.offsets, p.groups, p.rows, kPairRows);
-  }
   tc_fence_before_sync();
   __syncthreads();
   cluster_sync_all();  // the other CTA's barriers exist before anything reports to them
   tc_fence_after_sync();
+  if constexpr (kGrouped) groups::fill_table(table, p.offsets, p.groups, p.rows, kPairRows);
   const uint32_t tmem = *tmem_slot;
 
   const int tiles = (kGrouped ? table->tiles[p.groups] : p.tiles_m) * p.tiles_n, items = tiles * p.splits, all_stages = p.deep_stages * p.planes;
   if (warp == 0) {
     // ---------------------------------------------------------------- loads
     if (elect_one()) {
-      pdl_wait();
+      if constexpr (!kGrouped) pdl_wait();
       const uint32_t full = smem_u32(full_bar), empty = smem_u32(empty_bar), a_addr = smem_u32(smem_a), b_addr = smem_u32(smem_b);
       int s = 0;
       uint32_t ph = 0;
@@ -200,7 +198,7 @@ grad_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMAs, by the pair's leader
     if (rank == 0) {
-      pdl_wait();  // nothing lands earlier: keeps the bounded waits from running beside a long predecessor
+      if constexpr (!kGrouped) pdl_wait();  // nothing lands earlier: keeps the bounded waits from running beside a long predecessor
       if (elect_one()) {
         const uint32_t full = smem_u32(full_bar), empty = smem_u32(empty_bar), acc_full = smem_u32(acc_full_bar);
         const uint32_t empty_peer = map_to_cta(empty, 1), acc_full_peer = map_to_cta(acc_full, 1);
@@ -242,7 +240,7 @@ grad_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     __syncwarp();
   } else {
     // ---------------------------------------------------------------- epilogue
-    pdl_wait();  // the result's buffer may belong to the kernel before this one
+    if constexpr (!kGrouped) pdl_wait();  // the result's buffer may belong to the kernel before this one
     const int quarter = warp & 3, share = (warp - 2) >> 2;
     const uint32_t acc_empty = map_to_cta(smem_u32(acc_empty_bar), 0);
     // db, whose partial sums the kernel before left: a column a thread, in the chunks' order, while the first tile computes
@@ -606,7 +604,9 @@ int launch_grad_gemm(const CUtensorMap& map_a, const CUtensorMap& map_b, const G
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  // Grouped rows without programmatic serialization: started beside the end of the long preparing kernel, with its wait in front of the
+  // cluster's first barrier, one of some twenty thousand passes did not end.
+  cfg.numAttrs = pdl_enabled() && !kGrouped ? 2 : 1;
   // all pairs resident at once: how many there is room for depends on where the SMs lie
   static std::atomic<int> resident_on[64];
   int resident = (dev >= 0 && dev < 64) ? resident_on[dev].load(std::memory_order_acquire) : 0;

@@ -92,15 +92,12 @@ grouped_gemm_kernel(const __grid_constant__ RowMaps maps_a, const __grid_constan
     }
   }
   if (warp == 1) tmem_alloc<CTAS>(tmem_slot, Cfg::kTmemCols);
+  tc_fence_before_sync();
+  __syncthreads();
+  if constexpr (CTAS == 2) cluster_sync_all();  // the other CTA's barriers exist before anything reports to them
+  tc_fence_after_sync();
   pdl_wait();  // ends, operands and scales may come from the kernel before this one
   groups::fill_table(table, p.offsets, p.groups, p.M, Cfg::kTileRows);
-  tc_fence_before_sync();
-  if constexpr (CTAS == 2) {
-    cluster_sync_all();  // the other CTA's barriers exist before anything reports to them
-  } else {
-    __syncthreads();
-  }
-  tc_fence_after_sync();
   const uint32_t tmem = *tmem_slot;
 
   const int items = table->tiles[p.groups] * p.tiles_n;

@@ -65,6 +65,21 @@ struct Library {
   int64_t (*linear_grad_mxfp8_workspace_bytes)(int, int, int, int64_t, int64_t, int64_t);
   int (*linear_weight_grad_mxfp8)(const void*, int, const void*, const void*, void*, int, void*, int64_t, int64_t, int64_t, void*, int64_t, void*);
   int (*linear_input_grad_mxfp8)(const void*, int, const void*, const void*, void*, int, int64_t, int64_t, int64_t, void*, int64_t, void*);
+  int (*rms_norm_forward)(const void*, int, int64_t, int64_t, int64_t, int64_t, int64_t, const void*, int64_t, int64_t, int64_t, const void*, int, float,
+                          float, void*, void*, float*, void*, void*, void*);
+  int64_t (*rms_norm_backward_workspace_bytes)(int, int64_t, int64_t);
+  int (*rms_norm_backward)(const void*, int, int64_t, int64_t, int64_t, int64_t, int64_t, const void*, int64_t, int64_t, int64_t, const void*, int64_t,
+                           int64_t, int64_t, const float*, const void*, int, float, void*, void*, void*, int64_t, void*);
+  int64_t (*clip_grad_norm_workspace_bytes)(int64_t);
+  int (*clip_grad_norm)(void* const*, const int64_t*, const int*, int64_t, float, float*, void*, int64_t, void*);
+  int64_t (*grouped_mm_mxfp8_workspace_bytes)(int, int64_t, int64_t, int64_t);
+  int (*grouped_mm_mxfp8)(const void*, const void*, const void*, const void*, const int*, const void*, int, void*, int, int64_t, int64_t, int64_t, int64_t,
+                          void*, int64_t, void*);
+  int (*grouped_linear_mxfp8)(const void*, int, const void*, const void*, const int*, const void*, int, void*, int, int64_t, int64_t, int64_t, int64_t,
+                              void*, int64_t, void*);
+  int64_t (*grouped_input_grad_mxfp8_workspace_bytes)(int, int64_t, int64_t, int64_t, int64_t);
+  int (*grouped_input_grad_mxfp8)(const void*, int, const void*, const void*, const int*, void*, int, int64_t, int64_t, int64_t, int64_t, void*, int64_t,
+                                  void*);
   const char* (*last_error)();
 };
 Library lib = {};
@@ -456,6 +471,9 @@ PyObject* linear_mxfp8_from_float(PyObject*, Args a, Py_ssize_t n_args) {  // x,
 // ---- training ---------------------------------------------------------------------------------
 #include "ck_host_training.h"
 
+// ---- RMS norm, clipping, experts ---------------------------------------------------------------
+#include "ck_host_layers.h"
+
 // ---- set-up -----------------------------------------------------------------------------------
 // bind({name: address of ck_<name>}, torch.nn.Parameter)
 PyObject* bind(PyObject*, Args a, Py_ssize_t n_args) {
@@ -494,6 +512,16 @@ PyObject* bind(PyObject*, Args a, Py_ssize_t n_args) {
   CK_TAKE(linear_grad_mxfp8_workspace_bytes);
   CK_TAKE(linear_weight_grad_mxfp8);
   CK_TAKE(linear_input_grad_mxfp8);
+  CK_TAKE(rms_norm_forward);
+  CK_TAKE(rms_norm_backward_workspace_bytes);
+  CK_TAKE(rms_norm_backward);
+  CK_TAKE(clip_grad_norm_workspace_bytes);
+  CK_TAKE(clip_grad_norm);
+  CK_TAKE(grouped_mm_mxfp8_workspace_bytes);
+  CK_TAKE(grouped_mm_mxfp8);
+  CK_TAKE(grouped_linear_mxfp8);
+  CK_TAKE(grouped_input_grad_mxfp8_workspace_bytes);
+  CK_TAKE(grouped_input_grad_mxfp8);
   CK_TAKE(last_error);
 #undef CK_TAKE
   if (!complete) {
@@ -521,6 +549,12 @@ PyMethodDef methods[] = {CK_METHOD(bind),
                          CK_METHOD(gelu_checkpointed),
                          CK_METHOD(linear_weight_grad_mxfp8),
                          CK_METHOD(linear_input_grad_mxfp8),
+                         CK_METHOD(rms_norm),
+                         CK_METHOD(rms_norm_mxfp8),
+                         CK_METHOD(clip_grad_norm),
+                         CK_METHOD(grouped_mm_mxfp8),
+                         CK_METHOD(grouped_linear_mxfp8),
+                         CK_METHOD(grouped_input_grad_mxfp8),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_ck_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
