@@ -40,7 +40,9 @@ _own: dict = {}  # operator -> (its definition, the kernels it was defined with,
 
 def _remember(op) -> None:
     name = op._name
-    _own[name] = (op, dict(op._backend_fns), frozenset(f"comfy_kitchen/{name}/{key}" for key in _KEYS_IN_FRONT))
+    # (an operator that changes its arguments comes with a kernel of torch's own in front, which counts the change)
+    in_front = frozenset(f"comfy_kitchen/{name}/{key}" for key in _KEYS_IN_FRONT).difference(_registrations)
+    _own[name] = (op, dict(op._backend_fns), in_front)
 
 
 def replaced(name: str) -> bool:
