@@ -73,6 +73,11 @@ bool grad_few_rows_applies(int64_t M, int64_t N, int64_t K, int planes);
 int grad_few_rows(const void* dy, int planes, const void* codes, const void* scales, void* out, int out_dtype, int64_t M, int64_t N, int64_t K,
                   cudaStream_t stream);
 
+// The same for rows that are grouped by expert: rows of a tile, or 0 where the groups have too many.
+int grouped_few_rows_applies(int64_t M, int64_t N, int64_t K, int64_t E, int planes);
+int grouped_few_rows(const void* dy, int planes, const void* codes, const void* scales, const int* offsets, void* out, int out_dtype, int64_t M, int64_t N,
+                     int64_t K, int64_t E, cudaStream_t stream);
+
 // ---- programmatic dependent launch ------------------------------------------------------
 // The streaming kernels and the GEMMs of this library are launched with programmatic stream
 // serialization: each kernel lets its successor start being scheduled at once

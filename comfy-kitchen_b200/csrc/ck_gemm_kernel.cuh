@@ -1234,6 +1234,10 @@ EncodeTiledFn encode_tiled_fn() {
       fn = reinterpret_cast<EncodeTiledFn>(sym);
     }
   });
+  // The driver's call wants the device's context current on this thread, which the runtime has not made so where this is the thread's first
+  // call (a gradient on the autograd engine's thread).
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return nullptr;
   return fn;
 }
 

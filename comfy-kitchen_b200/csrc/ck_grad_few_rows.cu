@@ -10,9 +10,14 @@
 // The CTAs of a cluster share a strip's rows and add their sums through distributed shared memory, in their order.
 // Warp-wide MMAs (m16n8k16) in place of tcgen05 took 17 to 28 us for these sizes: one takes about 40 cycles here, and its
 // fragments want two rows' codes in one register.  dY in fp16 or fp32 enters as two or three bf16 numbers, exactly, as in the GEMM.
+//
+// Rows that are grouped by expert, few for each: the same stages in a kernel that stays.  A CTA takes tiles of up to a.padded rows of one group by
+// 128 columns one after another; its steps are numbered through all of them, so that the rings and their phases go on from tile to tile, and four
+// more warps store a tile's result while the others are at the next one.
 #include <atomic>
 
 #include "ck_gemm_kernel.cuh"
+#include "ck_groups.cuh"
 #include "ck_rows.cuh"
 
 namespace ck {
@@ -313,6 +318,271 @@ grad_few_rows_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_co
   if (warp == kCodeWarps + 1) tmem_dealloc<1>(tmem, tmem_cols);
 }
 
+// ---- grouped rows --------------------------------------------------------------------------------------------
+constexpr int kStoreWarps = 4, kGroupedThreads = kThreads + 32 * kStoreWarps;
+
+struct GroupedFewRowsArgs {
+  const uint8_t* scales;
+  void* out;
+  const int* offsets;
+  int out_dtype;
+  int groups, M, N, K;
+  int padded;       // rows of a tile, a multiple of 16
+  int planes;       // bf16 numbers whose sum is an element of dY
+  int parts;        // accumulators that the first of them take in turn; the others have one each, in front of these
+  int sets;         // of accumulators: two where tensor memory holds them, so that a tile is stored beside the next one's steps
+  int stages, raw_stages;
+  int strips;
+  int* status;
+};
+
+// A code and its scale for four rows of the operand, as the kernel above decodes them.
+__device__ __forceinline__ void decode_stage(const uint8_t* raw, uint32_t row_at, int row0, int unit, int step, int left) {
+  constexpr int kItems = kDeep / (4 * kGroupWarps);
+  const uint32_t low = ((unit & 3) * 2) ^ (row0 & 7), high = low ^ 1;
+#pragma unroll
+  for (int i = 0; i < kItems; ++i) {
+    const int row = row0 + 4 * kGroupWarps * i;
+    const uint4 codes = *reinterpret_cast<const uint4*>(raw + row * kCols + unit * 16);
+    uint32_t byte = raw[kDeep * kCols + (unit >> 1) + (row & 31) * 16 + (row >> 5) * 4 + (step & 1) * 8];  // a tile of scales is two stages high
+    if (row >= left) byte = 0;  // what stands for rows past the last one is nobody's
+    const float2 factor = both(e8m0_factor(byte));
+    const uint2 v0 = decode_four(codes.x, factor), v1 = decode_four(codes.y, factor);
+    const uint2 v2 = decode_four(codes.z, factor), v3 = decode_four(codes.w, factor);
+    const uint32_t to = row_at + 4 * kGroupWarps * i * 128;
+    st_shared_128(to + (low << 4), v0.x, v0.y, v1.x, v1.y);
+    st_shared_128(to + (high << 4), v2.x, v2.y, v3.x, v3.y);
+  }
+}
+
+__global__ void __launch_bounds__(kGroupedThreads)
+grouped_few_rows_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_constant__ CUtensorMap map_codes, const GroupedFewRowsArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t full_bar[kMaxStages], empty_bar[kMaxStages], raw_full_bar[kMaxRaw], raw_empty_bar[kMaxRaw], acc_full_bar[2], acc_empty_bar[2];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag;
+  pdl_launch_dependents();
+  uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));  // the operands' stages
+  uint8_t* const raw = smem + a.stages * (kHeldBytes + a.planes * a.padded * 128);                                       // the codes' stages
+  groups::Table* const table = reinterpret_cast<groups::Table*>(raw + a.raw_stages * kRawBytes);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int steps = (a.N + kDeep - 1) / kDeep;
+  const int plane_bytes = a.padded * 128, stage_bytes = kHeldBytes + a.planes * plane_bytes;
+  const int minor = a.planes - 1, set_cols = (minor + a.parts) * a.padded;
+  uint32_t tmem_cols = 32;
+  while (static_cast<int>(tmem_cols) < a.sets * set_cols) tmem_cols *= 2;
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int s = 0; s < a.stages; ++s) {
+      mbar_init(&full_bar[s], kGroupWarps + 1);  // the decoding warps, the loads of dY
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int s = 0; s < a.raw_stages; ++s) {
+      mbar_init(&raw_full_bar[s], 1);
+      mbar_init(&raw_empty_bar[s], kGroupWarps);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&acc_full_bar[s], 1);
+      mbar_init(&acc_empty_bar[s], kStoreWarps);
+    }
+    fence_barrier_init();
+    prefetch_tensormap(&map_dy);
+    prefetch_tensormap(&map_codes);
+  }
+  if (warp == kCodeWarps + 1) tmem_alloc<1>(&tmem_slot, tmem_cols);
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = tmem_slot;
+  const uint32_t full = smem_u32(full_bar), empty = smem_u32(empty_bar), raw_full = smem_u32(raw_full_bar), raw_empty = smem_u32(raw_empty_bar);
+  pdl_wait();
+  groups::fill_table(table, a.offsets, a.groups, a.M, a.padded);
+  // Tiles of this CTA: items worker, worker + workers, ...  Its steps count through them.
+  const int items = table->tiles[a.groups] * a.strips, worker = blockIdx.x, workers = gridDim.x;
+  const int mine = worker < items ? (items - worker + workers - 1) / workers : 0;
+  const auto place = [&](int i) { return groups::place(table, a.groups, a.strips, a.padded, worker + i * workers); };
+
+  if (warp < kCodeWarps) {
+    // ---------------------------------------------------------------- decoding
+    const int group = warp / kGroupWarps, odd = (lane >> 2) & 1, unit = (lane & 3) + (odd ^ ((lane >> 3) & 1)) * 4;
+    const int row0 = warp % kGroupWarps * 4 + odd + (lane >> 4) * 2;
+    const uint32_t row_at = smem_u32(smem) + (unit >> 2) * kBoxBytes + row0 * 128;
+    int stage = group, raw_stage = group;
+    uint32_t phase = 0, raw_phase = 0;
+    int step = group;  // within its tile
+    for (int left_tiles = mine; left_tiles > 0; step += kGroups) {
+      while (step >= steps) {
+        step -= steps;
+        if (--left_tiles == 0) break;
+      }
+      if (left_tiles == 0) break;
+      mbar_wait(raw_full + raw_stage * 8, raw_phase, &abort_flag);
+      mbar_wait(empty + stage * 8, phase ^ 1, &abort_flag);
+      decode_stage(raw + raw_stage * kRawBytes, row_at + stage * stage_bytes, row0, unit, step, a.N - step * kDeep);
+      fence_proxy_async();  // the MMAs read what was written here
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&raw_empty_bar[raw_stage]);
+        mbar_arrive(&full_bar[stage]);
+      }
+      stage += kGroups;
+      if (stage >= a.stages) {
+        stage -= a.stages;
+        phase ^= 1u;
+      }
+      raw_stage += kGroups;
+      if (raw_stage >= a.raw_stages) {
+        raw_stage -= a.raw_stages;
+        raw_phase ^= 1u;
+      }
+    }
+  } else if (warp == kCodeWarps) {
+    // ---------------------------------------------------------------- loads: codes and scales as far ahead as their ring goes, dY with its stage
+    if (elect_one() && mine > 0) {
+      const int64_t col_tiles = (a.K / 32 + 3) >> 2, group_tiles = (a.N + 127) / 128 * col_tiles;
+      int stage = 0, raw_stage = 0, ahead_item = 0, ahead_step = 0, fetched = 0;
+      uint32_t phase = 0, raw_phase = 0;
+      groups::Tile ahead = place(0);
+      const auto fetch = [&]() {
+        mbar_wait(raw_empty + raw_stage * 8, raw_phase ^ 1, &abort_flag);
+        const uint32_t bar = raw_full + raw_stage * 8, to = smem_u32(raw) + raw_stage * kRawBytes;
+        mbar_arrive_expect_tx(bar, kRawBytes);
+        asm volatile(
+            "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(to),
+            "l"(reinterpret_cast<uint64_t>(&map_codes)), "r"(bar), "r"(ahead.tile_n * kCols), "r"(ahead_step * kDeep), "r"(ahead.group)
+            : "memory");
+        bulk_load_1d(to + kDeep * kCols, a.scales + (ahead.group * group_tiles + (ahead_step >> 1) * col_tiles + ahead.tile_n) * kScaleBytes, kScaleBytes, bar);
+        ++fetched;
+        if (++ahead_step == steps) {
+          ahead_step = 0;
+          if (++ahead_item < mine) ahead = place(ahead_item);
+        }
+        if (++raw_stage == a.raw_stages) {
+          raw_stage = 0;
+          raw_phase ^= 1u;
+        }
+      };
+      while (ahead_item < mine && fetched < a.raw_stages) fetch();
+      for (int i = 0; i < mine; ++i) {
+        const groups::Tile t = place(i);
+        for (int step = 0; step < steps; ++step) {
+          mbar_wait(empty + stage * 8, phase ^ 1, &abort_flag);
+          const uint32_t bar = full + stage * 8, to = smem_u32(smem) + stage * stage_bytes + kHeldBytes;
+          mbar_arrive_expect_tx(bar, a.planes * plane_bytes);
+          for (int p = 0; p < a.planes; ++p) {
+            asm volatile(
+                "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(to + p * plane_bytes),
+                "l"(reinterpret_cast<uint64_t>(&map_dy)), "r"(bar), "r"(step * kDeep), "r"(t.row), "r"(p)
+                : "memory");
+          }
+          if (++stage == a.stages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+          if (ahead_item < mine) fetch();
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == kCodeWarps + 1) {
+    // ---------------------------------------------------------------- MMAs
+    if (elect_one()) {
+      const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (static_cast<uint32_t>(a.padded >> 3) << 17) | ((kCols >> 4) << 24);
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int i = 0; i < mine; ++i) {
+        const int set = a.sets == 2 ? i & 1 : 0;
+        const uint32_t base = tmem + set * set_cols;
+        mbar_wait(&acc_empty_bar[set], ((i / a.sets) & 1) ^ 1, &abort_flag);
+        tc_fence_after_sync();
+        int part = 0;
+        for (int step = 0; step < steps; ++step) {
+          mbar_wait(full + stage * 8, phase, &abort_flag);
+          tc_fence_after_sync();
+          const uint32_t at = smem_u32(smem) + stage * stage_bytes;
+          const uint64_t held = make_smem_desc(at, kBoxBytes, 1024, 2);
+          for (int p = 0; p < a.planes; ++p) {
+            const uint32_t to = base + (p == 0 ? (minor + part) * a.padded : (minor - p) * a.padded);  // the smallest in front
+            const bool begins = step == (p == 0 ? part : 0);
+            const uint64_t dy = make_operand_desc_sw128(at + kHeldBytes + p * plane_bytes);
+#pragma unroll
+            for (int q = 0; q < kDeep / 16; ++q) {  // 16 rows of 128 bytes, 32 bytes
+              mma_bf16(to, held + q * (2048 >> 4), dy + q * (32 >> 4), idesc, !begins || q != 0);
+            }
+          }
+          tc_commit<1>(empty + stage * 8);
+          if (++part == a.parts) part = 0;
+          if (++stage == a.stages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        tc_commit<1>(smem_u32(&acc_full_bar[set]));
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---------------------------------------------------------------- results: a warp has 32 of the strip's columns, one a lane
+    const int quarter = warp & 3, accumulators = minor + min(a.parts, steps);
+    for (int i = 0; i < mine; ++i) {
+      const groups::Tile t = place(i);
+      const int set = a.sets == 2 ? i & 1 : 0, k = t.tile_n * kCols + quarter * 32 + lane, count = min(a.padded, t.end - t.row);
+      mbar_wait(&acc_full_bar[set], (i / a.sets) & 1, &abort_flag);
+      __syncwarp();
+      tc_fence_after_sync();
+      for (int m0 = 0; m0 < count; m0 += 16) {
+        float f[16] = {};
+        for (int n = 0; n < accumulators; ++n) {
+          uint32_t v[16];
+          tmem_load_32x16(tmem + set * set_cols + (static_cast<uint32_t>(quarter * 32) << 16) + n * a.padded + m0, v);
+          tmem_load_wait();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) f[j] += __uint_as_float(v[j]);
+        }
+        if (m0 + 16 >= count) {  // read to the end
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&acc_empty_bar[set]);
+        }
+        if (k < a.K) {
+          const int64_t at = static_cast<int64_t>(t.row + m0) * a.K + k;
+          const auto store_rows = [&](auto* out) {
+            using OutT = std::remove_pointer_t<decltype(out)>;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              if (m0 + j < count) out[at + static_cast<int64_t>(j) * a.K] = from_float<OutT>(f[j]);
+            }
+          };
+          if (a.out_dtype == CK_DTYPE_BF16) {
+            store_rows(static_cast<__nv_bfloat16*>(a.out));
+          } else if (a.out_dtype == CK_DTYPE_F16) {
+            store_rows(static_cast<__half*>(a.out));
+          } else {
+            store_rows(static_cast<float*>(a.out));
+          }
+        }
+        __syncwarp();
+      }
+    }
+    // rows behind the last group, in units of 16 bytes (K is a multiple of 32)
+    const int64_t size = a.out_dtype == CK_DTYPE_F32 ? 4 : 2;
+    const int64_t begin = static_cast<int64_t>(table->bound[a.groups]) * a.K * size, end = static_cast<int64_t>(a.M) * a.K * size;
+    for (int64_t at = begin + (static_cast<int64_t>(blockIdx.x) * (32 * kStoreWarps) + threadIdx.x - kThreads) * 16; at < end;
+         at += static_cast<int64_t>(gridDim.x) * (32 * kStoreWarps) * 16) {
+      *reinterpret_cast<uint4*>(static_cast<uint8_t*>(a.out) + at) = make_uint4(0, 0, 0, 0);
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  if (abort_flag) {
+    if (threadIdx.x == 0) atomicExch(a.status, 1);
+    for (int i = 0; i < 200; ++i) __nanosleep(1000);  // copies that are in flight land before the memory is released
+    __syncthreads();
+  }
+  if (warp == kCodeWarps + 1) tmem_dealloc<1>(tmem, tmem_cols);
+}
+
 int make_code_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols) {
   return cached_map(map, MapKey{12, base, rows, cols, kDeep, 0}, [&](CUtensorMap* m) {
     EncodeTiledFn fn = encode_tiled_fn();
@@ -423,6 +693,88 @@ int grad_few_rows(const void* dy, int planes, const void* codes, const void* sca
   cfg.attrs = attr;
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
   CK_CUDA(cudaLaunchKernelEx(&cfg, grad_few_rows_kernel, map_dy, map_codes, a));
+  return CK_OK;
+}
+
+// ---- grouped rows --------------------------------------------------------------------------------------------
+namespace {
+
+constexpr int kGroupedSmem = 226 * 1024 - 1024;  // dynamic, beside the barriers
+
+// Rows of a tile for so many of a group, 0 if there are too many for their operand to find room.
+int grouped_few_rows_tile(int64_t rows, int planes) {
+  const int64_t padded = round_up(rows, 16);
+  const int64_t stage = kHeldBytes + planes * padded * 128;
+  return padded <= 256 && kMinStages * stage <= kGroupedSmem - 1024 - kGroups * kRawBytes - static_cast<int64_t>(sizeof(groups::Table)) ? static_cast<int>(padded) : 0;
+}
+
+// E4M3 [E, N, K], boxes of 128 columns x 64 rows of one matrix, as they lie in memory; rows past N and columns past K read as zeros.
+int make_experts_code_map(CUtensorMap* map, const void* base, int64_t E, int64_t N, int64_t K) {
+  return cached_map(map, MapKey{13, base, E, N, K, 0}, [&](CUtensorMap* m) {
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (fn == nullptr) return fail(CK_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(K), static_cast<cuuint64_t>(N), static_cast<cuuint64_t>(E)};
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(K), static_cast<cuuint64_t>(N) * static_cast<cuuint64_t>(K)};
+    const cuuint32_t box[3] = {kCols, kDeep, 1};
+    const cuuint32_t elem_strides[3] = {1, 1, 1};
+    const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(CK_ERR_CUDA, "cuTensorMapEncodeTiled (experts' codes) failed with code %d", static_cast<int>(r));
+    return static_cast<int>(CK_OK);
+  });
+}
+
+}  // namespace
+
+// Rows of a tile, or 0: the GEMM of ck_grad_gemm.cu.
+int grouped_few_rows_applies(int64_t M, int64_t N, int64_t K, int64_t E, int planes) {
+  const int64_t used = E < M ? E : M, rows = ceil_div(M, used);  // of a group, if they are alike
+  if (rows > 128 / planes) return 0;
+  // a quarter more than that, for groups that are not
+  return grouped_few_rows_tile(rows + rows / 4, planes);
+}
+
+// dy: bf16 [planes][M, N].
+int grouped_few_rows(const void* dy, int planes, const void* codes, const void* scales, const int* offsets, void* out, int out_dtype, int64_t M, int64_t N,
+                     int64_t K, int64_t E, cudaStream_t stream) {
+  GroupedFewRowsArgs a = {};
+  a.scales = static_cast<const uint8_t*>(scales);
+  a.out = out;
+  a.offsets = offsets;
+  a.out_dtype = out_dtype;
+  a.groups = static_cast<int>(E);
+  a.M = static_cast<int>(M);
+  a.N = static_cast<int>(N);
+  a.K = static_cast<int>(K);
+  a.padded = grouped_few_rows_applies(M, N, K, E, planes);
+  a.planes = planes;
+  a.strips = static_cast<int>(ceil_div(K, kCols));
+  // accumulators as for one weight: the second and third numbers' own, four for a result in fp32 where there is room for two sets of them
+  a.parts = 256 / a.padded - (planes - 1);
+  a.sets = a.parts >= 1 ? 2 : 1;
+  if (a.sets == 1) a.parts = 512 / a.padded - (planes - 1);
+  if (a.parts > (out_dtype == CK_DTYPE_F32 ? 4 : 1)) a.parts = out_dtype == CK_DTYPE_F32 ? 4 : 1;
+  CK_REQUIRE(a.padded > 0 && a.parts >= 1, "grouped_input_grad_mxfp8: no room for %d rows", a.padded);
+  const int stage = kHeldBytes + planes * a.padded * 128, room = kGroupedSmem - 1024 - static_cast<int>(sizeof(groups::Table));
+  a.raw_stages = (room - kMaxRaw * kRawBytes) / stage >= kMinStages ? kMaxRaw : kGroups;
+  a.stages = (room - a.raw_stages * kRawBytes) / stage;
+  CK_REQUIRE(a.stages >= kMinStages, "grouped_input_grad_mxfp8: %d stages", a.stages);
+  if (a.stages > kMaxStages) a.stages = kMaxStages;
+  if (int rc = gemm_status_word(&a.status)) return rc;
+  CUtensorMap map_dy, map_codes;
+  if (int rc = make_plane_map(&map_dy, dy, planes, M, N, a.padded, false)) return rc;
+  if (int rc = make_experts_code_map(&map_codes, codes, E, N, K)) return rc;
+  static std::atomic<bool> configured[64];
+  int dev = 0;
+  CK_CUDA(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64 || !configured[dev].load(std::memory_order_acquire)) {
+    CK_CUDA(cudaFuncSetAttribute(grouped_few_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kGroupedSmem));
+    if (dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_release);
+  }
+  // the most tiles that the groups can have; those that there are the device counts
+  const int64_t items = (M / a.padded + (E < M ? E : M)) * a.strips, workers = sm_count();
+  CK_CUDA(launch_pdl(grouped_few_rows_kernel, dim3(static_cast<unsigned>(items < workers ? items : workers)), dim3(kGroupedThreads), kGroupedSmem, stream,
+                     map_dy, map_codes, a));
   return CK_OK;
 }
 

@@ -723,11 +723,14 @@ int linear_grad(bool weight, const char* op, const void* dy, int dtype, const vo
 // Workspace: the groups' matrices in bf16 | dY's planes
 struct GroupedGradLayout {
   int64_t planes_off, total;
+  bool few_rows;  // the matrices are decoded on their way into the operand (ck_grad_few_rows.cu)
 };
 GroupedGradLayout grouped_grad_layout(int dtype, int64_t M, int64_t N, int64_t K, int64_t E) {
   GroupedGradLayout l;
-  l.planes_off = round_up(E * N * K * 2, 256);
+  l.few_rows = grouped_few_rows_applies(M, N, K, E, planes_of(dtype)) != 0;
+  l.planes_off = l.few_rows ? 0 : round_up(E * N * K * 2, 256);
   l.total = l.planes_off + (planes_of(dtype) > 1 ? planes_of(dtype) * M * N * 2 : 0);
+  if (l.total == 0) l.total = 256;
   return l;
 }
 
@@ -767,10 +770,12 @@ int grouped_input_grad(const char* op, const void* dy, int dtype, const void* co
   g.args.planes = reinterpret_cast<__nv_bfloat16*>(ws + l.planes_off);
   g.args.dy_rows = M;
   g.args.dy_cols = N;
-  g.args.held_blocks = static_cast<int>(E * ceil_div(N * (K / 32), 256));
+  g.args.held_blocks = l.few_rows ? 0 : static_cast<int>(E * ceil_div(N * (K / 32), 256));
   g.args.plane_blocks = planes > 1 ? static_cast<int>(ceil_div(M * N, 1024)) : 0;
   auto prepare = dtype == CK_DTYPE_BF16 ? prepare_groups_kernel<__nv_bfloat16> : dtype == CK_DTYPE_F16 ? prepare_groups_kernel<__half> : prepare_groups_kernel<float>;
-  CK_CUDA(launch_pdl(prepare, dim3(static_cast<unsigned>(g.args.held_blocks + g.args.plane_blocks)), dim3(256), 0, s, g));
+  const unsigned blocks = static_cast<unsigned>(g.args.held_blocks + g.args.plane_blocks);
+  if (blocks > 0) CK_CUDA(launch_pdl(prepare, dim3(blocks), dim3(256), 0, s, g));
+  if (l.few_rows) return grouped_few_rows(planes > 1 ? g.args.planes : dy, planes, codes, scales, offsets, out, out_dtype, M, N, K, E, s);
   CUtensorMap map_a, map_b;
   if (int rc = make_plane_map(&map_a, planes > 1 ? g.args.planes : dy, planes, M, N, 128, false)) return rc;
   if (int rc = make_plane_map(&map_b, ws, E, N, K, kDeep, false)) return rc;

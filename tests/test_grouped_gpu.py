@@ -300,3 +300,19 @@ def test_refusals(ck):
         ck.grouped_input_grad_mxfp8(x, codes, scales, ends)
     with pytest.raises(Exception):
         ck.grouped_mm_mxfp8(codes[0], codes, scales[:, :64], scales, ends)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("sizes,behind,n,k", [
+    ([17] * 9, 0, 72, 160), ([1, 2, 3, 60, 5, 0, 0, 90], 5, 1160, 288), ([200] + [0] * 30 + [3], 1, 64, 96), ([100, 120, 140], 0, 200, 1056),
+    ([40] * 24, 0, 328, 416), ([3] * 160, 0, 136, 64), ([130, 1], 0, 2056, 128), ([8], 0, 6208, 2624)])
+def test_input_grad_of_few_rows(ck, dtype, out, sizes, behind, n, k):
+    """Groups of up to about a hundred rows, among them some with several tiles' worth and some with none."""
+    dy = _made((sum(sizes) + behind, n), dtype, 23)
+    codes, scales, w = _weights(ck, len(sizes), n, k)
+    dx = ck.grouped_input_grad_mxfp8(dy, codes, scales, _ends(sizes), out_dtype=out)
+    assert dx.dtype == out
+    _check(dx, dy.double(), w, sizes, PARTS[dtype], name="dx")
+    for _ in range(3):
+        assert torch.equal(dx, ck.grouped_input_grad_mxfp8(dy, codes, scales, _ends(sizes), out_dtype=out))
