@@ -73,8 +73,8 @@ bool grad_few_rows_applies(int64_t M, int64_t N, int64_t K, int planes);
 int grad_few_rows(const void* dy, int planes, const void* codes, const void* scales, void* out, int out_dtype, int64_t M, int64_t N, int64_t K,
                   cudaStream_t stream);
 
-// The same for rows that are grouped by expert: rows of a tile, or 0 where the groups have too many.
-int grouped_few_rows_applies(int64_t M, int64_t N, int64_t K, int64_t E, int planes);
+// The same for rows that are grouped by expert.
+bool grouped_few_rows_applies(int64_t M, int64_t E);
 int grouped_few_rows(const void* dy, int planes, const void* codes, const void* scales, const int* offsets, void* out, int out_dtype, int64_t M, int64_t N,
                      int64_t K, int64_t E, cudaStream_t stream);
 

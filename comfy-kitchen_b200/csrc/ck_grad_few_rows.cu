@@ -79,6 +79,19 @@ __device__ __forceinline__ void store_result(const FewRowsArgs& a, int64_t at, f
   }
 }
 
+// Codes and a scale's byte as they came to shared memory, read where these stand: as ordinary loads they moved behind the wait that follows, and
+// where a copy into the same place may begin before that wait ends, what was read was a later stage's.
+__device__ __forceinline__ uint4 load_codes(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t load_scale(uint32_t at) {
+  uint32_t v;
+  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+  return v;
+}
+
 // Four codes -> four bf16 numbers times `factor`.
 __device__ __forceinline__ uint2 decode_four(uint32_t codes, float2 factor) {
   uint32_t lo, hi;
@@ -138,8 +151,7 @@ grad_few_rows_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_co
     constexpr int kItems = kDeep / (4 * kGroupWarps);
     const int group = warp / kGroupWarps, odd = (lane >> 2) & 1, unit = (lane & 3) + (odd ^ ((lane >> 3) & 1)) * 4;
     const int row0 = warp % kGroupWarps * 4 + odd + (lane >> 4) * 2;
-    const uint8_t* const code_at = raw + row0 * kCols + unit * 16;
-    const uint8_t* const scale_at = raw + kDeep * kCols + (unit >> 1);
+    const uint32_t code_at = smem_u32(raw) + row0 * kCols + unit * 16, scale_at = smem_u32(raw) + kDeep * kCols + (unit >> 1);
     const uint32_t row_at = smem_u32(smem) + (unit >> 2) * kBoxBytes + row0 * 128;
     const uint32_t low = ((unit & 3) * 2) ^ (row0 & 7), high = low ^ 1;  // the same for rows 16 apart
     int stage = group, raw_stage = group;
@@ -151,8 +163,8 @@ grad_few_rows_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_co
 #pragma unroll
       for (int i = 0; i < kItems; ++i) {
         const int row = row0 + 4 * kGroupWarps * i;
-        codes[i] = *reinterpret_cast<const uint4*>(code_at + raw_stage * kRawBytes + 4 * kGroupWarps * i * kCols);
-        byte[i] = scale_at[raw_stage * kRawBytes + (row & 31) * 16 + (row >> 5) * 4 + (step & 1) * 8];  // a tile of scales is two stages high
+        codes[i] = load_codes(code_at + raw_stage * kRawBytes + 4 * kGroupWarps * i * kCols);
+        byte[i] = load_scale(scale_at + raw_stage * kRawBytes + (row & 31) * 16 + (row >> 5) * 4 + (step & 1) * 8);  // a tile of scales is two stages high
       }
       if (const int left = a.N - step * kDeep; left < kDeep) {  // what stands in rows past the last one is nobody's: infinite, it would make NaN of zeros
 #pragma unroll
@@ -319,7 +331,8 @@ grad_few_rows_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_co
 }
 
 // ---- grouped rows --------------------------------------------------------------------------------------------
-constexpr int kStoreWarps = 4, kGroupedThreads = kThreads + 32 * kStoreWarps;
+constexpr int kRowBox = 16;  // rows of dY in a copy
+constexpr int kStoreWarps = 4, kGroupedThreads = kThreads + 32 * (kStoreWarps + 1);  // beside those of the kernel above, and the loads of dY apart from the codes
 
 struct GroupedFewRowsArgs {
   const uint8_t* scales;
@@ -327,7 +340,7 @@ struct GroupedFewRowsArgs {
   const int* offsets;
   int out_dtype;
   int groups, M, N, K;
-  int padded;       // rows of a tile, a multiple of 16
+  int padded;       // rows of a tile at most, a multiple of kRowBox
   int planes;       // bf16 numbers whose sum is an element of dY
   int parts;        // accumulators that the first of them take in turn; the others have one each, in front of these
   int sets;         // of accumulators: two where tensor memory holds them, so that a tile is stored beside the next one's steps
@@ -336,27 +349,9 @@ struct GroupedFewRowsArgs {
   int* status;
 };
 
-// A code and its scale for four rows of the operand, as the kernel above decodes them.
-__device__ __forceinline__ void decode_stage(const uint8_t* raw, uint32_t row_at, int row0, int unit, int step, int left) {
-  constexpr int kItems = kDeep / (4 * kGroupWarps);
-  const uint32_t low = ((unit & 3) * 2) ^ (row0 & 7), high = low ^ 1;
-#pragma unroll
-  for (int i = 0; i < kItems; ++i) {
-    const int row = row0 + 4 * kGroupWarps * i;
-    const uint4 codes = *reinterpret_cast<const uint4*>(raw + row * kCols + unit * 16);
-    uint32_t byte = raw[kDeep * kCols + (unit >> 1) + (row & 31) * 16 + (row >> 5) * 4 + (step & 1) * 8];  // a tile of scales is two stages high
-    if (row >= left) byte = 0;  // what stands for rows past the last one is nobody's
-    const float2 factor = both(e8m0_factor(byte));
-    const uint2 v0 = decode_four(codes.x, factor), v1 = decode_four(codes.y, factor);
-    const uint2 v2 = decode_four(codes.z, factor), v3 = decode_four(codes.w, factor);
-    const uint32_t to = row_at + 4 * kGroupWarps * i * 128;
-    st_shared_128(to + (low << 4), v0.x, v0.y, v1.x, v1.y);
-    st_shared_128(to + (high << 4), v2.x, v2.y, v3.x, v3.y);
-  }
-}
-
 __global__ void __launch_bounds__(kGroupedThreads)
-grouped_few_rows_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_constant__ CUtensorMap map_codes, const GroupedFewRowsArgs a) {
+grouped_few_rows_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_constant__ CUtensorMap map_dy_whole,
+                        const __grid_constant__ CUtensorMap map_codes, const GroupedFewRowsArgs a) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full_bar[kMaxStages], empty_bar[kMaxStages], raw_full_bar[kMaxRaw], raw_empty_bar[kMaxRaw], acc_full_bar[2], acc_empty_bar[2];
   __shared__ uint32_t tmem_slot;
@@ -387,6 +382,7 @@ grouped_few_rows_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid
     }
     fence_barrier_init();
     prefetch_tensormap(&map_dy);
+    prefetch_tensormap(&map_dy_whole);
     prefetch_tensormap(&map_codes);
   }
   if (warp == kCodeWarps + 1) tmem_alloc<1>(&tmem_slot, tmem_cols);
@@ -406,7 +402,10 @@ grouped_few_rows_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid
     // ---------------------------------------------------------------- decoding
     const int group = warp / kGroupWarps, odd = (lane >> 2) & 1, unit = (lane & 3) + (odd ^ ((lane >> 3) & 1)) * 4;
     const int row0 = warp % kGroupWarps * 4 + odd + (lane >> 4) * 2;
+    const uint32_t code_at = smem_u32(raw) + row0 * kCols + unit * 16, scale_at = smem_u32(raw) + kDeep * kCols + (unit >> 1);
     const uint32_t row_at = smem_u32(smem) + (unit >> 2) * kBoxBytes + row0 * 128;
+    const uint32_t low = ((unit & 3) * 2) ^ (row0 & 7), high = low ^ 1;  // the same for rows 16 apart
+    constexpr int kItems = kDeep / (4 * kGroupWarps);
     int stage = group, raw_stage = group;
     uint32_t phase = 0, raw_phase = 0;
     int step = group;  // within its tile
@@ -417,14 +416,31 @@ grouped_few_rows_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid
       }
       if (left_tiles == 0) break;
       mbar_wait(raw_full + raw_stage * 8, raw_phase, &abort_flag);
+      uint4 codes[kItems];
+      uint32_t byte[kItems];
+      const int left = a.N - step * kDeep;  // what stands for rows past the last one is nobody's
+#pragma unroll
+      for (int i = 0; i < kItems; ++i) {
+        const int row = row0 + 4 * kGroupWarps * i;
+        codes[i] = load_codes(code_at + raw_stage * kRawBytes + 4 * kGroupWarps * i * kCols);
+        byte[i] = load_scale(scale_at + raw_stage * kRawBytes + (row & 31) * 16 + (row >> 5) * 4 + (step & 1) * 8);  // a tile of scales is two stages high
+        if (row >= left) byte[i] = 0;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&raw_empty_bar[raw_stage]);
       mbar_wait(empty + stage * 8, phase ^ 1, &abort_flag);
-      decode_stage(raw + raw_stage * kRawBytes, row_at + stage * stage_bytes, row0, unit, step, a.N - step * kDeep);
+      const uint32_t to = row_at + stage * stage_bytes;
+#pragma unroll
+      for (int i = 0; i < kItems; ++i) {
+        const float2 factor = both(e8m0_factor(byte[i]));
+        const uint2 v0 = decode_four(codes[i].x, factor), v1 = decode_four(codes[i].y, factor);
+        const uint2 v2 = decode_four(codes[i].z, factor), v3 = decode_four(codes[i].w, factor);
+        st_shared_128(to + 4 * kGroupWarps * i * 128 + (low << 4), v0.x, v0.y, v1.x, v1.y);
+        st_shared_128(to + 4 * kGroupWarps * i * 128 + (high << 4), v2.x, v2.y, v3.x, v3.y);
+      }
       fence_proxy_async();  // the MMAs read what was written here
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&raw_empty_bar[raw_stage]);
-        mbar_arrive(&full_bar[stage]);
-      }
+      if (lane == 0) mbar_arrive(&full_bar[stage]);
       stage += kGroups;
       if (stage >= a.stages) {
         stage -= a.stages;
@@ -437,49 +453,60 @@ grouped_few_rows_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid
       }
     }
   } else if (warp == kCodeWarps) {
-    // ---------------------------------------------------------------- loads: codes and scales as far ahead as their ring goes, dY with its stage
-    if (elect_one() && mine > 0) {
+    // ---------------------------------------------------------------- loads of codes and scales, as far ahead as their ring goes
+    if (elect_one()) {
       const int64_t col_tiles = (a.K / 32 + 3) >> 2, group_tiles = (a.N + 127) / 128 * col_tiles;
-      int stage = 0, raw_stage = 0, ahead_item = 0, ahead_step = 0, fetched = 0;
-      uint32_t phase = 0, raw_phase = 0;
-      groups::Tile ahead = place(0);
-      const auto fetch = [&]() {
-        mbar_wait(raw_empty + raw_stage * 8, raw_phase ^ 1, &abort_flag);
-        const uint32_t bar = raw_full + raw_stage * 8, to = smem_u32(raw) + raw_stage * kRawBytes;
-        mbar_arrive_expect_tx(bar, kRawBytes);
-        asm volatile(
-            "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(to),
-            "l"(reinterpret_cast<uint64_t>(&map_codes)), "r"(bar), "r"(ahead.tile_n * kCols), "r"(ahead_step * kDeep), "r"(ahead.group)
-            : "memory");
-        bulk_load_1d(to + kDeep * kCols, a.scales + (ahead.group * group_tiles + (ahead_step >> 1) * col_tiles + ahead.tile_n) * kScaleBytes, kScaleBytes, bar);
-        ++fetched;
-        if (++ahead_step == steps) {
-          ahead_step = 0;
-          if (++ahead_item < mine) ahead = place(ahead_item);
-        }
-        if (++raw_stage == a.raw_stages) {
-          raw_stage = 0;
-          raw_phase ^= 1u;
-        }
-      };
-      while (ahead_item < mine && fetched < a.raw_stages) fetch();
+      int raw_stage = 0;
+      uint32_t raw_phase = 0;
       for (int i = 0; i < mine; ++i) {
         const groups::Tile t = place(i);
+        const uint8_t* const scales = a.scales + (t.group * group_tiles + t.tile_n) * kScaleBytes;
+        for (int step = 0; step < steps; ++step) {
+          mbar_wait(raw_empty + raw_stage * 8, raw_phase ^ 1, &abort_flag);
+          const uint32_t bar = raw_full + raw_stage * 8, to = smem_u32(raw) + raw_stage * kRawBytes;
+          mbar_arrive_expect_tx(bar, kRawBytes);
+          asm volatile(
+              "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(to),
+              "l"(reinterpret_cast<uint64_t>(&map_codes)), "r"(bar), "r"(t.tile_n * kCols), "r"(step * kDeep), "r"(t.group)
+              : "memory");
+          bulk_load_1d(to + kDeep * kCols, scales + (step >> 1) * col_tiles * kScaleBytes, kScaleBytes, bar);
+          if (++raw_stage == a.raw_stages) {
+            raw_stage = 0;
+            raw_phase ^= 1u;
+          }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == kCodeWarps + 2) {
+    // ---------------------------------------------------------------- loads of dY
+    if (elect_one()) {
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int i = 0; i < mine; ++i) {
+        const groups::Tile t = place(i);
+        // a tile's rows of dY in one box where it has more than half of them, in boxes of 16 otherwise
+        const int count = min(a.padded, t.end - t.row);
+        const bool whole = 2 * count > a.padded;
+        const int boxes = whole ? 1 : (count + kRowBox - 1) / kRowBox, box_rows = whole ? a.padded : kRowBox;
+        const CUtensorMap* const map = whole ? &map_dy_whole : &map_dy;
         for (int step = 0; step < steps; ++step) {
           mbar_wait(empty + stage * 8, phase ^ 1, &abort_flag);
           const uint32_t bar = full + stage * 8, to = smem_u32(smem) + stage * stage_bytes + kHeldBytes;
-          mbar_arrive_expect_tx(bar, a.planes * plane_bytes);
+          mbar_arrive_expect_tx(bar, a.planes * boxes * box_rows * 128);
           for (int p = 0; p < a.planes; ++p) {
-            asm volatile(
-                "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(to + p * plane_bytes),
-                "l"(reinterpret_cast<uint64_t>(&map_dy)), "r"(bar), "r"(step * kDeep), "r"(t.row), "r"(p)
-                : "memory");
+            for (int b = 0; b < boxes; ++b) {
+              asm volatile(
+                  "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+                      to + p * plane_bytes + b * (kRowBox * 128)),
+                  "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(step * kDeep), "r"(t.row + b * kRowBox), "r"(p)
+                  : "memory");
+            }
           }
           if (++stage == a.stages) {
             stage = 0;
             phase ^= 1u;
           }
-          if (ahead_item < mine) fetch();
         }
       }
     }
@@ -487,10 +514,13 @@ grouped_few_rows_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid
   } else if (warp == kCodeWarps + 1) {
     // ---------------------------------------------------------------- MMAs
     if (elect_one()) {
-      const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (static_cast<uint32_t>(a.padded >> 3) << 17) | ((kCols >> 4) << 24);
       int stage = 0;
       uint32_t phase = 0;
       for (int i = 0; i < mine; ++i) {
+        // as many of the MMA's columns as the tile has rows, in sixteens
+        const groups::Tile t = place(i);
+        const uint32_t columns = (min(a.padded, t.end - t.row) + 15) / 16 * 16;
+        const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | ((columns >> 3) << 17) | ((kCols >> 4) << 24);
         const int set = a.sets == 2 ? i & 1 : 0;
         const uint32_t base = tmem + set * set_cols;
         mbar_wait(&acc_empty_bar[set], ((i / a.sets) & 1) ^ 1, &abort_flag);
@@ -567,7 +597,7 @@ grouped_few_rows_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid
     // rows behind the last group, in units of 16 bytes (K is a multiple of 32)
     const int64_t size = a.out_dtype == CK_DTYPE_F32 ? 4 : 2;
     const int64_t begin = static_cast<int64_t>(table->bound[a.groups]) * a.K * size, end = static_cast<int64_t>(a.M) * a.K * size;
-    for (int64_t at = begin + (static_cast<int64_t>(blockIdx.x) * (32 * kStoreWarps) + threadIdx.x - kThreads) * 16; at < end;
+    for (int64_t at = begin + (static_cast<int64_t>(blockIdx.x) * (32 * kStoreWarps) + threadIdx.x - (kGroupedThreads - 32 * kStoreWarps)) * 16; at < end;
          at += static_cast<int64_t>(gridDim.x) * (32 * kStoreWarps) * 16) {
       *reinterpret_cast<uint4*>(static_cast<uint8_t*>(a.out) + at) = make_uint4(0, 0, 0, 0);
     }
@@ -701,11 +731,15 @@ namespace {
 
 constexpr int kGroupedSmem = 226 * 1024 - 1024;  // dynamic, beside the barriers
 
-// Rows of a tile for so many of a group, 0 if there are too many for their operand to find room.
+// Rows of a tile at most: as many as there is room for beside the fewest stages and eight of codes, or four where groups of so many rows would need
+// more.  A tile computes and loads what it has rows for, and a group in fewer tiles has its weight decoded less often; but codes four stages ahead come
+// late (64 experts of 2048 x 2048: 32 rows each of fp32 161 us with tiles of 48, 195 with 64; 64 of fp16 163 with 80, 195 with 112).
 int grouped_few_rows_tile(int64_t rows, int planes) {
-  const int64_t padded = round_up(rows, 16);
-  const int64_t stage = kHeldBytes + planes * padded * 128;
-  return padded <= 256 && kMinStages * stage <= kGroupedSmem - 1024 - kGroups * kRawBytes - static_cast<int64_t>(sizeof(groups::Table)) ? static_cast<int>(padded) : 0;
+  const auto most = [&](int raw_stages) {
+    const int room = (kGroupedSmem - 1024 - raw_stages * kRawBytes - static_cast<int>(sizeof(groups::Table))) / kMinStages - kHeldBytes;
+    return room / (planes * kRowBox * 128) * kRowBox;
+  };
+  return most(kMaxRaw) >= rows ? most(kMaxRaw) : most(kGroups);
 }
 
 // E4M3 [E, N, K], boxes of 128 columns x 64 rows of one matrix, as they lie in memory; rows past N and columns past K read as zeros.
@@ -726,12 +760,12 @@ int make_experts_code_map(CUtensorMap* map, const void* base, int64_t E, int64_t
 
 }  // namespace
 
-// Rows of a tile, or 0: the GEMM of ck_grad_gemm.cu.
-int grouped_few_rows_applies(int64_t M, int64_t N, int64_t K, int64_t E, int planes) {
-  const int64_t used = E < M ? E : M, rows = ceil_div(M, used);  // of a group, if they are alike
-  if (rows > 128 / planes) return 0;
-  // a quarter more than that, for groups that are not
-  return grouped_few_rows_tile(rows + rows / 4, planes);
+// Whether groups of so many rows are decoded here: for each tile of theirs once, where the GEMM of ck_grad_gemm.cu has all matrices
+// written as bf16 and reads them back (0.45 us for a million codes).  us, here / there: 64 experts of 2048 x 2048, 256 rows each, bf16 202 / 260, fp16
+// 425 / 450 to 490, 8 of 4096 x 2048, 256 rows of fp32, 163 / 208; 512 rows, bf16 16 of 1024 x 8192 251 / 186, fp32 32 of 1024 x 1024 181 / 165.
+bool grouped_few_rows_applies(int64_t M, int64_t E) {
+  const int64_t used = E < M ? E : M;
+  return ceil_div(M, used) <= 256;  // of a group, if they are alike
 }
 
 // dy: bf16 [planes][M, N].
@@ -746,7 +780,7 @@ int grouped_few_rows(const void* dy, int planes, const void* codes, const void* 
   a.M = static_cast<int>(M);
   a.N = static_cast<int>(N);
   a.K = static_cast<int>(K);
-  a.padded = grouped_few_rows_applies(M, N, K, E, planes);
+  a.padded = grouped_few_rows_tile(ceil_div(M, E < M ? E : M), planes);
   a.planes = planes;
   a.strips = static_cast<int>(ceil_div(K, kCols));
   // accumulators as for one weight: the second and third numbers' own, four for a result in fp32 where there is room for two sets of them
@@ -761,8 +795,9 @@ int grouped_few_rows(const void* dy, int planes, const void* codes, const void* 
   CK_REQUIRE(a.stages >= kMinStages, "grouped_input_grad_mxfp8: %d stages", a.stages);
   if (a.stages > kMaxStages) a.stages = kMaxStages;
   if (int rc = gemm_status_word(&a.status)) return rc;
-  CUtensorMap map_dy, map_codes;
-  if (int rc = make_plane_map(&map_dy, dy, planes, M, N, a.padded, false)) return rc;
+  CUtensorMap map_dy, map_dy_whole, map_codes;
+  if (int rc = make_plane_map(&map_dy, dy, planes, M, N, kRowBox, false)) return rc;
+  if (int rc = make_plane_map(&map_dy_whole, dy, planes, M, N, a.padded, false)) return rc;
   if (int rc = make_experts_code_map(&map_codes, codes, E, N, K)) return rc;
   static std::atomic<bool> configured[64];
   int dev = 0;
@@ -774,7 +809,7 @@ int grouped_few_rows(const void* dy, int planes, const void* codes, const void* 
   // the most tiles that the groups can have; those that there are the device counts
   const int64_t items = (M / a.padded + (E < M ? E : M)) * a.strips, workers = sm_count();
   CK_CUDA(launch_pdl(grouped_few_rows_kernel, dim3(static_cast<unsigned>(items < workers ? items : workers)), dim3(kGroupedThreads), kGroupedSmem, stream,
-                     map_dy, map_codes, a));
+                     map_dy, map_dy_whole, map_codes, a));
   return CK_OK;
 }
 

@@ -727,7 +727,7 @@ struct GroupedGradLayout {
 };
 GroupedGradLayout grouped_grad_layout(int dtype, int64_t M, int64_t N, int64_t K, int64_t E) {
   GroupedGradLayout l;
-  l.few_rows = grouped_few_rows_applies(M, N, K, E, planes_of(dtype)) != 0;
+  l.few_rows = grouped_few_rows_applies(M, E);
   l.planes_off = l.few_rows ? 0 : round_up(E * N * K * 2, 256);
   l.total = l.planes_off + (planes_of(dtype) > 1 ? planes_of(dtype) * M * N * 2 : 0);
   if (l.total == 0) l.total = 256;

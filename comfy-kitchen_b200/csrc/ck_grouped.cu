@@ -44,7 +44,8 @@ __device__ __forceinline__ float bias_at(const void* bias, int dtype, int64_t at
 template <int TILE_N, int NUM_ACC, int STAGES, int CTAS>
 struct GroupedConfig : Config<Kind::kMxfp8, TILE_N, NUM_ACC, STAGES, CTAS, 0> {
   using Base = Config<Kind::kMxfp8, TILE_N, NUM_ACC, STAGES, CTAS, 0>;
-  static constexpr int kSmem = Base::kRingBytes + 1024 + 256 + static_cast<int>(sizeof(groups::Table));
+  static constexpr int kTableBytes = (static_cast<int>(sizeof(groups::Table)) + 15) / 16 * 16, kBiasBytes = 128 * epilogue_warps(false, TILE_N) * (TILE_N / (epilogue_warps(false, TILE_N) / 4) / 32);
+  static constexpr int kSmem = Base::kRingBytes + 1024 + 256 + kTableBytes + kBiasBytes;
   static_assert(kSmem <= 227 * 1024, "shared memory budget exceeded");
 };
 
@@ -210,6 +211,7 @@ grouped_gemm_kernel(const __grid_constant__ RowMaps maps_a, const __grid_constan
     constexpr int kWarpCols = TILE_N / (kWarps / 4), kChunks = kWarpCols / 32;
     const uint32_t acc_empty = CTAS == 2 ? map_to_cta(smem_u32(acc_empty_bar), 0) : smem_u32(acc_empty_bar);
     OutT* out = static_cast<OutT*>(p.out);
+    float* const bias_s = reinterpret_cast<float*>(smem + Cfg::kRingBytes + 256 + Cfg::kTableBytes) + (warp - 2) * kWarpCols;
     // stores of 32 bytes where rows start on such boundaries, of 16 (N is a multiple of 8) otherwise
     const bool wide = (static_cast<int64_t>(p.N) * sizeof(OutT)) % 32 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 31u) == 0;
     int it = 0;
@@ -217,6 +219,15 @@ grouped_gemm_kernel(const __grid_constant__ RowMaps maps_a, const __grid_constan
       const groups::Tile t = groups::place(table, p.groups, p.tiles_n, Cfg::kTileRows, item);
       const int row = t.row + static_cast<int>(cta_rank) * kTileM + quarter * 32 + lane, col0 = t.tile_n * TILE_N + share * kWarpCols;
       const int acc = it % NUM_ACC;
+      // the warp's columns' bias, one a lane, fetched while the tile computes and passed round through shared memory
+      float bias[kChunks] = {};
+      if (p.bias != nullptr) {
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+          const int col = col0 + c * 32 + lane;
+          if (col < p.N) bias[c] = bias_at(p.bias, p.bias_dtype, static_cast<int64_t>(t.group) * p.N + col);
+        }
+      }
       mbar_wait(&acc_full_bar[acc], (it / NUM_ACC) & 1, abort_flag);
       __syncwarp();
       tc_fence_after_sync();
@@ -228,6 +239,11 @@ grouped_gemm_kernel(const __grid_constant__ RowMaps maps_a, const __grid_constan
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(acc_empty + acc * 8);
+      if (p.bias != nullptr) {
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) bias_s[c * 32 + lane] = bias[c];
+        __syncwarp();
+      }
       if (row >= t.end) continue;
       OutT* dst = out + static_cast<int64_t>(row) * p.N + col0;
 #pragma unroll
@@ -238,10 +254,13 @@ grouped_gemm_kernel(const __grid_constant__ RowMaps maps_a, const __grid_constan
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(buf[c][i]);
         if (p.bias != nullptr) {
-          const int64_t at = static_cast<int64_t>(t.group) * p.N + col0 + c * 32;
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            if (i < valid) v[i] += bias_at(p.bias, p.bias_dtype, at + i);
+          for (int i = 0; i < 8; ++i) {
+            const float4 q = reinterpret_cast<const float4*>(bias_s + c * 32)[i];
+            v[4 * i] += q.x;
+            v[4 * i + 1] += q.y;
+            v[4 * i + 2] += q.z;
+            v[4 * i + 3] += q.w;
           }
         }
         if (wide && valid == 32) {

@@ -316,3 +316,14 @@ def test_input_grad_of_few_rows(ck, dtype, out, sizes, behind, n, k):
     _check(dx, dy.double(), w, sizes, PARTS[dtype], name="dx")
     for _ in range(3):
         assert torch.equal(dx, ck.grouped_input_grad_mxfp8(dy, codes, scales, _ends(sizes), out_dtype=out))
+
+
+@pytest.mark.parametrize("dtype,rows,k", [(torch.bfloat16, 200, 256), (torch.float16, 96, 128), (torch.float16, 200, 256), (torch.float32, 200, 256)])
+def test_input_grad_again_and_again(ck, dtype, rows, k):
+    """A long contraction whose MMAs are behind the decoding: codes that were read late were those of a later step, in one pass of ten."""
+    dy = _made((rows, 4864), dtype, 24)
+    codes, scales, w = _weights(ck, 1, 4864, k)
+    first = ck.grouped_input_grad_mxfp8(dy, codes, scales, _ends([rows]), out_dtype=torch.float32)
+    _check(first, dy.double(), w, [rows], PARTS[dtype], name="dx")
+    for _ in range(300):
+        assert torch.equal(first, ck.grouped_input_grad_mxfp8(dy, codes, scales, _ends([rows]), out_dtype=torch.float32))
