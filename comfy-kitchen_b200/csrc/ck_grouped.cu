@@ -9,6 +9,10 @@
 // as they stand (1/32 of x).  The GEMM is the block-scaled one of ck_gemm_kernel.cuh (TMA producer, one issuing lane, epilogue
 // warps, two roles' distance by mbarriers) over a list of tiles that every CTA makes for itself from the groups' ends.  Rows are stored from
 // registers, those behind the group's end not at all; rows behind the last group are zeros.
+//
+// Many rows: bound by the tensor pipe and, in a loop, by the power limit (8192 x 8192 x 4096 of 8 experts from bf16 250 us, 2.2 PFLOP/s with the quantization;
+// 298 in a loop; one weight for all rows 202: the groups' last tiles are half empty).  Few rows: by the weights' bytes (64 experts of 2048 x 2048, 32 rows each, 57 us,
+// 5.1 TB/s); one token through eight of 64 experts, 25 MB, 10.7 us: two launches, first loads.
 #include "ck_gemm_kernel.cuh"
 #include "ck_groups.cuh"
 #include "ck_rows.cuh"
@@ -422,7 +426,10 @@ template <typename OutT>
 int launch_grouped_shape(const void* a, const void* b, const GroupedParams& p, cudaStream_t stream) {
   const int64_t used = p.groups < p.M ? p.groups : p.M, rows = ceil_div(p.M, used);  // of a group, if they are alike
   const int64_t pairs = used * ceil_div(rows, 256) * ceil_div(p.N, 256), tiles = used * ceil_div(rows, 128) * ceil_div(p.N, 128);
-  if (rows > 128 && pairs * 4 >= sm_count()) return launch_grouped<256, 1, 5, 2, OutT>(a, b, p, stream);
+  // Pairs for groups of more than one row block, from a fifth of the SMs on (us, pair / 128 x 128: 8 groups of 256 rows by 1024 x 1024 11.3 / 12.7, 4 by 4096 x
+  // 4096 30.8 / 38.3, 64 by 2048 x 2048 112 / 136; 3 of 200 by 2048 x 512 7.9 / 7.4).  Half tiles where whole ones leave half of the SMs without one (1 row
+  // of 1536 x 2048 8.8 / 9.1; 8 rows of as many experts, 96 tiles, 13.7 / 10.7).
+  if (rows > 128 && pairs * 5 >= sm_count()) return launch_grouped<256, 1, 5, 2, OutT>(a, b, p, stream);
   if (tiles * 2 <= sm_count()) return launch_grouped<64, 2, 6, 1, OutT>(a, b, p, stream);
   return launch_grouped<128, 2, 5, 1, OutT>(a, b, p, stream);
 }
