@@ -165,9 +165,9 @@ def clip_grad_norm_(parameters: Iterable[torch.Tensor] | torch.Tensor, max_norm:
         norm = grad_norm(grads)
         if not math.isfinite(norm.item()):
             raise RuntimeError(f"The total norm of the gradients is {norm.item()}, so it cannot be clipped")
-    if all(g.is_contiguous() for g in grads):
+    if all(g.is_contiguous() and not g.is_neg() for g in grads):
         return _list_call("clip_grads", grads, max_norm)
-    dense = [g.contiguous() for g in grads]
+    dense = [g.resolve_neg().contiguous() for g in grads]
     norm = _list_call("clip_grads", dense, max_norm)
     with torch.no_grad():
         for g, d in zip(grads, dense):

@@ -345,11 +345,19 @@ class CheckpointedLinear(nn.Linear):
 
 
 class CheckpointedMLP(nn.Module):
-    """``x + fc2(gelu(fc1(norm(x))))``, the MLP half of a transformer block, every activation that it keeps in MXFP8."""
+    """``x + fc2(gelu(fc1(norm(x))))``, the MLP half of a transformer block, every activation that it keeps in MXFP8; with ``norm="rms"`` an
+    RMS norm, which keeps x itself."""
 
-    def __init__(self, features: int, hidden: int, eps: float = 1e-5, device=None, dtype=None) -> None:
+    def __init__(self, features: int, hidden: int, eps: float = 1e-5, device=None, dtype=None, norm: str = "layer") -> None:
         super().__init__()
-        self.norm = CheckpointedLayerNorm(features, eps=eps, device=device, dtype=dtype)
+        if norm not in ("layer", "rms"):
+            raise ValueError(f"norm is 'layer' or 'rms', got {norm!r}")
+        if norm == "rms":
+            from .norms import RMSNorm  # built on this module
+
+            self.norm = RMSNorm(features, eps=eps, device=device, dtype=dtype)
+        else:
+            self.norm = CheckpointedLayerNorm(features, eps=eps, device=device, dtype=dtype)
         self.fc1 = CheckpointedLinear(features, hidden, device=device, dtype=dtype)
         self.act = CheckpointedGELU()
         self.fc2 = CheckpointedLinear(hidden, features, device=device, dtype=dtype)

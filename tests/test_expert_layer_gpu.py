@@ -1,0 +1,283 @@
+"""RMS norm, the experts' products and clipping together, on the GPU: a layer's step, its serving form, and the routes that a call can take."""
+from __future__ import annotations
+
+import sys
+
+import pytest
+import torch
+from conftest import PKG_DIR
+
+pytestmark = pytest.mark.gpu
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+@pytest.fixture(scope="module")
+def ck(cuda_device):
+    import comfy_kitchen
+
+    assert comfy_kitchen.list_backends()["cuda"]["available"]
+    return comfy_kitchen
+
+
+def _made(shape, dtype, seed, scale=1.0):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(shape, generator=gen, device="cuda") * scale).to(dtype)
+
+
+def _routed(tokens, experts, chosen, seed):
+    """(token of each row, ends): ``chosen`` different experts for each token, rows in the experts' order"""
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    picks = torch.rand(tokens, experts, generator=gen, device="cuda").topk(chosen, dim=1).indices.flatten()
+    order = picks.argsort(stable=True)
+    ends = torch.bincount(picks, minlength=experts).cumsum(0).to(torch.int32)
+    return order // chosen, ends
+
+
+class _Layer(torch.nn.Module):
+    """h + the sum over a token's experts of down(gelu(up(norm(h)))), h = x + residual"""
+
+    def __init__(self, ck, experts, features, hidden, dtype, seed):
+        super().__init__()
+        self.norm = ck.norms.RMSNorm(features, device="cuda", dtype=dtype)
+        self.norm.weight.data.copy_(_made((features,), dtype, seed, 0.1) + 1)
+        self.up = ck.experts.MXFP8Experts.from_float(_made((experts, hidden, features), torch.float32, seed + 1, features**-0.5))
+        self.down = ck.experts.MXFP8Experts.from_float(_made((experts, features, hidden), torch.float32, seed + 2, hidden**-0.5))
+
+    def forward(self, x, residual, token, ends):
+        y, h = self.norm(x, residual)
+        self.kept = (rows := y[token], u := self.up(rows, ends), g := torch.nn.functional.gelu(u, approximate="tanh"))
+        return h.index_add(0, token, self.down(g, ends))
+
+
+def test_a_layers_step(ck):
+    """Gradients of the norm's weight, of x and of the residual against the formulas in 64 bits, on the values that the MXFP8 products have seen.
+
+    fp32 throughout: each product is off by at most (640 / 16 + 4) 2^-22 of the sum of its terms' magnitudes, about 1e-5 (three bf16 parts of dY more), which is a
+    few times its value's norm; four of them in a row stay below 1e-4 of a gradient's norm in all but the worst alignment of signs."""
+    tokens, experts, chosen, features, hidden = 77, 6, 2, 256, 640
+    layer = _Layer(ck, experts, features, hidden, torch.float32, 1)
+    x, residual, dy = (_made((tokens, features), torch.float32, 10 + i) for i in range(3))
+    x.requires_grad_(), residual.requires_grad_()
+    token, ends = _routed(tokens, experts, chosen, 3)
+    layer(x, residual, token, ends).backward(dy)
+    rows, u, g = (t.detach() for t in layer.kept)
+
+    def values(m):
+        codes, scales = m.weight.view(torch.float8_e4m3fn), m.weight_scale.view(torch.float8_e8m0fnu)
+        return torch.stack([ck.dequantize_mxfp8(codes[e], scales[e], torch.float32) for e in range(experts)]).double()
+
+    up, down = values(layer.up), values(layer.down)
+    expert = torch.bucketize(torch.arange(tokens * chosen, device="cuda"), ends.long(), right=True)
+    d = dy.double()[token]
+    du = torch.einsum("rn,rnk->rk", d, down[expert])
+    u64 = u.double().requires_grad_()
+    torch.nn.functional.gelu(u64, approximate="tanh").backward(du)
+    drows = torch.einsum("rn,rnk->rk", u64.grad, up[expert])
+    dnormed = torch.zeros(tokens, features, dtype=torch.float64, device="cuda").index_add(0, token, drows)
+    h = (x + residual).detach().double().requires_grad_()
+    w = layer.norm.weight.detach().double().requires_grad_()
+    ((h * (h * h).mean(1, keepdim=True).add(1e-6).rsqrt() * w) * dnormed).sum().backward()
+    want = h.grad + dy.double()
+    for name, got, ref in (("x", x.grad, want), ("residual", residual.grad, want), ("weight", layer.norm.weight.grad, w.grad)):
+        assert (got.double() - ref).norm() <= 1e-4 * ref.norm(), name
+
+    norm = sum(t.grad.double().square().sum() for t in (x, residual, layer.norm.weight)).sqrt()
+    before = [t.grad.clone() for t in (x, residual, layer.norm.weight)]
+    said = ck.clip_grad_norm_([x, residual, layer.norm.weight], 0.5)
+    assert abs(said.double() - norm) <= 1e-5 * norm and norm > 0.5
+    for t, was in zip((x, residual, layer.norm.weight), before):
+        assert (t.grad.double() - was.double() * 0.5 / (norm + 1e-6)).norm() <= 2e-5 * t.grad.double().norm()
+
+
+def test_a_layers_step_captured(ck):
+    """Forward, backward and clipping in one graph, replayed on other tokens with other ends, give what the eager step gives."""
+    tokens, experts, features, hidden = 40, 5, 128, 192
+    layer = _Layer(ck, experts, features, hidden, torch.bfloat16, 21)
+    token, ends = _routed(tokens, experts, 2, 4)
+    x = _made((tokens, features), torch.bfloat16, 31).requires_grad_()
+    residual, dy = _made((tokens, features), torch.bfloat16, 32), _made((tokens, features), torch.bfloat16, 33)
+    leaves = (x, layer.norm.weight)
+
+    def step():
+        grads = torch.autograd.grad(layer(x, residual, token, ends), leaves, dy)
+        layer.kept = None
+        holders = [torch.nn.Parameter(t.detach()) for t in leaves]
+        for p, g in zip(holders, grads):
+            p.grad = g
+        return (ck.clip_grad_norm_(holders, 0.25), *grads)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in (50, 60):
+        other_token, other_ends = _routed(tokens, experts, 2, seed)
+        with torch.no_grad():
+            x.copy_(_made((tokens, features), torch.bfloat16, seed + 1))
+        dy.copy_(_made((tokens, features), torch.bfloat16, seed + 2))
+        token.copy_(other_token), ends.copy_(other_ends)
+        graph.replay()
+        # index_add over a token's two rows is an addition of two atomics onto one value: their order may change the last bit
+        for got, want in zip(out, step()):
+            assert (got.double() - want.double()).norm() <= 2**-6 * want.double().norm()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_one_token_through_its_experts(ck, dtype):
+    """The serving form: one row, as many times as it has experts, from the norm to the products without a dense result in between."""
+    experts, chosen, features, n = 16, 4, 256, 320
+    x, residual, w = _made((1, features), dtype, 41), _made((1, features), dtype, 42), _made((features,), dtype, 43)
+    weights, scales = ck.quantize_experts_mxfp8(_made((experts, n, features), torch.float32, 44, 0.06))
+    ends = torch.zeros(experts, dtype=torch.int32)
+    for e in (2, 3, 9, 15):
+        ends[e:] += 1
+    ends = ends.cuda()
+    codes, block_scales, h = ck.rms_norm_mxfp8(x.expand(chosen, -1), w, residual.expand(chosen, -1))
+    got = ck.grouped_mm_mxfp8(codes, weights, block_scales, scales, ends, out_dtype=dtype)
+    y, sums = ck.rms_norm(x, w, residual)
+    assert torch.equal(h, sums.expand(chosen, -1))
+    assert torch.equal(got, ck.grouped_linear_mxfp8(y.expand(chosen, -1), weights, scales, ends))
+    for row, e in enumerate((2, 3, 9, 15)):
+        one = ck.grouped_mm_mxfp8(codes[:1], weights[e:e + 1], block_scales, scales[e:e + 1], torch.ones(1, dtype=torch.int32, device="cuda"), out_dtype=dtype)
+        assert torch.equal(got[row:row + 1], one)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_same_without_the_native_host_half(ck, dtype, monkeypatch):
+    from comfy_kitchen.backends import cuda as backend
+
+    layer = _Layer(ck, 4, 64, 96, dtype, 71)
+    token, ends = torch.arange(24, device="cuda"), torch.tensor([5, 5, 20, 24], dtype=torch.int32, device="cuda")
+    x, residual, dy = _made((24, 64), dtype, 72).requires_grad_(), _made((24, 64), dtype, 73).requires_grad_(), _made((24, 64), dtype, 74)
+    leaves = (x, residual, layer.norm.weight)
+
+    def all_of_it():
+        with torch.no_grad():
+            quiet = (ck.rms_norm(x, layer.norm.weight), *ck.rms_norm_mxfp8(x, None, residual), layer(x, residual, token, ends))
+        grads = torch.autograd.grad(layer(x, residual, token, ends), leaves, dy)
+        holders = [torch.nn.Parameter(t.detach().clone()) for t in leaves]
+        for p, g in zip(holders, grads):
+            p.grad = g.clone()
+        return (*quiet, *grads, ck.grad_norm([p.grad for p in holders]), ck.clip_grad_norm_(holders, 0.3), *[p.grad for p in holders])
+
+    native = all_of_it()
+    with monkeypatch.context() as m:
+        m.setattr(backend, "_host", None)
+        plain = all_of_it()
+    assert len(native) == len(plain)
+    assert all(torch.equal(a.view(torch.uint8) if a.element_size() == 1 else a, b.view(torch.uint8) if b.element_size() == 1 else b)
+               for a, b in zip(native, plain))
+
+
+def test_compiled(ck):
+    layer = _Layer(ck, 4, 64, 96, torch.bfloat16, 81)
+    ends = torch.tensor([5, 5, 20, 24], dtype=torch.int32, device="cuda")
+    x, residual, dy = _made((24, 64), torch.bfloat16, 82).requires_grad_(), _made((24, 64), torch.bfloat16, 83).requires_grad_(), _made((24, 64), torch.bfloat16, 84)
+
+    def step(x, residual):
+        y, h = layer.norm(x, residual)
+        return h + layer.down(torch.nn.functional.gelu(layer.up(y, ends)), ends)
+
+    leaves = (x, residual, layer.norm.weight)
+    eager = torch.autograd.grad(step(x, residual), leaves, dy)
+    traced = torch.autograd.grad(torch.compile(step, backend="aot_eager")(x, residual), leaves, dy)
+    assert all(torch.equal(a, b) for a, b in zip(eager, traced))
+
+
+def test_recomputed_activations(ck):
+    """Inside torch's own checkpointing, which runs the forward pass again."""
+    from torch.utils.checkpoint import checkpoint
+
+    layer = _Layer(ck, 4, 64, 96, torch.float32, 91)
+    token, ends = torch.arange(24, device="cuda"), torch.tensor([5, 5, 20, 24], dtype=torch.int32, device="cuda")
+    x, residual, dy = _made((24, 64), torch.float32, 92).requires_grad_(), _made((24, 64), torch.float32, 93).requires_grad_(), _made((24, 64), torch.float32, 94)
+    leaves = (x, residual, layer.norm.weight)
+    plain = torch.autograd.grad(layer(x, residual, token, ends), leaves, dy)
+    again = torch.autograd.grad(checkpoint(layer, x, residual, token, ends, use_reentrant=False), leaves, dy)
+    assert all(torch.equal(a, b) for a, b in zip(plain, again))
+
+
+def _negated(t: torch.Tensor) -> torch.Tensor:
+    """-t as a strided view of complex memory"""
+    view = torch.complex(torch.zeros_like(t), t).conj().imag
+    assert view.is_neg()
+    return view
+
+
+def test_pending_negation(ck):
+    """Views whose memory holds the negative of their values."""
+    x, r, w = _made((24, 64), torch.float32, 101), _made((24, 64), torch.float32, 102), _made((64,), torch.float32, 103)
+    codes, scales = ck.quantize_experts_mxfp8(_made((2, 64, 64), torch.float32, 104, 0.1))
+    ends = torch.tensor([11, 24], dtype=torch.int32, device="cuda")
+    bias = _made((2, 64), torch.float32, 105)
+
+    def same(got, want):
+        for a, b in zip(got if isinstance(got, tuple) else (got,), want if isinstance(want, tuple) else (want,)):
+            assert torch.equal(a.view(torch.uint8) if a.element_size() == 1 else a, b.view(torch.uint8) if b.element_size() == 1 else b)
+
+    for neg in (_negated, torch._neg_view):
+        same(ck.rms_norm(neg(x), neg(w), neg(r)), ck.rms_norm(-x, -w, -r))
+        same(ck.rms_norm_mxfp8(neg(x), neg(w), neg(r)), ck.rms_norm_mxfp8(-x, -w, -r))
+        same(ck.grouped_linear_mxfp8(neg(x), codes, scales, ends, neg(bias)), ck.grouped_linear_mxfp8(-x, codes, scales, ends, -bias))
+        same(ck.grouped_input_grad_mxfp8(neg(x), codes, scales, ends), ck.grouped_input_grad_mxfp8(-x, codes, scales, ends))
+        same(ck.grad_norm([neg(x), r]), ck.grad_norm([-x, r]))
+        _, _, rstd = ck.rms_norm_forward(x, w)
+        same(ck.rms_norm_backward(neg(r), neg(x), rstd, neg(w)), ck.rms_norm_backward(-r, -x, rstd, -w))
+        p, q = torch.nn.Parameter(x.clone()), torch.nn.Parameter(x.clone())
+        p.grad, q.grad = neg(r), -r
+        same(ck.clip_grad_norm_([p], 0.5), ck.clip_grad_norm_([q], 0.5))
+        same(p.grad.resolve_neg().contiguous(), q.grad)
+
+
+def test_broadcast_gradients(ck):
+    """Gradients that are one value, or one row, for all (strides of zero), and inputs that are one row for all."""
+    x, w = _made((37, 96), torch.float32, 111).requires_grad_(), _made((96,), torch.float32, 112).requires_grad_()
+    for dy in (torch.ones((), device="cuda").expand(37, 96), _made((96,), torch.float32, 113).expand(37, 96), _made((37, 1), torch.float32, 114).expand(37, 96)):
+        got = torch.autograd.grad(ck.rms_norm(x, w), (x, w), dy)
+        want = torch.autograd.grad(ck.rms_norm(x, w), (x, w), dy.contiguous())
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    one = _made((96,), torch.float32, 115).requires_grad_()
+    g = _made((37, 96), torch.float32, 116)
+    got = torch.autograd.grad(ck.rms_norm(one.expand(37, 96), w), one, g)[0]
+    many = one.detach().repeat(37, 1).requires_grad_()
+    assert torch.equal(got, torch.autograd.grad(ck.rms_norm(many, w), many, g)[0].sum(0))
+
+
+def test_strict_mode_reports_a_wait_that_gave_up(ck, monkeypatch):
+    """The status word is set from the host here; no kernel is made to fail."""
+    from comfy_kitchen.backends import cuda as backend
+
+    lib = backend.load_library()
+    x = _made((24, 64), torch.bfloat16, 121)
+    codes, scales = ck.quantize_experts_mxfp8(_made((2, 64, 64), torch.float32, 122, 0.1))
+    ends = torch.tensor([11, 24], dtype=torch.int32, device="cuda")
+    q, s = ck.quantize_mxfp8(x)
+    backend.check_device_status("clean start")
+    monkeypatch.setenv("CK_STRICT", "1")
+    for call in (lambda: ck.rms_norm(x), lambda: ck.rms_norm_mxfp8(x), lambda: ck.grouped_linear_mxfp8(x, codes, scales, ends),
+                 lambda: ck.grouped_mm_mxfp8(q, codes, s, scales, ends), lambda: ck.grouped_input_grad_mxfp8(x, codes, scales, ends), lambda: ck.grad_norm([x])):
+        call()
+        assert lib.ck_debug_set_gemm_status(1) == 0
+        with pytest.raises(RuntimeError, match="gave up"):
+            call()
+    monkeypatch.setenv("CK_STRICT", "0")
+
+
+def test_the_example(ck):
+    """It runs, and its gradients are clipped where they are above the bound: the first step's norms of both kinds of layers agree up to bf16's and
+    MXFP8's roundings (blocks of 32 values, 2^-4 each: below a tenth of a norm)."""
+    if PKG_DIR not in sys.path:
+        sys.path.insert(0, PKG_DIR)
+    import train_mlp
+
+    said = []
+    ours = train_mlp.run(256, 128, 512, 2, 4, report=said.append, norm="rms", clip=0.01)
+    dense = train_mlp.run(256, 128, 512, 2, 4, dense=True, report=said.append, norm="rms", clip=0.01)
+    assert len(said) == 2 and len(ours["norms"]) == len(dense["norms"]) == 4
+    assert all(n > 0 for n in ours["norms"])
+    assert abs(ours["norms"][0] - dense["norms"][0]) <= 0.1 * dense["norms"][0]
+    assert ours["kept_bytes"] < dense["kept_bytes"]
