@@ -11,8 +11,9 @@
 // registers, those behind the group's end not at all; rows behind the last group are zeros.
 //
 // Many rows: bound by the tensor pipe and, in a loop, by the power limit (8192 x 8192 x 4096 of 8 experts from bf16 250 us, 2.2 PFLOP/s with the quantization;
-// 298 in a loop; one weight for all rows 202: the groups' last tiles are half empty).  Few rows: by the weights' bytes (64 experts of 2048 x 2048, 32 rows each, 57 us,
-// 5.1 TB/s); one token through eight of 64 experts, 25 MB, 10.7 us: two launches, first loads.
+// 298 in a loop; one weight for all rows 202: the groups' last tiles are half empty).  Few rows: by the weights' bytes (64 experts of 2048 x 2048, 32 rows each, 55 us,
+// 5.3 TB/s); one token through eight of 64 experts, 25 MB, 10.4 us: two launches, first loads (11.7 with the weights asked for behind the first kernel's end;
+// 777 rows of 40 experts of 1000 x 1056 16.4 and 18.3; a few megabytes of weights gain nothing, 64 rows of 8 experts of 1024 x 1024 7.1 and 6.9).
 #include "ck_gemm_kernel.cuh"
 #include "ck_groups.cuh"
 #include "ck_rows.cuh"
@@ -101,7 +102,8 @@ grouped_gemm_kernel(const __grid_constant__ RowMaps maps_a, const __grid_constan
   __syncthreads();
   if constexpr (CTAS == 2) cluster_sync_all();  // the other CTA's barriers exist before anything reports to them
   tc_fence_after_sync();
-  pdl_wait();  // ends, operands and scales may come from the kernel before this one
+  // The kernel before this one has waited for its own predecessor before it let this one start, so the ends, the weights and their scales are there;
+  // x's codes and scales are not.  Weights of the first stages are on their way while that kernel still runs.
   groups::fill_table(table, p.offsets, p.groups, p.M, Cfg::kTileRows);
   const uint32_t tmem = *tmem_slot;
 
@@ -112,8 +114,31 @@ grouped_gemm_kernel(const __grid_constant__ RowMaps maps_a, const __grid_constan
     if (elect_one()) {
       const uint32_t full = smem_u32(full_bar), empty = smem_u32(empty_bar);
       const uint32_t a_addr = smem_u32(smem_a), b_addr = smem_u32(smem_b), sfa_addr = smem_u32(smem_sfa), sfb_addr = smem_u32(smem_sfb);
-      int s = 0;
+      int s = 0, ahead = 0;  // stages whose weights have been asked for already
       uint32_t ph = 0;
+      if (worker < items) {
+        const groups::Tile t = groups::place(table, p.groups, p.tiles_n, Cfg::kTileRows, worker);
+        const int n0 = t.tile_n * TILE_N, left = t.end - t.row - static_cast<int>(cta_rank) * kTileM;
+        const int b_row = t.group * p.N + n0 + static_cast<int>(cta_rank) * Cfg::kBRows, rb_b = t.group * p.n_row_blocks_b + n0 / 128;
+        const uint32_t a_bytes = box_height(CTAS == 2 || left > box_height(1) ? 2 : left > box_height(0) ? 1 : 0) * kStageKBytes;
+        const int rb_b_count = min(Cfg::kSfbRowBlocks, p.n_row_blocks_b - n0 / 128);
+        ahead = min(STAGES, k_stages);
+        for (int ks = 0; ks < ahead; ++ks) {
+          const uint32_t bar = full + ks * 8;
+          if constexpr (CTAS == 2) {
+            if (cta_rank == 0) mbar_arrive_expect_tx(bar, 2 * Cfg::kStageBytes);  // both CTAs' loads report to the leader
+            tma_load_2d_pair(b_addr + ks * Cfg::kBBytes, &map_b, bar, ks * kStageKBytes, b_row);
+            tma_load_3d_pair(sfb_addr + ks * Cfg::kSfbBytes, &map_sfb, bar, 0, ks, rb_b);
+          } else {
+            mbar_arrive_expect_tx(bar, a_bytes + Cfg::kBBytes + 512u * (1 + rb_b_count));
+            tma_load_2d(b_addr + ks * Cfg::kBBytes, &map_b, bar, ks * kStageKBytes, b_row);
+            for (int r = 0; r < rb_b_count; ++r) {
+              bulk_load_1d(sfb_addr + ks * Cfg::kSfbBytes + r * 512, p.sfb + ((static_cast<int64_t>(rb_b) + r) * p.col_tiles + ks) * 512, 512, bar);
+            }
+          }
+        }
+      }
+      pdl_wait();  // also where there is no tile: this kernel does not end before the one in front of it
       for (int item = worker; item < items; item += workers) {
         const groups::Tile t = groups::place(table, p.groups, p.tiles_n, Cfg::kTileRows, item);
         const int m0 = t.row + static_cast<int>(cta_rank) * kTileM, n0 = t.tile_n * TILE_N;
@@ -130,20 +155,26 @@ grouped_gemm_kernel(const __grid_constant__ RowMaps maps_a, const __grid_constan
         for (int ks = 0; ks < k_stages; ++ks) {
           mbar_wait(empty + s * 8, ph ^ 1, abort_flag);
           const uint32_t bar = full + s * 8;
+          const bool whole = ahead == 0;
+          if (!whole) --ahead;
           if constexpr (CTAS == 2) {
-            if (cta_rank == 0) mbar_arrive_expect_tx(bar, 2 * Cfg::kStageBytes);  // both CTAs' loads report to the leader
-            tma_load_2d_pair(a_addr + s * Cfg::kABytes, map_a, bar, ks * kStageKBytes, m0);
-            tma_load_2d_pair(b_addr + s * Cfg::kBBytes, &map_b, bar, ks * kStageKBytes, b_row);
-            tma_load_3d_pair(sfa_addr + s * Cfg::kSfaBytes, &map_sfa, bar, 0, ks, rb_a);
-            tma_load_3d_pair(sfb_addr + s * Cfg::kSfbBytes, &map_sfb, bar, 0, ks, rb_b);
-          } else {
-            mbar_arrive_expect_tx(bar, a_bytes + Cfg::kBBytes + 512u * (1 + rb_b_count));
-            tma_load_2d(a_addr + s * Cfg::kABytes, map_a, bar, ks * kStageKBytes, m0);
-            tma_load_2d(b_addr + s * Cfg::kBBytes, &map_b, bar, ks * kStageKBytes, b_row);
-            bulk_load_1d(sfa_addr + s * Cfg::kSfaBytes, sfa_src + ks * 512, 512, bar);
-            for (int r = 0; r < rb_b_count; ++r) {
-              bulk_load_1d(sfb_addr + s * Cfg::kSfbBytes + r * 512, sfb_src + (static_cast<int64_t>(r) * p.col_tiles + ks) * 512, 512, bar);
+            if (whole) {
+              if (cta_rank == 0) mbar_arrive_expect_tx(bar, 2 * Cfg::kStageBytes);
+              tma_load_2d_pair(b_addr + s * Cfg::kBBytes, &map_b, bar, ks * kStageKBytes, b_row);
+              tma_load_3d_pair(sfb_addr + s * Cfg::kSfbBytes, &map_sfb, bar, 0, ks, rb_b);
             }
+            tma_load_2d_pair(a_addr + s * Cfg::kABytes, map_a, bar, ks * kStageKBytes, m0);
+            tma_load_3d_pair(sfa_addr + s * Cfg::kSfaBytes, &map_sfa, bar, 0, ks, rb_a);
+          } else {
+            if (whole) {
+              mbar_arrive_expect_tx(bar, a_bytes + Cfg::kBBytes + 512u * (1 + rb_b_count));
+              tma_load_2d(b_addr + s * Cfg::kBBytes, &map_b, bar, ks * kStageKBytes, b_row);
+              for (int r = 0; r < rb_b_count; ++r) {
+                bulk_load_1d(sfb_addr + s * Cfg::kSfbBytes + r * 512, sfb_src + (static_cast<int64_t>(r) * p.col_tiles + ks) * 512, 512, bar);
+              }
+            }
+            tma_load_2d(a_addr + s * Cfg::kABytes, map_a, bar, ks * kStageKBytes, m0);
+            bulk_load_1d(sfa_addr + s * Cfg::kSfaBytes, sfa_src + ks * 512, 512, bar);
           }
           if (++s == STAGES) {
             s = 0;
@@ -156,6 +187,7 @@ grouped_gemm_kernel(const __grid_constant__ RowMaps maps_a, const __grid_constan
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMAs, by the pair's leader
     if (cta_rank == 0 && elect_one()) {
+      pdl_wait();  // nothing is complete earlier: keeps the bounded waits from running beside a long predecessor
       const uint32_t a_lo0 = static_cast<uint32_t>(make_operand_desc_sw128(smem_u32(smem_a)));
       const uint32_t b_lo0 = static_cast<uint32_t>(make_operand_desc_sw128(smem_u32(smem_b)));
       const uint32_t op_hi = static_cast<uint32_t>(make_operand_desc_sw128(0) >> 32);
@@ -211,6 +243,7 @@ grouped_gemm_kernel(const __grid_constant__ RowMaps maps_a, const __grid_constan
     __syncwarp();
   } else {
     // ---------------------------------------------------------------- epilogue
+    pdl_wait();  // see above
     const int quarter = warp & 3, share = (warp - 2) >> 2;
     constexpr int kWarpCols = TILE_N / (kWarps / 4), kChunks = kWarpCols / 32;
     const uint32_t acc_empty = CTAS == 2 ? map_to_cta(smem_u32(acc_empty_bar), 0) : smem_u32(acc_empty_bar);
@@ -310,11 +343,11 @@ grouped_gemm_kernel(const __grid_constant__ RowMaps maps_a, const __grid_constan
 template <typename T>
 __global__ void __launch_bounds__(256) quantize_groups_kernel(const T* x, const int* offsets, int count, int rows, int64_t cols, uint8_t* codes,
                                                               uint8_t* scales) {
-  pdl_launch_dependents();
   const int64_t blocks = cols >> 5, col_tiles = ceil_div(blocks, 4);
   const int64_t index = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   const int64_t row = index / (col_tiles * 4), block = index - row * (col_tiles * 4);
   pdl_wait();
+  pdl_launch_dependents();  // not earlier: the GEMM reads the weights and the ends without waiting for this kernel's end
   uint32_t byte = 0;
   if (row < rows && block < blocks) {
     constexpr int kVec = 16 / static_cast<int>(sizeof(T));
@@ -352,11 +385,11 @@ __global__ void __launch_bounds__(256) quantize_groups_kernel(const T* x, const 
 
 // A word (one row, four blocks) a thread; the 128 words of a tile of x's scales beside one another.
 __global__ void __launch_bounds__(256) regroup_scales_kernel(const uint8_t* from, const int* offsets, int count, int rows, int64_t col_tiles, uint8_t* scales) {
-  pdl_launch_dependents();
   const int64_t index = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, tile = index >> 7;
   const int64_t row_block = tile / col_tiles, col = tile - row_block * col_tiles, row = row_block * 128 + (index & 127);
-  if (row >= rows) return;
   pdl_wait();
+  pdl_launch_dependents();  // not earlier, as above
+  if (row >= rows) return;
   const int e = groups::group_of_row(offsets, count, static_cast<int>(row));
   if (e == count) return;
   const int begin = groups::group_end(offsets, e - 1, rows);

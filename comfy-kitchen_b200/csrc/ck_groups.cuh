@@ -49,7 +49,7 @@ struct Table {
   int tiles[kMaxGroups + 1];  // row tiles of the groups before e
 };
 
-// Filled by all threads of the block, behind pdl_wait.
+// Filled by all threads of the block, when the ends are there.
 __device__ __forceinline__ void fill_table(Table* t, const int* offsets, int count, int rows, int tile_rows) {
   for (int e = threadIdx.x; e <= count; e += blockDim.x) t->bound[e] = group_end(offsets, e - 1, rows);
   __syncthreads();

@@ -281,3 +281,41 @@ def test_the_example(ck):
     assert all(n > 0 for n in ours["norms"])
     assert abs(ours["norms"][0] - dense["norms"][0]) <= 0.1 * dense["norms"][0]
     assert ours["kept_bytes"] < dense["kept_bytes"]
+
+
+def test_weights_of_the_kernel_before(ck):
+    """Weights and ends that the kernels right in front of the call have written, into memory that held others: two sets in turn, in a graph."""
+    experts, n, k, rows = 4, 256, 512, 50
+    dense = [_made((experts * n, k), torch.bfloat16, 131 + i, 0.05) for i in range(2)]
+    sizes = [torch.tensor(v, dtype=torch.int32, device="cuda") for v in ((10, 20, 30, 50), (0, 45, 45, 48))]
+    x = _made((rows, k), torch.bfloat16, 141)
+    q, s = ck.quantize_mxfp8(x)
+    dy = _made((rows, n), torch.bfloat16, 142)
+    source, ends = torch.empty_like(dense[0]), torch.empty_like(sizes[0])
+
+    def calls():
+        codes, scales = ck.quantize_mxfp8(source)
+        codes, scales = codes.view(experts, n, k), scales.view(experts, n, -1)
+        a = ck.grouped_linear_mxfp8(x, codes, scales, ends)
+        codes, scales = ck.quantize_mxfp8(source)
+        b = ck.grouped_mm_mxfp8(q, codes.view(experts, n, k), s, scales.view(experts, n, -1), ends)
+        codes, scales = ck.quantize_mxfp8(source)
+        return a, b, ck.grouped_input_grad_mxfp8(dy, codes.view(experts, n, k), scales.view(experts, n, -1), ends)
+
+    want = []
+    for i in range(2):
+        source.copy_(dense[i]), ends.copy_(sizes[i])
+        torch.cuda.synchronize()
+        want.append([t.clone() for t in calls()])
+        assert torch.equal(want[i][0], want[i][1])
+    assert not torch.equal(want[0][0], want[1][0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        source.copy_(dense[0]), ends.copy_(sizes[0])
+        first = calls()
+        source.copy_(dense[1]), ends.copy_(sizes[1])
+        second = calls()
+    for _ in range(200):
+        graph.replay()
+        for got, ref in zip((*first, *second), (*want[0], *want[1])):
+            assert torch.equal(got, ref)
