@@ -7,7 +7,7 @@
 // each, all fetched before the first is used; teams of up to 32 lanes share warps, wider rows have a block to themselves.
 // The result can be MXFP8 (the values rounded to x's type, then as ck_quantize_mxfp8 has them): the lanes that share a block of 32 elements
 // find its maximum, those that share four blocks write a word of scales.
-// Backward, the blocks stay: each takes every so-manieth row out of a ring in shared memory and adds dweight's terms of its columns in
+// Backward, the blocks stay: each takes its share of the rows, spread over all, out of a ring in shared memory and adds dweight's terms of its columns in
 // registers; a second kernel adds the blocks' sums in order.
 // 16384 x 4096 bf16 with a residual: forward 82 us (6.56 TB/s, 1.00 of the copy rate), with an MXFP8 result 83 (5.7), backward 89 (6.0); 20000 x 1001
 // 44 and 44; one row of 4096 2.6 and 6.7.
