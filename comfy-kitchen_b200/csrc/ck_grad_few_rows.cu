@@ -333,7 +333,7 @@ grad_few_rows_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_co
 // ---- grouped rows --------------------------------------------------------------------------------------------
 // dX[i] = dY[i] W_e for the rows i of group e: the same operand, but blocks that stay and take tiles (a group's rows, 128 columns of W_e) in turn, accumulators in two
 // sets, so that a tile is stored beside the next one's steps, and loads of dY and of codes by warps of their own.  Bound by the decoding, 2.9 million codes a microsecond: 64
-// groups of 32 rows, 2048 x 2048 each, bf16 92 us (fp32, three numbers an element, 161); eight rows of as many groups, 1536 x 2048, 13.8.
+// groups of 32 rows, 2048 x 2048 each, bf16 93 us (fp32, three numbers an element, 138); eight rows of as many groups, 1536 x 2048, 14.0.
 constexpr int kRowBox = 16;  // rows of dY in a copy
 constexpr int kStoreWarps = 4, kGroupedThreads = kThreads + 32 * (kStoreWarps + 1);  // beside those of the kernel above, and the loads of dY apart from the codes
 
@@ -735,14 +735,15 @@ namespace {
 constexpr int kGroupedSmem = 226 * 1024 - 1024;  // dynamic, beside the barriers
 
 // Rows of a tile at most: as many as there is room for beside the fewest stages and eight of codes, or four where groups of so many rows would need
-// more.  A tile computes and loads what it has rows for, and a group in fewer tiles has its weight decoded less often; but codes four stages ahead come
-// late (64 experts of 2048 x 2048: 32 rows each of fp32 161 us with tiles of 48, 195 with 64; 64 of fp16 163 with 80, 195 with 112).
+// more, or less than 64 fitted.  A tile computes and loads what it has rows for, and a group in fewer tiles has its weight decoded less often; codes that are fetched
+// four stages ahead come late at times (us, eight / four: 333 uneven rows of 16 experts of 1536 x 2048 in fp32, tiles of 48 / 64, 43.4 / 33.4, even ones 37.1 / 36.2, 64
+// experts of 2048 x 2048, 64 uneven rows each, 201 / 203; fp16, 80 / 112, 250 uneven rows each 405 / 415, 19 of 1024 x 1024 41.5 / 42.6; bf16, 160 / 224, 191 / 189).
 int grouped_few_rows_tile(int64_t rows, int planes) {
   const auto most = [&](int raw_stages) {
     const int room = (kGroupedSmem - 1024 - raw_stages * kRawBytes - static_cast<int>(sizeof(groups::Table))) / kMinStages - kHeldBytes;
     return room / (planes * kRowBox * 128) * kRowBox;
   };
-  return most(kMaxRaw) >= rows ? most(kMaxRaw) : most(kGroups);
+  return most(kMaxRaw) >= (rows > 64 ? rows : 64) ? most(kMaxRaw) : most(kGroups);
 }
 
 // E4M3 [E, N, K], boxes of 128 columns x 64 rows of one matrix, as they lie in memory; rows past N and columns past K read as zeros.
