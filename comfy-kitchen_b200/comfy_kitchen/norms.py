@@ -4,7 +4,8 @@
   the sum, which is returned beside the result: ``y, h = rms_norm(x, weight, residual)`` is one pass where a layer would add, write,
   read and normalize.  Differentiable in x, residual and weight.
 * :func:`rms_norm_mxfp8`: the same with the result in MXFP8, as the next layer's :func:`comfy_kitchen.scaled_mm_mxfp8` or
-  :func:`comfy_kitchen.grouped_mm_mxfp8` takes it; bit for bit ``quantize_mxfp8`` of :func:`rms_norm`'s rows.  For inference: codes carry no gradient.
+  :func:`comfy_kitchen.grouped_mm_mxfp8` takes it; what ``quantize_mxfp8`` gives for :func:`rms_norm`'s rows, up to the last bit of a row's norm (narrow rows
+  and ones off 32-byte boundaries have their squares added in another order).  For inference: codes carry no gradient.
 * :class:`RMSNorm`: a module around them.
 * :func:`grad_norm`, :func:`clip_grad_norm_`: the 2-norm over all gradients, and their scaling where it is above a bound, in two launches for up
   to 1024 tensors and without a read on the host.

@@ -362,8 +362,8 @@ CK_API int ck_linear_input_grad_mxfp8(const void* dy, int dy_dtype, const void* 
  *   y = h * rstd * f,  f = weight_offset + weight (1 where weight is null)
  * x, residual: [rows, cols] f32/f16/bf16, rows in two levels as ck_layer_norm_forward has them.  weight: [cols] of param_dtype, which is
  * dtype or f32.  h: [rows, cols] contiguous, null exactly where residual is.  rstd: [rows] f32 or null.  Either y ([rows, cols] contiguous
- * of dtype), or codes and block_scales: what ck_quantize_mxfp8 gives for y (cols % 32 == 0; rows of x and residual on
- * 32-byte boundaries, h and codes too, the weight on a 16-byte one).  fp32 arithmetic, one rounding (codes: behind that to dtype).
+ * of dtype), or codes and block_scales: what ck_quantize_mxfp8 gives for y, up to the last bit of a row's rstd (cols % 32 == 0; rows of x and
+ * residual on 32-byte boundaries, h and codes too, the weight on a 16-byte one).  fp32 arithmetic, one rounding (codes: behind that to dtype).
  */
 CK_API int ck_rms_norm_forward(const void* x, int dtype, int64_t rows, int64_t cols, int64_t x_inner, int64_t x_outer_stride,
                         int64_t x_inner_stride, const void* residual, int64_t r_inner, int64_t r_outer_stride,

@@ -268,3 +268,24 @@ def test_refusals(ck):
                 lambda: ck.rms_norm(x, w.view(1, 64))):
         with pytest.raises(Exception):
             bad()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols,start", [(30000, 32, 0), (20000, 64, 0), (9000, 128, 0), (2000, 1856, 3), (300, 6336, 8)])
+def test_mxfp8_of_many_rows(ck, dtype, rows, cols, start):
+    """Rows whose squares are added in another order than rms_norm's, so that a last bit may differ: values within the roundings to their type and to codes,
+    scales the smallest powers of two that hold a block (or twice that where its largest value stands on the border)."""
+    x = _made((rows, cols + start), dtype, 91)[:, start:]
+    w = _made((cols,), torch.float32, 92)
+    codes, scales = ck.rms_norm_mxfp8(x, w)
+    value = x.double() * (x.double().square().mean(-1, keepdim=True) + 1e-6).rsqrt() * w.double()
+    off_by = (40 + cols / 2048 + 4) * U + ROUND[dtype]  # the norm and the products in fp32, the rounding to x's type
+    blocks = value.abs().view(rows, -1, 32).amax(-1)
+    held = ck.dequantize_mxfp8(codes, scales, torch.float32).double()
+    r, c = torch.arange(rows, device="cuda").unsqueeze(1), torch.arange(cols // 32, device="cuda").unsqueeze(0)
+    at = ((r // 128) * (scales.shape[1] // 4) + c // 4) * 512 + (r % 32) * 16 + (r // 32 % 4) * 4 + c % 4
+    step = 2.0 ** (scales.view(torch.uint8).reshape(-1)[at].double() - 127)
+    assert (step * 448 >= blocks * (1 - 2 * off_by)).all() and (step * 224 <= blocks * (1 + 2 * off_by)).all()
+    # E4M3: half a step is 2^-4 of the value, or 2^-10 of the scale below 2^-6 of it
+    limit = off_by * value.abs() + 2.0**-4 * value.abs() * (1 + off_by) + 2.0**-10 * step.repeat_interleave(32, 1)
+    assert ((held - value).abs() <= limit).all()
