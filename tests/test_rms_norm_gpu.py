@@ -289,3 +289,22 @@ def test_mxfp8_of_many_rows(ck, dtype, rows, cols, start):
     # E4M3: half a step is 2^-4 of the value, or 2^-10 of the scale below 2^-6 of it
     limit = off_by * value.abs() + 2.0**-4 * value.abs() * (1 + off_by) + 2.0**-10 * step.repeat_interleave(32, 1)
     assert ((held - value).abs() <= limit).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_mxfp8_of_infinities_and_nan(ck, dtype):
+    """As the quantizer has them, and only in their own rows."""
+    x, w = _made((40, 256), dtype, 95), _made((256,), dtype, 96)
+    clean = ck.rms_norm_mxfp8(x, w)
+    x[3, 40], x[7, 200], x[20, 0] = float("inf"), float("nan"), float("-inf")
+    w2 = w.clone()
+    w2[100] = float("nan")
+    for weight in (w, w2):
+        codes, scales = ck.rms_norm_mxfp8(x, weight)
+        want, want_scales = ck.quantize_mxfp8(ck.rms_norm(x, weight))
+        assert torch.equal(codes.view(torch.uint8), want.view(torch.uint8)) and torch.equal(scales.view(torch.uint8), want_scales.view(torch.uint8))
+    rest = [i for i in range(40) if i not in (3, 7, 20)]
+    codes, scales = ck.rms_norm_mxfp8(x, w)
+    assert torch.equal(codes.view(torch.uint8)[rest], clean[0].view(torch.uint8)[rest])
+    linear = ck.dequantize_mxfp8(codes, scales, torch.float32)
+    assert torch.equal(linear[rest], ck.dequantize_mxfp8(*clean, torch.float32)[rest])
