@@ -7,13 +7,18 @@
 // A tile is rows of one group by columns: it begins at the group's first row, wherever in x that is (a TMA box may start at any row), and its
 // scales come from tiles of 128 rows that begin there too.  A first kernel writes those beside the quantization, or from the scales of x
 // as they stand (1/32 of x).  The GEMM is the block-scaled one of ck_gemm_kernel.cuh (TMA producer, one issuing lane, epilogue
-// warps, two roles' distance by mbarriers) over a list of tiles that every CTA makes for itself from the groups' ends.  Rows are stored from
-// registers, those behind the group's end not at all; rows behind the last group are zeros.
+// warps, two roles' distance by mbarriers) over a list of tiles that every CTA makes for itself from the groups' ends.  Rows behind the group's end are not stored;
+// rows behind the last group are zeros.
 //
-// Many rows: bound by the tensor pipe and, in a loop, by the power limit (8192 x 8192 x 4096 of 8 experts from bf16 250 us, 2.2 PFLOP/s with the quantization;
-// 298 in a loop; one weight for all rows 202: the groups' last tiles are half empty).  Few rows: by the weights' bytes (64 experts of 2048 x 2048, 32 rows each, 55 us,
+// CTA pairs, for many rows, compute W_e x^T: the weights' rows are the MMA's 256, x's rows its columns, of which there may be any multiple of 32, so that a group's last
+// tile costs what it has rows for.  The results come feature by feature and are turned in shared memory on their way out.  (With x's rows as the MMA's 256, last tiles
+// whole, us, so / before: 64 experts of 2048 x 2048, 140 rows each 62 / 69, 188 uneven ones 75 / 81, 256 88 / 92; 8 of 8192 x 4096, 1024 uneven rows 215 to 258 / 235 to 267;
+// 8 of 8192 x 512 48.9 / 47.5.)
+//
+// Many rows: bound by the tensor pipe and, in a loop, by the power limit (8192 x 8192 x 4096 of 8 experts from bf16 235 us, 2.3 PFLOP/s with the quantization;
+// one weight for all rows 202).  Few rows: by the weights' bytes (64 experts of 2048 x 2048, 32 rows each, 55 us,
 // 5.3 TB/s); one token through eight of 64 experts, 25 MB, 10.4 us: two launches, first loads (11.7 with the weights asked for behind the first kernel's end;
-// 777 rows of 40 experts of 1000 x 1056 16.4 and 18.3; a few megabytes of weights gain nothing, 64 rows of 8 experts of 1024 x 1024 7.1 and 6.9).
+// 777 rows of 40 experts of 1000 x 1056 16.3 and 18.3; a few megabytes of weights gain nothing, 64 rows of 8 experts of 1024 x 1024 7.1 and 6.9).
 #include "ck_gemm_kernel.cuh"
 #include "ck_groups.cuh"
 #include "ck_rows.cuh"
@@ -46,20 +51,65 @@ __device__ __forceinline__ float bias_at(const void* bias, int dtype, int64_t at
   return static_cast<const float*>(bias)[at];
 }
 
-template <int TILE_N, int NUM_ACC, int STAGES, int CTAS>
+template <int TILE_N, int NUM_ACC, int STAGES, int CTAS, int kOutBytes>
 struct GroupedConfig : Config<Kind::kMxfp8, TILE_N, NUM_ACC, STAGES, CTAS, 0> {
   using Base = Config<Kind::kMxfp8, TILE_N, NUM_ACC, STAGES, CTAS, 0>;
-  static constexpr int kTableBytes = (static_cast<int>(sizeof(groups::Table)) + 15) / 16 * 16, kBiasBytes = 128 * epilogue_warps(false, TILE_N) * (TILE_N / (epilogue_warps(false, TILE_N) / 4) / 32);
-  static constexpr int kSmem = Base::kRingBytes + 1024 + 256 + kTableBytes + kBiasBytes;
+  static constexpr int kTableBytes = (static_cast<int>(sizeof(groups::Table)) + 15) / 16 * 16, kWarps = epilogue_warps(false, TILE_N);
+  // a pair's warps turn 32 rows by 32 features; the others pass their columns' bias round
+  static constexpr int kEpilogueBytes = CTAS == 2 ? kWarps * 1024 * kOutBytes : kWarps * (TILE_N / (kWarps / 4)) * 4;
+  static constexpr int kSmem = Base::kRingBytes + 1024 + 256 + kTableBytes + kEpilogueBytes;
   static_assert(kSmem <= 227 * 1024, "shared memory budget exceeded");
 };
 
+// 32 x 32 numbers turned by a warp: a lane writes its feature's, one for each row, and reads 16 bytes of neighbouring features of row 32 / pieces * i + lane / pieces.
+// Numbers of 16 bits lie by feature, in pieces of eight rows whose places change with the feature so that neither the writes nor the transposing reads of 8 x 8
+// matrices (whose rows are the features 8 j + 2 m and 8 j + 2 m + 1, so that a lane gets eight in a row) meet a bank twice; those of 32 lie by row.
+__device__ __forceinline__ uint32_t turn_place(int feature, int piece) {
+  return static_cast<uint32_t>(feature * 64 + ((piece ^ (feature >> 1) ^ (feature >> 3)) & 3) * 16);
+}
+template <typename OutT>
+__device__ __forceinline__ void turn_write(uint32_t turn, int lane, const float* v) {
+  if constexpr (sizeof(OutT) == 2) {
+    uint32_t w[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float pair[2] = {v[2 * i], v[2 * i + 1]};
+      const rows::Raw<OutT, 2> r = rows::pack<OutT, 2>(pair);
+      w[i] = *reinterpret_cast<const uint32_t*>(&r);
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) st_shared_128(turn + turn_place(lane, q), w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) asm volatile("st.shared.f32 [%0], %1;" ::"r"(turn + (i * 32 + lane) * 4), "f"(v[i]) : "memory");
+  }
+}
+template <typename OutT>
+__device__ __forceinline__ rows::Raw<OutT, 16 / static_cast<int>(sizeof(OutT))> turn_read(uint32_t turn, int lane, int i) {
+  rows::Raw<OutT, 16 / static_cast<int>(sizeof(OutT))> r;
+  uint32_t* w = reinterpret_cast<uint32_t*>(&r);
+  if constexpr (sizeof(OutT) == 2) {
+    const int feature = (lane & 7) / 2 * 8 + (lane >> 3) * 2 + (lane & 1);
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                 : "r"(turn + turn_place(feature, i))
+                 : "memory");
+  } else {
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                 : "r"(turn + (i * 32 + lane) * 16)
+                 : "memory");
+  }
+  return r;
+}
+
 template <int TILE_N, int NUM_ACC, int STAGES, int CTAS, typename OutT>
 __global__ void __launch_bounds__(num_threads(false, TILE_N), 1)
-grouped_gemm_kernel(const __grid_constant__ RowMaps maps_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_sfa,
-                    const __grid_constant__ CUtensorMap map_sfb, const GroupedParams p) {
-  using Cfg = GroupedConfig<TILE_N, NUM_ACC, STAGES, CTAS>;
+grouped_gemm_kernel(const __grid_constant__ RowMaps maps_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_sfx,
+                    const __grid_constant__ CUtensorMap map_sfw, const GroupedParams p) {
+  using Cfg = GroupedConfig<TILE_N, NUM_ACC, STAGES, CTAS, static_cast<int>(sizeof(OutT))>;
   constexpr int kWarps = epilogue_warps(false, TILE_N);
+  constexpr int kTileCols = CTAS == 2 ? 2 * kTileM : TILE_N;  // output features of a tile
   pdl_launch_dependents();
   const uint32_t cta_rank = CTAS == 2 ? cluster_cta_rank() : 0u;
   const int worker = blockIdx.x / CTAS, workers = gridDim.x / CTAS;
@@ -90,11 +140,11 @@ grouped_gemm_kernel(const __grid_constant__ RowMaps maps_a, const __grid_constan
       mbar_init(&acc_empty_bar[a], kWarps * CTAS);
     }
     fence_barrier_init();
-    for (int h = 0; h < 3; ++h) prefetch_tensormap(&maps_a.m[h]);
-    prefetch_tensormap(&map_b);
+    for (int h = 0; h < 3; ++h) prefetch_tensormap(&maps_x.m[h]);
+    prefetch_tensormap(&map_w);
     if constexpr (CTAS == 2) {
-      prefetch_tensormap(&map_sfa);
-      prefetch_tensormap(&map_sfb);
+      prefetch_tensormap(&map_sfx);
+      prefetch_tensormap(&map_sfw);
     }
   }
   if (warp == 1) tmem_alloc<CTAS>(tmem_slot, Cfg::kTmemCols);
@@ -108,6 +158,12 @@ grouped_gemm_kernel(const __grid_constant__ RowMaps maps_a, const __grid_constan
   const uint32_t tmem = *tmem_slot;
 
   const int items = table->tiles[p.groups] * p.tiles_n;
+  // What of a tile's rows is computed on by a pair: as many of the MMA's columns, in steps of 32; and the box that holds a CTA's share of them.
+  const auto columns_of = [&](const groups::Tile& t) { return CTAS == 2 ? (min(256, t.end - t.row) + 31) / 32 * 32 : 0; };
+  const auto box_of = [&](const groups::Tile& t) {
+    const int need = CTAS == 2 ? columns_of(t) / 2 : t.end - t.row;
+    return need > box_height(1) ? 2 : CTAS == 2 || need > box_height(0) ? 1 : 0;
+  };
   const int k_stages = (p.k_bytes + kStageKBytes - 1) / kStageKBytes, total_mma = (p.k_bytes + kMmaKBytes - 1) / kMmaKBytes;
   if (warp == 0) {
     // ---------------------------------------------------------------- loads
@@ -118,40 +174,35 @@ grouped_gemm_kernel(const __grid_constant__ RowMaps maps_a, const __grid_constan
       uint32_t ph = 0;
       if (worker < items) {
         const groups::Tile t = groups::place(table, p.groups, p.tiles_n, Cfg::kTileRows, worker);
-        const int n0 = t.tile_n * TILE_N, left = t.end - t.row - static_cast<int>(cta_rank) * kTileM;
-        const int b_row = t.group * p.N + n0 + static_cast<int>(cta_rank) * Cfg::kBRows, rb_b = t.group * p.n_row_blocks_b + n0 / 128;
-        const uint32_t a_bytes = box_height(CTAS == 2 || left > box_height(1) ? 2 : left > box_height(0) ? 1 : 0) * kStageKBytes;
-        const int rb_b_count = min(Cfg::kSfbRowBlocks, p.n_row_blocks_b - n0 / 128);
+        const int n0 = t.tile_n * kTileCols, rank = static_cast<int>(cta_rank);
+        const int w_row = t.group * p.N + n0 + rank * kTileM, rb_w = t.group * p.n_row_blocks_b + n0 / 128 + rank;
+        const uint32_t x_bytes = box_height(box_of(t)) * kStageKBytes;
         ahead = min(STAGES, k_stages);
         for (int ks = 0; ks < ahead; ++ks) {
           const uint32_t bar = full + ks * 8;
           if constexpr (CTAS == 2) {
-            if (cta_rank == 0) mbar_arrive_expect_tx(bar, 2 * Cfg::kStageBytes);  // both CTAs' loads report to the leader
-            tma_load_2d_pair(b_addr + ks * Cfg::kBBytes, &map_b, bar, ks * kStageKBytes, b_row);
-            tma_load_3d_pair(sfb_addr + ks * Cfg::kSfbBytes, &map_sfb, bar, 0, ks, rb_b);
+            if (cta_rank == 0) mbar_arrive_expect_tx(bar, 2 * (Cfg::kABytes + x_bytes + Cfg::kSfaBytes + Cfg::kSfbBytes));  // both CTAs' loads report to the leader
+            tma_load_2d_pair(a_addr + ks * Cfg::kABytes, &map_w, bar, ks * kStageKBytes, w_row);
+            tma_load_3d_pair(sfa_addr + ks * Cfg::kSfaBytes, &map_sfw, bar, 0, ks, rb_w);
           } else {
-            mbar_arrive_expect_tx(bar, a_bytes + Cfg::kBBytes + 512u * (1 + rb_b_count));
-            tma_load_2d(b_addr + ks * Cfg::kBBytes, &map_b, bar, ks * kStageKBytes, b_row);
-            for (int r = 0; r < rb_b_count; ++r) {
-              bulk_load_1d(sfb_addr + ks * Cfg::kSfbBytes + r * 512, p.sfb + ((static_cast<int64_t>(rb_b) + r) * p.col_tiles + ks) * 512, 512, bar);
-            }
+            mbar_arrive_expect_tx(bar, x_bytes + Cfg::kBBytes + 512u * 2);
+            tma_load_2d(b_addr + ks * Cfg::kBBytes, &map_w, bar, ks * kStageKBytes, w_row);
+            bulk_load_1d(sfb_addr + ks * Cfg::kSfbBytes, p.sfb + (static_cast<int64_t>(rb_w) * p.col_tiles + ks) * 512, 512, bar);
           }
         }
       }
       pdl_wait();  // also where there is no tile: this kernel does not end before the one in front of it
       for (int item = worker; item < items; item += workers) {
         const groups::Tile t = groups::place(table, p.groups, p.tiles_n, Cfg::kTileRows, item);
-        const int m0 = t.row + static_cast<int>(cta_rank) * kTileM, n0 = t.tile_n * TILE_N;
-        const int b_row = t.group * p.N + n0 + static_cast<int>(cta_rank) * Cfg::kBRows;
-        const int rb_a = static_cast<int>(groups::first_scale_block(table->bound[t.group], t.group)) + t.index * CTAS + static_cast<int>(cta_rank);
-        const int rb_b = t.group * p.n_row_blocks_b + n0 / 128;
-        const int left = t.end - m0;
-        const int box = CTAS == 2 || left > box_height(1) ? 2 : left > box_height(0) ? 1 : 0;
-        const CUtensorMap* map_a = &maps_a.m[box];
-        const uint32_t a_bytes = box_height(box) * kStageKBytes;
-        const int rb_b_count = min(Cfg::kSfbRowBlocks, p.n_row_blocks_b - n0 / 128);
-        const uint8_t* sfa_src = p.sfa + static_cast<int64_t>(rb_a) * p.col_tiles * 512;
-        const uint8_t* sfb_src = p.sfb + static_cast<int64_t>(rb_b) * p.col_tiles * 512;
+        const int n0 = t.tile_n * kTileCols, rank = static_cast<int>(cta_rank);
+        const int w_row = t.group * p.N + n0 + rank * kTileM, rb_w = t.group * p.n_row_blocks_b + n0 / 128 + rank;
+        const int x_row = t.row + rank * (columns_of(t) / 2);  // (a pair's: half of the tile's rows each)
+        const int rb_x = static_cast<int>(groups::first_scale_block(table->bound[t.group], t.group)) + t.index * CTAS;
+        const int box = box_of(t);
+        const CUtensorMap* map_x = &maps_x.m[box];
+        const uint32_t x_bytes = box_height(box) * kStageKBytes;
+        const uint8_t* sfx_src = p.sfa + static_cast<int64_t>(rb_x) * p.col_tiles * 512;
+        const uint8_t* sfw_src = p.sfb + static_cast<int64_t>(rb_w) * p.col_tiles * 512;
         for (int ks = 0; ks < k_stages; ++ks) {
           mbar_wait(empty + s * 8, ph ^ 1, abort_flag);
           const uint32_t bar = full + s * 8;
@@ -159,22 +210,20 @@ grouped_gemm_kernel(const __grid_constant__ RowMaps maps_a, const __grid_constan
           if (!whole) --ahead;
           if constexpr (CTAS == 2) {
             if (whole) {
-              if (cta_rank == 0) mbar_arrive_expect_tx(bar, 2 * Cfg::kStageBytes);
-              tma_load_2d_pair(b_addr + s * Cfg::kBBytes, &map_b, bar, ks * kStageKBytes, b_row);
-              tma_load_3d_pair(sfb_addr + s * Cfg::kSfbBytes, &map_sfb, bar, 0, ks, rb_b);
+              if (cta_rank == 0) mbar_arrive_expect_tx(bar, 2 * (Cfg::kABytes + x_bytes + Cfg::kSfaBytes + Cfg::kSfbBytes));
+              tma_load_2d_pair(a_addr + s * Cfg::kABytes, &map_w, bar, ks * kStageKBytes, w_row);
+              tma_load_3d_pair(sfa_addr + s * Cfg::kSfaBytes, &map_sfw, bar, 0, ks, rb_w);
             }
-            tma_load_2d_pair(a_addr + s * Cfg::kABytes, map_a, bar, ks * kStageKBytes, m0);
-            tma_load_3d_pair(sfa_addr + s * Cfg::kSfaBytes, &map_sfa, bar, 0, ks, rb_a);
+            tma_load_2d_pair(b_addr + s * Cfg::kBBytes, map_x, bar, ks * kStageKBytes, x_row);
+            tma_load_3d_pair(sfb_addr + s * Cfg::kSfbBytes, &map_sfx, bar, 0, ks, rb_x);
           } else {
             if (whole) {
-              mbar_arrive_expect_tx(bar, a_bytes + Cfg::kBBytes + 512u * (1 + rb_b_count));
-              tma_load_2d(b_addr + s * Cfg::kBBytes, &map_b, bar, ks * kStageKBytes, b_row);
-              for (int r = 0; r < rb_b_count; ++r) {
-                bulk_load_1d(sfb_addr + s * Cfg::kSfbBytes + r * 512, sfb_src + (static_cast<int64_t>(r) * p.col_tiles + ks) * 512, 512, bar);
-              }
+              mbar_arrive_expect_tx(bar, x_bytes + Cfg::kBBytes + 512u * 2);
+              tma_load_2d(b_addr + s * Cfg::kBBytes, &map_w, bar, ks * kStageKBytes, w_row);
+              bulk_load_1d(sfb_addr + s * Cfg::kSfbBytes, sfw_src + ks * 512, 512, bar);
             }
-            tma_load_2d(a_addr + s * Cfg::kABytes, map_a, bar, ks * kStageKBytes, m0);
-            bulk_load_1d(sfa_addr + s * Cfg::kSfaBytes, sfa_src + ks * 512, 512, bar);
+            tma_load_2d(a_addr + s * Cfg::kABytes, map_x, bar, ks * kStageKBytes, x_row);
+            bulk_load_1d(sfa_addr + s * Cfg::kSfaBytes, sfx_src + ks * 512, 512, bar);
           }
           if (++s == STAGES) {
             s = 0;
@@ -201,7 +250,8 @@ grouped_gemm_kernel(const __grid_constant__ RowMaps maps_a, const __grid_constan
       for (int item = worker; item < items; item += workers, ++it) {
         // which half of a 128-row block of B's scales a 64-wide tile reads: its column's place in the band
         const groups::Tile t = groups::place(table, p.groups, p.tiles_n, Cfg::kTileRows, item);
-        const uint32_t sfb_shift = (t.tile_n * TILE_N % 128) / 32;
+        const uint32_t sfb_shift = CTAS == 2 ? 0u : (t.tile_n * TILE_N % 128) / 32;
+        const uint32_t idesc = CTAS == 2 ? (Cfg::kIdesc & ~(0x3Fu << 17)) | (static_cast<uint32_t>(columns_of(t) >> 3) << 17) : Cfg::kIdesc;
         const int acc = it % NUM_ACC;
         const uint32_t d = tmem + acc * Cfg::kAccCols;
         for (int ks = 0; ks < k_stages; ++ks) {
@@ -219,7 +269,7 @@ grouped_gemm_kernel(const __grid_constant__ RowMaps maps_a, const __grid_constan
             tc_fence_after_sync();
           }
           const auto mma = [&](int kb) {
-            mma_mxfp8<CTAS>(d, desc64(a_lo + kb * 2, op_hi), desc64(b_lo + kb * 2, op_hi), idesc_with_scale_ids(Cfg::kIdesc, kb), t_sfa, t_sfb + sfb_shift,
+            mma_mxfp8<CTAS>(d, desc64(a_lo + kb * 2, op_hi), desc64(b_lo + kb * 2, op_hi), idesc_with_scale_ids(idesc, kb), t_sfa, t_sfb + sfb_shift,
                             (ks != 0 || kb != 0) ? 1u : 0u);
           };
           const int n_mma = total_mma - ks * kMmaPerStage;
@@ -252,6 +302,51 @@ grouped_gemm_kernel(const __grid_constant__ RowMaps maps_a, const __grid_constan
     // stores of 32 bytes where rows start on such boundaries, of 16 (N is a multiple of 8) otherwise
     const bool wide = (static_cast<int64_t>(p.N) * sizeof(OutT)) % 32 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 31u) == 0;
     int it = 0;
+    if constexpr (CTAS == 2) {
+      // a lane has one output feature, a column of tensor memory one row
+      const uint32_t turn = smem_u32(smem + Cfg::kRingBytes + 256 + Cfg::kTableBytes) + (warp - 2) * 1024 * static_cast<int>(sizeof(OutT));
+      for (int item = worker; item < items; item += workers, ++it) {
+        const groups::Tile t = groups::place(table, p.groups, p.tiles_n, Cfg::kTileRows, item);
+        const int feature = t.tile_n * kTileCols + static_cast<int>(cta_rank) * kTileM + quarter * 32 + lane;
+        const int row0 = t.row + share * kWarpCols, rows = min(kWarpCols, t.end - row0);
+        const float bias = p.bias != nullptr && feature < p.N ? bias_at(p.bias, p.bias_dtype, static_cast<int64_t>(t.group) * p.N + feature) : 0.0f;
+        const int acc = it % NUM_ACC;
+        mbar_wait(&acc_full_bar[acc], (it / NUM_ACC) & 1, abort_flag);
+        __syncwarp();
+        tc_fence_after_sync();
+        const uint32_t from = tmem + acc * Cfg::kAccCols + (static_cast<uint32_t>(quarter * 32) << 16) + share * kWarpCols;
+        uint32_t buf[kChunks][32];
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+          if (c * 32 < rows) tmem_load_32x32(from + c * 32, buf[c]);
+        }
+        tmem_load_wait();
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(acc_empty + acc * 8);
+        // 32 rows at a time are turned in shared memory: stores are 16 bytes of a row's features
+        constexpr int kVec = 16 / static_cast<int>(sizeof(OutT)), kPieces = 32 / kVec, kRowsAtOnce = 32 / kPieces;
+        const int piece = lane % kPieces, at = t.tile_n * kTileCols + static_cast<int>(cta_rank) * kTileM + quarter * 32 + piece * kVec;
+        OutT* dst = out + static_cast<int64_t>(row0 + lane / kPieces) * p.N + at;
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+          if (c * 32 >= rows) break;
+          float v[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(buf[c][i]) + bias;
+          turn_write<OutT>(turn, lane, v);
+          __syncwarp();
+          rows::Raw<OutT, kVec> got[kPieces];
+#pragma unroll
+          for (int i = 0; i < kPieces; ++i) got[i] = turn_read<OutT>(turn, lane, i);
+#pragma unroll
+          for (int i = 0; i < kPieces; ++i) {
+            if (c * 32 + i * kRowsAtOnce + lane / kPieces < rows && at < p.N) rows::store(dst + static_cast<int64_t>(c * 32 + i * kRowsAtOnce) * p.N, got[i]);
+          }
+          __syncwarp();
+        }
+      }
+    } else
     for (int item = worker; item < items; item += workers, ++it) {
       const groups::Tile t = groups::place(table, p.groups, p.tiles_n, Cfg::kTileRows, item);
       const int row = t.row + static_cast<int>(cta_rank) * kTileM + quarter * 32 + lane, col0 = t.tile_n * TILE_N + share * kWarpCols;
@@ -404,22 +499,22 @@ __global__ void __launch_bounds__(256) regroup_scales_kernel(const uint8_t* from
 // ---------------------------------------------------------------------------
 template <int TILE_N, int NUM_ACC, int STAGES, int CTAS, typename OutT>
 int launch_grouped(const void* a, const void* b, GroupedParams p, cudaStream_t stream) {
-  using Cfg = GroupedConfig<TILE_N, NUM_ACC, STAGES, CTAS>;
+  using Cfg = GroupedConfig<TILE_N, NUM_ACC, STAGES, CTAS, static_cast<int>(sizeof(OutT))>;
   auto kernel = grouped_gemm_kernel<TILE_N, NUM_ACC, STAGES, CTAS, OutT>;
   int dev = 0;
   CK_CUDA(cudaGetDevice(&dev));
-  RowMaps maps_a;
-  CUtensorMap map_b, map_sfa = {}, map_sfb = {};
+  RowMaps maps_x;
+  CUtensorMap map_w, map_sfx = {}, map_sfw = {};
   for (int h = 0; h < 3; ++h) {
-    if (int rc = make_operand_map(&maps_a.m[h], a, p.M, p.k_bytes, box_height(h))) return rc;
+    if (int rc = make_operand_map(&maps_x.m[h], a, p.M, p.k_bytes, box_height(h))) return rc;
   }
   const int64_t row_blocks = groups::scale_blocks(p.M, p.groups);
-  if (int rc = make_operand_map(&map_b, b, static_cast<int64_t>(p.groups) * p.N, p.k_bytes, Cfg::kBRows)) return rc;
+  if (int rc = make_operand_map(&map_w, b, static_cast<int64_t>(p.groups) * p.N, p.k_bytes, CTAS == 2 ? kTileM : TILE_N)) return rc;
   if (CTAS == 2) {
-    if (int rc = make_scale_map(&map_sfa, p.sfa, row_blocks, p.col_tiles, 1, 1)) return rc;
-    if (int rc = make_scale_map(&map_sfb, p.sfb, static_cast<int64_t>(p.groups) * p.n_row_blocks_b, p.col_tiles, 1, Cfg::kSfbRowBlocks)) return rc;
+    if (int rc = make_scale_map(&map_sfx, p.sfa, row_blocks, p.col_tiles, 1, Cfg::kSfbRowBlocks)) return rc;
+    if (int rc = make_scale_map(&map_sfw, p.sfb, static_cast<int64_t>(p.groups) * p.n_row_blocks_b, p.col_tiles, 1, 1)) return rc;
   }
-  p.tiles_n = static_cast<int>(ceil_div(p.N, TILE_N));
+  p.tiles_n = static_cast<int>(ceil_div(p.N, CTAS == 2 ? 2 * kTileM : TILE_N));
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(num_threads(false, TILE_N));
   cfg.dynamicSmemBytes = Cfg::kSmem;
@@ -451,7 +546,7 @@ int launch_grouped(const void* a, const void* b, GroupedParams p, cudaStream_t s
   const int64_t used = p.groups < p.M ? p.groups : p.M;
   const int64_t items = (p.M / Cfg::kTileRows + used) * p.tiles_n;
   cfg.gridDim = dim3(CTAS * static_cast<unsigned>(items < resident ? items : resident));
-  CK_CUDA(cudaLaunchKernelEx(&cfg, kernel, maps_a, map_b, map_sfa, map_sfb, p));
+  CK_CUDA(cudaLaunchKernelEx(&cfg, kernel, maps_x, map_w, map_sfx, map_sfw, p));
   return CK_OK;
 }
 
@@ -459,9 +554,9 @@ template <typename OutT>
 int launch_grouped_shape(const void* a, const void* b, const GroupedParams& p, cudaStream_t stream) {
   const int64_t used = p.groups < p.M ? p.groups : p.M, rows = ceil_div(p.M, used);  // of a group, if they are alike
   const int64_t pairs = used * ceil_div(rows, 256) * ceil_div(p.N, 256), tiles = used * ceil_div(rows, 128) * ceil_div(p.N, 128);
-  // Pairs for groups of more than one row block, from a fifth of the SMs on (us, pair / 128 x 128: 8 groups of 256 rows by 1024 x 1024 11.3 / 12.7, 4 by 4096 x
-  // 4096 30.8 / 38.3, 64 by 2048 x 2048 112 / 136; 3 of 200 by 2048 x 512 7.9 / 7.4).  Half tiles where whole ones leave half of the SMs without one (1 row
-  // of 1536 x 2048 8.8 / 9.1; 8 rows of as many experts, 96 tiles, 13.7 / 10.7).
+  // Pairs for groups of more than 128 rows, from a fifth of the SMs on (us, pair / 128 x 128: 8 groups of 256 rows by 1024 x 1024 10.0 / 12.7, 4 of 150 by 4096 x
+  // 4096 19.7 / 24; 64 of 2048 x 2048, 117 uneven rows 62 / 71, 100 even ones 59 / 57, 8 of 113 by 4096 x 4096 34 / 31).  Half tiles where whole ones leave half of the SMs
+  // without one (1 row of 1536 x 2048 8.8 / 9.1; 8 rows of as many experts, 96 tiles, 14.1 / 10.4; 777 of 40 of 1000 x 1056 19.0 / 16.3).
   if (rows > 128 && pairs * 5 >= sm_count()) return launch_grouped<256, 1, 5, 2, OutT>(a, b, p, stream);
   if (tiles * 2 <= sm_count()) return launch_grouped<64, 2, 6, 1, OutT>(a, b, p, stream);
   return launch_grouped<128, 2, 5, 1, OutT>(a, b, p, stream);
