@@ -19,7 +19,10 @@
 // with the launch before it; 4608 x 12288 x 3072 to fp32 with db 233 (86 %, the sums in parts) and 264 to 300.
 //
 // Rows that are grouped by expert: dX[i] = dY[i] W_e for the rows i of group e.  The same GEMM over a list of tiles that every CTA makes for itself
-// from the groups' ends; a tile begins at its group's first row, wherever in dY that is, and stores the group's rows alone.  8192 rows of eight groups of 8192 x 4096
+// from the groups' ends, the operands' places changed round: W_e's columns are the MMA's 256 rows, dY's rows its columns, of which there may be any multiple of 32, so that a
+// group's last tile costs what it has rows for; results of 16 bits are turned in shared memory on their way out (us, so / with dY's rows as the MMA's: 64 groups of 2048 x
+// 2048, 312 uneven rows each, bf16 285 / 314, fp32 817 / 867; 40 of 1000 x 1056, 300 uneven ones, fp16 105 / 128; eight of 8192 x 4096, 1024 each, in a loop 574 / 576: the power
+// limit).  A tile begins at its group's first row, wherever in dY that is, and stores the group's rows alone.  8192 rows of eight groups of 8192 x 4096
 // bf16: 372 us cold (1.48 PFLOP/s, the pipe 90 % active), and 118 before it for the weights as bf16 (0.8 GB, 1.04 of the copy rate).  It starts in plain stream order.
 #include "ck_gemm_kernel.cuh"
 #include "ck_groups.cuh"
@@ -33,7 +36,8 @@ constexpr int kDeep = 64;                           // contraction steps of a st
 constexpr int kOperandBytes = 128 * kDeep * 2;      // of A or B, stage and CTA
 constexpr int kPairRows = 256, kPairCols = 256;     // a tile
 constexpr int kBoxBytes = 64 * kDeep * 2;           // 64 rows (A) or columns (B) of an MN-major operand
-constexpr int grad_smem(bool grouped) { return 1024 + kGradStages * 2 * kOperandBytes + 256 + (grouped ? static_cast<int>(sizeof(groups::Table)) : 0); }
+constexpr int kTableBytes = (static_cast<int>(sizeof(groups::Table)) + 15) / 16 * 16, kTurnBytes = 8 * 2048;  // of eight warps, 32 x 32 numbers of 16 bits
+constexpr int grad_smem(bool grouped) { return 1024 + kGradStages * 2 * kOperandBytes + 256 + (grouped ? kTableBytes + kTurnBytes : 0); }
 static_assert(grad_smem(true) <= 227 * 1024, "shared memory budget exceeded");
 // Epilogue warps: eight, 128 columns each; for fp32 results, whose sums go on in registers, sixteen of 64.
 constexpr int grad_epilogue_warps(bool parts) { return parts ? 16 : 8; }
@@ -42,8 +46,8 @@ template <typename OutT>
 constexpr bool kInParts = std::is_same<OutT, float>::value;
 
 // kind::f16: bf16 operands, fp32 accumulators; bit 15 / 16: A / B are MN-major
-constexpr uint32_t grad_idesc(bool a_mn) {
-  return (1u << 4) | (1u << 7) | (1u << 10) | ((a_mn ? 1u : 0u) << 15) | (1u << 16) | ((kPairCols >> 3) << 17) | ((kPairRows >> 4) << 24);
+constexpr uint32_t grad_idesc(bool a_mn, bool b_mn) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) | ((kPairCols >> 3) << 17) | ((kPairRows >> 4) << 24);
 }
 
 struct GradParams {
@@ -147,6 +151,8 @@ grad_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
   if constexpr (kGrouped) groups::fill_table(table, p.offsets, p.groups, p.rows, kPairRows);
   const uint32_t tmem = *tmem_slot;
 
+  // How many rows of a grouped tile are computed on: the MMA's columns, in steps of 32.
+  [[maybe_unused]] const auto columns_of = [](const groups::Tile& t) { return (min(kPairRows, t.end - t.row) + 31) / 32 * 32; };
   const int tiles = (kGrouped ? table->tiles[p.groups] : p.tiles_m) * p.tiles_n, items = tiles * p.splits, all_stages = p.deep_stages * p.planes;
   if (warp == 0) {
     // ---------------------------------------------------------------- loads
@@ -160,7 +166,7 @@ grad_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         int tile_m, tile_n, group = 0, m0 = static_cast<int>(rank) * 128;
         if constexpr (kGrouped) {
           const groups::Tile t = groups::place(table, p.groups, p.tiles_n, kPairRows, item);
-          m0 += t.row;
+          m0 = t.row + static_cast<int>(rank) * (columns_of(t) / 2);
           tile_n = t.tile_n;
           group = t.group;
         } else {
@@ -175,16 +181,17 @@ grad_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
           mbar_wait(empty + s * 8, ph ^ 1, abort_flag);
           const uint32_t bar = full + s * 8, a_to = a_addr + s * kOperandBytes, b_to = b_addr + s * kOperandBytes;
           if (rank == 0) mbar_arrive_expect_tx(bar, 2 * 2 * kOperandBytes);  // both CTAs' loads report to the leader
-          if constexpr (kMnA) {
-            tma_load_3d_pair(a_to, &map_a, bar, m0, l0, plane);
-            tma_load_3d_pair(a_to + kBoxBytes, &map_a, bar, m0 + 64, l0, plane);
+          if constexpr (kGrouped) {  // the operands' places changed round
+            tma_load_3d_pair(a_to, &map_b, bar, n0, l0, group);
+            tma_load_3d_pair(a_to + kBoxBytes, &map_b, bar, n0 + 64, l0, group);
+            tma_load_3d_pair(b_to, &map_a, bar, l0, m0, plane);
           } else {
-            tma_load_3d_pair(a_to, &map_a, bar, l0, m0, plane);
-          }
-          if constexpr (kGrouped) {
-            tma_load_3d_pair(b_to, &map_b, bar, n0, l0, group);
-            tma_load_3d_pair(b_to + kBoxBytes, &map_b, bar, n0 + 64, l0, group);
-          } else {
+            if constexpr (kMnA) {
+              tma_load_3d_pair(a_to, &map_a, bar, m0, l0, plane);
+              tma_load_3d_pair(a_to + kBoxBytes, &map_a, bar, m0 + 64, l0, plane);
+            } else {
+              tma_load_3d_pair(a_to, &map_a, bar, l0, m0, plane);
+            }
             tma_load_2d_pair(b_to, &map_b, bar, n0, l0);
             tma_load_2d_pair(b_to + kBoxBytes, &map_b, bar, n0 + 64, l0);
           }
@@ -203,15 +210,20 @@ grad_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       if (elect_one()) {
         const uint32_t full = smem_u32(full_bar), empty = smem_u32(empty_bar), acc_full = smem_u32(acc_full_bar);
         const uint32_t empty_peer = map_to_cta(empty, 1), acc_full_peer = map_to_cta(acc_full, 1);
-        const uint64_t a0 = kMnA ? make_mn_desc(smem_u32(smem_a)) : make_operand_desc_sw128(smem_u32(smem_a));
-        const uint64_t b0 = make_mn_desc(smem_u32(smem_b));
-        constexpr uint32_t kIdesc = grad_idesc(kMnA);
-        constexpr int kStepA = kMnA ? 2048 >> 4 : 32 >> 4, kStepB = 2048 >> 4;  // 16 contraction steps: 16 rows of 128 bytes, or 32 bytes
+        constexpr bool kA = kMnA || kGrouped, kB = !kGrouped;  // MN-major
+        const uint64_t a0 = kA ? make_mn_desc(smem_u32(smem_a)) : make_operand_desc_sw128(smem_u32(smem_a));
+        const uint64_t b0 = kB ? make_mn_desc(smem_u32(smem_b)) : make_operand_desc_sw128(smem_u32(smem_b));
+        uint32_t idesc = grad_idesc(kA, kB);
+        constexpr int kStepA = kA ? 2048 >> 4 : 32 >> 4, kStepB = kB ? 2048 >> 4 : 32 >> 4;  // 16 contraction steps: 16 rows of 128 bytes, or 32 bytes
         int s = 0, it = 0;
         uint32_t ph = 0;
         for (int item = worker; item < items; item += workers, ++it) {
           const int split = item / tiles, first = split * p.stages_per_split, last = min(all_stages, first + p.stages_per_split);
           const int part = kParts ? part_stages(last - first) : last - first;
+          if constexpr (kGrouped) {
+            const groups::Tile t = groups::place(table, p.groups, p.tiles_n, kPairRows, item);
+            idesc = (grad_idesc(kA, kB) & ~(0x3Fu << 17)) | (static_cast<uint32_t>(columns_of(t) >> 3) << 17);
+          }
           for (int begin = first; begin < last; begin += part) {
             const int end = min(last, begin + part);
             const int acc = it & 1;
@@ -223,7 +235,7 @@ grad_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
               tc_fence_after_sync();
               const uint64_t a = a0 + s * (kOperandBytes >> 4), b = b0 + s * (kOperandBytes >> 4);
 #pragma unroll
-              for (int k = 0; k < kDeep / 16; ++k) mma_bf16_pair(d, a + k * kStepA, b + k * kStepB, kIdesc, ks != begin || k != 0);
+              for (int k = 0; k < kDeep / 16; ++k) mma_bf16_pair(d, a + k * kStepA, b + k * kStepB, idesc, ks != begin || k != 0);
               tc_commit<2>(empty + s * 8);
               tc_commit<2>(empty_peer + s * 8);
               if (++s == kGradStages) {
@@ -267,21 +279,47 @@ grad_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(acc_empty + acc * 8);
       };
-      // this thread's row of the tile, its warp's columns
+      // this thread's row of the tile, its warp's columns; of a grouped tile its result's column, its warp's rows
       int end = p.rows;
       const auto place = [&](int* row, int* col0) {
         int tile_m, tile_n;
-        *row = static_cast<int>(rank) * 128 + quarter * 32 + lane;
         if constexpr (kGrouped) {
           const groups::Tile t = groups::place(table, p.groups, p.tiles_n, kPairRows, item);
-          *row += t.row;
-          tile_n = t.tile_n;
+          *row = t.row + share * kWarpCols;
+          *col0 = t.tile_n * kPairCols + static_cast<int>(rank) * 128 + quarter * 32;
           end = t.end;
         } else {
           tile_place(p, item - split * tiles, &tile_m, &tile_n);
-          *row += tile_m * kPairRows;
+          *row = tile_m * kPairRows + static_cast<int>(rank) * 128 + quarter * 32 + lane;
+          *col0 = tile_n * kPairCols + share * kWarpCols;
         }
-        *col0 = tile_n * kPairCols + share * kWarpCols;
+      };
+      // 32 rows by a lane's column each: fp32 as it is, lines of 128 bytes; 16 bits turned in shared memory on the way
+      const auto write_turned = [&](int row0, int col0, const uint32_t(&v)[32]) {
+        const int count = end - row0;
+        if (count <= 0) return;
+        if constexpr (kParts) {
+          OutT* out = static_cast<OutT*>(p.out) + static_cast<int64_t>(row0) * p.cols + col0 + lane;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            if (i < count && col0 + lane < p.cols) out[static_cast<int64_t>(i) * p.cols] = rows::from_float<OutT>(__uint_as_float(v[i]));
+          }
+        } else {
+          const uint32_t turn = smem_u32(smem + kGradStages * 2 * kOperandBytes + 256 + kTableBytes) + (warp - 2) * 2048;
+          float f[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(v[i]);
+          groups::turn_write<OutT>(turn, lane, f);
+          __syncwarp();
+          const int col = col0 + lane % 4 * 8;
+          OutT* out = static_cast<OutT*>(p.out) + static_cast<int64_t>(row0 + lane / 4) * p.cols + col;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const auto r = groups::turn_read<OutT>(turn, lane, i);
+            if (i * 8 + lane / 4 < count && col < p.cols) rows::store(out + static_cast<int64_t>(i * 8) * p.cols, r);
+          }
+          __syncwarp();
+        }
       };
       const auto write = [&](int row, int col, const uint32_t(&v)[32]) {
         if (row < end && col < p.cols) {
@@ -324,7 +362,11 @@ grad_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
           uint32_t v[32];
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(sum[32 * c + j]);
-          write(row, col0 + c * 32, v);
+          if constexpr (kGrouped) {
+            write_turned(row + c * 32, col0, v);
+          } else {
+            write(row, col0 + c * 32, v);
+          }
         }
       } else {
         const int acc = it & 1;
@@ -337,7 +379,11 @@ grad_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
           tmem_load_32x32(from + c * 32, v);
           tmem_load_wait();
           if (c == kWarpBoxes - 1) give_back(acc);  // read to the end
-          write(row, col0 + c * 32, v);
+          if constexpr (kGrouped) {
+            write_turned(row + c * 32, col0, v);
+          } else {
+            write(row, col0 + c * 32, v);
+          }
         }
       }
     }

@@ -61,48 +61,6 @@ struct GroupedConfig : Config<Kind::kMxfp8, TILE_N, NUM_ACC, STAGES, CTAS, 0> {
   static_assert(kSmem <= 227 * 1024, "shared memory budget exceeded");
 };
 
-// 32 x 32 numbers turned by a warp: a lane writes its feature's, one for each row, and reads 16 bytes of neighbouring features of row 32 / pieces * i + lane / pieces.
-// Numbers of 16 bits lie by feature, in pieces of eight rows whose places change with the feature so that neither the writes nor the transposing reads of 8 x 8
-// matrices (whose rows are the features 8 j + 2 m and 8 j + 2 m + 1, so that a lane gets eight in a row) meet a bank twice; those of 32 lie by row.
-__device__ __forceinline__ uint32_t turn_place(int feature, int piece) {
-  return static_cast<uint32_t>(feature * 64 + ((piece ^ (feature >> 1) ^ (feature >> 3)) & 3) * 16);
-}
-template <typename OutT>
-__device__ __forceinline__ void turn_write(uint32_t turn, int lane, const float* v) {
-  if constexpr (sizeof(OutT) == 2) {
-    uint32_t w[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float pair[2] = {v[2 * i], v[2 * i + 1]};
-      const rows::Raw<OutT, 2> r = rows::pack<OutT, 2>(pair);
-      w[i] = *reinterpret_cast<const uint32_t*>(&r);
-    }
-#pragma unroll
-    for (int q = 0; q < 4; ++q) st_shared_128(turn + turn_place(lane, q), w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 32; ++i) asm volatile("st.shared.f32 [%0], %1;" ::"r"(turn + (i * 32 + lane) * 4), "f"(v[i]) : "memory");
-  }
-}
-template <typename OutT>
-__device__ __forceinline__ rows::Raw<OutT, 16 / static_cast<int>(sizeof(OutT))> turn_read(uint32_t turn, int lane, int i) {
-  rows::Raw<OutT, 16 / static_cast<int>(sizeof(OutT))> r;
-  uint32_t* w = reinterpret_cast<uint32_t*>(&r);
-  if constexpr (sizeof(OutT) == 2) {
-    const int feature = (lane & 7) / 2 * 8 + (lane >> 3) * 2 + (lane & 1);
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                 : "r"(turn + turn_place(feature, i))
-                 : "memory");
-  } else {
-    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                 : "r"(turn + (i * 32 + lane) * 16)
-                 : "memory");
-  }
-  return r;
-}
-
 template <int TILE_N, int NUM_ACC, int STAGES, int CTAS, typename OutT>
 __global__ void __launch_bounds__(num_threads(false, TILE_N), 1)
 grouped_gemm_kernel(const __grid_constant__ RowMaps maps_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_sfx,
@@ -334,11 +292,11 @@ grouped_gemm_kernel(const __grid_constant__ RowMaps maps_x, const __grid_constan
           float v[32];
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(buf[c][i]) + bias;
-          turn_write<OutT>(turn, lane, v);
+          groups::turn_write<OutT>(turn, lane, v);
           __syncwarp();
           rows::Raw<OutT, kVec> got[kPieces];
 #pragma unroll
-          for (int i = 0; i < kPieces; ++i) got[i] = turn_read<OutT>(turn, lane, i);
+          for (int i = 0; i < kPieces; ++i) got[i] = groups::turn_read<OutT>(turn, lane, i);
 #pragma unroll
           for (int i = 0; i < kPieces; ++i) {
             if (c * 32 + i * kRowsAtOnce + lane / kPieces < rows && at < p.N) rows::store(dst + static_cast<int64_t>(c * 32 + i * kRowsAtOnce) * p.N, got[i]);

@@ -4,6 +4,8 @@
 #pragma once
 
 #include "ck_common.cuh"
+#include "ck_rows.cuh"
+#include "ck_sm100.cuh"
 
 namespace ck {
 namespace groups {
@@ -104,6 +106,48 @@ __device__ __forceinline__ Tile place(const Table* t, int count, int tiles_n, in
   p.row = t->bound[lo] + p.index * tile_rows;
   p.end = max(t->bound[lo], t->bound[lo + 1]);
   return p;
+}
+
+// 32 x 32 numbers turned by a warp: a lane writes its feature's, one for each row, and reads 16 bytes of neighbouring features of row 32 / pieces * i + lane / pieces.
+// Numbers of 16 bits lie by feature, in pieces of eight rows whose places change with the feature so that neither the writes nor the transposing reads of 8 x 8
+// matrices (whose rows are the features 8 j + 2 m and 8 j + 2 m + 1, so that a lane gets eight in a row) meet a bank twice; those of 32 lie by row.
+__device__ __forceinline__ uint32_t turn_place(int feature, int piece) {
+  return static_cast<uint32_t>(feature * 64 + ((piece ^ (feature >> 1) ^ (feature >> 3)) & 3) * 16);
+}
+template <typename OutT>
+__device__ __forceinline__ void turn_write(uint32_t turn, int lane, const float* v) {
+  if constexpr (sizeof(OutT) == 2) {
+    uint32_t w[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float pair[2] = {v[2 * i], v[2 * i + 1]};
+      const rows::Raw<OutT, 2> r = rows::pack<OutT, 2>(pair);
+      w[i] = *reinterpret_cast<const uint32_t*>(&r);
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) sm100::st_shared_128(turn + turn_place(lane, q), w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) asm volatile("st.shared.f32 [%0], %1;" ::"r"(turn + (i * 32 + lane) * 4), "f"(v[i]) : "memory");
+  }
+}
+template <typename OutT>
+__device__ __forceinline__ rows::Raw<OutT, 16 / static_cast<int>(sizeof(OutT))> turn_read(uint32_t turn, int lane, int i) {
+  rows::Raw<OutT, 16 / static_cast<int>(sizeof(OutT))> r;
+  uint32_t* w = reinterpret_cast<uint32_t*>(&r);
+  if constexpr (sizeof(OutT) == 2) {
+    const int feature = (lane & 7) / 2 * 8 + (lane >> 3) * 2 + (lane & 1);
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                 : "r"(turn + turn_place(feature, i))
+                 : "memory");
+  } else {
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                 : "r"(turn + (i * 32 + lane) * 16)
+                 : "memory");
+  }
+  return r;
 }
 
 }  // namespace groups
