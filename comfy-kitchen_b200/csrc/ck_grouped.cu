@@ -28,8 +28,8 @@ namespace {
 
 struct GroupedParams {
   const int* offsets;
-  const uint8_t* sfa;    // workspace: the groups' scale tiles
-  const uint8_t* sfb;    // [E][ceil(N / 128)][col_tiles] tiles of 512 bytes
+  const uint8_t* sfa;    // x's scales, in the workspace: the groups' tiles
+  const uint8_t* sfb;    // W's: [E][ceil(N / 128)][col_tiles] tiles of 512 bytes
   const void* bias;      // [E, N] or null
   void* out;             // [M, N]
   int bias_dtype;
@@ -39,7 +39,7 @@ struct GroupedParams {
   int* status;
 };
 
-// Boxes of A's rows: no more of them are fetched than a tile has, to the next of three heights.
+// Boxes of x's rows: no more of them are fetched than a tile has, to the next of three heights.
 constexpr int box_height(int box) { return box == 2 ? 128 : box == 1 ? 32 : 8; }
 struct RowMaps {
   CUtensorMap m[3];
@@ -304,65 +304,66 @@ grouped_gemm_kernel(const __grid_constant__ RowMaps maps_x, const __grid_constan
           __syncwarp();
         }
       }
-    } else
-    for (int item = worker; item < items; item += workers, ++it) {
-      const groups::Tile t = groups::place(table, p.groups, p.tiles_n, Cfg::kTileRows, item);
-      const int row = t.row + static_cast<int>(cta_rank) * kTileM + quarter * 32 + lane, col0 = t.tile_n * TILE_N + share * kWarpCols;
-      const int acc = it % NUM_ACC;
-      // the warp's columns' bias, one a lane, fetched while the tile computes and passed round through shared memory
-      float bias[kChunks] = {};
-      if (p.bias != nullptr) {
-#pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
-          const int col = col0 + c * 32 + lane;
-          if (col < p.N) bias[c] = bias_at(p.bias, p.bias_dtype, static_cast<int64_t>(t.group) * p.N + col);
-        }
-      }
-      mbar_wait(&acc_full_bar[acc], (it / NUM_ACC) & 1, abort_flag);
-      __syncwarp();
-      tc_fence_after_sync();
-      const uint32_t from = tmem + acc * Cfg::kAccCols + (static_cast<uint32_t>(quarter * 32) << 16) + share * kWarpCols;
-      uint32_t buf[kChunks][32];
-#pragma unroll
-      for (int c = 0; c < kChunks; ++c) tmem_load_32x32(from + c * 32, buf[c]);
-      tmem_load_wait();
-      tc_fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(acc_empty + acc * 8);
-      if (p.bias != nullptr) {
-#pragma unroll
-        for (int c = 0; c < kChunks; ++c) bias_s[c * 32 + lane] = bias[c];
-        __syncwarp();
-      }
-      if (row >= t.end) continue;
-      OutT* dst = out + static_cast<int64_t>(row) * p.N + col0;
-#pragma unroll
-      for (int c = 0; c < kChunks; ++c) {
-        const int valid = min(32, p.N - (col0 + c * 32));
-        if (valid <= 0) continue;
-        float v[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(buf[c][i]);
+    } else {
+      for (int item = worker; item < items; item += workers, ++it) {
+        const groups::Tile t = groups::place(table, p.groups, p.tiles_n, Cfg::kTileRows, item);
+        const int row = t.row + static_cast<int>(cta_rank) * kTileM + quarter * 32 + lane, col0 = t.tile_n * TILE_N + share * kWarpCols;
+        const int acc = it % NUM_ACC;
+        // the warp's columns' bias, one a lane, fetched while the tile computes and passed round through shared memory
+        float bias[kChunks] = {};
         if (p.bias != nullptr) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float4 q = reinterpret_cast<const float4*>(bias_s + c * 32)[i];
-            v[4 * i] += q.x;
-            v[4 * i + 1] += q.y;
-            v[4 * i + 2] += q.z;
-            v[4 * i + 3] += q.w;
+          for (int c = 0; c < kChunks; ++c) {
+            const int col = col0 + c * 32 + lane;
+            if (col < p.N) bias[c] = bias_at(p.bias, p.bias_dtype, static_cast<int64_t>(t.group) * p.N + col);
           }
         }
-        if (wide && valid == 32) {
-          store_row_chunk<OutT>(dst + c * 32, v, 32, true);
-        } else {
-          constexpr int kVec = 16 / static_cast<int>(sizeof(OutT));
+        mbar_wait(&acc_full_bar[acc], (it / NUM_ACC) & 1, abort_flag);
+        __syncwarp();
+        tc_fence_after_sync();
+        const uint32_t from = tmem + acc * Cfg::kAccCols + (static_cast<uint32_t>(quarter * 32) << 16) + share * kWarpCols;
+        uint32_t buf[kChunks][32];
 #pragma unroll
-          for (int i = 0; i < 32 / kVec; ++i) {
-            float f[kVec];
+        for (int c = 0; c < kChunks; ++c) tmem_load_32x32(from + c * 32, buf[c]);
+        tmem_load_wait();
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(acc_empty + acc * 8);
+        if (p.bias != nullptr) {
 #pragma unroll
-            for (int j = 0; j < kVec; ++j) f[j] = v[i * kVec + j];
-            if (i * kVec < valid) rows::store(dst + c * 32 + i * kVec, rows::pack<OutT, kVec>(f));
+          for (int c = 0; c < kChunks; ++c) bias_s[c * 32 + lane] = bias[c];
+          __syncwarp();
+        }
+        if (row >= t.end) continue;
+        OutT* dst = out + static_cast<int64_t>(row) * p.N + col0;
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+          const int valid = min(32, p.N - (col0 + c * 32));
+          if (valid <= 0) continue;
+          float v[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(buf[c][i]);
+          if (p.bias != nullptr) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float4 q = reinterpret_cast<const float4*>(bias_s + c * 32)[i];
+              v[4 * i] += q.x;
+              v[4 * i + 1] += q.y;
+              v[4 * i + 2] += q.z;
+              v[4 * i + 3] += q.w;
+            }
+          }
+          if (wide && valid == 32) {
+            store_row_chunk<OutT>(dst + c * 32, v, 32, true);
+          } else {
+            constexpr int kVec = 16 / static_cast<int>(sizeof(OutT));
+#pragma unroll
+            for (int i = 0; i < 32 / kVec; ++i) {
+              float f[kVec];
+#pragma unroll
+              for (int j = 0; j < kVec; ++j) f[j] = v[i * kVec + j];
+              if (i * kVec < valid) rows::store(dst + c * 32 + i * kVec, rows::pack<OutT, kVec>(f));
+            }
           }
         }
       }
