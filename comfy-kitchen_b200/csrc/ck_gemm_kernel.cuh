@@ -68,6 +68,12 @@ constexpr int epilogue_warps(bool fused, int tile_n) { return (fused && tile_n >
 constexpr int num_threads(bool fused, int tile_n) {
   return 64 + 32 * epilogue_warps(fused, tile_n);  // + TMA and MMA warps
 }
+// Tensor memory is never waited for: a kernel that allocates some of it asks for so much shared memory at least, one that takes more than half of the
+// 512 columns for so much that no other of them fits beside it on an SM (228 KB, a CTA's own 1 KB among them), and of those that take half three do not fit.
+constexpr int kLeastWithTensorMemory = 84 * 1024;
+constexpr bool alone_with_tensor_memory(int smem) { return smem + kLeastWithTensorMemory + 2 * 1024 > 228 * 1024; }
+static_assert(3 * (kLeastWithTensorMemory + 1024) > 228 * 1024, "two that take half at most");
+
 constexpr int pow2_at_least(int x) { return x <= 32 ? 32 : x <= 64 ? 64 : x <= 128 ? 128 : x <= 256 ? 256 : 512; }
 
 // CTAS == 2: a pair of CTAs (a 2-CTA cluster on neighbouring SMs) computes one 256 x TILE_N
@@ -115,6 +121,7 @@ struct Config {
   static_assert(CTAS == 1 || TILE_N % 32 == 0, "a CTA pair needs N % 32 == 0");
   static_assert(TILE_N % 16 == 0 && TILE_N >= 16 && TILE_N <= 256, "invalid MMA N");
   static_assert(kSmemBytes <= 227 * 1024, "shared memory budget exceeded");
+  static_assert(kSmemBytes >= kLeastWithTensorMemory && (kTmemCols <= 256 || alone_with_tensor_memory(kSmemBytes)), "no allocation waits");
   static constexpr uint32_t kIdesc = make_block_scaled_idesc(KIND == Kind::kNvfp4 ? 1u : 0u,
                                                              KIND == Kind::kNvfp4 ? 0u : 1u, kTileRows, TILE_N);
 };

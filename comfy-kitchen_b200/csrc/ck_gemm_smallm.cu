@@ -575,6 +575,7 @@ int launch(const void* w, const void* codes, SmallParams p, cudaStream_t stream)
   constexpr int kTwoToAnSm = 228 * 1024 / 2 - 1024 /*reserved*/ - 512 /*barriers, maxima*/;
   static_assert(Small<KIND>::smem_bytes(5, 16) <= kTwoToAnSm && Small<KIND>::smem_bytes(4, 32) <= kTwoToAnSm, "two CTAs to an SM");
   static_assert(Small<KIND>::smem_bytes(7, 32) <= kMaxSmemBytes, "one CTA to an SM");
+  static_assert(Small<KIND>::smem_bytes(5, 16) >= kLeastWithTensorMemory && Small<KIND>::smem_bytes(4, 32) >= kLeastWithTensorMemory, "no allocation of tensor memory waits");
   // Alone on its SM a CTA gets all the stages that tensor memory has columns for; where two share an SM, what leaves room for
   // both (MXFP8 8 x 18432 x 6144, us: four stages 22.7, five 21.9, seven 20.5; NVFP4 16 x 18432 x 12288 24.1 / 23.5 / 22.0, 8 x 9216
   // x 3072 6.40 / 6.13 / 5.92; but MXFP8 8 x 3072 x 12288, eight CTAs to a tile, 10.4 / 10.3 / 15.3).

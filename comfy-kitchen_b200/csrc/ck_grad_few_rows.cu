@@ -43,6 +43,7 @@ constexpr int kScaleBytes = 512, kRawBytes = kDeep * kCols + kScaleBytes;  // a 
 constexpr int kMaxRaw = 8;
 static_assert(kMaxRaw % kGroups == 0 && kMinStages >= kGroups, "no wait may take one phase for another");
 constexpr int kSmem = 208 * 1024;
+static_assert(alone_with_tensor_memory(kSmem), "no allocation of tensor memory waits");
 
 struct FewRowsArgs {
   const uint8_t* codes;
@@ -733,6 +734,7 @@ int grad_few_rows(const void* dy, int planes, const void* codes, const void* sca
 namespace {
 
 constexpr int kGroupedSmem = 226 * 1024 - 1024;  // dynamic, beside the barriers
+static_assert(alone_with_tensor_memory(kGroupedSmem), "no allocation of tensor memory waits");
 
 // Rows of a tile at most: as many as there is room for beside the fewest stages and eight of codes, or four where groups of so many rows would need
 // more, or less than 64 fitted.  A tile computes and loads what it has rows for, and a group in fewer tiles has its weight decoded less often; codes that are fetched

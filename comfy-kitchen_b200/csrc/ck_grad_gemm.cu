@@ -39,6 +39,7 @@ constexpr int kBoxBytes = 64 * kDeep * 2;           // 64 rows (A) or columns (B
 constexpr int kTableBytes = (static_cast<int>(sizeof(groups::Table)) + 15) / 16 * 16, kTurnBytes = 8 * 2048;  // of eight warps, 32 x 32 numbers of 16 bits
 constexpr int grad_smem(bool grouped) { return 1024 + kGradStages * 2 * kOperandBytes + 256 + (grouped ? kTableBytes + kTurnBytes : 0); }
 static_assert(grad_smem(true) <= 227 * 1024, "shared memory budget exceeded");
+static_assert(alone_with_tensor_memory(grad_smem(false)), "no allocation of tensor memory waits");
 // Epilogue warps: eight, 128 columns each; for fp32 results, whose sums go on in registers, sixteen of 64.
 constexpr int grad_epilogue_warps(bool parts) { return parts ? 16 : 8; }
 constexpr int grad_threads(bool parts) { return 64 + 32 * grad_epilogue_warps(parts); }  // beside them producer and issuer

@@ -59,6 +59,7 @@ struct GroupedConfig : Config<Kind::kMxfp8, TILE_N, NUM_ACC, STAGES, CTAS, 0> {
   static constexpr int kEpilogueBytes = CTAS == 2 ? kWarps * 1024 * kOutBytes : kWarps * (TILE_N / (kWarps / 4)) * 4;
   static constexpr int kSmem = Base::kRingBytes + 1024 + 256 + kTableBytes + kEpilogueBytes;
   static_assert(kSmem <= 227 * 1024, "shared memory budget exceeded");
+  static_assert(alone_with_tensor_memory(kSmem), "no allocation of tensor memory waits");
 };
 
 template <int TILE_N, int NUM_ACC, int STAGES, int CTAS, typename OutT>
@@ -111,7 +112,7 @@ grouped_gemm_kernel(const __grid_constant__ RowMaps maps_x, const __grid_constan
   if constexpr (CTAS == 2) cluster_sync_all();  // the other CTA's barriers exist before anything reports to them
   tc_fence_after_sync();
   // The kernel before this one has waited for its own predecessor before it let this one start, so the ends, the weights and their scales are there;
-  // x's codes and scales are not.  Weights of the first stages are on their way while that kernel still runs.
+  // x's codes and scales are not, where this is a single CTA.  Its first stages' weights are on their way while that kernel still runs.  (Pairs start behind it.)
   groups::fill_table(table, p.offsets, p.groups, p.M, Cfg::kTileRows);
   const uint32_t tmem = *tmem_slot;
 
@@ -486,7 +487,9 @@ int launch_grouped(const void* a, const void* b, GroupedParams p, cudaStream_t s
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  // Pairs in plain stream order, as the input gradient's (launch_grad_gemm): what has no limit to its wait, the kernel in front, the tensor memory and the
+  // cluster's barrier, then has nothing to wait for.
+  cfg.numAttrs = pdl_enabled() && CTAS == 1 ? 2 : 1;
   // all workers resident at once; how many pairs there is room for depends on where the SMs lie
   static std::atomic<int> resident_on[64];
   int resident = (dev >= 0 && dev < 64) ? resident_on[dev].load(std::memory_order_acquire) : 0;
@@ -512,11 +515,14 @@ int launch_grouped(const void* a, const void* b, GroupedParams p, cudaStream_t s
 template <typename OutT>
 int launch_grouped_shape(const void* a, const void* b, const GroupedParams& p, cudaStream_t stream) {
   const int64_t used = p.groups < p.M ? p.groups : p.M, rows = ceil_div(p.M, used);  // of a group, if they are alike
-  const int64_t pairs = used * ceil_div(rows, 256) * ceil_div(p.N, 256), tiles = used * ceil_div(rows, 128) * ceil_div(p.N, 128);
-  // Pairs for groups of more than 128 rows, from a fifth of the SMs on (us, pair / 128 x 128: 8 groups of 256 rows by 1024 x 1024 10.0 / 12.7, 4 of 150 by 4096 x
-  // 4096 19.7 / 24; 64 of 2048 x 2048, 117 uneven rows 62 / 71, 100 even ones 59 / 57, 8 of 113 by 4096 x 4096 34 / 31).  Half tiles where whole ones leave half of the SMs
-  // without one (1 row of 1536 x 2048 8.8 / 9.1; 8 rows of as many experts, 96 tiles, 14.1 / 10.4; 777 of 40 of 1000 x 1056 19.0 / 16.3).
-  if (rows > 128 && pairs * 5 >= sm_count()) return launch_grouped<256, 1, 5, 2, OutT>(a, b, p, stream);
+  const int64_t tiles = used * ceil_div(rows, 128) * ceil_div(p.N, 128), stages = ceil_div(p.k_bytes, kStageKBytes);
+  // Pairs for groups of more than 128 rows on average, where single CTAs would take turns and an SM's share is more than 32 stages: starting behind the
+  // first kernel's end costs pairs three microseconds (us, pair / 128 x 128: tiles 1024, 140 rows each of 64 by 2048 x 2048 77 / 95; 640, 200 uneven of 40 by 1000 x
+  // 1056 27.8 / 31.8; 256, 150 of 4 by 4096 x 4096 23.4 / 25.6; 512, 140 of 32 by 1024 x 1024 19.1 / 20.0; the other way 256, 1024 of 2 by 2048 x 2048 16.8 / 16.2; 384, 256 of 24 by 1024 x
+  // 1024 22.2 / 18.9; 128, 256 of 8 by 1024 x 4096 24.9 / 19.9; fewer rows, 100 of 64 by 2048 x 2048 71 / 65, 113 of 8 by 4096 x 4096 36 / 32).  The average cannot tell uneven groups from
+  // even ones: 117 uneven rows of 64 by 2048 x 2048 take 77 / 78.  Half tiles where whole ones leave half of the SMs without one (1 row of 1536 x 2048 8.8 / 9.1; 8 rows
+  // of as many experts, 96 tiles, 14.1 / 10.4; 777 of 40 of 1000 x 1056 19.0 / 16.3).
+  if (rows > 128 && tiles > sm_count() && tiles * stages > 32 * sm_count()) return launch_grouped<256, 1, 5, 2, OutT>(a, b, p, stream);
   if (tiles * 2 <= sm_count()) return launch_grouped<64, 2, 6, 1, OutT>(a, b, p, stream);
   return launch_grouped<128, 2, 5, 1, OutT>(a, b, p, stream);
 }
