@@ -20,6 +20,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -218,7 +219,8 @@ PyObject* pair(Tensor a, Tensor b) {
   return t;
 }
 
-// What `body` returns; None when that is null (refused) or something goes wrong in it: the call is the Python wrapper's then.
+// What `body` returns; None when that is null (refused) or something goes wrong in it: the call is the Python wrapper's then.  An error that Python
+// code raised on the way, a hook on saved tensors, is the caller's (non-reentrant checkpointing ends its recomputation with one).
 template <typename Body>
 PyObject* or_none(PyObject* const* args, Py_ssize_t got, Py_ssize_t wanted, Body&& body) {
   try {
@@ -226,8 +228,11 @@ PyObject* or_none(PyObject* const* args, Py_ssize_t got, Py_ssize_t wanted, Body
       PyObject* r = body();
       if (r != nullptr || PyErr_Occurred() != nullptr) return r;
     }
+  } catch (python_error& e) {
+    e.restore();
   } catch (const std::exception&) {
   }
+  if (PyErr_Occurred() != nullptr) return nullptr;
   Py_RETURN_NONE;
 }
 
