@@ -76,13 +76,14 @@ bool norm_params(const Tensor& x, const Tensor* weight, const Tensor* bias, Norm
     p->groups = some->size(0);
     if (x.dim() < 2 || x.size(0) != p->groups || some->numel() != p->groups * x.size(-1)) return false;
   }
-  for (const Tensor* t : {weight, bias}) {
-    if (t == nullptr) continue;
+  const auto take = [&](const Tensor* t, Tensor* to, int64_t* stride) {
+    if (t == nullptr) return true;
     if (x.size(-1) > 1 && t->stride(-1) != 1) return false;
-    (t == weight ? p->weight : p->bias) = *t;
-    (t == weight ? p->weight_stride : p->bias_stride) = t->dim() > 1 ? t->stride(0) : 0;
-  }
-  return true;
+    *to = *t;
+    *stride = t->dim() > 1 ? t->stride(0) : 0;
+    return true;
+  };
+  return take(weight, &p->weight, &p->weight_stride) && take(bias, &p->bias, &p->bias_stride);  // (they may be one tensor)
 }
 
 const void* data_of(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
