@@ -22,7 +22,7 @@ from torch.autograd.function import once_differentiable
 
 from .float_utils import roundup
 from .ops import DTYPE_TO_CODE, host_operator
-from .training import _call, _eager, _run, replaced
+from .training import _call, _eager, _no_tangents, _run, replaced
 
 __all__ = ["grouped_mm_mxfp8", "grouped_linear_mxfp8", "grouped_input_grad_mxfp8", "quantize_experts_mxfp8", "MXFP8Experts"]
 
@@ -83,6 +83,7 @@ def grouped_linear_mxfp8(x: torch.Tensor, w_codes: torch.Tensor, w_block_scales:
                 return out
     elif _eager((x, w_codes, w_block_scales, offsets, bias)) and not replaced("grouped_linear_mxfp8") and not replaced("grouped_input_grad_mxfp8"):
         return _GroupedLinear.apply(x, w_codes, w_block_scales, offsets, bias)
+    _no_tangents("grouped_linear_mxfp8", x, bias)
     return _call("grouped_linear_mxfp8", {"x": x, "w_codes": w_codes, "w_block_scales": w_block_scales, "offsets": offsets, "bias": bias})
 
 

@@ -11,6 +11,7 @@
   to 1024 tensors and without a read on the host.
 
 The arithmetic is fp32 with one rounding; the sum of x and residual is rounded to their type first, and the norm is of what stands there.
+Gradients of gradients and forward-mode derivatives are refused.
 """
 from __future__ import annotations
 
@@ -22,7 +23,7 @@ import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
 from .ops import host_operator, host_step
-from .training import _call, _eager, _run, replaced
+from .training import _call, _eager, _no_tangents, _run, replaced
 
 __all__ = ["rms_norm", "rms_norm_forward", "rms_norm_backward", "rms_norm_mxfp8", "RMSNorm", "grad_norm", "clip_grad_norm_"]
 
@@ -106,6 +107,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, residual: torc
             return _RmsNorm.apply(x, weight, residual, eps, weight_offset)
         y, h = _run("rms_norm_inference", {"x": x, "weight": weight, "residual": residual, "eps": eps, "weight_offset": weight_offset})
     else:
+        _no_tangents("rms_norm", x, weight, residual)
         y, h, _ = torch.ops.comfy_kitchen.rms_norm_forward(x, weight, residual, eps, weight_offset)
     return y if residual is None else (y, h)
 

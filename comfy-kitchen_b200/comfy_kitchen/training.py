@@ -15,7 +15,7 @@ so not exactly the derivative of anything (these values' own mean and variance a
 * :class:`CheckpointedLayerNorm`, :class:`CheckpointedGELU`, :class:`CheckpointedLinear`, :class:`CheckpointedMLP`: modules around them.
 
 The functions that these are built from (``layer_norm_forward`` ... ``linear_input_grad_mxfp8``) are operators of the package like
-the quantizers; statistics and copies that they return carry no gradient, and gradients of gradients are not available.
+the quantizers; statistics and copies that they return carry no gradient; gradients of gradients and forward-mode derivatives are refused.
 """
 from __future__ import annotations
 
@@ -129,6 +129,12 @@ def _eager(tensors) -> bool:
     return True
 
 
+def _no_tangents(name: str, *tensors) -> None:
+    """Refuses tensors that carry a forward-mode tangent: the dispatcher would drop it and the result would pass for a constant."""
+    if torch.autograd.forward_ad._current_level >= 0 and any(t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{name} has no forward-mode derivative")
+
+
 def _groups(*params) -> int:
     return next((p.shape[0] for p in params if p is not None and p.dim() > 1), 1)
 
@@ -193,6 +199,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
         if graph:
             return _LayerNorm.apply(x, weight, bias, eps, weight_offset, checkpoint)
         return _run("layer_norm_inference", {"x": x, "weight": weight, "bias": bias, "eps": eps, "weight_offset": weight_offset})
+    _no_tangents("layer_norm", x, weight, bias)
     op = torch.ops.comfy_kitchen.layer_norm_forward_mxfp8 if checkpoint and graph else torch.ops.comfy_kitchen.layer_norm_forward
     return op(x, weight, bias, eps, weight_offset)[0]
 
@@ -230,6 +237,7 @@ def gelu_checkpointed(x: torch.Tensor) -> torch.Tensor:
     if _eager((x2,)) and not any(replaced(name) for name in operators):
         y = _Gelu.apply(x2) if graph else _run("gelu_inference", {"x": x2})
     else:
+        _no_tangents("gelu_checkpointed", x2)
         y = torch.ops.comfy_kitchen.gelu_mxfp8_forward(x2)[0]
     return y if len(shape) == 2 else y.view(shape)
 
