@@ -80,8 +80,10 @@ __device__ __forceinline__ void store_result(const FewRowsArgs& a, int64_t at, f
   }
 }
 
-// Codes and a scale's byte as they came to shared memory, read where these stand: as ordinary loads they moved behind the wait that follows, and
-// where a copy into the same place may begin before that wait ends, what was read was a later stage's.
+// Codes and a scale's byte as they came to shared memory.  They are used behind a wait, and their place is given back in front of it, so nothing but a fence
+// between the proxies puts these reads before the next copy's writes: an arrival on a barrier does not.  Without it a warp's reads, held up where the MMAs keep shared memory busy,
+// met the codes of four steps later, in 3 to 70 passes of a hundred of one build (200 rows of bf16, 4864 x 256 and 4864 x 8192) and in none of another.  (Giving the place back behind
+// the decoding needs no fence and costs 4 % where four stages of codes are all there is room for: 64 experts of 2048 x 2048, 200 rows each, 126.7 us instead of 123.5.)
 __device__ __forceinline__ uint4 load_codes(uint32_t at) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
@@ -171,6 +173,7 @@ grad_few_rows_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_co
 #pragma unroll
         for (int i = 0; i < kItems; ++i) byte[i] = row0 + 4 * kGroupWarps * i < left ? byte[i] : 0u;
       }
+      fence_proxy_async();  // read before the next copy into this place (load_codes)
       __syncwarp();
       if (lane == 0) mbar_arrive(&raw_empty_bar[raw_stage]);
       mbar_wait(empty + stage * 8, phase ^ 1, &abort_flag);
@@ -430,6 +433,7 @@ grouped_few_rows_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid
         byte[i] = load_scale(scale_at + raw_stage * kRawBytes + (row & 31) * 16 + (row >> 5) * 4 + (step & 1) * 8);  // a tile of scales is two stages high
         if (row >= left) byte[i] = 0;
       }
+      fence_proxy_async();  // read before the next copy into this place (load_codes)
       __syncwarp();
       if (lane == 0) mbar_arrive(&raw_empty_bar[raw_stage]);
       mbar_wait(empty + stage * 8, phase ^ 1, &abort_flag);
