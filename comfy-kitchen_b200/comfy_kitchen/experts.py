@@ -2,8 +2,8 @@
 
 Rows come in the experts' order: expert e has the rows ``[offsets[e - 1], offsets[e])``, the first one from 0 on, with ``offsets`` an int32
 tensor ``[experts]`` on the device that nothing reads on the host, so a call can be captured in a CUDA graph and replayed with other ends.
-Ends that do not decrease and lie within the rows are the caller's to give; others give unspecified rows, and no access outside the
-tensors.  An expert may have no rows; rows behind the last expert's are zeros in the result.
+Ends that do not decrease and lie within the rows are the caller's to give; others give unspecified rows, no access outside the
+tensors and no more work than there are rows.  An expert may have no rows; rows behind the last expert's are zeros in the result.
 
 * :func:`grouped_mm_mxfp8`: both operands held in MXFP8, as :func:`comfy_kitchen.scaled_mm_mxfp8` takes them for one weight.
 * :func:`grouped_linear_mxfp8`: dense rows, quantized on the way; differentiable in the rows (the weights stay frozen, and the quantization

@@ -1,6 +1,6 @@
 // Rows that are grouped by expert: group e has the rows [offsets[e - 1], offsets[e]) of a matrix (the first one from 0 on), ends that
-// lie on the device.  What every kernel on such rows shares: the bounds, kept inside the matrix whatever the ends say, and
-// the walk over the groups' tiles, whose number only the device knows.
+// lie on the device.  What every kernel on such rows shares: the bounds, kept inside the matrix and from decreasing whatever the ends say (so
+// no row belongs to two groups, and the tiles are never more than the rows have), and the walk over the groups' tiles, whose number only the device knows.
 #pragma once
 
 #include "ck_common.cuh"
@@ -47,19 +47,25 @@ __host__ __device__ __forceinline__ int64_t scale_blocks(int64_t rows, int64_t c
 
 // In shared memory: the groups' bounds, and the numbers of row tiles before each.
 struct Table {
-  int bound[kMaxGroups + 1];  // group e: rows [bound[e], max(bound[e], bound[e + 1]))
+  int bound[kMaxGroups + 1];  // group e: rows [bound[e], bound[e + 1])
   int tiles[kMaxGroups + 1];  // row tiles of the groups before e
 };
 
-// Filled by all threads of the block, when the ends are there.
+// Filled by all threads of the block, when the ends are there.  An end below an earlier one counts as that one.
 __device__ __forceinline__ void fill_table(Table* t, const int* offsets, int count, int rows, int tile_rows) {
   for (int e = threadIdx.x; e <= count; e += blockDim.x) t->bound[e] = group_end(offsets, e - 1, rows);
   __syncthreads();
   if (threadIdx.x < 32) {
     int before = 0;
     for (int first = 0; first < count; first += 32) {
-      const int e = first + static_cast<int>(threadIdx.x);
-      const int own = e < count ? (max(t->bound[e + 1] - t->bound[e], 0) + tile_rows - 1) / tile_rows : 0;
+      const int e = first + static_cast<int>(threadIdx.x), from = min(e, count), to = min(e + 1, count);
+      if (__any_sync(0xFFFFFFFFu, t->bound[to] < t->bound[from])) {
+        if (threadIdx.x == 0) {
+          for (int i = first + 1; i <= count; ++i) t->bound[i] = max(t->bound[i], t->bound[i - 1]);
+        }
+        __syncwarp();
+      }
+      const int own = (t->bound[to] - t->bound[from] + tile_rows - 1) / tile_rows;
       int sum = own;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -104,7 +110,7 @@ __device__ __forceinline__ Tile place(const Table* t, int count, int tiles_n, in
   p.tile_n = in_band / height;
   p.index = band * kBand + in_band - p.tile_n * height;
   p.row = t->bound[lo] + p.index * tile_rows;
-  p.end = max(t->bound[lo], t->bound[lo + 1]);
+  p.end = t->bound[lo + 1];
   return p;
 }
 
