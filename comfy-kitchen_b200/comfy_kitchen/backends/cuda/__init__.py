@@ -510,7 +510,7 @@ def scaled_mm_nvfp4(a: torch.Tensor, b: torch.Tensor, tensor_scale_a: torch.Tens
     out = torch.empty((m, n), dtype=out_dtype, device=dev)
     with _on_device(dev):
         stream = _stream(dev)
-        need = _workspace_bytes("ck_scaled_mm_workspace_bytes", 0, m, n, k)
+        need = _workspace_bytes("ck_scaled_mm_workspace_bytes", 0, m, n, k, device=dev.index)
         ws = _workspace_for(need, dev, stream) if need > _ON_CHIP else None
         _check(lib.ck_scaled_mm_nvfp4_ws(a.data_ptr(), b.data_ptr(), block_scale_a.data_ptr(), block_scale_b.data_ptr(),
                                          tsa.data_ptr(), tsb.data_ptr(), _ptr(alpha_t), bias_ptr, bias_code, out.data_ptr(), DTYPE_TO_CODE[out_dtype], m, n, k,
@@ -611,7 +611,8 @@ def check_device_status(what: str = "kernel") -> None:
 
 
 @functools.lru_cache(maxsize=512)
-def _workspace_bytes(function: str, *shape: int) -> int:
+def _workspace_bytes(function: str, *shape: int, device: int | None = None) -> int:
+    """What the library asks for, kept by shape; where it depends on the number of SMs, by ``device`` too, which is current then."""
     return int(getattr(_lib, function)(*shape))
 
 
@@ -764,7 +765,7 @@ def scaled_mm_mxfp8(a: torch.Tensor, b: torch.Tensor, block_scale_a: torch.Tenso
     out = torch.empty((m, n), dtype=out_dtype, device=dev)
     with _on_device(dev):
         stream = _stream(dev)
-        need = _workspace_bytes("ck_scaled_mm_workspace_bytes", 1, m, n, k)
+        need = _workspace_bytes("ck_scaled_mm_workspace_bytes", 1, m, n, k, device=dev.index)
         ws = _workspace_for(need, dev, stream) if need > _ON_CHIP else None
         _check(lib.ck_scaled_mm_mxfp8_ws(a.data_ptr(), b.data_ptr(), block_scale_a.data_ptr(), block_scale_b.data_ptr(), bias_ptr, bias_code,
                                          out.data_ptr(), DTYPE_TO_CODE[out_dtype], m, n, k, _ptr(ws), need, stream),
@@ -906,8 +907,8 @@ def _layer_norm_backward(dy, x, codes, scales, mean, rstd, weight, weight_offset
             assert codes.shape == (rows, cols) and scales.shape == (roundup(rows, 128), roundup(cols // 32, 4)), "Invalid codes or scale shape"
             assert codes.is_contiguous() and scales.is_contiguous(), "codes and scales must be contiguous"
         dy, inner, outer_stride, inner_stride = _row_levels(dy, 16 if x is None else 1)
-        need = _workspace_bytes("ck_layer_norm_backward_workspace_bytes", rows, cols, groups) if weight_grad or bias_grad else 0
         with _on_device(dev):
+            need = _workspace_bytes("ck_layer_norm_backward_workspace_bytes", rows, cols, groups, device=dev.index) if weight_grad or bias_grad else 0
             ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
             _check(lib.ck_layer_norm_backward(dy.data_ptr(), DTYPE_TO_CODE[dy.dtype], rows, cols, inner, outer_stride, inner_stride, _ptr(x), x_inner,
                                               x_outer_stride, x_inner_stride, _ptr(codes), _ptr(scales), mean.data_ptr(), rstd.data_ptr(), _ptr(weight),
@@ -1008,8 +1009,8 @@ def linear_weight_grad_mxfp8(dy: torch.Tensor, x_codes: torch.Tensor, x_block_sc
     dweight = make((n, k), dtype=out_dtype, device=dev)
     dbias = make((n,), dtype=out_dtype, device=dev) if bias_grad else None
     if m > 0:
-        need = _workspace_bytes("ck_linear_grad_mxfp8_workspace_bytes", 1, DTYPE_TO_CODE[dy.dtype], int(bias_grad), m, n, k)
         with _on_device(dev):
+            need = _workspace_bytes("ck_linear_grad_mxfp8_workspace_bytes", 1, DTYPE_TO_CODE[dy.dtype], int(bias_grad), m, n, k, device=dev.index)
             ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
             _check(lib.ck_linear_weight_grad_mxfp8(dy.data_ptr(), DTYPE_TO_CODE[dy.dtype], codes.data_ptr(), scales.data_ptr(), dweight.data_ptr(),
                                                    DTYPE_TO_CODE[out_dtype], _ptr(dbias), m, n, k, ws.data_ptr(), need, _stream(dev)),
@@ -1030,8 +1031,8 @@ def linear_input_grad_mxfp8(dy: torch.Tensor, w_codes: torch.Tensor, w_block_sca
     m, dev, out_dtype = dy.shape[0], dy.device, out_dtype or dy.dtype
     dx = torch.empty((m, k), dtype=out_dtype, device=dev)
     if m > 0:
-        need = _workspace_bytes("ck_linear_grad_mxfp8_workspace_bytes", 0, DTYPE_TO_CODE[dy.dtype], 0, m, n, k)
         with _on_device(dev):
+            need = _workspace_bytes("ck_linear_grad_mxfp8_workspace_bytes", 0, DTYPE_TO_CODE[dy.dtype], 0, m, n, k, device=dev.index)
             ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
             _check(lib.ck_linear_input_grad_mxfp8(dy.data_ptr(), DTYPE_TO_CODE[dy.dtype], codes.data_ptr(), scales.data_ptr(), dx.data_ptr(),
                                                   DTYPE_TO_CODE[out_dtype], m, n, k, ws.data_ptr(), need, _stream(dev)),
@@ -1117,8 +1118,8 @@ def rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, rstd: torch.Tensor, wei
         dy, *dy_levels = _row_levels(dy)
         h, *h_levels = _row_levels(h)
         dh, *dh_levels = (None, 0, 0, 0) if dh is None else _row_levels(dh)
-        need = _workspace_bytes("ck_rms_norm_backward_workspace_bytes", DTYPE_TO_CODE[dy.dtype], rows, cols) if weight_grad else 0
         with _on_device(dev):
+            need = _workspace_bytes("ck_rms_norm_backward_workspace_bytes", DTYPE_TO_CODE[dy.dtype], rows, cols, device=dev.index) if weight_grad else 0
             ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
             _check(lib.ck_rms_norm_backward(dy.data_ptr(), DTYPE_TO_CODE[dy.dtype], rows, cols, *dy_levels, h.data_ptr(), *h_levels, _ptr(dh), *dh_levels,
                                             rstd.data_ptr(), _ptr(weight), code, weight_offset, dx.data_ptr(), _ptr(dweight), _ptr(ws), need, _stream(dev)),
@@ -1140,8 +1141,8 @@ def _clip(grads, max_norm: float):
         assert g.layout == torch.strided and g.is_contiguous(), "gradients must be contiguous"
     n = len(grads)
     norm = torch.empty((), dtype=torch.float32, device=dev)
-    need = _workspace_bytes("ck_clip_grad_norm_workspace_bytes", n)
     with _on_device(dev):
+        need = _workspace_bytes("ck_clip_grad_norm_workspace_bytes", n, device=dev.index)
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
         _check(lib.ck_clip_grad_norm((ctypes.c_void_p * n)(*[g.data_ptr() for g in grads]), (ctypes.c_int64 * n)(*[g.numel() for g in grads]),
                                      (ctypes.c_int * n)(*[DTYPE_TO_CODE[g.dtype] for g in grads]), n, max_norm, norm.data_ptr(), ws.data_ptr(), need,
