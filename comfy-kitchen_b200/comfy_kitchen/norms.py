@@ -138,16 +138,17 @@ def _list_call(name: str, grads: list[torch.Tensor], *args):
 
 
 def grad_norm(tensors: Iterable[torch.Tensor]) -> torch.Tensor:
-    """The 2-norm of all elements of the tensors (bf16, fp16 or fp32, on one GPU): a 0-d float32 tensor on that GPU."""
+    """The 2-norm of all elements of the tensors (bf16, fp16 or fp32, on one GPU): a 0-d float32 tensor on that GPU, for no tensors a zero on the CPU."""
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     if not tensors:
-        return torch.zeros(())
+        return torch.zeros((), dtype=torch.float32)
     dense = [t.detach() if t.is_contiguous() else t.detach().contiguous() for t in tensors]
     return _list_call("grad_norm", dense)
 
 
 def clip_grad_norm_(parameters: Iterable[torch.Tensor] | torch.Tensor, max_norm: float, error_if_nonfinite: bool = False) -> torch.Tensor:
-    """``torch.nn.utils.clip_grad_norm_`` for the 2-norm: every gradient times ``min(1, max_norm / (norm + 1e-6))``, in place; returns the norm.
+    """``torch.nn.utils.clip_grad_norm_`` for the 2-norm: every gradient times ``min(1, max_norm / (norm + 1e-6))``, in place; returns the norm,
+    0-d float32 (where no parameter has a gradient a zero on the first one's device).
 
     Gradients are bf16, fp16 or fp32, mixed at will, on one GPU, and do not overlap (a parameter that is given twice counts once).  Nothing is read
     on the host, so a step can be captured, except with ``error_if_nonfinite``, which raises before a gradient is changed."""
@@ -163,7 +164,7 @@ def clip_grad_norm_(parameters: Iterable[torch.Tensor] | torch.Tensor, max_norm:
                 return norm
     grads = list({id(p): p.grad for p in parameters if p.grad is not None}.values())
     if not grads:
-        return torch.zeros(())
+        return torch.zeros((), dtype=torch.float32, device=parameters[0].device if parameters else None)
     if error_if_nonfinite:
         norm = grad_norm(grads)
         if not math.isfinite(norm.item()):
