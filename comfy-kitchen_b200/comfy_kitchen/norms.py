@@ -113,7 +113,9 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, residual: torc
 
 
 class RMSNorm(nn.Module):
-    """``nn.RMSNorm`` over the last dimension; ``forward(x, residual)`` returns ``(y, x + residual)``."""
+    """RMS norm over the last dimension with a learned weight; ``forward(x, residual)`` returns ``(y, x + residual)``.
+
+    The parameter is named as ``nn.RMSNorm`` names it; ``eps`` is 1e-6 unless given, where torch's module takes the input type's epsilon."""
 
     def __init__(self, features: int, eps: float = 1e-6, device=None, dtype=None) -> None:
         super().__init__()

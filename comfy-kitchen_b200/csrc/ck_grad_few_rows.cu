@@ -337,7 +337,7 @@ grad_few_rows_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_co
 // ---- grouped rows --------------------------------------------------------------------------------------------
 // dX[i] = dY[i] W_e for the rows i of group e: the same operand, but blocks that stay and take tiles (a group's rows, 128 columns of W_e) in turn, accumulators in two
 // sets, so that a tile is stored beside the next one's steps, and loads of dY and of codes by warps of their own.  Bound by the decoding, 2.9 million codes a microsecond: 64
-// groups of 32 rows, 2048 x 2048 each, bf16 93 us (fp32, three numbers an element, 138); eight rows of as many groups, 1536 x 2048, 14.0.
+// groups of 32 rows, 2048 x 2048 each, bf16 94 us (fp32, three numbers an element, 143); eight rows of as many groups, 1536 x 2048, 13.6.
 constexpr int kRowBox = 16;  // rows of dY in a copy
 constexpr int kStoreWarps = 4, kGroupedThreads = kThreads + 32 * (kStoreWarps + 1);  // beside those of the kernel above, and the loads of dY apart from the codes
 

@@ -10,12 +10,13 @@
 // warps, two roles' distance by mbarriers) over a list of tiles that every CTA makes for itself from the groups' ends.  Rows behind the group's end are not stored;
 // rows behind the last group are zeros.
 //
-// CTA pairs, for many rows, compute W_e x^T: the weights' rows are the MMA's 256, x's rows its columns, of which there may be any multiple of 32, so that a group's last
-// tile costs what it has rows for.  The results come feature by feature and are turned in shared memory on their way out.  (With x's rows as the MMA's 256, last tiles
-// whole, us, so / before: 64 experts of 2048 x 2048, 140 rows each 62 / 69, 188 uneven ones 75 / 81, 256 88 / 92; 8 of 8192 x 4096, 1024 uneven rows 215 to 258 / 235 to 267;
-// 8 of 8192 x 512 48.9 / 47.5.)
+// CTA pairs, for many rows, compute W_e x^T: the weights' rows are the MMA's 256, x's rows its columns, of which there may be any multiple of 32, so that the MMAs of a
+// group's last tile cost what it has rows for; its loads of the weights are a whole tile's.  The results come feature by feature and are turned in shared memory on their way
+// out.  (With x's rows as the MMA's 256, last tiles whole, us, so / before: 64 experts of 2048 x 2048, 140 rows each 62 / 69, 188 uneven ones 75 / 81, 256 88 / 92; 8 of
+// 8192 x 4096, 1024 uneven rows 215 to 258 / 235 to 267; 8 of 8192 x 512 48.9 / 47.5; all of these with pairs that started beside the kernel in front.  Behind it, as now, from MXFP8 rows:
+// 140 each 65, 188 uneven 74, 256 74.)
 //
-// Many rows: bound by the tensor pipe and, in a loop, by the power limit (8192 x 8192 x 4096 of 8 experts from bf16 235 us, 2.3 PFLOP/s with the quantization;
+// Many rows: bound by the tensor pipe and, in a loop, by the power limit (8192 x 8192 x 4096 of 8 experts from bf16 234 us, 2.3 PFLOP/s with the quantization;
 // one weight for all rows 202).  Few rows: by the weights' bytes (64 experts of 2048 x 2048, 32 rows each, 55 us,
 // 5.3 TB/s); one token through eight of 64 experts, 25 MB, 10.4 us: two launches, first loads (11.7 with the weights asked for behind the first kernel's end;
 // 777 rows of 40 experts of 1000 x 1056 16.3 and 18.3; a few megabytes of weights gain nothing, 64 rows of 8 experts of 1024 x 1024 7.1 and 6.9).

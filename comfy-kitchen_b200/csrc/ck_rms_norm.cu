@@ -20,10 +20,10 @@ namespace {
 
 using sm100::smem_u32;
 
-// Rows in two levels: row r is row r % inner of outer index r / inner.  The quotient by a product and a shift, made for `inner` on the host: for
-// rows below 2^31, r / d = (high half of m * r + r) >> l with 2^l >= d and m = floor(2^32 (2^l - d) / d) + 1.  (The compiler's division, for
-// three tensors a row, kept the conversion unit busy for half of the backward kernel's time.)
-struct RowStrides {
+// rows::RowStrides with another quotient.  Row r is row r % inner of outer index r / inner; the quotient by a product and a shift, made for `inner` on the
+// host, is the division by an invariant integer of Granlund and Montgomery (1994): for rows below 2^31, r / d = (high half of m * r + r) >> l with 2^l >= d
+// and m = floor(2^32 (2^l - d) / d) + 1.  (The compiler's division, for three tensors a row, kept the conversion unit busy for half of the backward kernel's time.)
+struct DividedRows {
   int64_t outer_stride, inner_stride;  // elements
   uint32_t inner, m, l;
   __device__ __forceinline__ int64_t offset(uint32_t row) const {
@@ -42,7 +42,7 @@ struct RmsArgs {
   uint8_t* codes;
   uint8_t* scales;
   int64_t rows, cols;
-  RowStrides x_strides, r_strides;
+  DividedRows x_strides, r_strides;
   float eps, offset;
   bool weight_f32;
   int lanes;             // of a team
@@ -57,7 +57,7 @@ struct RmsBackwardArgs {
   void* dx;
   float* partials;     // [blocks][cols], or null
   int64_t rows, cols;
-  RowStrides dy_strides, h_strides, dh_strides;
+  DividedRows dy_strides, h_strides, dh_strides;
   float offset;
   bool weight_f32;
   int lanes;
@@ -729,7 +729,7 @@ int lanes_of(int size, Form form, int64_t cols, int vecs, int least, int most) {
   return pow2;
 }
 
-RowStrides strides_of(const Rows& r, int64_t rows) {
+DividedRows strides_of(const Rows& r, int64_t rows) {
   const uint32_t d = static_cast<uint32_t>(r.inner < rows ? r.inner : rows);
   uint32_t l = 0;
   while ((1ull << l) < d) ++l;
